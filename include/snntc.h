@@ -19,8 +19,8 @@
  *                         REGISTER_OP("SnnCvGrad") snntc/snncvgrad_ops.cc:6-20
  *
  * Conventions
- *  - All tensors are float32, row-major (images NHWC), and live in DEVICE memory, except
- *    `params`, which is a HOST pointer (the reference pins it with HostMemory("params"),
+ *  - All tensors are float32 (the operators over tokens and choices take 16-bit types where they say so),
+ *    row-major (images NHWC), and live in DEVICE memory, except `params`, which is a HOST pointer (the reference pins it with HostMemory("params"),
  *    snntc/snnfc_kernels.cc:224, snntc/snncv_kernels.cc:259).
  *  - The caller owns every buffer, including the scratch `workspace` (device memory, 256-byte
  *    aligned, at least snntc_*_workspace_bytes() long).  The library allocates nothing, keeps no
@@ -298,6 +298,92 @@ SNNTC_API int snntc_weight_cost_grad(const float* const* w, float* const* grad, 
 SNNTC_API int snntc_recipe_total(const int64_t* rows, const int64_t* cols, int64_t count, float k, float k2,
                        const float* sample_loss, const int32_t* correct, int64_t B, float* total, int64_t* n_correct,
                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Element types of the tensors below that need not be float32 (tables, gates, the losses' times and the gradients of
+ * each).  Arithmetic is float32 throughout; a result is rounded to its type once, to nearest even.
+ * ------------------------------------------------------------------------------------------- */
+enum { SNNTC_F32 = 0, SNNTC_BF16 = 1, SNNTC_F16 = 2 };
+
+/* ---------------------------------------------------------------------------------------------
+ * Spike times of tokens: tokens[N] (token_bytes 4: int32, 8: int64), table[V,D] of table_type.
+ *   z[n,:] = scale table[tokens[n],:], or exp(1 - scale table[tokens[n],:]) with encode != 0 (float32; the encoding of
+ *   snntc_encode_time).  A token outside [0, V) leaves NaN in its row.
+ *   dtable[v,:] = k_v sum over { n : tokens[n] = v } of grad[n,:], k_v = scale, or -scale exp(1 - scale table[v,:]): every
+ *   row of dtable is written, rows are added in the order of their positions, with the same sums on every call.  Positions
+ *   whose token lies outside the table add nothing.  table may be NULL in the backward call where encode is 0.
+ * Errors: a negative size, a token_bytes or table_type that is none of the above, a NULL required pointer, V = 0 with N > 0
+ * -> BAD_ARGUMENT; N, V or D above INT32_MAX -> TOO_LARGE (products may exceed it); a workspace below
+ * _workspace_bytes -> WORKSPACE.
+ * ------------------------------------------------------------------------------------------- */
+SNNTC_API int snntc_embed_forward(const void* tokens, int token_bytes, const void* table, int table_type, float* z, int64_t N,
+                        int64_t V, int64_t D, float scale, int encode, void* stream);
+SNNTC_API int snntc_embed_backward_workspace_bytes(int64_t N, int64_t V, int64_t D, size_t* bytes);
+SNNTC_API int snntc_embed_backward(const float* grad, const void* tokens, int token_bytes, const void* table, int table_type,
+                         void* dtable, int64_t N, int64_t V, int64_t D, float scale, int encode, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Gated running mean of spike times along a sequence, x[B,T,D], gate[B,T,D] of gate_type:
+ *   a_t = sigmoid(gate_t),  h_t = a_t h_{t-1} + (1 - a_t) x_t,  y_t = h_t,  h_0 = state[B,D] (NULL: zeros)
+ * lengths[B] (int64, NULL: all T; values outside [0, T] count as the nearer end): steps behind a sequence's length are
+ * not read, y there is 0, and final_state[B,D] (may be NULL) is h at the sequence's length (the initial state for
+ * length 0).
+ * Backward, with y the forward output and u_t the gradient that reaches h_t:
+ *   u_t = dy_t + a_{t+1} u_{t+1} (dfinal at a sequence's end),  dx_t = (1 - a_t) u_t,
+ *   dgate_t = u_t (h_{t-1} - x_t) a_t (1 - a_t),  dstate = a_1 u_1
+ * dy, dfinal, state: NULL counts as zeros.  dx, dgate (of gate_type), dstate: NULL is not computed.  dx and dgate are 0
+ * behind a sequence's length, dy there is not read.  One workspace size serves both directions.
+ * snntc_gated_step is one step of n independent channels: out = a state + (1 - a) x (state NULL: zeros; out may be state).
+ * Errors: a negative size, a gate_type that is none of the above, a NULL required pointer -> BAD_ARGUMENT; B, T or D
+ * above INT32_MAX -> TOO_LARGE; a workspace below _workspace_bytes -> WORKSPACE.
+ * ------------------------------------------------------------------------------------------- */
+SNNTC_API int snntc_gated_scan_workspace_bytes(int64_t B, int64_t T, int64_t D, size_t* bytes);
+SNNTC_API int snntc_gated_scan_forward(const float* x, const void* gate, int gate_type, const float* state, const int64_t* lengths,
+                             float* y, float* final_state, int64_t B, int64_t T, int64_t D, void* workspace,
+                             size_t workspace_bytes, void* stream);
+SNNTC_API int snntc_gated_scan_backward(const float* dy, const float* dfinal, const float* x, const void* gate, int gate_type,
+                              const float* y, const float* state, const int64_t* lengths, float* dx, void* dgate,
+                              float* dstate, int64_t B, int64_t T, int64_t D, void* workspace, size_t workspace_bytes,
+                              void* stream);
+SNNTC_API int snntc_gated_step(const float* x, const void* gate, int gate_type, const float* state, float* out, int64_t n,
+                     void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Losses over choices: every row times[r,:] of J spike times stands for softmax(-times), and one output of it was chosen
+ * (tokens[r], int64).  logp[r] = log softmax(-times[r])[tokens[r]]; a token outside [0, J) leaves NaN in its row.
+ * A row of weight 0 is not read: its logp and loss are 0 and its gradient is 0.
+ *   snntc_time_logp           logp[rows] and, for the backward call, stats[rows,2] (8-byte aligned; may be NULL).
+ *   snntc_time_logp_backward  dtimes[r,j] = upstream coef[r] (softmax(-times[r])[j] - [j = tokens[r]]), of times' type, the
+ *                             gradient where coef[r] is a loss's derivative by logp[r] (upstream: a device scalar, NULL = 1).
+ *   snntc_policy_loss         clipped policy loss with a KL term, ratio = exp(logp - old_logp), d = ref_logp - logp:
+ *       row_loss = kl_coef (exp(d) - d - 1) - min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A),  A = advantage[r]
+ *       (ref_logp NULL: no KL term).  The objective is sum_r weight[r] row_loss[r], weight NULL: the mean.  stats, coef[rows]
+ *       and dtimes: its saved values for the backward call, its derivative by each logp, its gradient; each may be NULL, logp too.
+ *   snntc_preference_loss     P pairs of sequences of T rows each, the preferred ones first (times[2P,T,J], tokens and
+ *       weight[2P,T], ref_logp[2P] = log-probability of each sequence under the reference):
+ *       seq_logp[q] = sum_t weight[q,t] logp[q,t],  m = beta ((seq_logp - ref_logp)[p] - (seq_logp - ref_logp)[P + p])
+ *       pair_loss[p] = -(1 - smoothing) log sigmoid(m) - smoothing log sigmoid(-m)
+ *       The objective is the mean of pair_loss.  weight NULL: all 1.  stats, coef[2P,T], dtimes as above.
+ *   snntc_loss_total          total = sum_i weight[i] loss[i] (weight NULL: the mean), added in a fixed order.
+ * Errors: a negative size, a times_type that is none of the above, a NULL required pointer, J = 0 with rows, a clip below 0
+ * or a clip_low above 1, smoothing outside [0, 1], a beta or kl_coef that is not finite -> BAD_ARGUMENT; more than 2^24 - 1
+ * rows, J above INT32_MAX -> TOO_LARGE; a workspace below _workspace_bytes (of all rows) -> WORKSPACE.
+ * ------------------------------------------------------------------------------------------- */
+SNNTC_API int snntc_choice_workspace_bytes(int64_t rows, int64_t J, size_t* bytes);
+SNNTC_API int snntc_time_logp(const void* times, int times_type, const int64_t* tokens, const float* weight, float* logp,
+                    float* stats, int64_t rows, int64_t J, void* workspace, size_t workspace_bytes, void* stream);
+SNNTC_API int snntc_time_logp_backward(const void* times, int times_type, const int64_t* tokens, const float* stats,
+                             const float* coef, const float* upstream, void* dtimes, int64_t rows, int64_t J, void* stream);
+SNNTC_API int snntc_policy_loss(const void* times, int times_type, const int64_t* actions, const float* old_logp,
+                      const float* advantage, const float* ref_logp, const float* weight, float clip_low, float clip_high,
+                      float kl_coef, float* row_loss, float* logp, float* stats, float* coef, void* dtimes, int64_t rows,
+                      int64_t J, void* workspace, size_t workspace_bytes, void* stream);
+SNNTC_API int snntc_preference_loss(const void* times, int times_type, const int64_t* tokens, const float* ref_logp,
+                          const float* weight, float beta, float smoothing, float* pair_loss, float* seq_logp, float* stats,
+                          float* coef, void* dtimes, int64_t P, int64_t T, int64_t J, void* workspace,
+                          size_t workspace_bytes, void* stream);
+SNNTC_API int snntc_loss_total(const float* loss, const float* weight, float* total, int64_t n, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Health of the bounded wait described at snntc_fc_forward (no counterpart in the reference, whose scan

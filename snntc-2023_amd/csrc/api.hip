@@ -539,6 +539,184 @@ int snntc_recipe_total(const int64_t* rows, const int64_t* cols, int64_t count, 
                                static_cast<float*>(workspace), static_cast<hipStream_t>(stream));
 }
 
+// ---- sequences of tokens and choices -----------------------------------------------------------------
+
+static bool known_type(int type) { return type == SNNTC_F32 || type == SNNTC_BF16 || type == SNNTC_F16; }
+
+static int embed_check(int64_t N, int64_t V, int64_t D, const char* who) {
+    if (N < 0 || V < 0 || D < 0) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: negative size", who);
+    if (N > kInt32Max || V > kInt32Max || D > kInt32Max)
+        return fail(SNNTC_ERR_TOO_LARGE, "%s: a dimension exceeds INT32_MAX", who);
+    return SNNTC_OK;
+}
+
+static int embed_types(int64_t N, int64_t V, int token_bytes, int table_type, const char* who) {
+    if (token_bytes != 4 && token_bytes != 8) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: tokens of %d bytes", who, token_bytes);
+    if (!known_type(table_type)) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: unknown table type %d", who, table_type);
+    if (N > 0 && V == 0) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: tokens but an empty table", who);
+    return SNNTC_OK;
+}
+
+int snntc_embed_forward(const void* tokens, int token_bytes, const void* table, int table_type, float* z, int64_t N, int64_t V,
+                        int64_t D, float scale, int encode, void* stream) {
+    int rc = embed_check(N, V, D, "snntc_embed_forward");
+    if (!rc) rc = embed_types(N, V, token_bytes, table_type, "snntc_embed_forward");
+    if (rc || N == 0 || D == 0) return rc;
+    if (!tokens || !table || !z) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_embed_forward: null pointer");
+    return launch_embed_forward(tokens, token_bytes, table, table_type, z, N, V, D, scale, encode != 0, static_cast<hipStream_t>(stream));
+}
+
+int snntc_embed_backward_workspace_bytes(int64_t N, int64_t V, int64_t D, size_t* bytes) {
+    const int rc = embed_check(N, V, D, "snntc_embed_backward_workspace_bytes");
+    if (rc) return rc;
+    if (!bytes) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_embed_backward_workspace_bytes: bytes is NULL");
+    *bytes = embed_backward_workspace(N, V, D);
+    return SNNTC_OK;
+}
+
+int snntc_embed_backward(const float* grad, const void* tokens, int token_bytes, const void* table, int table_type, void* dtable,
+                         int64_t N, int64_t V, int64_t D, float scale, int encode, void* workspace, size_t workspace_bytes,
+                         void* stream) {
+    int rc = embed_check(N, V, D, "snntc_embed_backward");
+    if (!rc) rc = embed_types(N, V, token_bytes, table_type, "snntc_embed_backward");
+    if (rc || V == 0 || D == 0) return rc;
+    if (!dtable || (N > 0 && (!grad || !tokens)) || (encode && !table))
+        return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_embed_backward: null pointer");
+    rc = check_workspace(workspace, workspace_bytes, embed_backward_workspace(N, V, D));
+    if (rc) return rc;
+    return launch_embed_backward(grad, tokens, token_bytes, table, table_type, dtable, N, V, D, scale, encode != 0, workspace,
+                                 static_cast<hipStream_t>(stream));
+}
+
+static int gated_check(int64_t B, int64_t T, int64_t D, int gate_type, const char* who) {
+    if (B < 0 || T < 0 || D < 0) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: negative size", who);
+    if (!known_type(gate_type)) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: unknown gate type %d", who, gate_type);
+    if (B > kInt32Max || T > kInt32Max || D > kInt32Max)
+        return fail(SNNTC_ERR_TOO_LARGE, "%s: a dimension exceeds INT32_MAX", who);
+    return SNNTC_OK;
+}
+
+int snntc_gated_scan_workspace_bytes(int64_t B, int64_t T, int64_t D, size_t* bytes) {
+    const int rc = gated_check(B, T, D, SNNTC_F32, "snntc_gated_scan_workspace_bytes");
+    if (rc) return rc;
+    if (!bytes) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_gated_scan_workspace_bytes: bytes is NULL");
+    *bytes = gated_scan_workspace(B, T, D);
+    return SNNTC_OK;
+}
+
+int snntc_gated_scan_forward(const float* x, const void* gate, int gate_type, const float* state, const int64_t* lengths, float* y,
+                             float* final_state, int64_t B, int64_t T, int64_t D, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = gated_check(B, T, D, gate_type, "snntc_gated_scan_forward");
+    if (rc || B == 0 || D == 0 || (T == 0 && !final_state)) return rc;
+    if (T > 0 && (!x || !gate || !y)) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_gated_scan_forward: null pointer");
+    rc = check_workspace(workspace, workspace_bytes, gated_scan_workspace(B, T, D));
+    if (rc) return rc;
+    return launch_gated_scan_forward(x, gate, gate_type, state, lengths, y, final_state, B, T, D, workspace,
+                                     static_cast<hipStream_t>(stream));
+}
+
+int snntc_gated_scan_backward(const float* dy, const float* dfinal, const float* x, const void* gate, int gate_type, const float* y,
+                              const float* state, const int64_t* lengths, float* dx, void* dgate, float* dstate, int64_t B, int64_t T,
+                              int64_t D, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = gated_check(B, T, D, gate_type, "snntc_gated_scan_backward");
+    if (rc || B == 0 || D == 0 || (T == 0 && !dstate) || (!dx && !dgate && !dstate)) return rc;
+    if (T > 0 && (!x || !gate || !y)) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_gated_scan_backward: null pointer");
+    rc = check_workspace(workspace, workspace_bytes, gated_scan_workspace(B, T, D));
+    if (rc) return rc;
+    return launch_gated_scan_backward(dy, dfinal, x, gate, gate_type, y, state, lengths, dx, dgate, dstate, B, T, D, workspace,
+                                      static_cast<hipStream_t>(stream));
+}
+
+int snntc_gated_step(const float* x, const void* gate, int gate_type, const float* state, float* out, int64_t n, void* stream) {
+    if (n < 0) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_gated_step: negative size");
+    if (!known_type(gate_type)) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_gated_step: unknown gate type %d", gate_type);
+    if (n == 0) return SNNTC_OK;
+    if (!x || !gate || !out) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_gated_step: null pointer");
+    return launch_gated_step(x, gate, gate_type, state, out, n, static_cast<hipStream_t>(stream));
+}
+
+static int choice_check(int64_t rows, int64_t J, int times_type, const char* who) {
+    if (rows < 0 || J < 0) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: negative size", who);
+    if (!known_type(times_type)) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: unknown type of times %d", who, times_type);
+    if (rows > 0 && J == 0) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: rows without outputs", who);
+    if (rows >= (1 << 24)) return fail(SNNTC_ERR_TOO_LARGE, "%s: more than 2^24 - 1 rows", who);
+    if (J > kInt32Max) return fail(SNNTC_ERR_TOO_LARGE, "%s: more than INT32_MAX outputs", who);
+    return SNNTC_OK;
+}
+
+int snntc_choice_workspace_bytes(int64_t rows, int64_t J, size_t* bytes) {
+    const int rc = choice_check(rows, J, SNNTC_F32, "snntc_choice_workspace_bytes");
+    if (rc) return rc;
+    if (!bytes) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_choice_workspace_bytes: bytes is NULL");
+    *bytes = choice_workspace(rows, J);
+    return SNNTC_OK;
+}
+
+int snntc_time_logp(const void* times, int times_type, const int64_t* tokens, const float* weight, float* logp, float* stats,
+                    int64_t rows, int64_t J, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = choice_check(rows, J, times_type, "snntc_time_logp");
+    if (rc || rows == 0) return rc;
+    if (!times || !tokens || !logp) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_time_logp: null pointer");
+    rc = check_workspace(workspace, workspace_bytes, choice_workspace(rows, J));
+    if (rc) return rc;
+    return launch_time_logp(times, times_type, tokens, weight, logp, stats, rows, J, workspace, static_cast<hipStream_t>(stream));
+}
+
+int snntc_time_logp_backward(const void* times, int times_type, const int64_t* tokens, const float* stats, const float* coef,
+                             const float* upstream, void* dtimes, int64_t rows, int64_t J, void* stream) {
+    const int rc = choice_check(rows, J, times_type, "snntc_time_logp_backward");
+    if (rc || rows == 0) return rc;
+    if (!times || !tokens || !stats || !coef || !dtimes) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_time_logp_backward: null pointer");
+    return launch_time_logp_backward(times, times_type, tokens, stats, coef, upstream, dtimes, rows, J, static_cast<hipStream_t>(stream));
+}
+
+int snntc_policy_loss(const void* times, int times_type, const int64_t* actions, const float* old_logp, const float* advantage,
+                      const float* ref_logp, const float* weight, float clip_low, float clip_high, float kl_coef, float* row_loss,
+                      float* logp, float* stats, float* coef, void* dtimes, int64_t rows, int64_t J, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+    int rc = choice_check(rows, J, times_type, "snntc_policy_loss");
+    if (rc) return rc;
+    if (!(clip_low >= 0.0f && clip_low <= 1.0f && clip_high >= 0.0f) || !isfinite(kl_coef))
+        return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_policy_loss: clip (%g, %g) or kl_coef %g outside its range", (double)clip_low,
+                    (double)clip_high, (double)kl_coef);
+    if (rows == 0) return SNNTC_OK;
+    if (!times || !actions || !old_logp || !advantage || !row_loss)
+        return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_policy_loss: null pointer");
+    rc = check_workspace(workspace, workspace_bytes, choice_workspace(rows, J));
+    if (rc) return rc;
+    const PolicyArgs a{old_logp, advantage, ref_logp, weight, 1.0f - clip_low, 1.0f + clip_high, kl_coef, 1.0f / (float)rows};
+    return launch_policy_loss(times, times_type, actions, a, row_loss, logp, stats, coef, dtimes, rows, J, workspace,
+                              static_cast<hipStream_t>(stream));
+}
+
+int snntc_preference_loss(const void* times, int times_type, const int64_t* tokens, const float* ref_logp, const float* weight,
+                          float beta, float smoothing, float* pair_loss, float* seq_logp, float* stats, float* coef, void* dtimes,
+                          int64_t P, int64_t T, int64_t J, void* workspace, size_t workspace_bytes, void* stream) {
+    if (P < 0 || T < 0) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_preference_loss: negative size");
+    if (P > kInt32Max || T > kInt32Max) return fail(SNNTC_ERR_TOO_LARGE, "snntc_preference_loss: too many pairs or steps");
+    const int64_t rows = 2 * P * T;
+    int rc = choice_check(rows, J, times_type, "snntc_preference_loss");
+    if (rc) return rc;
+    if (!(smoothing >= 0.0f && smoothing <= 1.0f) || !isfinite(beta))
+        return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_preference_loss: beta %g or smoothing %g outside its range", (double)beta,
+                    (double)smoothing);
+    if (P == 0) return SNNTC_OK;
+    if (P >= (1 << 24)) return fail(SNNTC_ERR_TOO_LARGE, "snntc_preference_loss: more than 2^24 - 1 pairs");
+    if (!ref_logp || !pair_loss || !seq_logp || (rows > 0 && (!times || !tokens)))
+        return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_preference_loss: null pointer");
+    rc = check_workspace(workspace, workspace_bytes, choice_workspace(rows, J));
+    if (rc) return rc;
+    const PreferenceArgs a{ref_logp, weight, beta, smoothing};
+    return launch_preference_loss(times, times_type, tokens, a, pair_loss, seq_logp, stats, coef, dtimes, P, T, J, workspace,
+                                  static_cast<hipStream_t>(stream));
+}
+
+int snntc_loss_total(const float* loss, const float* weight, float* total, int64_t n, void* stream) {
+    if (n < 0) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_loss_total: negative size");
+    if (!total || (n > 0 && !loss)) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_loss_total: null pointer");
+    return launch_loss_total(loss, weight, total, n, static_cast<hipStream_t>(stream));
+}
+
 int snntc_scan_status(int64_t* giveups, void* stream) {
     if (!giveups) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_scan_status: giveups is NULL");
     return read_scan_giveups(giveups, static_cast<hipStream_t>(stream));

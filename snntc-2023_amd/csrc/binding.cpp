@@ -55,7 +55,11 @@ using torch::autograd::variable_list;
     F(snntc_cv_backward_workspace_bytes) F(snntc_softmax_time_loss) F(snntc_sgd_update)                            \
     F(snntc_min_pool_forward) F(snntc_min_pool_forward_chained) F(snntc_min_pool_backward)                         \
     F(snntc_pad_time_forward) F(snntc_pad_time_backward) F(snntc_encode_time) F(snntc_label_loss)                  \
-    F(snntc_weight_cost_workspace_bytes) F(snntc_weight_cost_sums) F(snntc_weight_cost_grad) F(snntc_recipe_total)
+    F(snntc_weight_cost_workspace_bytes) F(snntc_weight_cost_sums) F(snntc_weight_cost_grad) F(snntc_recipe_total)    \
+    F(snntc_embed_forward) F(snntc_embed_backward) F(snntc_embed_backward_workspace_bytes)                         \
+    F(snntc_gated_scan_forward) F(snntc_gated_scan_backward) F(snntc_gated_scan_workspace_bytes)                   \
+    F(snntc_gated_step) F(snntc_choice_workspace_bytes) F(snntc_time_logp) F(snntc_time_logp_backward)             \
+    F(snntc_policy_loss) F(snntc_preference_loss) F(snntc_loss_total)
 
 struct Library {
 #define SNNTC_FIELD(f) decltype(&::f) f = nullptr;
@@ -107,6 +111,51 @@ Tensor dev_f32(const Tensor& t, const char* name, int64_t ndim) {
     TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat, name, " must be float32, got ", t.scalar_type());
     TORCH_CHECK_VALUE(t.dim() == ndim, name, " must have ", ndim, " dimensions, got shape ", shape_text(t));
     return t.contiguous();
+}
+
+// A device tensor of float32 or a 16-bit float type.
+Tensor dev_float(const Tensor& t, const char* name) {
+    if (!t.is_cuda())
+        raise_class(g_library_error, message_args, 0, std::string(name) + " lives on " + t.device().str() +
+                    ": the SNN-TC ops run on a ROCm GPU only (no CPU fallback)");
+    const at::ScalarType s = t.scalar_type();
+    TORCH_CHECK_TYPE(s == at::kFloat || s == at::kBFloat16 || s == at::kHalf, name, " must be float32, bfloat16 or float16, got ", s);
+    return t.contiguous();
+}
+
+int float_type(const Tensor& t) {
+    return t.scalar_type() == at::kFloat ? SNNTC_F32 : t.scalar_type() == at::kBFloat16 ? SNNTC_BF16 : SNNTC_F16;
+}
+
+void same_device(const Tensor& t, const Tensor& with, const char* name) {
+    if (!t.is_cuda())
+        raise_class(g_library_error, message_args, 0, std::string(name) + " lives on " + t.device().str() +
+                    ": the SNN-TC ops run on a ROCm GPU only (no CPU fallback)");
+    TORCH_CHECK_VALUE(t.device() == with.device(), name, " lives on ", t.device().str(), ", not on ", with.device().str());
+}
+
+// A float32 tensor of the given shape on the device of `with`; undefined stays undefined.
+Tensor f32_like(const Tensor& t, const Tensor& with, at::IntArrayRef sizes, const char* name) {
+    if (!t.defined()) return t;
+    same_device(t, with, name);
+    TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat, name, " must be float32, got ", t.scalar_type());
+    TORCH_CHECK_VALUE(t.sizes() == sizes, name, " must have shape ", sizes, ", got ", shape_text(t));
+    return t.contiguous();
+}
+
+Tensor index_like(const Tensor& t, const Tensor& with, const char* name, bool narrow) {
+    same_device(t, with, name);
+    TORCH_CHECK_TYPE(t.scalar_type() == at::kLong || (narrow && t.scalar_type() == at::kInt), name, " must be ",
+                     narrow ? "int64 or int32" : "int64", ", got ", t.scalar_type());
+    return t.contiguous();
+}
+
+int64_t* i64(const Tensor& t) { return t.defined() ? static_cast<int64_t*>(t.data_ptr()) : nullptr; }
+void* raw(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+void no_gradient(std::initializer_list<std::pair<const Tensor*, const char*>> tensors, const char* who) {
+    for (const auto& t : tensors)
+        TORCH_CHECK_VALUE(!t.first->defined() || !t.first->requires_grad(), who, ": ", t.second, " must not require a gradient");
 }
 
 float* f32(const Tensor& t) { return t.defined() ? static_cast<float*>(t.data_ptr()) : nullptr; }
@@ -285,6 +334,185 @@ LossOut time_loss(const Tensor& times, const Tensor& label, bool want_loss, bool
     check(lib.snntc_softmax_time_loss(f32(times), f32(label), f32(r.loss), f32(r.grad), times.size(0), times.size(1),
                                       stream_of(times)));
     return r;
+}
+
+// ---- sequences of tokens and choices ---------------------------------------------------------------------------------
+
+struct EmbedArgs { Tensor tokens, table; float scale; bool encode; };
+
+EmbedArgs embed_args(const Tensor& tokens, const Tensor& table, float scale, bool encode) {
+    EmbedArgs a{Tensor(), dev_float(table, "table"), scale, encode};
+    TORCH_CHECK_VALUE(table.dim() == 2, "table must have 2 dimensions, got shape ", shape_text(table));
+    a.tokens = index_like(tokens, a.table, "tokens", true);
+    return a;
+}
+
+Tensor embed_tokens(const EmbedArgs& a) {
+    const c10::DeviceGuard guard(a.table.device());
+    std::vector<int64_t> sizes = a.tokens.sizes().vec();
+    sizes.push_back(a.table.size(1));
+    const Tensor z = at::empty(sizes, a.table.options().dtype(at::kFloat));
+    check(lib.snntc_embed_forward(raw(a.tokens), (int)a.tokens.element_size(), raw(a.table), float_type(a.table), f32(z), a.tokens.numel(),
+                                  a.table.size(0), a.table.size(1), a.scale, a.encode, stream_of(a.table)));
+    return z;
+}
+
+Tensor embed_tokens_grad(const Tensor& grad_in, const EmbedArgs& a) {
+    std::vector<int64_t> sizes = a.tokens.sizes().vec();
+    sizes.push_back(a.table.size(1));
+    const Tensor grad = f32_like(grad_in, a.table, sizes, "grad");
+    const c10::DeviceGuard guard(a.table.device());
+    const int64_t N = a.tokens.numel(), V = a.table.size(0), D = a.table.size(1);
+    size_t need = 0;
+    check(lib.snntc_embed_backward_workspace_bytes(N, V, D, &need));
+    const Tensor ws = scratch(a.table, need), d = empty(a.table, a.table.sizes());
+    check(lib.snntc_embed_backward(f32(grad), raw(a.tokens), (int)a.tokens.element_size(), raw(a.table), float_type(a.table), raw(d), N, V,
+                                   D, a.scale, a.encode, ws.data_ptr(), ws.numel(), stream_of(a.table)));
+    return d;
+}
+
+struct GatedArgs { Tensor x, gate, state, lengths; };
+
+GatedArgs gated_args(const Tensor& x_in, const Tensor& gate_in, const Tensor& state, const Tensor& lengths) {
+    GatedArgs a;
+    a.x = dev_f32(x_in, "x", 3);
+    TORCH_CHECK_VALUE(gate_in.sizes() == a.x.sizes(), "gate ", shape_text(gate_in), " does not match x ", shape_text(a.x));
+    a.gate = dev_float(gate_in, "gate");
+    same_device(a.gate, a.x, "gate");
+    a.state = f32_like(state, a.x, {a.x.size(0), a.x.size(2)}, "state");
+    if (lengths.defined()) {
+        a.lengths = index_like(lengths, a.x, "lengths", false);
+        TORCH_CHECK_VALUE(a.lengths.dim() == 1 && a.lengths.size(0) == a.x.size(0), "lengths must have one entry per sequence, got shape ",
+                          shape_text(a.lengths), " for x ", shape_text(a.x));
+    }
+    return a;
+}
+
+struct Scanned { Tensor y, final; };
+
+Tensor gated_scratch(const GatedArgs& a) {
+    size_t need = 0;
+    check(lib.snntc_gated_scan_workspace_bytes(a.x.size(0), a.x.size(1), a.x.size(2), &need));
+    return scratch(a.x, need);
+}
+
+Scanned gated_scan(const GatedArgs& a) {
+    const c10::DeviceGuard guard(a.x.device());
+    const int64_t B = a.x.size(0), T = a.x.size(1), D = a.x.size(2);
+    const Tensor ws = gated_scratch(a);
+    Scanned r{empty(a.x, a.x.sizes()), empty(a.x, {B, D})};
+    check(lib.snntc_gated_scan_forward(f32(a.x), raw(a.gate), float_type(a.gate), f32(a.state), i64(a.lengths), f32(r.y), f32(r.final), B,
+                                       T, D, ws.data_ptr(), ws.numel(), stream_of(a.x)));
+    return r;
+}
+
+struct ScanGrads { Tensor dx, dgate, dstate; };
+
+ScanGrads gated_scan_grad(const Tensor& dy_in, const Tensor& dfinal_in, const GatedArgs& a, const Tensor& y_in, bool want_dx, bool want_dgate,
+                          bool want_dstate) {
+    const c10::DeviceGuard guard(a.x.device());
+    const int64_t B = a.x.size(0), T = a.x.size(1), D = a.x.size(2);
+    TORCH_CHECK_VALUE(y_in.defined(), "y, the forward output, is required");
+    const Tensor y = f32_like(y_in, a.x, a.x.sizes(), "y"), dy = f32_like(dy_in, a.x, a.x.sizes(), "grad_y"),
+                 dfinal = f32_like(dfinal_in, a.x, {B, D}, "grad_final");
+    const Tensor ws = gated_scratch(a);
+    ScanGrads g;
+    if (want_dx) g.dx = empty(a.x, a.x.sizes());
+    if (want_dgate) g.dgate = empty(a.gate, a.x.sizes());
+    if (want_dstate) g.dstate = empty(a.x, {B, D});
+    check(lib.snntc_gated_scan_backward(f32(dy), f32(dfinal), f32(a.x), raw(a.gate), float_type(a.gate), f32(y), f32(a.state),
+                                        i64(a.lengths), f32(g.dx), raw(g.dgate), f32(g.dstate), B, T, D, ws.data_ptr(), ws.numel(),
+                                        stream_of(a.x)));
+    return g;
+}
+
+Tensor gated_step(const Tensor& x_in, const Tensor& gate_in, const Tensor& state_in, const Tensor& out_in) {
+    const Tensor x = dev_f32(x_in, "x", x_in.dim());
+    TORCH_CHECK_VALUE(gate_in.sizes() == x.sizes(), "gate ", shape_text(gate_in), " does not match x ", shape_text(x));
+    const Tensor gate = dev_float(gate_in, "gate");
+    same_device(gate, x, "gate");
+    const Tensor state = f32_like(state_in, x, x.sizes(), "state");
+    const c10::DeviceGuard guard(x.device());
+    Tensor out = f32_like(out_in, x, x.sizes(), "out");
+    if (!out.defined()) out = empty(x, x.sizes());
+    else TORCH_CHECK_VALUE(out.is_same(out_in), "out must be contiguous");
+    check(lib.snntc_gated_step(f32(x), raw(gate), float_type(gate), f32(state), f32(out), x.numel(), stream_of(x)));
+    if (out_in.defined()) written_behind_autograd(out);
+    return out;
+}
+
+// times[..., J] with one token per row.
+struct ChoiceArgs { Tensor times, tokens, weight; int64_t rows = 0, J = 0; };
+
+ChoiceArgs choice_args(const Tensor& times, const Tensor& tokens, const Tensor& weight, const char* name) {
+    ChoiceArgs a;
+    a.times = dev_float(times, "times");
+    TORCH_CHECK_VALUE(times.dim() >= 2, "times must have at least 2 dimensions, got shape ", shape_text(times));
+    const at::IntArrayRef rows = times.sizes().slice(0, times.dim() - 1);
+    a.tokens = index_like(tokens, a.times, name, false);
+    TORCH_CHECK_VALUE(tokens.sizes() == rows, name, " must have shape ", rows, ", got ", shape_text(tokens));
+    a.weight = f32_like(weight, a.times, rows, "weight");
+    a.rows = tokens.numel();
+    a.J = times.size(-1);
+    return a;
+}
+
+Tensor row_floats(const ChoiceArgs& a, at::IntArrayRef sizes) { return at::empty(sizes, a.times.options().dtype(at::kFloat)); }
+
+Tensor choice_scratch(const ChoiceArgs& a) {
+    size_t need = 0;
+    check(lib.snntc_choice_workspace_bytes(a.rows, a.J, &need));
+    return scratch(a.times, need);
+}
+
+Tensor time_logp(const ChoiceArgs& a) {
+    const c10::DeviceGuard guard(a.times.device());
+    const Tensor ws = choice_scratch(a), logp = row_floats(a, a.tokens.sizes());
+    check(lib.snntc_time_logp(raw(a.times), float_type(a.times), i64(a.tokens), f32(a.weight), f32(logp), nullptr, a.rows, a.J,
+                              ws.data_ptr(), ws.numel(), stream_of(a.times)));
+    return logp;
+}
+
+// Loss per row or pair, log-probabilities and, as asked for, the gradient of the objective or what its backward pass needs.
+struct ChoiceOut { Tensor loss, logp, dtimes, stats, coef; };
+
+struct PolicyIn { Tensor old_logp, advantage, ref_logp; float low, high, kl; };
+
+ChoiceOut policy_loss(const ChoiceArgs& a, const PolicyIn& p, bool want_grad, bool save) {
+    const c10::DeviceGuard guard(a.times.device());
+    const at::IntArrayRef rows = a.tokens.sizes();
+    TORCH_CHECK_VALUE(p.old_logp.defined() && p.advantage.defined(), "old_logp and advantage are required");
+    const Tensor old_logp = f32_like(p.old_logp, a.times, rows, "old_logp"), advantage = f32_like(p.advantage, a.times, rows, "advantage"),
+                 ref = f32_like(p.ref_logp, a.times, rows, "ref_logp");
+    const Tensor ws = choice_scratch(a);
+    ChoiceOut r{row_floats(a, rows), row_floats(a, rows), Tensor(), Tensor(), Tensor()};
+    if (want_grad) r.dtimes = empty(a.times, a.times.sizes());
+    if (save) { r.stats = row_floats(a, {a.rows, 2}); r.coef = row_floats(a, {a.rows}); }
+    check(lib.snntc_policy_loss(raw(a.times), float_type(a.times), i64(a.tokens), f32(old_logp), f32(advantage), f32(ref), f32(a.weight),
+                                p.low, p.high, p.kl, f32(r.loss), f32(r.logp), f32(r.stats), f32(r.coef), raw(r.dtimes), a.rows, a.J,
+                                ws.data_ptr(), ws.numel(), stream_of(a.times)));
+    return r;
+}
+
+ChoiceOut preference_loss(const ChoiceArgs& a, const Tensor& ref_in, float beta, float smoothing, bool want_grad, bool save) {
+    const c10::DeviceGuard guard(a.times.device());
+    TORCH_CHECK_VALUE(a.tokens.dim() == 2 && a.tokens.size(0) % 2 == 0, "tokens must be [2 pairs, steps], got shape ", shape_text(a.tokens));
+    TORCH_CHECK_VALUE(ref_in.defined(), "ref_logp is required");
+    const int64_t P = a.tokens.size(0) / 2, T = a.tokens.size(1);
+    const Tensor ref = f32_like(ref_in, a.times, {2 * P}, "ref_logp"), ws = choice_scratch(a);
+    ChoiceOut r{row_floats(a, {P}), row_floats(a, {2 * P}), Tensor(), Tensor(), Tensor()};
+    if (want_grad) r.dtimes = empty(a.times, a.times.sizes());
+    if (save) { r.stats = row_floats(a, {a.rows, 2}); r.coef = row_floats(a, {a.rows}); }
+    check(lib.snntc_preference_loss(raw(a.times), float_type(a.times), i64(a.tokens), f32(ref), f32(a.weight), beta, smoothing, f32(r.loss),
+                                    f32(r.logp), f32(r.stats), f32(r.coef), raw(r.dtimes), P, T, a.J, ws.data_ptr(), ws.numel(),
+                                    stream_of(a.times)));
+    return r;
+}
+
+Tensor loss_total(const Tensor& loss, const Tensor& weight) {
+    const Tensor total = empty(loss, {});
+    check(lib.snntc_loss_total(f32(loss), f32(weight), f32(total), loss.numel(), stream_of(loss)));
+    return total;
 }
 
 // ---- autograd nodes ------------------------------------------------------------------------------------------------
@@ -530,6 +758,141 @@ void sgd_update(const std::vector<Tensor>& ws, const std::vector<Tensor>& gs, fl
     }
     const c10::DeviceGuard guard(ws[0].device());
     check(lib.snntc_sgd_update(wp.data(), gp.data(), n.data(), (int64_t)n.size(), lr, stream_of(ws[0])));
+}
+
+// ---- layers and losses over sequences ---------------------------------------------------------------------------------
+
+struct EmbedNode : public Node {
+    SavedVariable tokens, table;
+    float scale;
+    bool encode;
+    std::string name() const override { return "SnnEmbedBackward"; }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        tokens.reset_data(); table.reset_data();
+    }
+    variable_list apply(variable_list&& grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        if (!grads[0].defined() || !task_should_compute_output(0)) return variable_list(1);
+        const Tensor tok = tokens.unpack(), tab = table.unpack();
+        at::AutoGradMode no_grad(false);
+        return {embed_tokens_grad(grads[0], embed_args(tok, tab, scale, encode))};
+    }
+};
+
+Tensor embed_layer(const Tensor& tokens, const Tensor& table, float scale, bool encode) {
+    const EmbedArgs a = embed_args(tokens, table, scale, encode);
+    Tensor z;
+    {
+        at::AutoGradMode no_grad(false);
+        z = embed_tokens(a);
+    }
+    if (!wants_grad(a.table)) return z;
+    auto node = make_node<EmbedNode>({a.table});
+    node->scale = scale; node->encode = encode;
+    node->tokens = SavedVariable(a.tokens, false); node->table = SavedVariable(a.table, false);
+    return with_history(z, node);
+}
+
+struct GatedNode : public Node {
+    SavedVariable x, gate, state, lengths, y;
+    bool has_state, has_lengths;
+    std::string name() const override { return "SnnGatedScanBackward"; }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        x.reset_data(); gate.reset_data(); state.reset_data(); lengths.reset_data(); y.reset_data();
+    }
+    variable_list apply(variable_list&& grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        variable_list out(3);
+        if (!grads[0].defined() && !grads[1].defined()) return out;
+        const Tensor X = x.unpack(), G = gate.unpack(), S = has_state ? state.unpack() : Tensor(),
+                     L = has_lengths ? lengths.unpack() : Tensor(), Y = y.unpack();
+        at::AutoGradMode no_grad(false);
+        ScanGrads g = gated_scan_grad(grads[0], grads[1], GatedArgs{X, G, S, L}, Y, task_should_compute_output(0),
+                                      task_should_compute_output(1), has_state && task_should_compute_output(2));
+        out[0] = g.dx; out[1] = g.dgate; out[2] = g.dstate;
+        return out;
+    }
+};
+
+Scanned gated_layer(const Tensor& x, const Tensor& gate, const Tensor& state, const Tensor& lengths) {
+    const GatedArgs a = gated_args(x, gate, state, lengths);
+    Scanned r;
+    {
+        at::AutoGradMode no_grad(false);
+        r = gated_scan(a);
+    }
+    if (!wants_grad(a.x, a.gate) && !(a.state.defined() && wants_grad(a.state))) return r;
+    std::shared_ptr<GatedNode> node(new GatedNode(), torch::autograd::deleteNode);
+    torch::autograd::edge_list edges{torch::autograd::impl::gradient_edge(a.x), torch::autograd::impl::gradient_edge(a.gate),
+                                     a.state.defined() ? torch::autograd::impl::gradient_edge(a.state) : torch::autograd::Edge()};
+    node->set_next_edges(std::move(edges));
+    node->has_state = a.state.defined(); node->has_lengths = a.lengths.defined();
+    node->x = SavedVariable(a.x, false); node->gate = SavedVariable(a.gate, false);
+    if (node->has_state) node->state = SavedVariable(a.state, false);
+    if (node->has_lengths) node->lengths = SavedVariable(a.lengths, false);
+    node->y = SavedVariable(r.y.detach(), false);            // a detached alias, or the output would keep itself alive
+    torch::autograd::set_history(r.y, node);
+    torch::autograd::set_history(r.final, node);
+    return r;
+}
+
+// The objective of a loss over choices: its gradient by the times is made in the backward pass, from the row statistics and the
+// derivative by each row's log-probability that the forward pass has left.
+struct ChoiceNode : public Node {
+    SavedVariable times, tokens, stats, coef;
+    std::string name() const override { return "ChoiceLossBackward"; }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        times.reset_data(); tokens.reset_data(); stats.reset_data(); coef.reset_data();
+    }
+    variable_list apply(variable_list&& grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        if (!grads[0].defined() || !task_should_compute_output(0)) return variable_list(1);
+        const Tensor t = times.unpack(), k = tokens.unpack(), s = stats.unpack(), c = coef.unpack();
+        at::AutoGradMode no_grad(false);
+        const c10::DeviceGuard guard(t.device());
+        const Tensor up = grads[0].contiguous(), d = empty(t, t.sizes());
+        check(lib.snntc_time_logp_backward(raw(t), float_type(t), i64(k), f32(s), f32(c), f32(up), raw(d), k.numel(), t.size(-1),
+                                           stream_of(t)));
+        return {d};
+    }
+};
+
+Tensor choice_history(const Tensor& total, const ChoiceArgs& a, const ChoiceOut& r) {
+    auto node = make_node<ChoiceNode>({a.times});
+    node->times = SavedVariable(a.times, false); node->tokens = SavedVariable(a.tokens, false);
+    node->stats = SavedVariable(r.stats, false); node->coef = SavedVariable(r.coef, false);
+    return with_history(total, node);
+}
+
+Tensor policy_layer(const ChoiceArgs& a, const PolicyIn& p) {
+    no_gradient({{&p.old_logp, "old_logp"}, {&p.advantage, "advantage"}, {&p.ref_logp, "ref_logp"}, {&a.weight, "weight"}}, "policy loss");
+    const bool grad = wants_grad(a.times);
+    ChoiceOut r;
+    Tensor total;
+    {
+        at::AutoGradMode no_grad(false);
+        r = policy_loss(a, p, false, grad);
+        const c10::DeviceGuard guard(a.times.device());
+        total = loss_total(r.loss, a.weight);
+    }
+    return grad ? choice_history(total, a, r) : total;
+}
+
+Tensor preference_layer(const ChoiceArgs& a, const Tensor& ref, float beta, float smoothing) {
+    no_gradient({{&ref, "ref_logp"}, {&a.weight, "weight"}}, "preference loss");
+    const bool grad = wants_grad(a.times);
+    ChoiceOut r;
+    Tensor total;
+    {
+        at::AutoGradMode no_grad(false);
+        r = preference_loss(a, ref, beta, smoothing, false, grad);
+        const c10::DeviceGuard guard(a.times.device());
+        total = loss_total(r.loss, Tensor());
+    }
+    return grad ? choice_history(total, a, r) : total;
 }
 
 // ---- the example training recipe -------------------------------------------------------------------------------------
@@ -1071,6 +1434,228 @@ SNNTC_METHOD(py_recipe_step) {
     END_HANDLE_TH_ERRORS
 }
 
+// embed_tokens(tokens, table, scale, encode) -> z[..., D]
+SNNTC_METHOD(py_embed_tokens) {
+    HANDLE_TH_ERRORS
+    arity(n, 4, "embed_tokens");
+    const Tensor tok = tensor_arg(a[0], "tokens"), tab = tensor_arg(a[1], "table");
+    const float scale = float_arg(a[2]);
+    const bool encode = bool_arg(a[3]);
+    Tensor z;
+    {
+        NoGil nogil;
+        at::AutoGradMode no_grad(false);
+        z = embed_tokens(embed_args(tok, tab, scale, encode));
+    }
+    return wrap(z);
+    END_HANDLE_TH_ERRORS
+}
+
+// embed_tokens_grad(grad, tokens, table, scale, encode) -> gradient of the table
+SNNTC_METHOD(py_embed_tokens_grad) {
+    HANDLE_TH_ERRORS
+    arity(n, 5, "embed_tokens_grad");
+    const Tensor g = tensor_arg(a[0], "grad"), tok = tensor_arg(a[1], "tokens"), tab = tensor_arg(a[2], "table");
+    const float scale = float_arg(a[3]);
+    const bool encode = bool_arg(a[4]);
+    Tensor d;
+    {
+        NoGil nogil;
+        at::AutoGradMode no_grad(false);
+        d = embed_tokens_grad(g, embed_args(tok, tab, scale, encode));
+    }
+    return wrap(d);
+    END_HANDLE_TH_ERRORS
+}
+
+// embed_layer(tokens, table, scale, encode) -> z, differentiable in the table
+SNNTC_METHOD(py_embed_layer) {
+    HANDLE_TH_ERRORS
+    arity(n, 4, "embed_layer");
+    const Tensor tok = tensor_arg(a[0], "tokens"), tab = tensor_arg(a[1], "table");
+    if (!plain({tok, tab})) return general("embed_layer", a, n);
+    const float scale = float_arg(a[2]);
+    const bool encode = bool_arg(a[3]);
+    Tensor z;
+    {
+        NoGil nogil;
+        z = embed_layer(tok, tab, scale, encode);
+    }
+    return wrap(z);
+    END_HANDLE_TH_ERRORS
+}
+
+// gated_scan(x, gate, state, lengths) -> (y, final)
+SNNTC_METHOD(py_gated_scan) {
+    HANDLE_TH_ERRORS
+    arity(n, 4, "gated_scan");
+    const Tensor x = tensor_arg(a[0], "x"), g = tensor_arg(a[1], "gate"), s = optional_tensor(a[2], "state"),
+                 l = optional_tensor(a[3], "lengths");
+    Scanned r;
+    {
+        NoGil nogil;
+        at::AutoGradMode no_grad(false);
+        r = gated_scan(gated_args(x, g, s, l));
+    }
+    return wrap2(r.y, r.final);
+    END_HANDLE_TH_ERRORS
+}
+
+// gated_scan_grad(grad_y, grad_final, x, gate, y, state, lengths, want_dx, want_dgate, want_dstate) -> (dx, dgate, dstate)
+SNNTC_METHOD(py_gated_scan_grad) {
+    HANDLE_TH_ERRORS
+    arity(n, 10, "gated_scan_grad");
+    const Tensor dy = optional_tensor(a[0], "grad_y"), df = optional_tensor(a[1], "grad_final"), x = tensor_arg(a[2], "x"),
+                 g = tensor_arg(a[3], "gate"), y = tensor_arg(a[4], "y"), s = optional_tensor(a[5], "state"),
+                 l = optional_tensor(a[6], "lengths");
+    const bool want_dx = bool_arg(a[7]), want_dgate = bool_arg(a[8]), want_dstate = bool_arg(a[9]);
+    ScanGrads r;
+    {
+        NoGil nogil;
+        at::AutoGradMode no_grad(false);
+        r = gated_scan_grad(dy, df, gated_args(x, g, s, l), y, want_dx, want_dgate, want_dstate);
+    }
+    return wrap3(r.dx, r.dgate, r.dstate);
+    END_HANDLE_TH_ERRORS
+}
+
+// gated_layer(x, gate, state, lengths) -> (y, final), differentiable in x, gate and state
+SNNTC_METHOD(py_gated_layer) {
+    HANDLE_TH_ERRORS
+    arity(n, 4, "gated_layer");
+    const Tensor x = tensor_arg(a[0], "x"), g = tensor_arg(a[1], "gate"), s = optional_tensor(a[2], "state"),
+                 l = optional_tensor(a[3], "lengths");
+    if (!plain({x, g, s, l})) return general("gated_layer", a, n);
+    Scanned r;
+    {
+        NoGil nogil;
+        r = gated_layer(x, g, s, l);
+    }
+    return wrap2(r.y, r.final);
+    END_HANDLE_TH_ERRORS
+}
+
+// gated_step(x, gate, state, out) -> the new state
+SNNTC_METHOD(py_gated_step) {
+    HANDLE_TH_ERRORS
+    arity(n, 4, "gated_step");
+    const Tensor x = tensor_arg(a[0], "x"), g = tensor_arg(a[1], "gate"), s = optional_tensor(a[2], "state"),
+                 o = optional_tensor(a[3], "out");
+    Tensor out;
+    {
+        NoGil nogil;
+        at::AutoGradMode no_grad(false);
+        out = gated_step(x, g, s, o);
+    }
+    return wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// time_logp(times, tokens, weight) -> logp
+SNNTC_METHOD(py_time_logp) {
+    HANDLE_TH_ERRORS
+    arity(n, 3, "time_logp");
+    const Tensor t = tensor_arg(a[0], "times"), k = tensor_arg(a[1], "tokens"), w = optional_tensor(a[2], "weight");
+    Tensor logp;
+    {
+        NoGil nogil;
+        at::AutoGradMode no_grad(false);
+        logp = time_logp(choice_args(t, k, w, "tokens"));
+    }
+    return wrap(logp);
+    END_HANDLE_TH_ERRORS
+}
+
+PolicyIn policy_in(PyObject* const* a) {
+    return PolicyIn{tensor_arg(a[0], "old_logp"), tensor_arg(a[1], "advantage"), optional_tensor(a[2], "ref_logp"), float_arg(a[4]),
+                    float_arg(a[5]), float_arg(a[6])};
+}
+
+// policy_loss(times, actions, old_logp, advantage, ref_logp, weight, clip_low, clip_high, kl_coef, want_grad) -> (row_loss, logp, dtimes)
+SNNTC_METHOD(py_policy_loss) {
+    HANDLE_TH_ERRORS
+    arity(n, 10, "policy_loss");
+    const Tensor t = tensor_arg(a[0], "times"), k = tensor_arg(a[1], "actions"), w = optional_tensor(a[5], "weight");
+    const PolicyIn p = policy_in(a + 2);
+    const bool want_grad = bool_arg(a[9]);
+    ChoiceOut r;
+    {
+        NoGil nogil;
+        at::AutoGradMode no_grad(false);
+        r = policy_loss(choice_args(t, k, w, "actions"), p, want_grad, false);
+    }
+    return wrap3(r.loss, r.logp, r.dtimes);
+    END_HANDLE_TH_ERRORS
+}
+
+// policy_layer(times, actions, old_logp, advantage, ref_logp, weight, clip_low, clip_high, kl_coef) -> objective, differentiable
+SNNTC_METHOD(py_policy_layer) {
+    HANDLE_TH_ERRORS
+    arity(n, 9, "policy_layer");
+    const Tensor t = tensor_arg(a[0], "times"), k = tensor_arg(a[1], "actions"), w = optional_tensor(a[5], "weight");
+    const PolicyIn p = policy_in(a + 2);
+    if (!plain({t, k, w, p.old_logp, p.advantage, p.ref_logp})) return general("policy_layer", a, n);
+    Tensor total;
+    {
+        NoGil nogil;
+        total = policy_layer(choice_args(t, k, w, "actions"), p);
+    }
+    return wrap(total);
+    END_HANDLE_TH_ERRORS
+}
+
+// preference_loss(times, tokens, ref_logp, weight, beta, smoothing, want_grad) -> (pair_loss, seq_logp, dtimes)
+SNNTC_METHOD(py_preference_loss) {
+    HANDLE_TH_ERRORS
+    arity(n, 7, "preference_loss");
+    const Tensor t = tensor_arg(a[0], "times"), k = tensor_arg(a[1], "tokens"), ref = tensor_arg(a[2], "ref_logp"),
+                 w = optional_tensor(a[3], "weight");
+    const float beta = float_arg(a[4]), smoothing = float_arg(a[5]);
+    const bool want_grad = bool_arg(a[6]);
+    ChoiceOut r;
+    {
+        NoGil nogil;
+        at::AutoGradMode no_grad(false);
+        r = preference_loss(choice_args(t, k, w, "tokens"), ref, beta, smoothing, want_grad, false);
+    }
+    return wrap3(r.loss, r.logp, r.dtimes);
+    END_HANDLE_TH_ERRORS
+}
+
+// preference_layer(times, tokens, ref_logp, weight, beta, smoothing) -> objective, differentiable
+SNNTC_METHOD(py_preference_layer) {
+    HANDLE_TH_ERRORS
+    arity(n, 6, "preference_layer");
+    const Tensor t = tensor_arg(a[0], "times"), k = tensor_arg(a[1], "tokens"), ref = tensor_arg(a[2], "ref_logp"),
+                 w = optional_tensor(a[3], "weight");
+    const float beta = float_arg(a[4]), smoothing = float_arg(a[5]);
+    if (!plain({t, k, ref, w})) return general("preference_layer", a, n);
+    Tensor total;
+    {
+        NoGil nogil;
+        total = preference_layer(choice_args(t, k, w, "tokens"), ref, beta, smoothing);
+    }
+    return wrap(total);
+    END_HANDLE_TH_ERRORS
+}
+
+// loss_total(loss, weight) -> sum of weight loss, or the mean
+SNNTC_METHOD(py_loss_total) {
+    HANDLE_TH_ERRORS
+    arity(n, 2, "loss_total");
+    const Tensor l = tensor_arg(a[0], "loss"), w = optional_tensor(a[1], "weight");
+    Tensor total;
+    {
+        NoGil nogil;
+        at::AutoGradMode no_grad(false);
+        const Tensor lc = dev_f32(l, "loss", l.dim());
+        const c10::DeviceGuard guard(lc.device());
+        total = loss_total(lc, f32_like(w, lc, lc.sizes(), "weight"));
+    }
+    return wrap(total);
+    END_HANDLE_TH_ERRORS
+}
+
 // bind(path, SnntcLibraryError, SnntcError, params_array, general paths): looks the C ABI up in the library loaded from `path`
 SNNTC_METHOD(py_bind) {
     HANDLE_TH_ERRORS
@@ -1099,7 +1684,11 @@ PyMethodDef g_methods[] = {SNNTC_ENTRY(bind), SNNTC_ENTRY(fc_forward), SNNTC_ENT
                            SNNTC_ENTRY(cv_forward), SNNTC_ENTRY(cv_layer), SNNTC_ENTRY(cv_same), SNNTC_ENTRY(cv_backward),
                            SNNTC_ENTRY(min_pool), SNNTC_ENTRY(min_pool_layer), SNNTC_ENTRY(pad_layer), SNNTC_ENTRY(time_loss),
                            SNNTC_ENTRY(loss_layer), SNNTC_ENTRY(sgd_update), SNNTC_ENTRY(plain), SNNTC_ENTRY(encode_time),
-                           SNNTC_ENTRY(constraint_cost), SNNTC_ENTRY(recipe_step), {nullptr, nullptr, 0, nullptr}};
+                           SNNTC_ENTRY(constraint_cost), SNNTC_ENTRY(recipe_step), SNNTC_ENTRY(embed_tokens),
+                           SNNTC_ENTRY(embed_tokens_grad), SNNTC_ENTRY(embed_layer), SNNTC_ENTRY(gated_scan),
+                           SNNTC_ENTRY(gated_scan_grad), SNNTC_ENTRY(gated_layer), SNNTC_ENTRY(gated_step), SNNTC_ENTRY(time_logp),
+                           SNNTC_ENTRY(policy_loss), SNNTC_ENTRY(policy_layer), SNNTC_ENTRY(preference_loss),
+                           SNNTC_ENTRY(preference_layer), SNNTC_ENTRY(loss_total), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_binding", "Native host path of the SNN-TC ops.", -1, g_methods,
                         nullptr, nullptr, nullptr, nullptr};

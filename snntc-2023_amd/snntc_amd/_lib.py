@@ -38,6 +38,10 @@ EXPORTS = (
     "snntc_pad_time_forward", "snntc_pad_time_backward",
     "snntc_encode_time", "snntc_label_loss", "snntc_weight_cost_workspace_bytes", "snntc_weight_cost_sums",
     "snntc_weight_cost_grad", "snntc_recipe_total",
+    "snntc_embed_forward", "snntc_embed_backward_workspace_bytes", "snntc_embed_backward",
+    "snntc_gated_scan_workspace_bytes", "snntc_gated_scan_forward", "snntc_gated_scan_backward", "snntc_gated_step",
+    "snntc_choice_workspace_bytes", "snntc_time_logp", "snntc_time_logp_backward", "snntc_policy_loss",
+    "snntc_preference_loss", "snntc_loss_total",
     "snntc_scan_status", "snntc_debug_set_scan_wait_polls", "snntc_debug_order_tile",
     "snntc_profile_enable", "snntc_profile_collect", "snntc_profile_entry",
 )
@@ -129,6 +133,20 @@ def load():
     lib.snntc_weight_cost_grad.argtypes = [c.POINTER(vp), c.POINTER(vp), pi64, pi64, i64, c.c_float, c.c_float, vp, c.c_int,
                                            vp, sz, vp]
     lib.snntc_recipe_total.argtypes = [pi64, pi64, i64, c.c_float, c.c_float, vp, vp, i64, vp, vp, vp, sz, vp]
+    i32, f32, psz = c.c_int, c.c_float, c.POINTER(sz)
+    lib.snntc_embed_forward.argtypes = [vp, i32, vp, i32, vp, i64, i64, i64, f32, i32, vp]
+    lib.snntc_embed_backward_workspace_bytes.argtypes = [i64, i64, i64, psz]
+    lib.snntc_embed_backward.argtypes = [vp, vp, i32, vp, i32, vp, i64, i64, i64, f32, i32, vp, sz, vp]
+    lib.snntc_gated_scan_workspace_bytes.argtypes = [i64, i64, i64, psz]
+    lib.snntc_gated_scan_forward.argtypes = [vp, vp, i32, vp, vp, vp, vp, i64, i64, i64, vp, sz, vp]
+    lib.snntc_gated_scan_backward.argtypes = [vp, vp, vp, vp, i32, vp, vp, vp, vp, vp, vp, i64, i64, i64, vp, sz, vp]
+    lib.snntc_gated_step.argtypes = [vp, vp, i32, vp, vp, i64, vp]
+    lib.snntc_choice_workspace_bytes.argtypes = [i64, i64, psz]
+    lib.snntc_time_logp.argtypes = [vp, i32, vp, vp, vp, vp, i64, i64, vp, sz, vp]
+    lib.snntc_time_logp_backward.argtypes = [vp, i32, vp, vp, vp, vp, vp, i64, i64, vp]
+    lib.snntc_policy_loss.argtypes = [vp, i32, vp, vp, vp, vp, vp, f32, f32, f32, vp, vp, vp, vp, vp, i64, i64, vp, sz, vp]
+    lib.snntc_preference_loss.argtypes = [vp, i32, vp, vp, vp, f32, f32, vp, vp, vp, vp, vp, i64, i64, i64, vp, sz, vp]
+    lib.snntc_loss_total.argtypes = [vp, vp, vp, i64, vp]
     lib.snntc_scan_status.argtypes = [c.POINTER(i64), vp]
     lib.snntc_debug_set_scan_wait_polls.argtypes = [c.c_int]
     lib.snntc_debug_order_tile.argtypes = [i64, i64, i64, i64, fparams, c.c_int, c.POINTER(i64)]

@@ -16,7 +16,8 @@ import torch
 import torch.nn.functional as F
 
 from ._lib import SnntcLibraryError, native
-from .ops import SnnCvSame, SnnCvTimes, SnnMinPool, SnnPadTime, SoftmaxTimeLoss
+from .ops import (PolicyTimeLoss, PreferenceTimeLoss, SnnCvSame, SnnCvTimes, SnnEmbed, SnnGatedScan, SnnMinPool, SnnPadTime,
+                  SoftmaxTimeLoss, gated_step)
 
 # Mirrors the reference's module-level switch (SNN_TC_Modules.py:11): when True the layers keep
 # the largest batch and element count they have seen in ``maxD`` (every tensor must stay below
@@ -308,6 +309,69 @@ class SNN_flatten(torch.nn.Module):
         return input.reshape(input.shape[0], -1)
 
 
+class SNN_embedding(torch.nn.Module):
+    """Tokens to spike times: tokens[...] (int64 or int32) -> times[..., dim], exp(1 - scale * weight[token]) (or
+    scale * weight[token] with encode=False); weight[num_tokens, dim], by default intensities in [0, 1) as pixels have."""
+
+    def __init__(self, num_tokens, dim, scale=1.0, encode=True, weight=None, name=None):
+        super().__init__()
+        self.num_tokens, self.dim, self.scale, self.encode = num_tokens, dim, float(scale), bool(encode)
+        self.name = name
+        weight = np.random.rand(num_tokens, dim) if weight is None else np.array(weight)
+        if tuple(weight.shape) != (num_tokens, dim):
+            raise ValueError(f"weight shape {tuple(weight.shape)} != {(num_tokens, dim)}")
+        self.weight = torch.nn.Parameter(torch.from_numpy(weight.astype(np.float32)))
+
+    def forward(self, tokens):
+        return SnnEmbed.apply(tokens, self.weight, self.scale, self.encode)
+
+
+class SNN_recurrence(torch.nn.Module):
+    """Gated running mean of spike times along a sequence, x[B,T,dim] -> y[B,T,dim]: the gates are a linear map of each
+    step's own times, gate = x @ weight[:-1] + weight[-1] (weight[dim + 1, dim], the last row a bias, by default 2: a mean
+    over some eight steps).  `step` is the same layer on rows that are served token by token."""
+
+    def __init__(self, dim, weight=None, name=None):
+        super().__init__()
+        self.dim = dim
+        self.name = name
+        if weight is None:
+            weight = np.concatenate((np.random.randn(dim, dim) * (0.5 / dim), np.full([1, dim], 2.0)), axis=0)
+        else:
+            weight = np.array(weight)
+        if tuple(weight.shape) != (dim + 1, dim):
+            raise ValueError(f"weight shape {tuple(weight.shape)} != {(dim + 1, dim)}")
+        self.weight = torch.nn.Parameter(torch.from_numpy(weight.astype(np.float32)))
+
+    def gates(self, x):
+        """[..., dim] -> [..., dim]"""
+        rows = x.reshape(-1, self.dim)
+        return torch.addmm(self.weight[-1], rows, self.weight[:-1]).view(x.shape)
+
+    def forward(self, x, state=None, lengths=None, return_state=False):
+        _require_device(x, "input")
+        if x.dim() != 3 or x.shape[2] != self.dim:
+            raise ValueError(f"input must be [B,T,{self.dim}], got shape {tuple(x.shape)}")
+        y, final = SnnGatedScan.apply(x, self.gates(x), state, lengths)
+        return (y, final) if return_state else y
+
+    @torch.no_grad()
+    def step(self, x, state=None, out=None):
+        """x[B,dim], one token's times of every row, and the rows' state[B,dim] -> the new state, which is the step's
+        output (written into `out` if given, which may be `state`)."""
+        _require_device(x, "input")
+        if x.dim() != 2 or x.shape[1] != self.dim:
+            raise ValueError(f"input must be [B,{self.dim}], got shape {tuple(x.shape)}")
+        return gated_step(x, self.gates(x), state, out)
+
+
+class SNN_steps(torch.nn.Module):
+    """[B,T,D] -> [B*T,D]: every step of every sequence a row for the dense layers that follow."""
+
+    def forward(self, input):
+        return input.reshape(-1, input.shape[-1])
+
+
 class SNN_avgpool2d(_Pool2d):
     """Average pooling after padding with 1e5 (SNN_TC_Modules.py:251-281)."""
 
@@ -327,3 +391,15 @@ def loss_func(logit=None, label=None):
     if label.requires_grad:
         raise ValueError("label must not require a gradient: the loss kernel differentiates the spike times only")
     return SoftmaxTimeLoss.apply(logit, label)               # one fused kernel for loss and gradient
+
+
+def policy_loss(times, actions, old_logp, advantage, ref_logp=None, weight=None, clip=(0.2, 0.2), kl_coef=0.0):
+    """Clipped policy loss with a KL term over softmax(-times), the mean of the rows or their weighted sum, differentiable
+    in times (see ops.policy_time_loss for the formula)."""
+    return PolicyTimeLoss.apply(times, actions, old_logp, advantage, ref_logp, weight, clip, kl_coef)
+
+
+def preference_loss(times, tokens, ref_logp, weight=None, beta=0.1, smoothing=0.0):
+    """Mean loss of pairs of preferred and rejected sequences over softmax(-times), differentiable in times (see
+    ops.preference_time_loss for the formula)."""
+    return PreferenceTimeLoss.apply(times, tokens, ref_logp, weight, beta, smoothing)

@@ -8,6 +8,9 @@ A network is described by a list of tuples
     ("gmin",)                                 SNN_globalminpool2d
     ("flatten",)                              SNN_flatten
     ("dense", n_in, n_out)                    SNN_dense, bias input
+    ("embed", tokens, dim)                    SNN_embedding: tokens to spike times
+    ("recur", dim)                            SNN_recurrence: gated running mean along a sequence
+    ("steps",)                                SNN_steps: every step of a sequence a row
 
 in the style of the reference's example models (snntc-mnist.py:36-53, snntc-cifar10.py:73-106,
 snntc-imagenet-example/snntc-imagenet.py:21-58), which stack these layer types.
@@ -46,20 +49,31 @@ def baseline_weight(rng, fan_in, fan_out, bias=True):
 
 
 def layer_weight_shapes(spec):
-    """[(fan_in, fan_out)] of the weighted layers of `spec`, in order."""
+    """[(fan_in, fan_out)] of the weighted layers of `spec`, in order (an embedding's: its table)."""
     out = []
     for item in spec:
         if item[0] == "conv":
             _, ci, co, k, _s = item
             out.append((k * k * ci, co))
-        elif item[0] == "dense":
+        elif item[0] in ("dense", "embed"):
             out.append((item[1], item[2]))
+        elif item[0] == "recur":
+            out.append((item[1], item[1]))
     return out
 
 
 def draw_weights(spec, rng):
-    """One baseline_weight draw per weighted layer of `spec` (with bias rows)."""
-    return [baseline_weight(rng, fi, fo) for fi, fo in layer_weight_shapes(spec)]
+    """One draw per weighted layer of `spec`: baseline_weight (with bias rows) for the spiking layers, intensities in [0, 1) for
+    an embedding, small gate weights with a bias of 2 for a recurrence."""
+    out = []
+    for item, (fi, fo) in zip([i for i in spec if i[0] in ("conv", "dense", "embed", "recur")], layer_weight_shapes(spec)):
+        if item[0] == "embed":
+            out.append(rng.random((fi, fo)).astype(np.float32))
+        elif item[0] == "recur":
+            out.append(np.concatenate((rng.standard_normal((fi, fo)) * (0.5 / fi), np.full((1, fo), 2.0))).astype(np.float32))
+        else:
+            out.append(baseline_weight(rng, fi, fo))
+    return out
 
 
 class SnnSequential(torch.nn.Sequential):
@@ -120,6 +134,12 @@ def build(spec, weights=None, rng=None, chain=False):
             mods.append(L.SNN_globalminpool2d())
         elif kind == "flatten":
             mods.append(L.SNN_flatten())
+        elif kind == "embed":
+            mods.append(L.SNN_embedding(item[1], item[2], weight=weights.pop(0)))
+        elif kind == "recur":
+            mods.append(L.SNN_recurrence(item[1], weight=weights.pop(0)))
+        elif kind == "steps":
+            mods.append(L.SNN_steps())
         else:
             raise ValueError(f"unknown layer kind {kind!r}")
     if weights:

@@ -1,4 +1,4 @@
-"""The four SNN-TC ops over PyTorch-ROCm tensors, each a thin call into the C ABI.
+"""The four SNN-TC ops, and those around them, over PyTorch-ROCm tensors, each a thin call into the C ABI.
 
 Counterparts of the reference's op handles (SNN_TC_Modules.py:29-33, 89-93):
 
@@ -7,8 +7,11 @@ Counterparts of the reference's op handles (SNN_TC_Modules.py:29-33, 89-93):
     snncv(Xpad, W, Params)                   -> Y[2B, Nh, Nw, Kc]
     snncv_grad(grad, Xpad, W, Params, Y)     -> (dXpad, dW, dParams)
 
+Around them: loss, pooling, padding and update of an image network; for networks over sequences of tokens embed_tokens,
+gated_scan / gated_step, policy_time_loss and preference_time_loss.
+
 ``SnnFc`` / ``SnnCv`` are the differentiable ops that replace ``@ops.RegisterGradient``.
-Tensors must be float32 on a ROCm device; ``Params`` is the host-side float32 vector the layers
+Tensors must be float32 on a ROCm device (tables, gates and the last two losses' times may be 16-bit floats); ``Params`` is the host-side float32 vector the layers
 build.  PyTorch supplies device memory, the current HIP stream and the autograd engine; the host side
 of a call (checks, allocation, launches, graph nodes) is csrc/binding.cpp.  The differentiable ops are
 ``torch.autograd.Function`` classes whose ``apply`` is that native path; it hands a call with forward-mode
@@ -426,6 +429,147 @@ class SnnPadTime(torch.autograd.Function):
         return pad_time_grad(dxpad, *ctx.geom), None, None, None, None, None
 
 
+# ---- sequences of tokens and choices ----------------------------------------------------------------------------
+
+
+def embed_tokens(tokens, table, scale=1.0, encode=False):
+    """Rows of table[V,D] as spike times: scale * table[tokens], or exp(1 - scale * table[tokens]) with encode=True,
+    the encoding train.encode_input gives pixels.  tokens: int64 or int32 of any shape; table: float32, bfloat16 or
+    float16; the result is float32 [..., D].  A token outside the table leaves NaN in its row."""
+    return _lib.native().embed_tokens(tokens, table, scale, encode)
+
+
+def embed_tokens_grad(grad, tokens, table, scale=1.0, encode=False):
+    """Gradient of embed_tokens with respect to the table, of its type: every row's grads added up in float32 in the
+    order of their positions (the same sums on every call), rounded once; rows without a token are zero."""
+    return _lib.native().embed_tokens_grad(grad, tokens, table, scale, encode)
+
+
+class SnnEmbed(torch.autograd.Function):
+    """z = embed_tokens(tokens, table, scale, encode), differentiable in the table."""
+
+    @classmethod
+    def apply(cls, tokens, table, scale=1.0, encode=False):
+        return _lib.native().embed_layer(tokens, table, scale, encode)
+
+    @staticmethod
+    def forward(ctx, tokens, table, scale, encode):
+        ctx.save_for_backward(tokens, table)
+        ctx.how = (scale, encode)
+        return embed_tokens(tokens, table, scale, encode)
+
+    @staticmethod
+    def backward(ctx, grad):
+        return None, embed_tokens_grad(grad, *ctx.saved_tensors, *ctx.how), None, None
+
+
+def gated_scan(x, gate, state=None, lengths=None):
+    """Gated running mean of spike times along a sequence: with a = sigmoid(gate),
+    h_t = a_t h_{t-1} + (1 - a_t) x_t per channel of x[B,T,D] -> (y[B,T,D] = all h_t, final[B,D]).
+    gate[B,T,D]: float32, bfloat16 or float16.  state[B,D]: h before the first step (None: zeros).  lengths[B]
+    (int64): steps behind a sequence's length are not read and 0 in y, final is h at the length."""
+    return _lib.native().gated_scan(x, gate, state, lengths)
+
+
+def gated_scan_grad(grad_y, grad_final, x, gate, y, state=None, lengths=None, want_dx=True, want_dgate=True, want_dstate=True):
+    """Gradients of gated_scan, y being its output -> (dx, dgate, dstate).  grad_y or grad_final may be None (zeros).  A
+    want_* flag set to False skips that gradient (None is returned in its place)."""
+    return _lib.native().gated_scan_grad(grad_y, grad_final, x, gate, y, state, lengths, want_dx, want_dgate, want_dstate)
+
+
+def gated_step(x, gate, state=None, out=None):
+    """One step of gated_scan for rows that are served token by token: sigmoid(gate) * state + (1 - sigmoid(gate)) * x,
+    all of x's shape (state=None: zeros).  out may be a preallocated tensor, also state itself.  Not differentiable."""
+    return _lib.native().gated_step(x, gate, state, out)
+
+
+class SnnGatedScan(torch.autograd.Function):
+    """(y, final) = gated_scan(x, gate, state, lengths), differentiable in x, gate and state."""
+
+    @classmethod
+    def apply(cls, x, gate, state=None, lengths=None):
+        return _lib.native().gated_layer(x, gate, state, lengths)
+
+    @staticmethod
+    def forward(ctx, x, gate, state, lengths):
+        y, final = gated_scan(x, gate, state, lengths)
+        ctx.save_for_backward(x, gate, y, state, lengths)
+        return y, final
+
+    @staticmethod
+    def backward(ctx, grad_y, grad_final):
+        want = ctx.needs_input_grad
+        return *gated_scan_grad(grad_y, grad_final, *ctx.saved_tensors, want[0], want[1], want[2]), None
+
+
+def time_logp(times, tokens, weight=None):
+    """log softmax(-times)[token] of every row of times[..., J] (float32, bfloat16 or float16), tokens[...] int64: what
+    the old and reference log-probabilities of the losses below are made by.  Rows of weight 0 (weight[...] float32) are
+    not read and give 0; a token outside the classes gives NaN.  Not differentiable: the losses are."""
+    return _lib.native().time_logp(times, tokens, weight)
+
+
+def policy_time_loss(times, actions, old_logp, advantage, ref_logp=None, weight=None, clip=(0.2, 0.2), kl_coef=0.0,
+                     want_grad=True):
+    """Clipped policy loss over softmax(-times), times[..., J], with an estimate of the divergence from a reference:
+    with ratio = exp(logp - old_logp) and d = ref_logp - logp, row by row
+        kl_coef * (exp(d) - d - 1) - min(ratio * advantage, clip(ratio, 1 - clip[0], 1 + clip[1]) * advantage).
+    The objective is the sum of weight * row loss (weight=None: the mean); rows of weight 0 are not read.
+    Returns (row_loss[...], logp[...], gradient of the objective with respect to times or None)."""
+    return _lib.native().policy_loss(times, actions, old_logp, advantage, ref_logp, weight, clip[0], clip[1], kl_coef, want_grad)
+
+
+def _weighted_total(loss, weight):
+    return _lib.native().loss_total(loss, weight)
+
+
+class PolicyTimeLoss(torch.autograd.Function):
+    """The objective of policy_time_loss, differentiable in times."""
+
+    @classmethod
+    def apply(cls, times, actions, old_logp, advantage, ref_logp=None, weight=None, clip=(0.2, 0.2), kl_coef=0.0):
+        return _lib.native().policy_layer(times, actions, old_logp, advantage, ref_logp, weight, clip[0], clip[1], kl_coef)
+
+    @staticmethod
+    def forward(ctx, times, actions, old_logp, advantage, ref_logp, weight, clip, kl_coef):
+        loss, _, grad = policy_time_loss(times, actions, old_logp, advantage, ref_logp, weight, clip, kl_coef,
+                                         want_grad=times.requires_grad)
+        ctx.save_for_backward(*[] if grad is None else [grad])
+        return _weighted_total(loss, weight)
+
+    @staticmethod
+    def backward(ctx, upstream):
+        return (ctx.saved_tensors[0] * upstream if ctx.saved_tensors else None), None, None, None, None, None, None, None
+
+
+def preference_time_loss(times, tokens, ref_logp, weight=None, beta=0.1, smoothing=0.0, want_grad=True):
+    """Loss of pairs of sequences, the P preferred ones before the P rejected ones: times[2P,T,J], tokens[2P,T], and
+    ref_logp[2P], each sequence's log-probability under a reference.  With S = sum_t weight * logp of a sequence
+    (weight[2P,T], None: all ones) and m = beta * ((S - ref)[preferred] - (S - ref)[rejected]), pair by pair
+        -(1 - smoothing) * log sigmoid(m) - smoothing * log sigmoid(-m).
+    The objective is the mean over the pairs; rows of weight 0 are not read.
+    Returns (pair_loss[P], S[2P], gradient of the objective with respect to times or None)."""
+    return _lib.native().preference_loss(times, tokens, ref_logp, weight, beta, smoothing, want_grad)
+
+
+class PreferenceTimeLoss(torch.autograd.Function):
+    """The objective of preference_time_loss, differentiable in times."""
+
+    @classmethod
+    def apply(cls, times, tokens, ref_logp, weight=None, beta=0.1, smoothing=0.0):
+        return _lib.native().preference_layer(times, tokens, ref_logp, weight, beta, smoothing)
+
+    @staticmethod
+    def forward(ctx, times, tokens, ref_logp, weight, beta, smoothing):
+        loss, _, grad = preference_time_loss(times, tokens, ref_logp, weight, beta, smoothing, want_grad=times.requires_grad)
+        ctx.save_for_backward(*[] if grad is None else [grad])
+        return _weighted_total(loss, None)
+
+    @staticmethod
+    def backward(ctx, upstream):
+        return (ctx.saved_tensors[0] * upstream if ctx.saved_tensors else None), None, None, None, None, None
+
+
 def _function(cls, *args):
     return super(cls, cls).apply(*args)                     # torch.autograd.Function's own
 
@@ -440,4 +584,10 @@ GENERAL = {
         SnnMinPool, x, (kh, kw), (sh, sw), (top, left), (nh, nw), value, next_xpad, (ntop, nleft)),
     "pad_layer": lambda x, top, bottom, left, right, value: _function(SnnPadTime, x, top, bottom, left, right, value),
     "loss_layer": lambda times, label: _function(SoftmaxTimeLoss, times, label),
+    "embed_layer": lambda tokens, table, scale, encode: _function(SnnEmbed, tokens, table, scale, encode),
+    "gated_layer": lambda x, gate, state, lengths: _function(SnnGatedScan, x, gate, state, lengths),
+    "policy_layer": lambda times, actions, old, adv, ref, weight, low, high, kl: _function(
+        PolicyTimeLoss, times, actions, old, adv, ref, weight, (low, high), kl),
+    "preference_layer": lambda times, tokens, ref, weight, beta, smoothing: _function(
+        PreferenceTimeLoss, times, tokens, ref, weight, beta, smoothing),
 }

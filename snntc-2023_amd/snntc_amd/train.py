@@ -1,6 +1,6 @@
 """The training-step glue of the reference's example scripts, for models built from the SNN layers:
 input encoding, the weight-constraint cost, one Adam/SGD step and the evaluation step
-(snntc-mnist.py:55-59, 73-96).  On a ROCm device the encoding, the loss with its count of correct samples
+(snntc-mnist.py:55-59, 73-96), and steps on choices and preferences for networks over tokens.  On a ROCm device the encoding, the loss with its count of correct samples
 and the weight-constraint cost with its gradient are five kernels (csrc/recipe.hip).  Everything else, and
 all of it on other devices and types, with tangents, transforms or tracers at work, or with tensors as cost
 factors, is stock PyTorch around the gfx950 ops.  Weights are saved and restored with ``model.state_dict()``
@@ -9,7 +9,7 @@ factors, is stock PyTorch around the gfx950 ops.  Weights are saved and restored
 import torch
 
 from ._lib import native
-from .layers import loss_func
+from .layers import loss_func, policy_loss, preference_loss
 
 
 def encode_input(images):
@@ -95,3 +95,25 @@ def test_step(model, images, labels, num_classes, weight_k=100.0, weight_k2=1e-2
     onehot = torch.nn.functional.one_hot(labels, num_classes).to(inputs.dtype)
     loss = loss_func(logit=predictions, label=onehot) + constraint_cost(model, weight_k, weight_k2)
     return loss, (predictions_to_classes(predictions) == labels).sum()
+
+
+def policy_step(model, optimizer, inputs, actions, old_logp, advantage, ref_logp=None, weight=None, clip=(0.2, 0.2), kl_coef=0.0):
+    """One optimisation step of a policy on choices it has made: model(inputs) -> spike times with a row per action.  old_logp,
+    ref_logp: ops.time_logp of the model that made the choices and of the reference.  Returns the loss."""
+    optimizer.zero_grad(set_to_none=True)
+    times = model(inputs)
+    loss = policy_loss(times.view(*actions.shape, times.shape[-1]), actions, old_logp, advantage, ref_logp, weight, clip, kl_coef)
+    loss.backward()
+    optimizer.step()
+    return loss.detach()
+
+
+def preference_step(model, optimizer, inputs, tokens, ref_logp, weight=None, beta=0.1, smoothing=0.0):
+    """One optimisation step on pairs of sequences, the preferred ones first: model(inputs) -> spike times with a row per token
+    of tokens[2P,T].  ref_logp[2P]: the sequences' log-probabilities under the reference.  Returns the loss."""
+    optimizer.zero_grad(set_to_none=True)
+    times = model(inputs)
+    loss = preference_loss(times.view(*tokens.shape, times.shape[-1]), tokens, ref_logp, weight, beta, smoothing)
+    loss.backward()
+    optimizer.step()
+    return loss.detach()
