@@ -313,7 +313,7 @@ enum { SNNTC_F32 = 0, SNNTC_BF16 = 1, SNNTC_F16 = 2 };
  *   row of dtable is written, rows are added in the order of their positions, with the same sums on every call.  Positions
  *   whose token lies outside the table add nothing.  table may be NULL in the backward call where encode is 0.
  * Errors: a negative size, a token_bytes or table_type that is none of the above, a NULL required pointer, V = 0 with N > 0
- * -> BAD_ARGUMENT; N, V or D above INT32_MAX -> TOO_LARGE (products may exceed it); a workspace below
+ * -> BAD_ARGUMENT; N or D above 2^30, V above INT32_MAX -> TOO_LARGE (products may exceed it); a workspace below
  * _workspace_bytes -> WORKSPACE.
  * ------------------------------------------------------------------------------------------- */
 SNNTC_API int snntc_embed_forward(const void* tokens, int token_bytes, const void* table, int table_type, float* z, int64_t N,

@@ -545,8 +545,8 @@ static bool known_type(int type) { return type == SNNTC_F32 || type == SNNTC_BF1
 
 static int embed_check(int64_t N, int64_t V, int64_t D, const char* who) {
     if (N < 0 || V < 0 || D < 0) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: negative size", who);
-    if (N > kInt32Max || V > kInt32Max || D > kInt32Max)
-        return fail(SNNTC_ERR_TOO_LARGE, "%s: a dimension exceeds INT32_MAX", who);
+    if (N > (1 << 30) || V > kInt32Max || D > (1 << 30))
+        return fail(SNNTC_ERR_TOO_LARGE, "%s: more than 2^30 tokens or columns, or INT32_MAX rows", who);
     return SNNTC_OK;
 }
 

@@ -3,10 +3,59 @@
 //     dE[v,:] = k_v sum over the n with tok_n = v of g[n,:],   k_v = scale, or -scale exp(1 - scale E[v,:])
 // The gradient is a sum of rows by token.  Atomic adds would make its last digits depend on the order in which workgroups run;
 // here the tokens are sorted first (by token, then by position), and the rows are added in that order.
+#include <algorithm>
+
 #include "snntc_common.h"
 
 namespace snntc {
 namespace {
+
+constexpr int kCols = 4;                            // columns of a lane
+constexpr int kSlice = kCols * kWave;               // columns of a wavefront
+
+// Column q of a lane: four neighbours (VEC: one access for all of them) or one of every 64.
+template <bool VEC>
+__device__ __forceinline__ int column(int slice, int lane, int q) { return slice * kSlice + (VEC ? lane * kCols + q : q * kWave + lane); }
+
+template <typename E>
+struct alignas(kCols * sizeof(E)) Four { E v[kCols]; };
+
+template <typename E, bool VEC>
+__device__ __forceinline__ void load_cols(const E* row, int slice, int lane, int D, float (&v)[kCols]) {
+    if (VEC) {
+        const int d = column<true>(slice, lane, 0);
+        Four<E> f{};
+        if (d < D) f = *reinterpret_cast<const Four<E>*>(row + d);
+#pragma unroll
+        for (int q = 0; q < kCols; ++q) v[q] = (float)f.v[q];
+    } else {
+#pragma unroll
+        for (int q = 0; q < kCols; ++q) {
+            const int d = column<false>(slice, lane, q);
+            v[q] = d < D ? (float)row[d] : 0.0f;
+        }
+    }
+}
+
+template <typename E, bool VEC>
+__device__ __forceinline__ void store_cols(E* row, int slice, int lane, int D, const float (&v)[kCols]) {
+    if (VEC) {
+        const int d = column<true>(slice, lane, 0);
+        Four<E> f;
+#pragma unroll
+        for (int q = 0; q < kCols; ++q) f.v[q] = (E)v[q];
+        if (d < D) *reinterpret_cast<Four<E>*>(row + d) = f;
+    } else {
+#pragma unroll
+        for (int q = 0; q < kCols; ++q) {
+            const int d = column<false>(slice, lane, q);
+            if (d < D) row[d] = (E)v[q];
+        }
+    }
+}
+
+// Whether rows of D elements from p on can be accessed four elements at a time.
+inline bool fours(const void* p, int64_t D, size_t element) { return D % kCols == 0 && (uintptr_t)p % (kCols * element) == 0; }
 
 // ---- forward -------------------------------------------------------------------------------------
 
@@ -14,107 +63,501 @@ __device__ __forceinline__ float time_of(float e, float scale, bool encode) {
     return encode ? expf(1.0f - scale * e) : scale * e;
 }
 
-template <typename E, typename I>
+// A wavefront owns 256 columns of TOKENS consecutive tokens and requests their rows together.
+template <typename E, typename I, bool VEC, int TOKENS>
 __global__ void __launch_bounds__(256)
-embed_forward_kernel(const I* __restrict__ tokens, const E* __restrict__ table, float* __restrict__ z, int V, int D, float scale,
-                     bool encode) {
-    const int64_t n = blockIdx.x;
-    const long long tok = tokens[n];
-    const bool known = tok >= 0 && tok < V;
-    const E* __restrict__ row = table + (size_t)(known ? tok : 0) * D;
-    for (int d = threadIdx.x; d < D; d += 256) z[(size_t)n * D + d] = known ? time_of((float)row[d], scale, encode) : NAN;
+embed_forward_kernel(const I* __restrict__ tokens, const E* __restrict__ table, float* __restrict__ z, int N, int V, int D, int slices,
+                     int64_t units, float scale, bool encode) {
+    const int64_t unit = (int64_t)blockIdx.x * (256 / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    if (unit >= units) return;
+    const int64_t n0 = unit / slices * TOKENS;
+    const int slice = (int)(unit % slices), lane = threadIdx.x % kWave;
+    float v[TOKENS][kCols];
+    bool known[TOKENS];
+#pragma unroll
+    for (int k = 0; k < TOKENS; ++k) {
+        const long long tok = tokens[min(n0 + k, (int64_t)N - 1)];
+        known[k] = tok >= 0 && tok < V;
+        load_cols<E, VEC>(table + (size_t)(known[k] ? tok : 0) * D, slice, lane, D, v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < TOKENS; ++k) {
+        if (n0 + k >= N) return;
+#pragma unroll
+        for (int q = 0; q < kCols; ++q) v[k][q] = known[k] ? time_of(v[k][q], scale, encode) : NAN;
+        store_cols<float, VEC>(z + (size_t)(n0 + k) * D, slice, lane, D, v[k]);
+    }
 }
 
 // ---- gradient ------------------------------------------------------------------------------------
+//
+// 1. The positions are put in the order (token, position).  Up to kRankMost of them by counting, for each, those that come
+//    before it: N^2 compares spread over the whole chip in one launch, 64 in one instruction and one count of its mask (N = 8192:
+//    1.7 us of compares), where a sort that works by passes is several launches.  More go by stable radix passes of at most ten
+//    bits, two launches each.  The same first launch clears dtable: rows of tokens that do not occur stay like that.
+// 2. The sorted positions are cut into chunks of equal length, whatever the tokens' frequencies are; a wavefront owns a chunk and
+//    256 columns.  It adds up the rows of each token in order; a token that lies wholly in the chunk is finished there, the
+//    first and last one may reach beyond it and leave partial sums.
+// 3. Partial sums of one token are added in the order of their chunks.
 
-// Place of every position in the order (token, position): the number of positions that come before it.  Positions whose token
-// lies outside the table count as token V and end up last.
-constexpr int kRankThreads = 256;
+constexpr int kRankThreads = 1024;
+constexpr int kRankWaves = kRankThreads / kWave;
+constexpr int kRankOwn = 32;                        // positions a workgroup ranks
+constexpr int kRankMost = 16 * kRankThreads;
+
+// Positions whose token lies outside the table count as token V and end up last.
 template <typename I>
-__global__ void __launch_bounds__(kRankThreads)
-token_rank_kernel(const I* __restrict__ tokens, int* __restrict__ sorted_token, int* __restrict__ sorted_pos, int N, int V) {
-    const int n = blockIdx.x * kRankThreads + threadIdx.x;
-    auto key = [&](int i) {
-        const long long t = tokens[i];
-        return t >= 0 && t < V ? (int)t : V;
-    };
-    __shared__ int tile[kRankThreads];
-    const int own = n < N ? key(n) : 0;
-    int rank = 0;
-    for (int i0 = 0; i0 < N; i0 += kRankThreads) {
-        __syncthreads();
-        if (i0 + (int)threadIdx.x < N) tile[threadIdx.x] = key(i0 + threadIdx.x);
-        __syncthreads();
-        const int count = min(kRankThreads, N - i0);
-        for (int i = 0; i < count; ++i) rank += tile[i] < own || (tile[i] == own && i0 + i < n);
+__device__ __forceinline__ int token_key(const I* tokens, int i, int V) {
+    const long long t = tokens[i];
+    return t >= 0 && t < V ? (int)t : V;
+}
+
+// What clears a tensor: workgroups from first_block on, 16 bytes a thread and step; the bytes before the first 16-byte boundary and
+// behind the last one by themselves.
+struct ClearArgs {
+    char* p;
+    int64_t bytes;
+    int first_block;
+    __device__ __forceinline__ bool mine() const { return (int)blockIdx.x >= first_block; }
+    __device__ __forceinline__ void run() const {
+        const int64_t block = blockIdx.x - first_block, blocks = gridDim.x - first_block;
+        const int64_t lead = min(bytes, (int64_t)(-(uintptr_t)p & 15)), n16 = (bytes - lead) / 16, tail = lead + n16 * 16;
+        uint4* q = reinterpret_cast<uint4*>(p + lead);
+        for (int64_t e = block * blockDim.x + threadIdx.x; e < n16; e += blocks * blockDim.x) q[e] = uint4{0, 0, 0, 0};
+        if (block == 0 && (int64_t)threadIdx.x < lead) p[threadIdx.x] = 0;
+        if (block == 0 && tail + threadIdx.x < bytes) p[tail + threadIdx.x] = 0;
     }
-    if (n < N) {
-        sorted_token[rank] = own;
-        sorted_pos[rank] = n;
+};
+__global__ void __launch_bounds__(256) clear_kernel(ClearArgs clear) { clear.run(); }
+
+// A wavefront holds R x 64 tokens, the workgroup all of them; each of its kRankOwn positions is compared with all.
+template <typename I, int R>
+__global__ void __launch_bounds__(kRankThreads)
+token_rank_kernel(const I* __restrict__ tokens, int* __restrict__ sorted_token, int* __restrict__ sorted_pos, int N, int V, ClearArgs clear) {
+    if (clear.mine()) { clear.run(); return; }
+    __shared__ int own_key[kRankOwn], part[kRankOwn][kRankWaves];
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int n0 = blockIdx.x * kRankOwn;
+    if ((int)threadIdx.x < kRankOwn) own_key[threadIdx.x] = n0 + (int)threadIdx.x < N ? token_key(tokens, n0 + threadIdx.x, V) : V;
+    int key[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int i = (wave * R + r) * kWave + lane;
+        key[r] = i < N ? token_key(tokens, i, V) : 0x7fffffff;       // behind everything: never counted
+    }
+    __syncthreads();
+    for (int k = 0; k < kRankOwn; ++k) {
+        const int own = __builtin_amdgcn_readfirstlane(own_key[k]);
+        int before = 0;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            // equal tokens count where their position is lower; the owned positions all lie in one group of 64
+            const int i0 = (wave * R + r) * kWave;
+            if (i0 + kWave <= n0) before += __popcll(__ballot(key[r] <= own));
+            else if (i0 > n0) before += __popcll(__ballot(key[r] < own));
+            else before += __popcll(__ballot(key[r] < own || (key[r] == own && i0 + lane < n0 + k)));
+        }
+        if (lane == 0) part[k][wave] = before;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < kRankOwn && n0 + (int)threadIdx.x < N) {
+        int rank = 0;
+#pragma unroll
+        for (int w = 0; w < kRankWaves; ++w) rank += part[threadIdx.x][w];
+        sorted_token[rank] = own_key[threadIdx.x];
+        sorted_pos[rank] = n0 + threadIdx.x;
     }
 }
 
-// A wavefront owns 64 columns of one table row and adds up its rows of g in order.
-template <typename E>
+// One pass of the radix sort: digits of `bits` bits from bit `shift` on.  A workgroup owns `chunk` consecutive entries; counts[g][d]
+// is how often digit d occurs in chunk g.  The first pass reads tokens (and positions are its indices), later ones key and pos.
+constexpr int kRadixThreads = 256;
+constexpr int kRadixWaves = kRadixThreads / kWave;
+constexpr int kRadixBits = 10;
+constexpr int kRadixChunk = 2048, kRadixChunks = 256;
+
+template <typename I, bool FIRST>
+__device__ __forceinline__ int entry_key(const I* tokens, const int* key, int i, int V) {
+    return FIRST ? token_key(tokens, i, V) : key[i];
+}
+
+template <typename I, bool FIRST>
+__global__ void __launch_bounds__(kRadixThreads)
+radix_count_kernel(const I* __restrict__ tokens, const int* __restrict__ key, int* __restrict__ counts, int N, int V, int shift, int bits,
+                   int chunk, ClearArgs clear) {
+    if (clear.mine()) { clear.run(); return; }
+    __shared__ int hist[1 << kRadixBits];
+    const int bins = 1 << bits;
+    for (int d = threadIdx.x; d < bins; d += kRadixThreads) hist[d] = 0;
+    __syncthreads();
+    const int64_t i0 = (int64_t)blockIdx.x * chunk;
+    const int i1 = (int)min((int64_t)N, i0 + chunk);
+    for (int64_t i = i0 + threadIdx.x; i < i1; i += kRadixThreads)
+        atomicAdd(&hist[(entry_key<I, FIRST>(tokens, key, (int)i, V) >> shift) & (bins - 1)], 1);
+    __syncthreads();
+    for (int d = threadIdx.x; d < bins; d += kRadixThreads) counts[(size_t)blockIdx.x * bins + d] = hist[d];
+}
+
+template <typename I, bool FIRST>
+__global__ void __launch_bounds__(kRadixThreads)
+radix_place_kernel(const I* __restrict__ tokens, const int* __restrict__ key, const int* __restrict__ pos, const int* __restrict__ counts,
+                   int* __restrict__ out_key, int* __restrict__ out_pos, int N, int V, int shift, int bits, int chunk, int chunks) {
+    __shared__ int start[1 << kRadixBits], seen[kRadixWaves][1 << kRadixBits], wave_sum[kRadixWaves];
+    const int bins = 1 << bits, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const int g = blockIdx.x;
+    // where digit d of this chunk begins: all lower digits, and the same digit in earlier chunks
+    constexpr int kPer = (1 << kRadixBits) / kRadixThreads;
+    int total[kPer], before[kPer], sum = 0;
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+        const int d = threadIdx.x * kPer + q;
+        total[q] = before[q] = 0;
+        if (d < bins) {
+#pragma unroll 8
+            for (int h = 0; h < chunks; ++h) {
+                const int c = counts[(size_t)h * bins + d];
+                total[q] += c;
+                if (h < g) before[q] += c;
+            }
+        }
+        sum += total[q];
+    }
+    int upto = sum;
+#pragma unroll
+    for (int s = 1; s < kWave; s <<= 1) {
+        const int v = __shfl_up(upto, s, kWave);
+        if (lane >= s) upto += v;
+    }
+    if (lane == kWave - 1) wave_sum[wave] = upto;
+    for (int d = threadIdx.x; d < kRadixWaves * bins; d += kRadixThreads) (&seen[0][0])[(d / bins) * (1 << kRadixBits) + d % bins] = 0;
+    __syncthreads();
+    int base = upto - sum;
+    for (int w = 0; w < wave; ++w) base += wave_sum[w];
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+        const int d = threadIdx.x * kPer + q;
+        if (d < bins) start[d] = base + before[q];
+        base += total[q];
+    }
+    // each wavefront takes a consecutive quarter of the chunk, 64 entries at a time: first to count its digits, then, knowing what the
+    // wavefronts before it hold, to place them
+    const int64_t w0 = (int64_t)g * chunk + (int64_t)wave * (chunk / kRadixWaves);
+    const int64_t end = min((int64_t)N, w0 + chunk / kRadixWaves);
+    auto same_digit = [&](int digit, bool there) {
+        unsigned long long same = __ballot(there);
+        for (int b = 0; b < bits; ++b) {
+            const unsigned long long ones = __ballot((digit >> b) & 1);
+            same &= (digit >> b) & 1 ? ones : ~ones;
+        }
+        return same;
+    };
+    for (int64_t i = w0; i < end; i += kWave) {
+        const bool there = i + lane < end;
+        const int digit = there ? (entry_key<I, FIRST>(tokens, key, (int)(i + lane), V) >> shift) & (bins - 1) : 0;
+        if (there) atomicAdd(&seen[wave][digit], 1);
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < bins; d += kRadixThreads) {
+        int at = start[d];
+#pragma unroll
+        for (int w = 0; w < kRadixWaves; ++w) {
+            const int c = seen[w][d];
+            seen[w][d] = at;
+            at += c;
+        }
+    }
+    __syncthreads();
+    for (int64_t i = w0; i < end; i += kWave) {
+        const bool there = i + lane < end;
+        const int k = there ? entry_key<I, FIRST>(tokens, key, (int)(i + lane), V) : 0;
+        const int digit = (k >> shift) & (bins - 1);
+        const unsigned long long same = same_digit(digit, there);
+        const int ahead = __popcll(same & ((1ull << lane) - 1));
+        int at = 0;
+        if (there) {
+            at = seen[wave][digit] + ahead;
+            out_key[at] = k;
+            out_pos[at] = FIRST ? (int)(i + lane) : pos[i + lane];
+        }
+        // the last of equal digits moves the mark on, after all have read it (one wavefront: its LDS accesses are in order)
+        if (there && (same >> lane) == 1) seen[wave][digit] = at + 1;
+    }
+}
+
+// ---- sums of rows
+
+constexpr int kBatch = 8;                           // rows requested together
+
+// The finished sum of table row v.
+template <typename E, bool VEC>
+__device__ __forceinline__ void store_row(E* dtable, const E* table, int v, int slice, int lane, int D, float scale, bool encode,
+                                          const float (&s)[kCols]) {
+    float g[kCols];
+    if (encode) {
+        load_cols<E, VEC>(table + (size_t)v * D, slice, lane, D, g);
+#pragma unroll
+        for (int q = 0; q < kCols; ++q) g[q] = -scale * expf(1.0f - scale * g[q]) * s[q];
+    } else {
+#pragma unroll
+        for (int q = 0; q < kCols; ++q) g[q] = scale * s[q];
+    }
+    store_cols<E, VEC>(dtable + (size_t)v * D, slice, lane, D, g);
+}
+
+// partial[chunk][0]: what a chunk adds to the token that began before it; [1]: the token that begins in it and goes on behind it.
+template <typename E, bool VEC>
 __global__ void __launch_bounds__(256)
-embed_backward_kernel(const float* __restrict__ grad, const int* __restrict__ sorted_token, const int* __restrict__ sorted_pos,
-                      const E* __restrict__ table, E* __restrict__ dtable, int N, int D, float scale, bool encode) {
-    const int v = blockIdx.x;
-    int lo = 0, hi = N;
-    while (lo < hi) {
-        const int mid = lo + (hi - lo) / 2;
-        if (sorted_token[mid] < v) lo = mid + 1;
-        else hi = mid;
+embed_sums_kernel(const float* __restrict__ grad, const int* __restrict__ sorted_token, const int* __restrict__ sorted_pos,
+                  const E* __restrict__ table, E* __restrict__ dtable, float* __restrict__ partial, int N, int V, int D, int chunk,
+                  int slices, int64_t units, float scale, bool encode) {
+    const int64_t unit = (int64_t)blockIdx.x * (256 / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    if (unit >= units) return;
+    const int c = (int)(unit / slices), slice = (int)(unit % slices), lane = threadIdx.x % kWave;
+    const int i0 = c * chunk, i1 = min(N, i0 + chunk);                   // (N is at most 2^30)
+    const int first = sorted_token[i0];
+    bool head = i0 > 0 && sorted_token[i0 - 1] == first;                 // the first token began before
+    const bool open = i1 < N && sorted_token[i1] == sorted_token[i1 - 1];
+    float s[kCols] = {0.0f, 0.0f, 0.0f, 0.0f}, next[kBatch][kCols];
+    int tok = first;
+    auto request = [&](int i) {
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+            load_cols<float, VEC>(grad + (size_t)sorted_pos[min(i + k, i1 - 1)] * D, slice, lane, D, next[k]);
+    };
+    request(i0);
+    for (int i = i0; i < i1; i += kBatch) {
+        float v[kBatch][kCols];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+            for (int q = 0; q < kCols; ++q) v[k][q] = next[k][q];
+        if (i + kBatch < i1) request(i + kBatch);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            if (i + k >= i1) break;
+            const int t = sorted_token[i + k];
+            if (t != tok) {                                              // (uniform)
+                if (head) store_cols<float, VEC>(partial + (size_t)c * 2 * D, slice, lane, D, s);
+                else if (tok < V) store_row<E, VEC>(dtable, table, tok, slice, lane, D, scale, encode, s);
+                head = false;
+                tok = t;
+#pragma unroll
+                for (int q = 0; q < kCols; ++q) s[q] = 0.0f;
+            }
+            if (t >= V) return;                                          // the rest lies outside the table
+#pragma unroll
+            for (int q = 0; q < kCols; ++q) s[q] += v[k][q];
+        }
     }
-    for (int d = threadIdx.x; d < D; d += 256) {
+    if (head) store_cols<float, VEC>(partial + (size_t)c * 2 * D, slice, lane, D, s);
+    else if (open) store_cols<float, VEC>(partial + ((size_t)c * 2 + 1) * D, slice, lane, D, s);
+    else store_row<E, VEC>(dtable, table, tok, slice, lane, D, scale, encode, s);
+}
+
+// A workgroup joins the token that begins in chunk c and goes on behind it, if there is one: each wavefront a consecutive part of
+// its chunks, then the parts in order.
+constexpr int kJoinWaves = 16;
+template <typename E>
+__global__ void __launch_bounds__(kJoinWaves * kWave)
+embed_join_kernel(const float* __restrict__ partial, const int* __restrict__ sorted_token, const E* __restrict__ table, E* __restrict__ dtable,
+                  int N, int V, int D, int chunk, int chunks, float scale, bool encode) {
+    __shared__ float part[kJoinWaves][kWave];
+    const int c = blockIdx.x, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const int64_t i0 = (int64_t)c * chunk, i1 = i0 + chunk;
+    if (i1 >= N) return;
+    const int tok = sorted_token[i1];
+    if (tok >= V || sorted_token[i1 - 1] != tok) return;                 // nothing goes on behind this chunk
+    if (i0 > 0 && sorted_token[i0 - 1] == tok) return;                   // it began earlier
+    int last = c + 1;                                                    // the last chunk that begins with this token
+    while (last + 1 < chunks) {
+        const int at = last + 1 + lane;
+        const unsigned long long more = __ballot(at < chunks && sorted_token[(int64_t)min(at, chunks - 1) * chunk] == tok);
+        const int run = more == ~0ull ? kWave : __ffsll((long long)~more) - 1;
+        last += run;
+        if (run < kWave) break;
+    }
+    const int rows = last - c + 1;                                       // partial sums: the begun one, then one a chunk
+    const int per = (rows + kJoinWaves - 1) / kJoinWaves, r0 = min(rows, wave * per), r1 = min(rows, r0 + per);
+    for (int d0 = 0; d0 < D; d0 += kWave) {
+        const int d = d0 + lane;
         float s = 0.0f;
-        for (int i = lo; i < N && sorted_token[i] == v; ++i) s += grad[(size_t)sorted_pos[i] * D + d];
-        const size_t e = (size_t)v * D + d;
-        dtable[e] = (E)(encode ? -scale * expf(1.0f - scale * (float)table[e]) * s : scale * s);
+        if (d < D) {
+#pragma unroll 8
+            for (int r = r0; r < r1; ++r) s += partial[((size_t)(c + r) * 2 + (r == 0)) * D + d];
+        }
+        part[wave][lane] = s;
+        __syncthreads();
+        if (wave == 0 && d < D) {
+            s = part[0][lane];
+            for (int w = 1; w < kJoinWaves && w * per < rows; ++w) s += part[w][lane];
+            const size_t e = (size_t)tok * D + d;
+            dtable[e] = (E)(encode ? -scale * expf(1.0f - scale * (float)table[e]) * s : scale * s);
+        }
+        __syncthreads();
     }
+}
+
+// How the sorted positions are cut: chunks long enough that few tokens are cut, short enough that some 2048 wavefronts are at work.
+struct SumPlan { int chunk, chunks, slices; };
+SumPlan sum_plan(int64_t N, int64_t D) {
+    SumPlan p;
+    p.slices = (int)((D + kSlice - 1) / kSlice);
+    int64_t chunk = N * p.slices / 2048;
+    chunk = (chunk + kBatch - 1) / kBatch * kBatch;
+    chunk = chunk < 16 ? 16 : chunk > 256 ? 256 : chunk;
+    p.chunk = (int)chunk;
+    p.chunks = (int)((N + chunk - 1) / chunk);
+    return p;
+}
+
+struct RadixPlan { int passes, bits, chunk, chunks; };
+RadixPlan radix_plan(int64_t N, int64_t V) {
+    RadixPlan p;
+    int bits = 1;
+    while (bits < 32 && (V >> bits) > 0) ++bits;                         // of keys 0 .. V
+    p.passes = (bits + kRadixBits - 1) / kRadixBits;
+    p.bits = (bits + p.passes - 1) / p.passes;
+    int64_t chunk = (N + kRadixChunks - 1) / kRadixChunks;
+    chunk = (chunk + 4 * kWave - 1) / (4 * kWave) * (4 * kWave);
+    p.chunk = (int)(chunk < kRadixChunk ? kRadixChunk : chunk);
+    p.chunks = (int)((N + p.chunk - 1) / p.chunk);
+    return p;
+}
+
+struct SortWs {
+    int *token, *pos, *other_token, *other_pos, *counts;
+    float* partial;
+    size_t bytes;
+    SortWs(void* ws, int64_t N, int64_t V, int64_t D) {
+        char* base = static_cast<char*>(ws);
+        size_t used = 0;
+        auto take = [&](size_t b) { char* p = base + used; used += align_up(b); return p; };
+        token = reinterpret_cast<int*>(take(N * sizeof(int)));
+        pos = reinterpret_cast<int*>(take(N * sizeof(int)));
+        const SumPlan s = sum_plan(N, D);
+        partial = reinterpret_cast<float*>(take((size_t)s.chunks * 2 * D * sizeof(float)));
+        other_token = other_pos = counts = nullptr;
+        if (N > kRankMost) {
+            const RadixPlan r = radix_plan(N, V);
+            other_token = reinterpret_cast<int*>(take(N * sizeof(int)));
+            other_pos = reinterpret_cast<int*>(take(N * sizeof(int)));
+            counts = reinterpret_cast<int*>(take((size_t)r.chunks * (1 << r.bits) * sizeof(int)));
+        }
+        bytes = used;
+    }
+};
+
+template <typename I>
+int sort_tokens(const I* tokens, const SortWs& w, int64_t N, int64_t V, void* dtable, int64_t table_bytes, hipStream_t stream) {
+    // workgroups that clear: 16 KiB a workgroup and step, up to four a CU
+    const int64_t clear_blocks = std::max<int64_t>(1, std::min<int64_t>(1024, table_bytes / (16 * 1024)));
+    if (N <= kRankMost) {
+        const int blocks = (int)((N + kRankOwn - 1) / kRankOwn);
+        const dim3 grid((unsigned)(blocks + clear_blocks));
+        const ClearArgs clear{static_cast<char*>(dtable), table_bytes, blocks};
+        const int held = (int)((N + kRankThreads - 1) / kRankThreads);
+        KernelTimerScope timer_("token_rank", stream);
+        auto kern = held <= 1 ? token_rank_kernel<I, 1> : held <= 2 ? token_rank_kernel<I, 2> : held <= 4 ? token_rank_kernel<I, 4>
+                    : held <= 8 ? token_rank_kernel<I, 8> : token_rank_kernel<I, 16>;
+        hipLaunchKernelGGL(kern, grid, dim3(kRankThreads), 0, stream, tokens, w.token, w.pos, (int)N, (int)V, clear);
+        SNNTC_HIP_CHECK(hipGetLastError());
+        return SNNTC_OK;
+    }
+    const RadixPlan r = radix_plan(N, V);
+    // the last pass ends in token / pos
+    int *to_key = r.passes % 2 ? w.token : w.other_token, *to_pos = r.passes % 2 ? w.pos : w.other_pos;
+    const int *key = nullptr, *pos = nullptr;
+    for (int pass = 0; pass < r.passes; ++pass) {
+        const int shift = pass * r.bits;
+        const ClearArgs clear{static_cast<char*>(dtable), table_bytes, r.chunks};
+        {
+            KernelTimerScope timer_("radix_count", stream);
+            if (pass == 0)
+                hipLaunchKernelGGL((radix_count_kernel<I, true>), dim3((unsigned)(r.chunks + 2 * clear_blocks)), dim3(kRadixThreads), 0, stream,
+                                   tokens, key, w.counts, (int)N, (int)V, shift, r.bits, r.chunk, clear);
+            else
+                hipLaunchKernelGGL((radix_count_kernel<I, false>), dim3((unsigned)r.chunks), dim3(kRadixThreads), 0, stream, tokens, key,
+                                   w.counts, (int)N, (int)V, shift, r.bits, r.chunk, clear);
+        }
+        SNNTC_HIP_CHECK(hipGetLastError());
+        {
+            KernelTimerScope timer_("radix_place", stream);
+            if (pass == 0)
+                hipLaunchKernelGGL((radix_place_kernel<I, true>), dim3((unsigned)r.chunks), dim3(kRadixThreads), 0, stream, tokens, key, pos,
+                                   w.counts, to_key, to_pos, (int)N, (int)V, shift, r.bits, r.chunk, r.chunks);
+            else
+                hipLaunchKernelGGL((radix_place_kernel<I, false>), dim3((unsigned)r.chunks), dim3(kRadixThreads), 0, stream, tokens, key, pos,
+                                   w.counts, to_key, to_pos, (int)N, (int)V, shift, r.bits, r.chunk, r.chunks);
+        }
+        SNNTC_HIP_CHECK(hipGetLastError());
+        key = to_key; pos = to_pos;
+        to_key = key == w.token ? w.other_token : w.token;
+        to_pos = pos == w.pos ? w.other_pos : w.pos;
+    }
+    return SNNTC_OK;
 }
 
 }  // namespace
 
 int launch_embed_forward(const void* tokens, int token_bytes, const void* table, int type, float* z, int64_t N, int64_t V, int64_t D,
                          float scale, bool encode, hipStream_t stream) {
+    const int slices = (int)((D + kSlice - 1) / kSlice);
+    // four rows in flight a wavefront once that still leaves every SIMD two of them
+    const int each = N * slices >= 8192 ? 4 : 1;
+    const int64_t units = (N + each - 1) / each * slices, blocks = (units + 3) / 4;
+    if (blocks > (1 << 24) - 1) return fail(SNNTC_ERR_TOO_LARGE, "embed: too many rows");
+    const bool vec = fours(table, D, type_bytes(type)) && fours(z, D, sizeof(float));
     with_type(type, [&](auto e) {
         using E = decltype(e);
         KernelTimerScope timer_("embed_forward", stream);
-        if (token_bytes == 8)
-            hipLaunchKernelGGL((embed_forward_kernel<E, int64_t>), dim3((unsigned)N), dim3(256), 0, stream,
-                               static_cast<const int64_t*>(tokens), static_cast<const E*>(table), z, (int)V, (int)D, scale, encode);
-        else
-            hipLaunchKernelGGL((embed_forward_kernel<E, int32_t>), dim3((unsigned)N), dim3(256), 0, stream,
-                               static_cast<const int32_t*>(tokens), static_cast<const E*>(table), z, (int)V, (int)D, scale, encode);
+        auto launch = [&](auto i) {
+            using I = decltype(i);
+            auto kern = vec ? (each == 4 ? embed_forward_kernel<E, I, true, 4> : embed_forward_kernel<E, I, true, 1>)
+                            : (each == 4 ? embed_forward_kernel<E, I, false, 4> : embed_forward_kernel<E, I, false, 1>);
+            hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), 0, stream, static_cast<const I*>(tokens),
+                               static_cast<const E*>(table), z, (int)N, (int)V, (int)D, slices, units, scale, encode);
+        };
+        if (token_bytes == 8) launch(int64_t{});
+        else launch(int32_t{});
         return 0;
     });
     SNNTC_HIP_CHECK(hipGetLastError());
     return SNNTC_OK;
 }
 
-size_t embed_backward_workspace(int64_t N, int64_t, int64_t) { return align_up((size_t)N * sizeof(int)) * 2; }
+size_t embed_backward_workspace(int64_t N, int64_t V, int64_t D) { return N > 0 ? SortWs(nullptr, N, V, D).bytes : 0; }
 
 int launch_embed_backward(const float* grad, const void* tokens, int token_bytes, const void* table, int type, void* dtable, int64_t N,
                           int64_t V, int64_t D, float scale, bool encode, void* ws, hipStream_t stream) {
-    int* sorted_token = static_cast<int*>(ws);
-    int* sorted_pos = reinterpret_cast<int*>(static_cast<char*>(ws) + align_up((size_t)N * sizeof(int)));
-    if (N > 0) {
-        KernelTimerScope timer_("token_rank", stream);
-        const dim3 grid((unsigned)((N + kRankThreads - 1) / kRankThreads));
-        if (token_bytes == 8)
-            hipLaunchKernelGGL(token_rank_kernel<int64_t>, grid, dim3(kRankThreads), 0, stream, static_cast<const int64_t*>(tokens),
-                               sorted_token, sorted_pos, (int)N, (int)V);
-        else
-            hipLaunchKernelGGL(token_rank_kernel<int32_t>, grid, dim3(kRankThreads), 0, stream, static_cast<const int32_t*>(tokens),
-                               sorted_token, sorted_pos, (int)N, (int)V);
+    const int64_t table_bytes = V * D * (int64_t)type_bytes(type);
+    if (N == 0) {
+        KernelTimerScope timer_("embed_clear", stream);
+        hipLaunchKernelGGL(clear_kernel, dim3(1024), dim3(256), 0, stream, ClearArgs{static_cast<char*>(dtable), table_bytes, 0});
+        SNNTC_HIP_CHECK(hipGetLastError());
+        return SNNTC_OK;
     }
-    SNNTC_HIP_CHECK(hipGetLastError());
+    const SumPlan p = sum_plan(N, D);
+    const int64_t units = (int64_t)p.chunks * p.slices, blocks = (units + 3) / 4;
+    if (blocks > (1 << 24) - 1) return fail(SNNTC_ERR_TOO_LARGE, "embed: too many rows of gradients");
+    const SortWs w(ws, N, V, D);
+    int rc = token_bytes == 8 ? sort_tokens(static_cast<const int64_t*>(tokens), w, N, V, dtable, table_bytes, stream)
+                              : sort_tokens(static_cast<const int32_t*>(tokens), w, N, V, dtable, table_bytes, stream);
+    if (rc) return rc;
+    const size_t element = type_bytes(type);
+    const bool vec = fours(grad, D, sizeof(float)) && fours(dtable, D, element) && (!encode || fours(table, D, element));
     with_type(type, [&](auto e) {
         using E = decltype(e);
-        KernelTimerScope timer_("embed_backward", stream);
-        hipLaunchKernelGGL(embed_backward_kernel<E>, dim3((unsigned)V), dim3(256), 0, stream, grad, sorted_token, sorted_pos,
-                           static_cast<const E*>(table), static_cast<E*>(dtable), (int)N, (int)D, scale, encode);
+        {
+            KernelTimerScope timer_("embed_sums", stream);
+            auto kern = vec ? embed_sums_kernel<E, true> : embed_sums_kernel<E, false>;
+            hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), 0, stream, grad, w.token, w.pos, static_cast<const E*>(table),
+                               static_cast<E*>(dtable), w.partial, (int)N, (int)V, (int)D, p.chunk, p.slices, units, scale, encode);
+        }
+        if (p.chunks > 1) {
+            KernelTimerScope timer_("embed_join", stream);
+            hipLaunchKernelGGL(embed_join_kernel<E>, dim3((unsigned)(p.chunks - 1)), dim3(kJoinWaves * kWave), 0, stream, w.partial, w.token,
+                               static_cast<const E*>(table), static_cast<E*>(dtable), (int)N, (int)V, (int)D, p.chunk, p.chunks, scale, encode);
+        }
         return 0;
     });
     SNNTC_HIP_CHECK(hipGetLastError());

@@ -58,7 +58,9 @@ def test_forward_and_gradient(N, V, D, dtype, bits):
 
 
 @pytest.mark.parametrize("N,V,D,dtype", [(20000, 30, 64, torch.float32), (17000, 50000, 33, torch.bfloat16), (40000, 1, 20, torch.float32),
-                                         (70001, 300000, 8, torch.float16), (33000, 5000, 300, torch.float32)])
+                                         (70001, 300000, 8, torch.float16), (33000, 5000, 300, torch.float32),
+                                         (16384, 700, 12, torch.float32), (16385, 1023, 12, torch.float32), (16385, 1024, 7, torch.float32),
+                                         (20000, 1200000, 4, torch.bfloat16), (600000, 77, 3, torch.float32)])
 def test_many_tokens(N, V, D, dtype):
     """More positions than the short sort takes; tokens that occur tens of thousands of times; tables most of whose rows are unused."""
     import snntc_amd as snn
