@@ -93,7 +93,7 @@ embed_forward_kernel(const I* __restrict__ tokens, const E* __restrict__ table, 
 //
 // 1. The positions are put in the order (token, position).  Up to kRankMost of them by counting, for each, those that come
 //    before it: N^2 compares spread over the whole chip in one launch, 64 in one instruction and one count of its mask (N = 8192:
-//    1.7 us of compares), where a sort that works by passes is several launches.  More go by stable radix passes of at most ten
+//    1.7 us of compares), where a sort that works by passes is several launches.  More go by stable radix passes of at most nine
 //    bits, two launches each.  The same first launch clears dtable: rows of tokens that do not occur stay like that.
 // 2. The sorted positions are cut into chunks of equal length, whatever the tokens' frequencies are; a wavefront owns a chunk and
 //    256 columns.  It adds up the rows of each token in order; a token that lies wholly in the chunk is finished there, the
@@ -130,50 +130,54 @@ struct ClearArgs {
 };
 __global__ void __launch_bounds__(256) clear_kernel(ClearArgs clear) { clear.run(); }
 
-// A wavefront holds R x 64 tokens, the workgroup all of them; each of its kRankOwn positions is compared with all.
+// A wavefront holds R x 64 tokens, the workgroup all of them; each of its kRankOwn positions is compared with all.  Equal tokens
+// count where their position is lower: a token before the owned positions is held as 2 token, one behind them as 2 token + 1, and
+// both count where they lie below 2 own + 1.  The owned ones among themselves are counted apart.
 template <typename I, int R>
 __global__ void __launch_bounds__(kRankThreads)
 token_rank_kernel(const I* __restrict__ tokens, int* __restrict__ sorted_token, int* __restrict__ sorted_pos, int N, int V, ClearArgs clear) {
     if (clear.mine()) { clear.run(); return; }
-    __shared__ int own_key[kRankOwn], part[kRankOwn][kRankWaves];
+    __shared__ int part[kRankWaves][kRankOwn];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int n0 = blockIdx.x * kRankOwn;
-    if ((int)threadIdx.x < kRankOwn) own_key[threadIdx.x] = n0 + (int)threadIdx.x < N ? token_key(tokens, n0 + threadIdx.x, V) : V;
-    int key[R];
+    const int own = lane < kRankOwn && n0 + lane < N ? token_key(tokens, n0 + lane, V) : V;
+    unsigned held[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const int i = (wave * R + r) * kWave + lane;
-        key[r] = i < N ? token_key(tokens, i, V) : 0x7fffffff;       // behind everything: never counted
+        held[r] = i >= N || (i >= n0 && i < n0 + kRankOwn) ? ~0u : 2u * (unsigned)token_key(tokens, i, V) + (i >= n0);
     }
-    __syncthreads();
+    int before = 0;
+#pragma unroll 4
     for (int k = 0; k < kRankOwn; ++k) {
-        const int own = __builtin_amdgcn_readfirstlane(own_key[k]);
-        int before = 0;
+        const unsigned bound = 2u * (unsigned)__builtin_amdgcn_readlane(own, k) + 1u;
+        int count = 0;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            // equal tokens count where their position is lower; the owned positions all lie in one group of 64
-            const int i0 = (wave * R + r) * kWave;
-            if (i0 + kWave <= n0) before += __popcll(__ballot(key[r] <= own));
-            else if (i0 > n0) before += __popcll(__ballot(key[r] < own));
-            else before += __popcll(__ballot(key[r] < own || (key[r] == own && i0 + lane < n0 + k)));
-        }
-        if (lane == 0) part[k][wave] = before;
+        for (int r = 0; r < R; ++r) count += __popcll(__ballot(held[r] < bound));
+        before = lane == k ? count : before;
     }
+    if (lane < kRankOwn) part[wave][lane] = before;
     __syncthreads();
-    if ((int)threadIdx.x < kRankOwn && n0 + (int)threadIdx.x < N) {
+    if (wave == 0) {
         int rank = 0;
 #pragma unroll
-        for (int w = 0; w < kRankWaves; ++w) rank += part[threadIdx.x][w];
-        sorted_token[rank] = own_key[threadIdx.x];
-        sorted_pos[rank] = n0 + threadIdx.x;
+        for (int w = 0; w < kRankWaves; ++w) rank += part[w][lane % kRankOwn];
+        for (int k = 0; k < kRankOwn; ++k) {
+            const int other = __builtin_amdgcn_readlane(own, k);
+            rank += other < own || (other == own && k < lane);
+        }
+        if (lane < kRankOwn && n0 + lane < N) {
+            sorted_token[rank] = own;
+            sorted_pos[rank] = n0 + lane;
+        }
     }
 }
 
 // One pass of the radix sort: digits of `bits` bits from bit `shift` on.  A workgroup owns `chunk` consecutive entries; counts[g][d]
 // is how often digit d occurs in chunk g.  The first pass reads tokens (and positions are its indices), later ones key and pos.
-constexpr int kRadixThreads = 256;
+constexpr int kRadixThreads = 1024;
 constexpr int kRadixWaves = kRadixThreads / kWave;
-constexpr int kRadixBits = 10;
+constexpr int kRadixBits = 9;
 constexpr int kRadixChunk = 2048, kRadixChunks = 256;
 
 template <typename I, bool FIRST>
@@ -202,44 +206,42 @@ template <typename I, bool FIRST>
 __global__ void __launch_bounds__(kRadixThreads)
 radix_place_kernel(const I* __restrict__ tokens, const int* __restrict__ key, const int* __restrict__ pos, const int* __restrict__ counts,
                    int* __restrict__ out_key, int* __restrict__ out_pos, int N, int V, int shift, int bits, int chunk, int chunks) {
-    __shared__ int start[1 << kRadixBits], seen[kRadixWaves][1 << kRadixBits], wave_sum[kRadixWaves];
+    __shared__ int total[1 << kRadixBits], start[1 << kRadixBits], seen[kRadixWaves][1 << kRadixBits], wave_sum[kRadixWaves];
     const int bins = 1 << bits, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const int g = blockIdx.x;
-    // where digit d of this chunk begins: all lower digits, and the same digit in earlier chunks
-    constexpr int kPer = (1 << kRadixBits) / kRadixThreads;
-    int total[kPer], before[kPer], sum = 0;
-#pragma unroll
-    for (int q = 0; q < kPer; ++q) {
-        const int d = threadIdx.x * kPer + q;
-        total[q] = before[q] = 0;
-        if (d < bins) {
-#pragma unroll 8
-            for (int h = 0; h < chunks; ++h) {
-                const int c = counts[(size_t)h * bins + d];
-                total[q] += c;
-                if (h < g) before[q] += c;
-            }
+    // where digit d of this chunk begins: all lower digits, and the same digit in earlier chunks; a digit's counts are read by
+    // several threads, each of which requests sixteen chunks together
+    for (int d = threadIdx.x; d < bins; d += kRadixThreads) total[d] = start[d] = 0;
+    for (int e = threadIdx.x; e < (kRadixWaves << bits); e += kRadixThreads) seen[e >> bits][e & (bins - 1)] = 0;
+    __syncthreads();
+    {
+        const int d = threadIdx.x & (bins - 1), parts = kRadixThreads >> bits;
+        int all = 0, earlier = 0;
+#pragma unroll 16
+        for (int h = threadIdx.x >> bits; h < chunks; h += parts) {
+            const int c = counts[((size_t)h << bits) + d];
+            all += c;
+            earlier += h < g ? c : 0;
         }
-        sum += total[q];
+        atomicAdd(&total[d], all);
+        atomicAdd(&start[d], earlier);
     }
-    int upto = sum;
+    __syncthreads();
+    const int own = (int)threadIdx.x < bins ? total[threadIdx.x] : 0;
+    int upto = own;
 #pragma unroll
     for (int s = 1; s < kWave; s <<= 1) {
         const int v = __shfl_up(upto, s, kWave);
         if (lane >= s) upto += v;
     }
     if (lane == kWave - 1) wave_sum[wave] = upto;
-    for (int d = threadIdx.x; d < kRadixWaves * bins; d += kRadixThreads) (&seen[0][0])[(d / bins) * (1 << kRadixBits) + d % bins] = 0;
     __syncthreads();
-    int base = upto - sum;
-    for (int w = 0; w < wave; ++w) base += wave_sum[w];
-#pragma unroll
-    for (int q = 0; q < kPer; ++q) {
-        const int d = threadIdx.x * kPer + q;
-        if (d < bins) start[d] = base + before[q];
-        base += total[q];
+    if ((int)threadIdx.x < bins) {
+        int base = upto - own;
+        for (int w = 0; w < wave; ++w) base += wave_sum[w];
+        start[threadIdx.x] += base;
     }
-    // each wavefront takes a consecutive quarter of the chunk, 64 entries at a time: first to count its digits, then, knowing what the
+    // each wavefront takes a consecutive part of the chunk, 64 entries at a time: first to count its digits, then, knowing what the
     // wavefronts before it hold, to place them
     const int64_t w0 = (int64_t)g * chunk + (int64_t)wave * (chunk / kRadixWaves);
     const int64_t end = min((int64_t)N, w0 + chunk / kRadixWaves);
@@ -314,57 +316,61 @@ embed_sums_kernel(const float* __restrict__ grad, const int* __restrict__ sorted
     if (unit >= units) return;
     const int c = (int)(unit / slices), slice = (int)(unit % slices), lane = threadIdx.x % kWave;
     const int i0 = c * chunk, i1 = min(N, i0 + chunk);                   // (N is at most 2^30)
-    const int first = sorted_token[i0];
-    bool head = i0 > 0 && sorted_token[i0 - 1] == first;                 // the first token began before
-    const bool open = i1 < N && sorted_token[i1] == sorted_token[i1 - 1];
-    float s[kCols] = {0.0f, 0.0f, 0.0f, 0.0f}, next[kBatch][kCols];
-    int tok = first;
-    auto request = [&](int i) {
+    float s[kCols] = {0.0f, 0.0f, 0.0f, 0.0f};
+    bool head = i0 > 0 && sorted_token[i0 - 1] == sorted_token[i0];      // the first token began before
+    int tok = V;
+    for (int g = i0; g < i1; g += kWave) {
+        // 64 entries at a time: lane k holds the token and the row of entry g + k, and whether the token ends there
+        const int here = min(kWave, i1 - g), at = min(g + lane, i1 - 1);
+        const int token = sorted_token[at], row = sorted_pos[at], follows = at + 1 < N ? sorted_token[at + 1] : V;
+        const unsigned long long ends = __ballot(token != follows), known = __ballot(lane < here && token < V);
+        const int rows = __popcll(known);                                // (tokens outside the table come last)
+        float next[kBatch][kCols];
+        auto request = [&](int k0) {
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k)
-            load_cols<float, VEC>(grad + (size_t)sorted_pos[min(i + k, i1 - 1)] * D, slice, lane, D, next[k]);
-    };
-    request(i0);
-    for (int i = i0; i < i1; i += kBatch) {
-        float v[kBatch][kCols];
+            for (int k = 0; k < kBatch; ++k)
+                load_cols<float, VEC>(grad + (size_t)__builtin_amdgcn_readlane(row, min(k0 + k, kWave - 1)) * D, slice, lane, D, next[k]);
+        };
+        if (rows > 0) request(0);
+        for (int k0 = 0; k0 < rows; k0 += kBatch) {
+            float v[kBatch][kCols];
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k)
+            for (int k = 0; k < kBatch; ++k)
 #pragma unroll
-            for (int q = 0; q < kCols; ++q) v[k][q] = next[k][q];
-        if (i + kBatch < i1) request(i + kBatch);
+                for (int q = 0; q < kCols; ++q) v[k][q] = next[k][q];
+            if (k0 + kBatch < rows) request(k0 + kBatch);
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-            if (i + k >= i1) break;
-            const int t = sorted_token[i + k];
-            if (t != tok) {                                              // (uniform)
-                if (head) store_cols<float, VEC>(partial + (size_t)c * 2 * D, slice, lane, D, s);
-                else if (tok < V) store_row<E, VEC>(dtable, table, tok, slice, lane, D, scale, encode, s);
-                head = false;
-                tok = t;
+            for (int k = 0; k < kBatch; ++k) {
+                if (k0 + k >= rows) break;
 #pragma unroll
-                for (int q = 0; q < kCols; ++q) s[q] = 0.0f;
+                for (int q = 0; q < kCols; ++q) s[q] += v[k][q];
+                tok = __builtin_amdgcn_readlane(token, k0 + k);
+                if ((ends >> (k0 + k)) & 1) {                            // (uniform)
+                    if (head) store_cols<float, VEC>(partial + (size_t)c * 2 * D, slice, lane, D, s);
+                    else store_row<E, VEC>(dtable, table, tok, slice, lane, D, scale, encode, s);
+                    head = false;
+                    tok = V;
+#pragma unroll
+                    for (int q = 0; q < kCols; ++q) s[q] = 0.0f;
+                }
             }
-            if (t >= V) return;                                          // the rest lies outside the table
-#pragma unroll
-            for (int q = 0; q < kCols; ++q) s[q] += v[k][q];
         }
+        if (rows < here) return;
     }
-    if (head) store_cols<float, VEC>(partial + (size_t)c * 2 * D, slice, lane, D, s);
-    else if (open) store_cols<float, VEC>(partial + ((size_t)c * 2 + 1) * D, slice, lane, D, s);
-    else store_row<E, VEC>(dtable, table, tok, slice, lane, D, scale, encode, s);
+    if (tok < V)                                                         // it goes on behind this chunk
+        store_cols<float, VEC>(partial + ((size_t)c * 2 + (head ? 0 : 1)) * D, slice, lane, D, s);
 }
 
-// A workgroup joins the token that begins in chunk c and goes on behind it, if there is one: each wavefront a consecutive part of
-// its chunks, then the parts in order.
+// A workgroup joins the token that begins in chunk c and goes on behind it, if there is one.  Its sixteen wavefronts share the
+// slices of 256 columns, and where those are fewer the chunks of a slice, each a consecutive part; the parts are added in order.
 constexpr int kJoinWaves = 16;
-template <typename E>
+template <typename E, bool VEC>
 __global__ void __launch_bounds__(kJoinWaves * kWave)
 embed_join_kernel(const float* __restrict__ partial, const int* __restrict__ sorted_token, const E* __restrict__ table, E* __restrict__ dtable,
-                  int N, int V, int D, int chunk, int chunks, float scale, bool encode) {
-    __shared__ float part[kJoinWaves][kWave];
-    const int c = blockIdx.x, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+                  int N, int V, int D, int chunk, int chunks, int slices, float scale, bool encode) {
+    __shared__ float part[kJoinWaves][kCols][kWave];
+    const int c = blockIdx.x, lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int64_t i0 = (int64_t)c * chunk, i1 = i0 + chunk;
-    if (i1 >= N) return;
     const int tok = sorted_token[i1];
     if (tok >= V || sorted_token[i1 - 1] != tok) return;                 // nothing goes on behind this chunk
     if (i0 > 0 && sorted_token[i0 - 1] == tok) return;                   // it began earlier
@@ -377,32 +383,41 @@ embed_join_kernel(const float* __restrict__ partial, const int* __restrict__ sor
         if (run < kWave) break;
     }
     const int rows = last - c + 1;                                       // partial sums: the begun one, then one a chunk
-    const int per = (rows + kJoinWaves - 1) / kJoinWaves, r0 = min(rows, wave * per), r1 = min(rows, r0 + per);
-    for (int d0 = 0; d0 < D; d0 += kWave) {
-        const int d = d0 + lane;
-        float s = 0.0f;
-        if (d < D) {
+    int parts = 1;
+    while (parts * 2 * slices <= kJoinWaves) parts *= 2;
+    const int together = kJoinWaves / parts;                             // slices at a time
+    const int per = (rows + parts - 1) / parts, p = wave / together, r0 = min(rows, p * per), r1 = min(rows, r0 + per);
+    for (int first = 0; first < slices; first += together) {
+        const int slice = first + wave % together;
+        float s[kCols] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (slice < slices) {
 #pragma unroll 8
-            for (int r = r0; r < r1; ++r) s += partial[((size_t)(c + r) * 2 + (r == 0)) * D + d];
+            for (int r = r0; r < r1; ++r) {
+                float v[kCols];
+                load_cols<float, VEC>(partial + ((size_t)(c + r) * 2 + (r == 0)) * D, slice, lane, D, v);
+#pragma unroll
+                for (int q = 0; q < kCols; ++q) s[q] += v[q];
+            }
         }
-        part[wave][lane] = s;
+#pragma unroll
+        for (int q = 0; q < kCols; ++q) part[wave][q][lane] = s[q];
         __syncthreads();
-        if (wave == 0 && d < D) {
-            s = part[0][lane];
-            for (int w = 1; w < kJoinWaves && w * per < rows; ++w) s += part[w][lane];
-            const size_t e = (size_t)tok * D + d;
-            dtable[e] = (E)(encode ? -scale * expf(1.0f - scale * (float)table[e]) * s : scale * s);
+        if (p == 0 && slice < slices) {
+            for (int other = 1; other < parts && other * per < rows; ++other)
+#pragma unroll
+                for (int q = 0; q < kCols; ++q) s[q] += part[other * together + wave][q][lane];
+            store_row<E, VEC>(dtable, table, tok, slice, lane, D, scale, encode, s);
         }
         __syncthreads();
     }
 }
 
-// How the sorted positions are cut: chunks long enough that few tokens are cut, short enough that some 2048 wavefronts are at work.
+// How the sorted positions are cut: chunks long enough that few tokens are cut, short enough that some 4096 wavefronts are at work.
 struct SumPlan { int chunk, chunks, slices; };
 SumPlan sum_plan(int64_t N, int64_t D) {
     SumPlan p;
     p.slices = (int)((D + kSlice - 1) / kSlice);
-    int64_t chunk = N * p.slices / 2048;
+    int64_t chunk = N * p.slices / 4096;
     chunk = (chunk + kBatch - 1) / kBatch * kBatch;
     chunk = chunk < 16 ? 16 : chunk > 256 ? 256 : chunk;
     p.chunk = (int)chunk;
@@ -418,7 +433,7 @@ RadixPlan radix_plan(int64_t N, int64_t V) {
     p.passes = (bits + kRadixBits - 1) / kRadixBits;
     p.bits = (bits + p.passes - 1) / p.passes;
     int64_t chunk = (N + kRadixChunks - 1) / kRadixChunks;
-    chunk = (chunk + 4 * kWave - 1) / (4 * kWave) * (4 * kWave);
+    chunk = (chunk + kRadixThreads - 1) / kRadixThreads * kRadixThreads;
     p.chunk = (int)(chunk < kRadixChunk ? kRadixChunk : chunk);
     p.chunks = (int)((N + p.chunk - 1) / p.chunk);
     return p;
@@ -473,7 +488,7 @@ int sort_tokens(const I* tokens, const SortWs& w, int64_t N, int64_t V, void* dt
         {
             KernelTimerScope timer_("radix_count", stream);
             if (pass == 0)
-                hipLaunchKernelGGL((radix_count_kernel<I, true>), dim3((unsigned)(r.chunks + 2 * clear_blocks)), dim3(kRadixThreads), 0, stream,
+                hipLaunchKernelGGL((radix_count_kernel<I, true>), dim3((unsigned)(r.chunks + clear_blocks)), dim3(kRadixThreads), 0, stream,
                                    tokens, key, w.counts, (int)N, (int)V, shift, r.bits, r.chunk, clear);
             else
                 hipLaunchKernelGGL((radix_count_kernel<I, false>), dim3((unsigned)r.chunks), dim3(kRadixThreads), 0, stream, tokens, key,
@@ -555,8 +570,10 @@ int launch_embed_backward(const float* grad, const void* tokens, int token_bytes
         }
         if (p.chunks > 1) {
             KernelTimerScope timer_("embed_join", stream);
-            hipLaunchKernelGGL(embed_join_kernel<E>, dim3((unsigned)(p.chunks - 1)), dim3(kJoinWaves * kWave), 0, stream, w.partial, w.token,
-                               static_cast<const E*>(table), static_cast<E*>(dtable), (int)N, (int)V, (int)D, p.chunk, p.chunks, scale, encode);
+            auto kern = vec ? embed_join_kernel<E, true> : embed_join_kernel<E, false>;
+            hipLaunchKernelGGL(kern, dim3((unsigned)(p.chunks - 1)), dim3(kJoinWaves * kWave), 0, stream, w.partial, w.token,
+                               static_cast<const E*>(table), static_cast<E*>(dtable), (int)N, (int)V, (int)D, p.chunk, p.chunks, p.slices,
+                               scale, encode);
         }
         return 0;
     });
