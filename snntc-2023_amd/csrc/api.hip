@@ -591,8 +591,8 @@ int snntc_embed_backward(const float* grad, const void* tokens, int token_bytes,
 static int gated_check(int64_t B, int64_t T, int64_t D, int gate_type, const char* who) {
     if (B < 0 || T < 0 || D < 0) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: negative size", who);
     if (!known_type(gate_type)) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: unknown gate type %d", who, gate_type);
-    if (B > kInt32Max || T > kInt32Max || D > kInt32Max)
-        return fail(SNNTC_ERR_TOO_LARGE, "%s: a dimension exceeds INT32_MAX", who);
+    if (B > (1 << 30) || T > (1 << 30) || D > (1 << 30) || B * ((D + kWave - 1) / kWave) >= (1 << 20))
+        return fail(SNNTC_ERR_TOO_LARGE, "%s: a dimension above 2^30, or 2^20 and more groups of 64 channels", who);
     return SNNTC_OK;
 }
 

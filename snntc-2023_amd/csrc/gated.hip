@@ -4,6 +4,8 @@
 //     u_t = dy_t + a_{t+1} u_{t+1}  (the last step of a sequence: dy_t + dfinal)
 //     dx_t = (1 - a_t) u_t,   dgate_t = u_t (h_{t-1} - x_t) a_t (1 - a_t),   dstate = a_1 u_1
 // A step mixes two spike times, so what comes out lies between those that went in and is a spike time itself.
+#include <algorithm>
+
 #include "snntc_common.h"
 
 namespace snntc {
@@ -24,54 +26,265 @@ __device__ __forceinline__ int length_of(const int64_t* lengths, int64_t b, int6
     return (int)(n < 0 ? 0 : n > T ? T : n);
 }
 
-template <typename G>
-__global__ void __launch_bounds__(256)
-gated_scan_forward_kernel(const float* __restrict__ x, const G* __restrict__ gate, const float* __restrict__ state,
-                          const int64_t* __restrict__ lengths, float* __restrict__ y, float* __restrict__ final_state, int T, int D) {
-    const int64_t b = blockIdx.y;
-    const int d = blockIdx.x * 256 + threadIdx.x;
-    if (d >= D) return;
-    const int n = length_of(lengths, b, T);
-    const size_t base = (size_t)b * T * D + d;
-    float h = state ? state[b * D + d] : 0.0f;
-    for (int t = 0; t < T; ++t) {
-        const size_t e = base + (size_t)t * D;
-        if (t < n) {
-            const Gate g = gate_of((float)gate[e]);
-            h = g.a * h + g.rest * x[e];
-        }
-        y[e] = t < n ? h : 0.0f;
+// A workgroup owns 64 neighbouring channels of a sequence and walks along it in tiles of kWaves x kSteps steps: each wavefront holds
+// kSteps of them in registers (lane = channel).  A run of steps maps the state it is given to A h + H, so the wavefronts exchange
+// (A, H) of their runs through LDS, every one composes those before its own, and goes through its steps a second time with the
+// right start.  The next tile's loads are under way meanwhile; every value is read once and written once.
+//
+// Where that makes fewer than kFill workgroups, sequences are also cut along time: a first kernel composes (A, H) of each part, and
+// a workgroup starts from the composition of the parts before its own.  The order of composition depends on sizes alone.
+constexpr int kWaves = 8, kSteps = 8, kTile = kWaves * kSteps;
+constexpr int kThreads = kWaves * kWave;
+constexpr int kFill = 256, kCutFill = 1024;
+
+struct Map { float A, H; };                         // h -> A h + H
+__device__ __forceinline__ Map then(const Map& first, const Map& second) { return Map{first.A * second.A, fmaf(second.A, first.H, second.H)}; }
+
+struct Geometry {
+    int B, T, D, groups, parts, part;               // groups of 64 channels, parts of `part` steps (a multiple of kTile)
+};
+struct Place {
+    int64_t b;
+    int d, s, lane, wave;
+    bool valid;                                     // lanes behind the last channel repeat it and store nothing
+};
+__device__ __forceinline__ Place place_of(const Geometry& g, int64_t block) {
+    Place p;
+    p.lane = threadIdx.x % kWave;
+    p.wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int64_t rest = block / g.groups;
+    const int d = (int)(block % g.groups) * kWave + p.lane;
+    p.valid = d < g.D;
+    p.d = p.valid ? d : g.D - 1;
+    p.s = (int)(rest % g.parts);
+    p.b = rest / g.parts;
+    return p;
+}
+
+// Composition of maps[w][lane] over the wavefronts, w ascending (or descending) from the state h: what comes in at wavefront `wave`
+// and what goes out at the end.
+template <bool DOWN>
+__device__ __forceinline__ float through(const Map (*maps)[kWave], const Place& p, float h, float* in) {
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) {
+        const int w = DOWN ? kWaves - 1 - k : k;
+        if (w == p.wave) *in = h;
+        const Map m = maps[w][p.lane];
+        h = fmaf(m.A, h, m.H);
     }
-    if (final_state) final_state[b * D + d] = h;
+    return h;
+}
+
+// The state with which part s begins, from the maps of the parts on its way: each wavefront composes a consecutive share of them.
+template <bool DOWN>
+__device__ __forceinline__ float enter_part(const Map* parts, const Geometry& g, const Place& p, Map (*maps)[kWave], float h) {
+    const int count = DOWN ? g.parts - 1 - p.s : p.s;
+    if (count == 0) return h;
+    const int first = DOWN ? p.s + 1 : 0, per = (count + kWaves - 1) / kWaves;
+    const int r0 = min(count, p.wave * per), r1 = min(count, r0 + per);
+    Map m{1.0f, 0.0f};
+#pragma unroll 8
+    for (int r = r0; r < r1; ++r) {
+        // ascending in time; going down, the later part acts first
+        const Map next = parts[((size_t)p.b * g.parts + first + r) * g.D + p.d];
+        m = DOWN ? then(next, m) : then(m, next);
+    }
+    maps[p.wave][p.lane] = m;
+    __syncthreads();
+    float unused;
+    h = through<DOWN>(maps, p, h, &unused);
+    __syncthreads();
+    return h;
 }
 
 template <typename G>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kThreads)
+gated_scan_forward_kernel(const float* __restrict__ x, const G* __restrict__ gate, const float* __restrict__ state,
+                          const int64_t* __restrict__ lengths, float* __restrict__ y, float* __restrict__ final_state,
+                          const Map* __restrict__ parts, Geometry g) {
+    __shared__ Map maps[2][kWaves][kWave];
+    const Place p = place_of(g, blockIdx.x);
+    const int t0 = p.s * g.part, t1 = min(g.T, t0 + g.part);
+    const int n = min(length_of(lengths, p.b, g.T), t1);                 // steps from n on are not there
+    float h = state ? state[p.b * g.D + p.d] : 0.0f;
+    h = enter_part<false>(parts, g, p, maps[0], h);
+    const size_t base = (size_t)p.b * g.T * g.D + p.d;
+    float xn[kSteps];
+    G gn[kSteps];
+    auto request = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const size_t e = base + (size_t)max(0, min(t + i, n - 1)) * g.D;
+            xn[i] = x[e];
+            gn[i] = gate[e];
+        }
+    };
+    int buffer = 0;
+    if (t0 < n) request(t0 + p.wave * kSteps);
+    for (int tile = t0; tile < t1; tile += kTile) {
+        const int t = tile + p.wave * kSteps;
+        float* __restrict__ out = y + base;
+        if (tile >= n) {                                                 // (uniform) nothing there any more
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i)
+                if (t + i < t1 && p.valid) out[(size_t)(t + i) * g.D] = 0.0f;
+            continue;
+        }
+        float a[kSteps], b[kSteps];
+        Map m{1.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const Gate q = gate_of((float)gn[i]);
+            a[i] = t + i < n ? q.a : 1.0f;
+            b[i] = t + i < n ? q.rest * xn[i] : 0.0f;
+            m.H = fmaf(a[i], m.H, b[i]);
+            m.A *= a[i];
+        }
+        maps[buffer][p.wave][p.lane] = m;
+        if (tile + kTile < n) request(t + kTile);
+        __syncthreads();
+        float in = h;
+        h = through<false>(maps[buffer], p, h, &in);
+        buffer ^= 1;                                                     // (the other half is written behind the next barrier's readers)
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            in = fmaf(a[i], in, b[i]);
+            if (t + i < t1 && p.valid) out[(size_t)(t + i) * g.D] = t + i < n ? in : 0.0f;
+        }
+    }
+    if (final_state && p.s == g.parts - 1 && p.wave == 0 && p.valid) final_state[p.b * g.D + p.d] = h;
+}
+
+// (A, H) of every part but the last on the way: forward of x and the gates, backward (DOWN) of the gradients v_t = a_t (dy_t + v_{t+1}).
+template <typename G, bool DOWN>
+__global__ void __launch_bounds__(kThreads)
+gated_scan_parts_kernel(const float* __restrict__ x, const G* __restrict__ gate, const int64_t* __restrict__ lengths, Map* __restrict__ parts,
+                        Geometry g) {
+    __shared__ Map maps[kWaves][kWave];
+    // the grid leaves out the last part on the way: renumbered over parts - 1
+    Geometry less = g;
+    less.parts = g.parts - 1;
+    Place p = place_of(less, blockIdx.x);
+    if (DOWN) ++p.s;
+    const int t0 = p.s * g.part, t1 = min(g.T, t0 + g.part);
+    const int n = min(length_of(lengths, p.b, g.T), t1);
+    const size_t base = (size_t)p.b * g.T * g.D + p.d;
+    // each wavefront composes a consecutive share of the part's steps; shares are joined once
+    const int share = g.part / kWaves, w0 = t0 + p.wave * share, w1 = min(n, w0 + share);
+    Map m{1.0f, 0.0f};
+    float xn[kSteps];
+    G gn[kSteps];
+    auto at = [&](int i) { return DOWN ? w1 - 1 - i : w0 + i; };        // the i-th step on the way
+    const int count = w1 - w0;
+    auto request = [&](int i0) {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const size_t e = base + (size_t)at(min(i0 + i, count - 1)) * g.D;
+            xn[i] = x ? x[e] : 0.0f;
+            gn[i] = gate[e];
+        }
+    };
+    if (count > 0) request(0);
+    for (int i0 = 0; i0 < count; i0 += kSteps) {
+        float xv[kSteps];
+        G gv[kSteps];
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) { xv[i] = xn[i]; gv[i] = gn[i]; }
+        if (i0 + kSteps < count) request(i0 + kSteps);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            if (i0 + i >= count) break;
+            const Gate q = gate_of((float)gv[i]);
+            m.H = DOWN ? q.a * (m.H + xv[i]) : fmaf(q.a, m.H, q.rest * xv[i]);
+            m.A *= q.a;
+        }
+    }
+    maps[p.wave][p.lane] = m;
+    __syncthreads();
+    if (p.wave != 0) return;
+    m = maps[DOWN ? kWaves - 1 : 0][p.lane];
+#pragma unroll
+    for (int k = 1; k < kWaves; ++k) m = then(m, maps[DOWN ? kWaves - 1 - k : k][p.lane]);
+    if (p.valid) parts[((size_t)p.b * g.parts + p.s) * g.D + p.d] = m;
+}
+
+// The same walk from the end: v_t = a_t u_t, u_t = dy_t + v_{t+1}, v behind the last step = dfinal.
+template <typename G>
+__global__ void __launch_bounds__(kThreads)
 gated_scan_backward_kernel(const float* __restrict__ dy, const float* __restrict__ dfinal, const float* __restrict__ x,
                            const G* __restrict__ gate, const float* __restrict__ y, const float* __restrict__ state,
                            const int64_t* __restrict__ lengths, float* __restrict__ dx, G* __restrict__ dgate, float* __restrict__ dstate,
-                           int T, int D) {
-    const int64_t b = blockIdx.y;
-    const int d = blockIdx.x * 256 + threadIdx.x;
-    if (d >= D) return;
-    const int n = length_of(lengths, b, T);
-    const size_t base = (size_t)b * T * D + d;
-    float u = dfinal ? dfinal[b * D + d] : 0.0f;
-    for (int t = T - 1; t >= 0; --t) {
-        const size_t e = base + (size_t)t * D;
-        if (t >= n) {
-            if (dx) dx[e] = 0.0f;
-            if (dgate) dgate[e] = (G)0.0f;
+                           const Map* __restrict__ parts, Geometry g) {
+    __shared__ Map maps[2][kWaves][kWave];
+    const Place p = place_of(g, blockIdx.x);
+    const int t0 = p.s * g.part, t1 = min(g.T, t0 + g.part);
+    const int n = min(length_of(lengths, p.b, g.T), t1);
+    float v = dfinal ? dfinal[p.b * g.D + p.d] : 0.0f;
+    v = enter_part<true>(parts, g, p, maps[0], v);
+    const float start = state ? state[p.b * g.D + p.d] : 0.0f;
+    const size_t base = (size_t)p.b * g.T * g.D + p.d;
+    float un[kSteps], xn[kSteps], hn[kSteps];
+    G gn[kSteps];
+    auto request = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const int at = max(0, min(t + i, n - 1));
+            const size_t e = base + (size_t)at * g.D;
+            gn[i] = gate[e];
+            un[i] = dy ? dy[e] : 0.0f;
+            xn[i] = x[e];
+            hn[i] = y[at > 0 ? e - g.D : e];
+        }
+    };
+    int buffer = 0;
+    const int last = t0 + (t1 - t0 - 1) / kTile * kTile;
+    bool asked = false;
+    for (int tile = last; tile >= t0; tile -= kTile) {
+        const int t = tile + p.wave * kSteps;
+        if (tile >= n) {                                                 // (uniform) nothing there
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i)
+                if (t + i < t1 && p.valid) {
+                    const size_t e = base + (size_t)(t + i) * g.D;
+                    if (dx) dx[e] = 0.0f;
+                    if (dgate) dgate[e] = (G)0.0f;
+                }
             continue;
         }
-        const Gate g = gate_of((float)gate[e]);
-        const float before = t > 0 ? y[e - D] : state ? state[b * D + d] : 0.0f;
-        if (dy) u += dy[e];
-        if (dx) dx[e] = g.rest * u;
-        if (dgate) dgate[e] = (G)(u * (before - x[e]) * (g.a * g.rest));
-        u *= g.a;
+        if (!asked) request(t);
+        asked = true;
+        Gate q[kSteps];
+        float up[kSteps], lead[kSteps];
+        Map m{1.0f, 0.0f};
+#pragma unroll
+        for (int i = kSteps - 1; i >= 0; --i) {
+            const bool there = t + i < n;
+            q[i] = gate_of((float)gn[i]);
+            if (!there) q[i] = Gate{1.0f, 0.0f};
+            up[i] = there ? un[i] : 0.0f;
+            lead[i] = (t + i > 0 ? hn[i] : start) - xn[i];
+            m.H = q[i].a * (m.H + up[i]);
+            m.A *= q[i].a;
+        }
+        maps[buffer][p.wave][p.lane] = m;
+        if (tile > t0) request(t - kTile);
+        __syncthreads();
+        float in = v;
+        v = through<true>(maps[buffer], p, v, &in);
+        buffer ^= 1;
+#pragma unroll
+        for (int i = kSteps - 1; i >= 0; --i) {
+            const float u = up[i] + in;
+            in = q[i].a * u;
+            if (t + i < t1 && p.valid) {
+                const bool there = t + i < n;
+                const size_t e = base + (size_t)(t + i) * g.D;
+                if (dx) dx[e] = there ? q[i].rest * u : 0.0f;
+                if (dgate) dgate[e] = (G)(there ? u * lead[i] * (q[i].a * q[i].rest) : 0.0f);
+            }
+        }
     }
-    if (dstate) dstate[b * D + d] = u;
+    if (dstate && p.s == 0 && p.wave == 0 && p.valid) dstate[p.b * g.D + p.d] = v;
 }
 
 template <typename G>
@@ -85,16 +298,36 @@ gated_step_kernel(const float* x, const G* gate, const float* state, float* out,
 
 }  // namespace
 
-size_t gated_scan_workspace(int64_t, int64_t, int64_t) { return 0; }
+namespace {
+Geometry geometry(int64_t B, int64_t T, int64_t D) {
+    Geometry g{(int)B, (int)T, (int)D, (int)((D + kWave - 1) / kWave), 1, 0};
+    const int64_t rows = B * g.groups, tiles = (T + kTile - 1) / kTile;
+    if (rows < kFill && tiles > 1) g.parts = (int)std::min(tiles, (kCutFill + rows - 1) / rows);
+    g.part = (int)((tiles + g.parts - 1) / g.parts * kTile);
+    g.parts = T > 0 ? (int)((T + g.part - 1) / g.part) : 1;
+    return g;
+}
+}  // namespace
+
+size_t gated_scan_workspace(int64_t B, int64_t T, int64_t D) {
+    const Geometry g = geometry(B, T, D);
+    return g.parts > 1 ? align_up((size_t)B * g.parts * D * sizeof(Map)) : 0;
+}
 
 int launch_gated_scan_forward(const float* x, const void* gate, int type, const float* state, const int64_t* lengths, float* y,
-                              float* final_state, int64_t B, int64_t T, int64_t D, void*, hipStream_t stream) {
-    if (B > 65535) return fail(SNNTC_ERR_TOO_LARGE, "gated scan: too many sequences");
-    with_type(type, [&](auto g) {
-        using G = decltype(g);
+                              float* final_state, int64_t B, int64_t T, int64_t D, void* ws, hipStream_t stream) {
+    const Geometry g = geometry(B, T, D);
+    const int64_t rows = B * g.groups;
+    with_type(type, [&](auto e) {
+        using G = decltype(e);
+        if (g.parts > 1) {
+            KernelTimerScope timer_("gated_scan_parts", stream);
+            hipLaunchKernelGGL((gated_scan_parts_kernel<G, false>), dim3((unsigned)(rows * (g.parts - 1))), dim3(kThreads), 0, stream, x,
+                               static_cast<const G*>(gate), lengths, static_cast<Map*>(ws), g);
+        }
         KernelTimerScope timer_("gated_scan_forward", stream);
-        hipLaunchKernelGGL(gated_scan_forward_kernel<G>, dim3((unsigned)((D + 255) / 256), (unsigned)B), dim3(256), 0, stream, x,
-                           static_cast<const G*>(gate), state, lengths, y, final_state, (int)T, (int)D);
+        hipLaunchKernelGGL(gated_scan_forward_kernel<G>, dim3((unsigned)(rows * g.parts)), dim3(kThreads), 0, stream, x,
+                           static_cast<const G*>(gate), state, lengths, y, final_state, static_cast<const Map*>(ws), g);
         return 0;
     });
     SNNTC_HIP_CHECK(hipGetLastError());
@@ -103,13 +336,20 @@ int launch_gated_scan_forward(const float* x, const void* gate, int type, const 
 
 int launch_gated_scan_backward(const float* dy, const float* dfinal, const float* x, const void* gate, int type, const float* y,
                                const float* state, const int64_t* lengths, float* dx, void* dgate, float* dstate, int64_t B, int64_t T,
-                               int64_t D, void*, hipStream_t stream) {
-    if (B > 65535) return fail(SNNTC_ERR_TOO_LARGE, "gated scan: too many sequences");
-    with_type(type, [&](auto g) {
-        using G = decltype(g);
+                               int64_t D, void* ws, hipStream_t stream) {
+    const Geometry g = geometry(B, T, D);
+    const int64_t rows = B * g.groups;
+    with_type(type, [&](auto e) {
+        using G = decltype(e);
+        if (g.parts > 1) {
+            KernelTimerScope timer_("gated_scan_parts_down", stream);
+            hipLaunchKernelGGL((gated_scan_parts_kernel<G, true>), dim3((unsigned)(rows * (g.parts - 1))), dim3(kThreads), 0, stream, dy,
+                               static_cast<const G*>(gate), lengths, static_cast<Map*>(ws), g);
+        }
         KernelTimerScope timer_("gated_scan_backward", stream);
-        hipLaunchKernelGGL(gated_scan_backward_kernel<G>, dim3((unsigned)((D + 255) / 256), (unsigned)B), dim3(256), 0, stream, dy, dfinal,
-                           x, static_cast<const G*>(gate), y, state, lengths, dx, static_cast<G*>(dgate), dstate, (int)T, (int)D);
+        hipLaunchKernelGGL(gated_scan_backward_kernel<G>, dim3((unsigned)(rows * g.parts)), dim3(kThreads), 0, stream, dy, dfinal, x,
+                           static_cast<const G*>(gate), y, state, lengths, dx, static_cast<G*>(dgate), dstate, static_cast<const Map*>(ws),
+                           g);
         return 0;
     });
     SNNTC_HIP_CHECK(hipGetLastError());
