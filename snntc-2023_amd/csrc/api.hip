@@ -640,7 +640,7 @@ static int choice_check(int64_t rows, int64_t J, int times_type, const char* who
     if (!known_type(times_type)) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: unknown type of times %d", who, times_type);
     if (rows > 0 && J == 0) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: rows without outputs", who);
     if (rows >= (1 << 24)) return fail(SNNTC_ERR_TOO_LARGE, "%s: more than 2^24 - 1 rows", who);
-    if (J > kInt32Max) return fail(SNNTC_ERR_TOO_LARGE, "%s: more than INT32_MAX outputs", who);
+    if (J > (1 << 30)) return fail(SNNTC_ERR_TOO_LARGE, "%s: more than 2^30 outputs", who);
     return SNNTC_OK;
 }
 

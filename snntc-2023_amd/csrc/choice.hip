@@ -14,131 +14,378 @@
 namespace snntc {
 namespace {
 
-constexpr int kThreads = 256;
-
 // Running maximum m and sum s of exp(v - m); empty: m = -inf, s = 0.
 struct Soft { float m, s; };
+// exp by the hardware's base-2 exponential: the argument's product with log2(e) adds its own size in half steps to the result's
+// error, of terms that shrink faster than that grows.
+__device__ __forceinline__ float exp_fast(float v) { return __builtin_amdgcn_exp2f(v * 1.44269504f); }
 __device__ __forceinline__ Soft join(const Soft& a, const Soft& b) {
     const float m = fmaxf(a.m, b.m);
     if (m == -INFINITY) return Soft{m, a.s + b.s};                     // nothing yet (or a NaN sum to keep)
-    return Soft{m, a.s * expf(a.m - m) + b.s * expf(b.m - m)};
+    return Soft{m, a.s * exp_fast(a.m - m) + b.s * exp_fast(b.m - m)};
 }
-__device__ __forceinline__ Soft wave_join(Soft v) {
+template <int WIDTH>
+__device__ __forceinline__ float group_max(float v) {
 #pragma unroll
-    for (int d = kWave / 2; d > 0; d >>= 1) v = join(v, Soft{__shfl_xor(v.m, d, kWave), __shfl_xor(v.s, d, kWave)});
+    for (int d = WIDTH / 2; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, kWave));
+    return v;
+}
+template <int WIDTH>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+    for (int d = WIDTH / 2; d > 0; d >>= 1) v += __shfl_xor(v, d, kWave);
     return v;
 }
 
 __device__ __forceinline__ float row_weight(const float* weight, int64_t r) { return weight ? weight[r] : 1.0f; }
 
-// logp of the row's token; NaN for a token outside [0, J).
-template <typename E>
-__device__ __forceinline__ float token_logp(const E* t, long long token, int J, float2 soft) {
-    return token >= 0 && token < J ? (-(float)t[token] - soft.x) - soft.y : NAN;
-}
-
-template <typename E>
-__global__ void __launch_bounds__(kThreads)
-time_logp_kernel(const E* __restrict__ times, const long long* __restrict__ tokens, const float* __restrict__ weight,
-                 float* __restrict__ logp, float2* __restrict__ stats, int J) {
-    __shared__ Soft part[kThreads / kWave];
-    const int64_t r = blockIdx.x;
-    if (row_weight(weight, r) == 0.0f) {
-        if (threadIdx.x == 0) { logp[r] = 0.0f; if (stats) stats[r] = float2{0.0f, 0.0f}; }
-        return;
-    }
-    const E* __restrict__ t = times + (size_t)r * J;
-    float m = -INFINITY;
-    for (int j = threadIdx.x; j < J; j += kThreads) m = fmaxf(m, -(float)t[j]);
-    float s = 0.0f;
-    for (int j = threadIdx.x; j < J; j += kThreads) s += expf(-(float)t[j] - (m == -INFINITY ? 0.0f : m));
-    const Soft w = wave_join(Soft{m, s});
-    if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = w;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        Soft v = part[0];
-        for (int i = 1; i < kThreads / kWave; ++i) v = join(v, part[i]);
-        const float2 soft{v.m, logf(v.s)};
-        logp[r] = token_logp(t, tokens[r], J, soft);
-        if (stats) stats[r] = soft;
-    }
-}
-
-template <typename E>
-__global__ void __launch_bounds__(kThreads)
-time_logp_backward_kernel(const E* __restrict__ times, const long long* __restrict__ tokens, const float2* __restrict__ stats,
-                          const float* __restrict__ coef, const float* __restrict__ upstream, E* __restrict__ dtimes, int J) {
-    const int64_t r = blockIdx.x;
-    const float c = coef[r];
-    const float up = upstream ? *upstream : 1.0f;
-    E* __restrict__ g = dtimes + (size_t)r * J;
-    if (c == 0.0f) {
-        for (int j = threadIdx.x; j < J; j += kThreads) g[j] = (E)0.0f;
-        return;
-    }
-    const E* __restrict__ t = times + (size_t)r * J;
-    const long long token = tokens[r];
-    const float2 soft = stats[r];
-    const float cu = c * up;
-    for (int j = threadIdx.x; j < J; j += kThreads) g[j] = (E)(cu * (expf((-(float)t[j] - soft.x) - soft.y) - (j == token ? 1.0f : 0.0f)));
-}
-
-__global__ void __launch_bounds__(kThreads)
-policy_rows_kernel(const float* __restrict__ logp, PolicyArgs a, float* __restrict__ row_loss, float* __restrict__ coef, int64_t rows) {
-    const int64_t r = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (r >= rows) return;
-    const float w = a.weight ? a.weight[r] : a.mean;
-    if (w == 0.0f) {
-        row_loss[r] = 0.0f;
-        coef[r] = 0.0f;
-        return;
-    }
-    const float lp = logp[r], adv = a.advantage[r];
+struct RowLoss { float loss, coef; };
+// The policy loss of a row, and its derivative by logp.
+__device__ __forceinline__ RowLoss policy_row(const PolicyArgs& a, int64_t r, float lp) {
+    const float adv = a.advantage[r];
     const float ratio = expf(lp - a.old_logp[r]);
     const float plain = ratio * adv, clipped = fminf(fmaxf(ratio, a.low), a.high) * adv;
-    float loss = -(plain <= clipped ? plain : clipped), c = plain <= clipped ? -plain : 0.0f;
-    if (isnan(ratio) || isnan(plain)) loss = c = NAN;
+    RowLoss out{-(plain <= clipped ? plain : clipped), plain <= clipped ? -plain : 0.0f};
+    if (isnan(ratio) || isnan(plain)) out.loss = out.coef = NAN;
     if (a.ref_logp && a.kl != 0.0f) {
         const float d = a.ref_logp[r] - lp, e = expm1f(d);
-        loss += a.kl * (d == INFINITY ? d : e - d);                    // (inf - inf where the output can never be chosen)
-        c -= a.kl * e;
+        out.loss += a.kl * (d == INFINITY ? d : e - d);                // (inf - inf where the output can never be chosen)
+        out.coef -= a.kl * e;
     }
-    row_loss[r] = loss;
-    coef[r] = c * w;
+    return out;
 }
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int d = kWave / 2; d > 0; d >>= 1) v += __shfl_xor(v, d, kWave);
-    return v;
+// What a kernel over rows does with them.
+enum Mode {
+    LOGP,                                           // logp and statistics
+    POLICY,                                         // the same, the row's loss and, if wanted, its gradient
+    GRAD                                            // the gradient from statistics and coef
+};
+struct RowArgs {
+    const long long* tokens;
+    const float* weight;
+    float* logp;
+    float2* stats;
+    float* coef;
+    float* row_loss;
+    const float* upstream;                          // GRAD: a factor, NULL: 1
+    PolicyArgs policy;
+    int64_t rows;
+    int J;
+};
+
+// A row in pieces of VEC elements (16 bytes): those at 16-byte boundaries, `lead` elements before the first and `tail` behind the
+// last one.  VEC = 1: every element a piece, for times and dtimes that lie differently to such boundaries.
+template <typename E, int VEC>
+struct alignas(VEC * sizeof(E)) Piece { E v[VEC]; };
+// Keeps the compiler from carrying a piece's elements in float32 from one use to the next: sixteen 16-bit pieces a thread would take
+// all registers that way, eight half of the wavefronts a SIMD can have.
+template <typename P>
+__device__ __forceinline__ void forget(P& p) {
+    if constexpr (sizeof(P) == 16) {
+        typedef unsigned Words __attribute__((ext_vector_type(4)));
+        Words w = __builtin_bit_cast(Words, p);
+        asm volatile("" : "+v"(w));
+        p = __builtin_bit_cast(P, w);
+    }
 }
+struct Cut { int lead, pieces, tail; };
+template <typename E, int VEC>
+__device__ __forceinline__ Cut cut_row(const E* t, int J) {
+    if (VEC == 1) return Cut{0, J, 0};
+    Cut c;
+    c.lead = min(J, (int)((-(uintptr_t)t & (VEC * sizeof(E) - 1)) / sizeof(E)));
+    c.pieces = (J - c.lead) / VEC;
+    c.tail = J - c.lead - c.pieces * VEC;
+    return c;
+}
+// The single element thread k < 2 * VEC takes apart from its pieces, -1: none.
+template <int VEC>
+__device__ __forceinline__ int odd_element(const Cut& c, int k) {
+    if (VEC == 1) return -1;
+    if (k < c.lead) return k;
+    return k >= VEC && k < VEC + c.tail ? c.lead + c.pieces * VEC + k - VEC : -1;
+}
+
+__device__ __forceinline__ float grad_of(float t, const float2& soft, float c) { return c * exp_fast((-t - soft.x) - soft.y); }
+
+// WIDTH threads own a row and hold all of it in registers, so that it is read once: R pieces each, at most WIDTH * R * VEC elements and
+// the odd ones.  Up to 64 threads a row: several rows a workgroup.
+template <typename E, int VEC, int WIDTH, int R, Mode MODE>
+__global__ void __launch_bounds__(WIDTH < 256 ? 256 : WIDTH)
+choice_row_kernel(const E* __restrict__ times, E* __restrict__ dtimes, RowArgs a) {
+    constexpr int kRows = WIDTH < 256 ? 256 / WIDTH : 1, kWaves = WIDTH <= kWave ? 1 : WIDTH / kWave;
+    constexpr int kGroup = WIDTH < kWave ? WIDTH : kWave;
+    __shared__ Soft part[kWaves];
+    using P = Piece<E, VEC>;
+    const int k = threadIdx.x % WIDTH;
+    // the gradient pass begins with the rows that were read last: they may still be in a cache
+    const int64_t block = MODE == GRAD ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+    const int64_t r = block * kRows + threadIdx.x / WIDTH;
+    if (r >= a.rows) return;                                             // (whole rows; no barrier where rows share a workgroup)
+    const E* __restrict__ t = times + (size_t)r * a.J;
+    E* __restrict__ g = dtimes + (size_t)r * a.J;
+    const Cut cut = cut_row<E, VEC>(t, a.J);
+    const int odd = odd_element<VEC>(cut, k);
+    const float w = MODE == GRAD ? a.coef[r] : MODE == POLICY && !a.weight ? a.policy.mean : row_weight(a.weight, r);
+    if (w == 0.0f) {
+        if (MODE != GRAD && k == 0) {
+            if (a.logp) a.logp[r] = 0.0f;
+            if (a.stats) a.stats[r] = float2{0.0f, 0.0f};
+            if (MODE == POLICY) a.row_loss[r] = 0.0f;
+            if (MODE == POLICY && a.coef) a.coef[r] = 0.0f;
+        }
+        if (MODE == LOGP || !dtimes) return;
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            if (i * WIDTH + k < cut.pieces) reinterpret_cast<P*>(g + cut.lead)[i * WIDTH + k] = P{};
+        if (odd >= 0) g[odd] = (E)0.0f;
+        return;
+    }
+    P held[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+        if (i * WIDTH < cut.pieces) held[i] = reinterpret_cast<const P*>(t + cut.lead)[min(i * WIDTH + k, cut.pieces - 1)];
+    const float single = odd >= 0 ? (float)t[odd] : INFINITY;            // (infinity adds nothing)
+    const long long token = a.tokens[r];
+    const bool known = token >= 0 && token < a.J;
+    float2 soft;
+    float c = w;
+    if (MODE == GRAD) {
+        soft = a.stats[r];
+        if (a.upstream) c *= *a.upstream;
+    } else {
+        const float chosen = known ? (float)t[token] : NAN;
+        float m = -single;
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            if (i * WIDTH + k < cut.pieces)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) m = fmaxf(m, -(float)held[i].v[v]);
+        m = group_max<kGroup>(m);
+        const float base = m == -INFINITY ? 0.0f : m;
+        float sum = odd >= 0 ? exp_fast(-single - base) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            if (R >= 8) forget(held[i]);
+            if (i * WIDTH + k < cut.pieces)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) sum += exp_fast(-(float)held[i].v[v] - base);
+        }
+        Soft all{m, group_sum<kGroup>(sum)};
+        if (kWaves > 1) {
+            if (k % kWave == 0) part[k / kWave] = all;
+            __syncthreads();
+            all = part[0];
+#pragma unroll
+            for (int i = 1; i < kWaves; ++i) all = join(all, part[i]);
+        }
+        soft = float2{all.m, logf(all.s)};
+        const float lp = (-chosen - soft.x) - soft.y;
+        RowLoss loss{0.0f, 0.0f};
+        if (MODE == POLICY) {
+            loss = policy_row(a.policy, r, lp);
+            c = loss.coef * w;
+        }
+        if (k == 0) {
+            if (a.logp) a.logp[r] = lp;
+            if (a.stats) a.stats[r] = soft;
+            if (MODE == POLICY) a.row_loss[r] = loss.loss;
+            if (MODE == POLICY && a.coef) a.coef[r] = c;
+        }
+        if (MODE == LOGP || !dtimes) return;
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        if (i * WIDTH + k >= cut.pieces) continue;
+        if (R >= 8) forget(held[i]);
+        const int j0 = cut.lead + (i * WIDTH + k) * VEC;
+        float d[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) d[v] = grad_of((float)held[i].v[v], soft, c);
+        if (token >= j0 && token < j0 + VEC) {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) d[v] -= token == j0 + v ? c : 0.0f;
+        }
+        P out;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) out.v[v] = (E)d[v];
+        reinterpret_cast<P*>(g + cut.lead)[i * WIDTH + k] = out;
+    }
+    if (odd >= 0) g[odd] = (E)(grad_of(single, soft, c) - (token == odd ? c : 0.0f));
+}
+
+// Rows longer than a workgroup holds: slices of kSlicePieces pieces, a workgroup each.  One pass leaves (maximum, sum) of every slice, the
+// next joins those of a row in order, the third reads the row again for its gradient.
+constexpr int kSliceThreads = 256;
+template <int VEC>
+constexpr int slice_pieces() { return VEC == 1 ? 4096 : 1024; }          // 16 KiB of float32, 8 or 16 of 16-bit times
+
+template <typename E, int VEC>
+__global__ void __launch_bounds__(kSliceThreads)
+choice_slice_kernel(const E* __restrict__ times, const float* __restrict__ weight, Soft* __restrict__ partial, int J, int slices) {
+    __shared__ Soft part[kSliceThreads / kWave];
+    using P = Piece<E, VEC>;
+    constexpr int kPieces = slice_pieces<VEC>(), kEach = kPieces / kSliceThreads, kBatch = 4;
+    const int64_t r = blockIdx.x / slices;
+    const int slice = blockIdx.x % slices, k = threadIdx.x;
+    if (row_weight(weight, r) == 0.0f) return;
+    const E* __restrict__ t = times + (size_t)r * J;
+    const Cut cut = cut_row<E, VEC>(t, J);
+    const int odd = slice == 0 ? odd_element<VEC>(cut, k) : -1;
+    const P* __restrict__ pieces = reinterpret_cast<const P*>(t + cut.lead);
+    Soft all{-INFINITY, 0.0f};
+    if (odd >= 0) all = Soft{-(float)t[odd], 1.0f};
+    if (odd >= 0 && !(fabsf(all.m) < INFINITY)) all.s = all.m == -INFINITY ? 0.0f : NAN;
+#pragma unroll
+    for (int i0 = 0; i0 < kEach; i0 += kBatch) {
+        const int first = slice * kPieces + i0 * kSliceThreads;
+        if (first >= cut.pieces) break;                                  // (uniform)
+        P held[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) held[i] = pieces[min(first + i * kSliceThreads + k, cut.pieces - 1)];
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+            if (first + i * kSliceThreads + k < cut.pieces)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) m = fmaxf(m, -(float)held[i].v[v]);
+        const float base = m == -INFINITY ? 0.0f : m;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+            if (first + i * kSliceThreads + k < cut.pieces)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) sum += exp_fast(-(float)held[i].v[v] - base);
+        all = join(all, Soft{m, sum});
+    }
+    const float m = group_max<kWave>(all.m);
+    all = Soft{m, group_sum<kWave>(m == -INFINITY ? all.s : all.s * exp_fast(all.m - m))};
+    if (k % kWave == 0) part[k / kWave] = all;
+    __syncthreads();
+    if (k != 0) return;
+#pragma unroll
+    for (int i = 1; i < kSliceThreads / kWave; ++i) all = join(all, part[i]);
+    partial[r * slices + slice] = all;
+}
+
+template <typename E, Mode MODE>
+__global__ void __launch_bounds__(kWave)
+choice_join_kernel(const E* __restrict__ times, const Soft* __restrict__ partial, RowArgs a, int slices) {
+    const int64_t r = blockIdx.x;
+    const int lane = threadIdx.x;
+    const float w = MODE == POLICY && !a.weight ? a.policy.mean : row_weight(a.weight, r);
+    Soft all{-INFINITY, 0.0f};
+    float2 soft{0.0f, 0.0f};
+    float lp = 0.0f;
+    RowLoss loss{0.0f, 0.0f};
+    if (w != 0.0f) {
+        for (int i = lane; i < slices; i += kWave) all = join(all, partial[r * slices + i]);
+        const float m = group_max<kWave>(all.m);
+        all = Soft{m, group_sum<kWave>(m == -INFINITY ? all.s : all.s * exp_fast(all.m - m))};
+        soft = float2{all.m, logf(all.s)};
+        const long long token = a.tokens[r];
+        const float chosen = token >= 0 && token < a.J ? (float)times[(size_t)r * a.J + token] : NAN;
+        lp = (-chosen - soft.x) - soft.y;
+        if (MODE == POLICY) loss = policy_row(a.policy, r, lp);
+    }
+    if (lane != 0) return;
+    if (a.logp) a.logp[r] = lp;
+    if (a.stats) a.stats[r] = soft;
+    if (MODE == POLICY) a.row_loss[r] = loss.loss;
+    if (MODE == POLICY && a.coef) a.coef[r] = loss.coef * w;
+}
+
+template <typename E, int VEC>
+__global__ void __launch_bounds__(kSliceThreads)
+choice_slice_grad_kernel(const E* __restrict__ times, E* __restrict__ dtimes, RowArgs a, int slices) {
+    using P = Piece<E, VEC>;
+    constexpr int kPieces = slice_pieces<VEC>(), kEach = kPieces / kSliceThreads, kBatch = 4;
+    const int64_t block = gridDim.x - 1 - blockIdx.x;                    // (what was read last comes first)
+    const int64_t r = block / slices;
+    const int slice = block % slices, k = threadIdx.x;
+    const E* __restrict__ t = times + (size_t)r * a.J;
+    E* __restrict__ g = dtimes + (size_t)r * a.J;
+    const Cut cut = cut_row<E, VEC>(t, a.J);
+    const int odd = slice == 0 ? odd_element<VEC>(cut, k) : -1;
+    float c = a.coef[r];
+    const bool off = c == 0.0f;
+    if (a.upstream) c *= *a.upstream;
+    const float2 soft = off ? float2{0.0f, 0.0f} : a.stats[r];
+    const long long token = off ? -1 : a.tokens[r];
+#pragma unroll
+    for (int i0 = 0; i0 < kEach; i0 += kBatch) {
+        const int first = slice * kPieces + i0 * kSliceThreads;
+        if (first >= cut.pieces) break;                                  // (uniform)
+        P held[kBatch];
+        if (!off) {
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) held[i] = reinterpret_cast<const P*>(t + cut.lead)[min(first + i * kSliceThreads + k, cut.pieces - 1)];
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int piece = first + i * kSliceThreads + k, j0 = cut.lead + piece * VEC;
+            if (piece >= cut.pieces) continue;
+            P out{};
+            if (!off) {
+                float d[VEC];
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) d[v] = grad_of((float)held[i].v[v], soft, c);
+                if (token >= j0 && token < j0 + VEC) {
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) d[v] -= token == j0 + v ? c : 0.0f;
+                }
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) out.v[v] = (E)d[v];
+            }
+            reinterpret_cast<P*>(g + cut.lead)[piece] = out;
+        }
+    }
+    if (odd >= 0) g[odd] = off ? (E)0.0f : (E)(grad_of((float)t[odd], soft, c) - (token == odd ? c : 0.0f));
+}
+
+__device__ __forceinline__ float wave_sum(float v) { return group_sum<kWave>(v); }
 
 // log(1 + exp(v))
 __device__ __forceinline__ float softplus(float v) { return fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v))); }
 
-// One wavefront per pair.
-__global__ void __launch_bounds__(kWave)
+// One workgroup per pair.
+constexpr int kPairThreads = 256;
+__global__ void __launch_bounds__(kPairThreads)
 preference_pairs_kernel(const float* __restrict__ logp, PreferenceArgs a, float* __restrict__ pair_loss, float* __restrict__ seq_logp,
                         float* __restrict__ coef, int64_t P, int T) {
+    __shared__ float part[2][kPairThreads / kWave];
     const int64_t p = blockIdx.x;
-    float seq[2];
-    for (int half = 0; half < 2; ++half) {
-        const int64_t q = p + half * P;
-        float s = 0.0f;
-        for (int t = threadIdx.x; t < T; t += kWave) {
-            const float w = row_weight(a.weight, q * T + t);
-            if (w != 0.0f) s = fmaf(w, logp[q * T + t], s);
+    // (logp is 0 where the weight is, so both are requested together)
+    float sum[2] = {0.0f, 0.0f}, seq[2];
+    for (int t = threadIdx.x; t < T; t += kPairThreads)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int64_t e = (p + half * P) * T + t;
+            sum[half] = fmaf(row_weight(a.weight, e), logp[e], sum[half]);
         }
-        seq[half] = wave_sum(s);
-        if (threadIdx.x == 0) seq_logp[q] = seq[half];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const float s = wave_sum(sum[half]);
+        if (threadIdx.x % kWave == 0) part[half][threadIdx.x / kWave] = s;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        seq[half] = part[half][0];
+#pragma unroll
+        for (int i = 1; i < kPairThreads / kWave; ++i) seq[half] += part[half][i];
+        if (threadIdx.x == 0) seq_logp[p + half * P] = seq[half];
     }
     const float m = a.beta * ((seq[0] - a.ref_logp[p]) - (seq[1] - a.ref_logp[p + P]));
     if (threadIdx.x == 0) pair_loss[p] = (1.0f - a.smoothing) * softplus(-m) + a.smoothing * softplus(m);
     const float slope = a.beta / (float)P * (a.smoothing / (1.0f + expf(-m)) - (1.0f - a.smoothing) / (1.0f + expf(m)));
-    for (int half = 0; half < 2; ++half) {
-        const int64_t q = p + half * P;
-        for (int t = threadIdx.x; t < T; t += kWave) coef[q * T + t] = row_weight(a.weight, q * T + t) * (half ? -slope : slope);
-    }
+    for (int t = threadIdx.x; t < T; t += kPairThreads)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int64_t e = (p + half * P) * T + t;
+            coef[e] = row_weight(a.weight, e) * (half ? -slope : slope);
+        }
 }
 
 // total = sum weight loss, or the mean where weight is NULL; one workgroup, so that the order of the sum is fixed.
@@ -162,74 +409,149 @@ loss_total_kernel(const float* __restrict__ loss, const float* __restrict__ weig
 
 }  // namespace
 
-size_t choice_workspace(int64_t rows, int64_t) { return align_up((size_t)rows * sizeof(float)) * 4; }
-
-int launch_time_logp(const void* times, int type, const int64_t* tokens, const float* weight, float* logp, float* stats, int64_t rows,
-                     int64_t J, void*, hipStream_t stream) {
-    with_type(type, [&](auto e) {
-        using E = decltype(e);
-        KernelTimerScope timer_("time_logp", stream);
-        hipLaunchKernelGGL(time_logp_kernel<E>, dim3((unsigned)rows), dim3(kThreads), 0, stream, static_cast<const E*>(times),
-                           reinterpret_cast<const long long*>(tokens), weight, logp, reinterpret_cast<float2*>(stats), (int)J);
-        return 0;
-    });
-    SNNTC_HIP_CHECK(hipGetLastError());
-    return SNNTC_OK;
-}
-
-int launch_time_logp_backward(const void* times, int type, const int64_t* tokens, const float* stats, const float* coef,
-                              const float* upstream, void* dtimes, int64_t rows, int64_t J, hipStream_t stream) {
-    with_type(type, [&](auto e) {
-        using E = decltype(e);
-        KernelTimerScope timer_("time_logp_backward", stream);
-        hipLaunchKernelGGL(time_logp_backward_kernel<E>, dim3((unsigned)rows), dim3(kThreads), 0, stream, static_cast<const E*>(times),
-                           reinterpret_cast<const long long*>(tokens), reinterpret_cast<const float2*>(stats), coef, upstream, static_cast<E*>(dtimes), (int)J);
-        return 0;
-    });
-    SNNTC_HIP_CHECK(hipGetLastError());
-    return SNNTC_OK;
-}
-
 namespace {
-// Row arrays the caller does not want are kept in the workspace.
+
+// Rows of up to so many pieces are held by a workgroup; longer ones are sliced.  Nothing has to be held for a gradient from
+// statistics: there the slices' smaller workgroups serve from 1024 pieces on.
+constexpr int kMostPieces = 16 * 1024;
+template <Mode MODE>
+constexpr int held_pieces() { return MODE == GRAD ? 1024 : kMostPieces; }
+
+template <typename E, int VEC, Mode MODE>
+int launch_rows(const E* times, E* dtimes, const RowArgs& a, hipStream_t stream) {
+    const int pieces = VEC == 1 ? a.J : a.J / VEC;
+    auto launch = [&](auto kern, int width) -> int {
+        const int64_t per = width < 256 ? 256 / width : 1, blocks = (a.rows + per - 1) / per, threads = width < 256 ? 256 : width;
+        if (blocks * threads >= (1ll << 32)) return fail(SNNTC_ERR_TOO_LARGE, "loss: too many long rows");
+        {
+            KernelTimerScope timer_(MODE == LOGP ? "time_logp" : MODE == POLICY ? "policy_loss" : "time_logp_backward", stream);
+            hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3((unsigned)threads), 0, stream, times, dtimes, a);
+        }
+        SNNTC_HIP_CHECK(hipGetLastError());
+        return SNNTC_OK;
+    };
+    if (pieces <= 16) return launch(choice_row_kernel<E, VEC, 16, 1, MODE>, 16);
+    if (pieces <= 64) return launch(choice_row_kernel<E, VEC, 64, 1, MODE>, 64);
+    if constexpr (VEC == 1) {
+        if (pieces <= 1024) return launch(choice_row_kernel<E, 1, 64, 16, MODE>, 64);
+        if constexpr (MODE != GRAD) return launch(choice_row_kernel<E, 1, 1024, 16, MODE>, 1024);
+    } else {
+        if (pieces <= 256) return launch(choice_row_kernel<E, VEC, 64, 4, MODE>, 64);
+        if (pieces <= 1024) return launch(choice_row_kernel<E, VEC, 256, 4, MODE>, 256);
+        if constexpr (MODE != GRAD) {
+            if (pieces <= 2048) return launch(choice_row_kernel<E, VEC, 256, 8, MODE>, 256);
+            if (pieces <= 4096) return launch(choice_row_kernel<E, VEC, 512, 8, MODE>, 512);
+            if (pieces <= 8192) return launch(choice_row_kernel<E, VEC, 1024, 8, MODE>, 1024);
+            return launch(choice_row_kernel<E, VEC, 1024, 16, MODE>, 1024);
+        }
+    }
+    return fail(SNNTC_ERR_UNSUPPORTED, "loss: a row of %d pieces", pieces);
+}
+
+template <typename E, int VEC, Mode MODE>
+int launch_slices(const E* times, E* dtimes, const RowArgs& a, Soft* partial, hipStream_t stream) {
+    const int per = slice_pieces<VEC>(), pieces = a.J / VEC, slices = (pieces + per - 1) / per;
+    const int64_t blocks = a.rows * slices;
+    if (blocks >= (1 << 24)) return fail(SNNTC_ERR_TOO_LARGE, "loss: too many long rows");
+    if constexpr (MODE != GRAD) {
+        {
+            KernelTimerScope timer_("choice_slice", stream);
+            hipLaunchKernelGGL((choice_slice_kernel<E, VEC>), dim3((unsigned)blocks), dim3(kSliceThreads), 0, stream, times, a.weight,
+                               partial, a.J, slices);
+        }
+        KernelTimerScope timer_("choice_join", stream);
+        hipLaunchKernelGGL((choice_join_kernel<E, MODE>), dim3((unsigned)a.rows), dim3(kWave), 0, stream, times, partial, a, slices);
+    }
+    if (MODE == GRAD || (MODE == POLICY && dtimes)) {
+        KernelTimerScope timer_("choice_slice_grad", stream);
+        hipLaunchKernelGGL((choice_slice_grad_kernel<E, VEC>), dim3((unsigned)blocks), dim3(kSliceThreads), 0, stream, times, dtimes, a,
+                           slices);
+    }
+    SNNTC_HIP_CHECK(hipGetLastError());
+    return SNNTC_OK;
+}
+
+// Everything a mode does with the rows.  The statistics and coef that a sliced gradient needs are in `a`.
+template <Mode MODE>
+int launch_choice(const void* times, int type, void* dtimes, const RowArgs& a, Soft* partial, hipStream_t stream) {
+    return with_type(type, [&](auto e) -> int {
+        using E = decltype(e);
+        constexpr int VEC = 16 / sizeof(E);
+        const E* t = static_cast<const E*>(times);
+        E* g = static_cast<E*>(dtimes);
+        // pieces of 16 bytes where times and dtimes lie alike to 16-byte boundaries (and to their own type's)
+        const bool vec = ((uintptr_t)t % sizeof(E)) == 0 && (!g || (((uintptr_t)t ^ (uintptr_t)g) & 15) == 0);
+        if (vec)
+            return a.J / VEC <= held_pieces<MODE>() ? launch_rows<E, VEC, MODE>(t, g, a, stream) : launch_slices<E, VEC, MODE>(t, g, a, partial, stream);
+        return a.J <= held_pieces<MODE>() ? launch_rows<E, 1, MODE>(t, g, a, stream) : launch_slices<E, 1, MODE>(t, g, a, partial, stream);
+    });
+}
+
+// The workspace: row arrays the caller does not want, and the slices' sums.
 struct RowArrays {
     float *logp, *stats, *coef;
-    RowArrays(float* logp_, float* stats_, float* coef_, int64_t rows, void* ws) : logp(logp_), stats(stats_), coef(coef_) {
+    Soft* partial;
+    size_t bytes;
+    RowArrays(float* logp_, float* stats_, float* coef_, int64_t rows, int64_t J, void* ws) : logp(logp_), stats(stats_), coef(coef_) {
         char* scratch = static_cast<char*>(ws);
         const size_t piece = align_up((size_t)rows * sizeof(float));
         if (!coef) coef = reinterpret_cast<float*>(scratch);
         if (!logp) logp = reinterpret_cast<float*>(scratch + piece);
         if (!stats) stats = reinterpret_cast<float*>(scratch + 2 * piece);
+        partial = reinterpret_cast<Soft*>(scratch + 4 * piece);
+        bytes = 4 * piece + (J > kMostPieces ? align_up((size_t)rows * (J / 4096 + 1) * sizeof(Soft)) : 0);
     }
 };
+
+RowArgs row_args(const int64_t* tokens, const float* weight, float* logp, float* stats, float* coef, int64_t rows, int64_t J) {
+    RowArgs a{};
+    a.tokens = reinterpret_cast<const long long*>(tokens);
+    a.weight = weight;
+    a.logp = logp; a.stats = reinterpret_cast<float2*>(stats); a.coef = coef;
+    a.rows = rows; a.J = (int)J;
+    return a;
+}
+
 }  // namespace
 
-int launch_policy_loss(const void* times, int type, const int64_t* actions, const PolicyArgs& a, float* row_loss, float* logp, float* stats,
+size_t choice_workspace(int64_t rows, int64_t J) { return RowArrays(nullptr, nullptr, nullptr, rows, J, nullptr).bytes; }
+
+int launch_time_logp(const void* times, int type, const int64_t* tokens, const float* weight, float* logp, float* stats, int64_t rows,
+                     int64_t J, void* ws, hipStream_t stream) {
+    const RowArrays ra(logp, stats, nullptr, rows, J, ws);
+    return launch_choice<LOGP>(times, type, nullptr, row_args(tokens, weight, logp, stats, nullptr, rows, J), ra.partial, stream);
+}
+
+int launch_time_logp_backward(const void* times, int type, const int64_t* tokens, const float* stats, const float* coef,
+                              const float* upstream, void* dtimes, int64_t rows, int64_t J, hipStream_t stream) {
+    RowArgs a = row_args(tokens, nullptr, nullptr, const_cast<float*>(stats), const_cast<float*>(coef), rows, J);
+    a.upstream = upstream;
+    return launch_choice<GRAD>(times, type, dtimes, a, nullptr, stream);
+}
+
+int launch_policy_loss(const void* times, int type, const int64_t* actions, const PolicyArgs& p, float* row_loss, float* logp, float* stats,
                        float* coef, void* dtimes, int64_t rows, int64_t J, void* ws, hipStream_t stream) {
-    const RowArrays ra(logp, stats, coef, rows, ws);
-    int rc = launch_time_logp(times, type, actions, a.weight, ra.logp, ra.stats, rows, J, ws, stream);
-    if (rc) return rc;
-    {
-        KernelTimerScope timer_("policy_rows", stream);
-        hipLaunchKernelGGL(policy_rows_kernel, dim3((unsigned)((rows + kThreads - 1) / kThreads)), dim3(kThreads), 0, stream, ra.logp, a,
-                           row_loss, ra.coef, rows);
-    }
-    SNNTC_HIP_CHECK(hipGetLastError());
-    return dtimes ? launch_time_logp_backward(times, type, actions, ra.stats, ra.coef, nullptr, dtimes, rows, J, stream) : SNNTC_OK;
+    const RowArrays ra(logp, stats, coef, rows, J, ws);
+    // a row that is sliced is read again for its gradient, which then needs these two
+    const bool sliced = dtimes && J > kMostPieces;
+    RowArgs a = row_args(actions, p.weight, logp, sliced ? ra.stats : stats, sliced ? ra.coef : coef, rows, J);
+    a.row_loss = row_loss;
+    a.policy = p;
+    return launch_choice<POLICY>(times, type, dtimes, a, ra.partial, stream);
 }
 
 int launch_preference_loss(const void* times, int type, const int64_t* tokens, const PreferenceArgs& a, float* pair_loss,
                            float* seq_logp, float* stats, float* coef, void* dtimes, int64_t P, int64_t T, int64_t J, void* ws,
                            hipStream_t stream) {
     const int64_t rows = 2 * P * T;
-    const RowArrays ra(nullptr, stats, coef, rows, ws);
+    const RowArrays ra(nullptr, stats, coef, rows, J, ws);
     int rc = SNNTC_OK;
     if (rows > 0) rc = launch_time_logp(times, type, tokens, a.weight, ra.logp, ra.stats, rows, J, ws, stream);
     if (rc) return rc;
     {
         KernelTimerScope timer_("preference_pairs", stream);
-        hipLaunchKernelGGL(preference_pairs_kernel, dim3((unsigned)P), dim3(kWave), 0, stream, ra.logp, a, pair_loss, seq_logp, ra.coef, P,
-                           (int)T);
+        hipLaunchKernelGGL(preference_pairs_kernel, dim3((unsigned)P), dim3(kPairThreads), 0, stream, ra.logp, a, pair_loss, seq_logp, ra.coef,
+                           P, (int)T);
     }
     SNNTC_HIP_CHECK(hipGetLastError());
     if (!dtimes || rows == 0) return SNNTC_OK;
