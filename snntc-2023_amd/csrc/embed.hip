@@ -37,14 +37,19 @@ __device__ __forceinline__ void load_cols(const E* row, int slice, int lane, int
     }
 }
 
-template <typename E, bool VEC>
+// STREAM: past the caches, for more than they hold.
+template <typename E, bool VEC, bool STREAM = false>
 __device__ __forceinline__ void store_cols(E* row, int slice, int lane, int D, const float (&v)[kCols]) {
     if (VEC) {
         const int d = column<true>(slice, lane, 0);
-        Four<E> f;
+        typedef E Words __attribute__((ext_vector_type(kCols)));
+        Words f;
 #pragma unroll
-        for (int q = 0; q < kCols; ++q) f.v[q] = (E)v[q];
-        if (d < D) *reinterpret_cast<Four<E>*>(row + d) = f;
+        for (int q = 0; q < kCols; ++q) f[q] = (E)v[q];
+        if (d < D) {
+            if (STREAM) __builtin_nontemporal_store(f, reinterpret_cast<Words*>(row + d));
+            else *reinterpret_cast<Words*>(row + d) = f;
+        }
     } else {
 #pragma unroll
         for (int q = 0; q < kCols; ++q) {
@@ -64,7 +69,7 @@ __device__ __forceinline__ float time_of(float e, float scale, bool encode) {
 }
 
 // A wavefront owns 256 columns of TOKENS consecutive tokens and requests their rows together.
-template <typename E, typename I, bool VEC, int TOKENS>
+template <typename E, typename I, bool VEC, int TOKENS, bool STREAM>
 __global__ void __launch_bounds__(256)
 embed_forward_kernel(const I* __restrict__ tokens, const E* __restrict__ table, float* __restrict__ z, int N, int V, int D, int slices,
                      int64_t units, float scale, bool encode) {
@@ -85,7 +90,7 @@ embed_forward_kernel(const I* __restrict__ tokens, const E* __restrict__ table, 
         if (n0 + k >= N) return;
 #pragma unroll
         for (int q = 0; q < kCols; ++q) v[k][q] = known[k] ? time_of(v[k][q], scale, encode) : NAN;
-        store_cols<float, VEC>(z + (size_t)(n0 + k) * D, slice, lane, D, v[k]);
+        store_cols<float, VEC, STREAM>(z + (size_t)(n0 + k) * D, slice, lane, D, v[k]);
     }
 }
 
@@ -514,6 +519,10 @@ int sort_tokens(const I* tokens, const SortWs& w, int64_t N, int64_t V, void* dt
 
 }  // namespace
 
+// Outputs above this size are stored past the caches, which hold 256 MB: 131072 x 1024 (537 MB) and its gradient 366 -> 327 us; below
+// it, what follows finds them there.
+constexpr int64_t kStreamBytes = 256ll << 20;
+
 int launch_embed_forward(const void* tokens, int token_bytes, const void* table, int type, float* z, int64_t N, int64_t V, int64_t D,
                          float scale, bool encode, hipStream_t stream) {
     const int slices = (int)((D + kSlice - 1) / kSlice);
@@ -522,13 +531,15 @@ int launch_embed_forward(const void* tokens, int token_bytes, const void* table,
     const int64_t units = (N + each - 1) / each * slices, blocks = (units + 3) / 4;
     if (blocks > (1 << 24) - 1) return fail(SNNTC_ERR_TOO_LARGE, "embed: too many rows");
     const bool vec = fours(table, D, type_bytes(type)) && fours(z, D, sizeof(float));
+    const bool stream_out = N * D * (int64_t)sizeof(float) > kStreamBytes;
     with_type(type, [&](auto e) {
         using E = decltype(e);
         KernelTimerScope timer_("embed_forward", stream);
         auto launch = [&](auto i) {
             using I = decltype(i);
-            auto kern = vec ? (each == 4 ? embed_forward_kernel<E, I, true, 4> : embed_forward_kernel<E, I, true, 1>)
-                            : (each == 4 ? embed_forward_kernel<E, I, false, 4> : embed_forward_kernel<E, I, false, 1>);
+            auto kern = !vec ? (each == 4 ? embed_forward_kernel<E, I, false, 4, false> : embed_forward_kernel<E, I, false, 1, false>)
+                        : stream_out ? embed_forward_kernel<E, I, true, 4, true>
+                        : each == 4 ? embed_forward_kernel<E, I, true, 4, false> : embed_forward_kernel<E, I, true, 1, false>;
             hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), 0, stream, static_cast<const I*>(tokens),
                                static_cast<const E*>(table), z, (int)N, (int)V, (int)D, slices, units, scale, encode);
         };
