@@ -31,11 +31,14 @@ __device__ __forceinline__ int length_of(const int64_t* lengths, int64_t b, int6
 // (A, H) of their runs through LDS, every one composes those before its own, and goes through its steps a second time with the
 // right start.  The next tile's loads are under way meanwhile; every value is read once and written once.
 //
-// Where that makes fewer than kFill workgroups, sequences are also cut along time: a first kernel composes (A, H) of each part, and
-// a workgroup starts from the composition of the parts before its own.  The order of composition depends on sizes alone.
+// Where that makes fewer than kFill workgroups of more than kShort tiles, sequences are also cut along time: a first kernel composes
+// (A, H) of each part, and a workgroup starts from the composition of the parts before its own.  The order of composition depends on
+// sizes alone.  Forward + backward in us, sequences whole / cut, 16-bit gates: 4096 steps, 16 groups of 64 channels 104 + 168 / 18 + 24,
+// 128 groups 117 + 190 / 105 + 138, 192 groups 125 + 208 / 157 + 228; 512 steps, 16 groups 16 + 24 / 12 + 14, 128 groups 17 + 25 /
+// 18 + 23; 128 steps, any number 8 + 10 / 12 + 13.
 constexpr int kWaves = 8, kSteps = 8, kTile = kWaves * kSteps;
 constexpr int kThreads = kWaves * kWave;
-constexpr int kFill = 256, kCutFill = 1024;
+constexpr int kFill = 160, kShort = 4, kCutFill = 1024;
 
 struct Map { float A, H; };                         // h -> A h + H
 __device__ __forceinline__ Map then(const Map& first, const Map& second) { return Map{first.A * second.A, fmaf(second.A, first.H, second.H)}; }
@@ -302,7 +305,7 @@ namespace {
 Geometry geometry(int64_t B, int64_t T, int64_t D) {
     Geometry g{(int)B, (int)T, (int)D, (int)((D + kWave - 1) / kWave), 1, 0};
     const int64_t rows = B * g.groups, tiles = (T + kTile - 1) / kTile;
-    if (rows < kFill && tiles > 1) g.parts = (int)std::min(tiles, (kCutFill + rows - 1) / rows);
+    if (rows < kFill && tiles > kShort) g.parts = (int)std::min(tiles, (kCutFill + rows - 1) / rows);
     g.part = (int)((tiles + g.parts - 1) / g.parts * kTile);
     g.parts = T > 0 ? (int)((T + g.part - 1) / g.part) : 1;
     return g;
