@@ -368,9 +368,11 @@ SNNTC_API int snntc_gated_step(const float* x, const void* gate, int gate_type, 
  *   snntc_loss_total          total = sum_i weight[i] loss[i] (weight NULL: the mean), added in a fixed order.
  * Errors: a negative size, a times_type that is none of the above, a NULL required pointer, J = 0 with rows, a clip below 0
  * or a clip_low above 1, smoothing outside [0, 1], a beta or kl_coef that is not finite -> BAD_ARGUMENT; more than 2^24 - 1
- * rows, J above 2^30 -> TOO_LARGE; a workspace below _workspace_bytes (of all rows) -> WORKSPACE.
+ * rows, J above 2^30 -> TOO_LARGE; a workspace below snntc_choice_workspace_bytes (time_logp,
+ * policy_loss; 0 where J <= 16384) or snntc_preference_workspace_bytes -> WORKSPACE.
  * ------------------------------------------------------------------------------------------- */
 SNNTC_API int snntc_choice_workspace_bytes(int64_t rows, int64_t J, size_t* bytes);
+SNNTC_API int snntc_preference_workspace_bytes(int64_t P, int64_t T, int64_t J, size_t* bytes);
 SNNTC_API int snntc_time_logp(const void* times, int times_type, const int64_t* tokens, const float* weight, float* logp,
                     float* stats, int64_t rows, int64_t J, void* workspace, size_t workspace_bytes, void* stream);
 SNNTC_API int snntc_time_logp_backward(const void* times, int times_type, const int64_t* tokens, const float* stats,

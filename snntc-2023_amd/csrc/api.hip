@@ -652,6 +652,20 @@ int snntc_choice_workspace_bytes(int64_t rows, int64_t J, size_t* bytes) {
     return SNNTC_OK;
 }
 
+static int preference_check(int64_t P, int64_t T, int64_t J, int times_type, const char* who) {
+    if (P < 0 || T < 0) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: negative size", who);
+    if (P >= (1 << 24) || T >= (1 << 24)) return fail(SNNTC_ERR_TOO_LARGE, "%s: more than 2^24 - 1 pairs or steps", who);
+    return choice_check(2 * P * T, J, times_type, who);
+}
+
+int snntc_preference_workspace_bytes(int64_t P, int64_t T, int64_t J, size_t* bytes) {
+    const int rc = preference_check(P, T, J, SNNTC_F32, "snntc_preference_workspace_bytes");
+    if (rc) return rc;
+    if (!bytes) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_preference_workspace_bytes: bytes is NULL");
+    *bytes = preference_workspace(2 * P * T, J);
+    return SNNTC_OK;
+}
+
 int snntc_time_logp(const void* times, int times_type, const int64_t* tokens, const float* weight, float* logp, float* stats,
                     int64_t rows, int64_t J, void* workspace, size_t workspace_bytes, void* stream) {
     int rc = choice_check(rows, J, times_type, "snntc_time_logp");
@@ -692,19 +706,16 @@ int snntc_policy_loss(const void* times, int times_type, const int64_t* actions,
 int snntc_preference_loss(const void* times, int times_type, const int64_t* tokens, const float* ref_logp, const float* weight,
                           float beta, float smoothing, float* pair_loss, float* seq_logp, float* stats, float* coef, void* dtimes,
                           int64_t P, int64_t T, int64_t J, void* workspace, size_t workspace_bytes, void* stream) {
-    if (P < 0 || T < 0) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_preference_loss: negative size");
-    if (P > kInt32Max || T > kInt32Max) return fail(SNNTC_ERR_TOO_LARGE, "snntc_preference_loss: too many pairs or steps");
-    const int64_t rows = 2 * P * T;
-    int rc = choice_check(rows, J, times_type, "snntc_preference_loss");
+    int rc = preference_check(P, T, J, times_type, "snntc_preference_loss");
     if (rc) return rc;
+    const int64_t rows = 2 * P * T;
     if (!(smoothing >= 0.0f && smoothing <= 1.0f) || !isfinite(beta))
         return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_preference_loss: beta %g or smoothing %g outside its range", (double)beta,
                     (double)smoothing);
     if (P == 0) return SNNTC_OK;
-    if (P >= (1 << 24)) return fail(SNNTC_ERR_TOO_LARGE, "snntc_preference_loss: more than 2^24 - 1 pairs");
     if (!ref_logp || !pair_loss || !seq_logp || (rows > 0 && (!times || !tokens)))
         return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_preference_loss: null pointer");
-    rc = check_workspace(workspace, workspace_bytes, choice_workspace(rows, J));
+    rc = check_workspace(workspace, workspace_bytes, preference_workspace(rows, J));
     if (rc) return rc;
     const PreferenceArgs a{ref_logp, weight, beta, smoothing};
     return launch_preference_loss(times, times_type, tokens, a, pair_loss, seq_logp, stats, coef, dtimes, P, T, J, workspace,

@@ -58,7 +58,8 @@ using torch::autograd::variable_list;
     F(snntc_weight_cost_workspace_bytes) F(snntc_weight_cost_sums) F(snntc_weight_cost_grad) F(snntc_recipe_total)    \
     F(snntc_embed_forward) F(snntc_embed_backward) F(snntc_embed_backward_workspace_bytes)                         \
     F(snntc_gated_scan_forward) F(snntc_gated_scan_backward) F(snntc_gated_scan_workspace_bytes)                   \
-    F(snntc_gated_step) F(snntc_choice_workspace_bytes) F(snntc_time_logp) F(snntc_time_logp_backward)             \
+    F(snntc_gated_step) F(snntc_choice_workspace_bytes) F(snntc_preference_workspace_bytes) F(snntc_time_logp)     \
+    F(snntc_time_logp_backward)                                                                                    \
     F(snntc_policy_loss) F(snntc_preference_loss) F(snntc_loss_total)
 
 struct Library {
@@ -390,11 +391,14 @@ GatedArgs gated_args(const Tensor& x_in, const Tensor& gate_in, const Tensor& st
 
 struct Scanned { Tensor y, final; };
 
+// (Undefined where the sequences need none.)
 Tensor gated_scratch(const GatedArgs& a) {
     size_t need = 0;
     check(lib.snntc_gated_scan_workspace_bytes(a.x.size(0), a.x.size(1), a.x.size(2), &need));
-    return scratch(a.x, need);
+    return need ? scratch(a.x, need) : Tensor();
 }
+
+size_t bytes_of(const Tensor& t) { return t.defined() ? (size_t)t.numel() : 0; }
 
 Scanned gated_scan(const GatedArgs& a) {
     const c10::DeviceGuard guard(a.x.device());
@@ -402,7 +406,7 @@ Scanned gated_scan(const GatedArgs& a) {
     const Tensor ws = gated_scratch(a);
     Scanned r{empty(a.x, a.x.sizes()), empty(a.x, {B, D})};
     check(lib.snntc_gated_scan_forward(f32(a.x), raw(a.gate), float_type(a.gate), f32(a.state), i64(a.lengths), f32(r.y), f32(r.final), B,
-                                       T, D, ws.data_ptr(), ws.numel(), stream_of(a.x)));
+                                       T, D, raw(ws), bytes_of(ws), stream_of(a.x)));
     return r;
 }
 
@@ -421,8 +425,7 @@ ScanGrads gated_scan_grad(const Tensor& dy_in, const Tensor& dfinal_in, const Ga
     if (want_dgate) g.dgate = empty(a.gate, a.x.sizes());
     if (want_dstate) g.dstate = empty(a.x, {B, D});
     check(lib.snntc_gated_scan_backward(f32(dy), f32(dfinal), f32(a.x), raw(a.gate), float_type(a.gate), f32(y), f32(a.state),
-                                        i64(a.lengths), f32(g.dx), raw(g.dgate), f32(g.dstate), B, T, D, ws.data_ptr(), ws.numel(),
-                                        stream_of(a.x)));
+                                        i64(a.lengths), f32(g.dx), raw(g.dgate), f32(g.dstate), B, T, D, raw(ws), bytes_of(ws), stream_of(a.x)));
     return g;
 }
 
@@ -459,17 +462,18 @@ ChoiceArgs choice_args(const Tensor& times, const Tensor& tokens, const Tensor& 
 
 Tensor row_floats(const ChoiceArgs& a, at::IntArrayRef sizes) { return at::empty(sizes, a.times.options().dtype(at::kFloat)); }
 
+// (Undefined where the rows need none.)
 Tensor choice_scratch(const ChoiceArgs& a) {
     size_t need = 0;
     check(lib.snntc_choice_workspace_bytes(a.rows, a.J, &need));
-    return scratch(a.times, need);
+    return need ? scratch(a.times, need) : Tensor();
 }
 
 Tensor time_logp(const ChoiceArgs& a) {
     const c10::DeviceGuard guard(a.times.device());
     const Tensor ws = choice_scratch(a), logp = row_floats(a, a.tokens.sizes());
     check(lib.snntc_time_logp(raw(a.times), float_type(a.times), i64(a.tokens), f32(a.weight), f32(logp), nullptr, a.rows, a.J,
-                              ws.data_ptr(), ws.numel(), stream_of(a.times)));
+                              raw(ws), bytes_of(ws), stream_of(a.times)));
     return logp;
 }
 
@@ -490,7 +494,7 @@ ChoiceOut policy_loss(const ChoiceArgs& a, const PolicyIn& p, bool want_grad, bo
     if (save) { r.stats = row_floats(a, {a.rows, 2}); r.coef = row_floats(a, {a.rows}); }
     check(lib.snntc_policy_loss(raw(a.times), float_type(a.times), i64(a.tokens), f32(old_logp), f32(advantage), f32(ref), f32(a.weight),
                                 p.low, p.high, p.kl, f32(r.loss), f32(r.logp), f32(r.stats), f32(r.coef), raw(r.dtimes), a.rows, a.J,
-                                ws.data_ptr(), ws.numel(), stream_of(a.times)));
+                                raw(ws), bytes_of(ws), stream_of(a.times)));
     return r;
 }
 
@@ -499,7 +503,10 @@ ChoiceOut preference_loss(const ChoiceArgs& a, const Tensor& ref_in, float beta,
     TORCH_CHECK_VALUE(a.tokens.dim() == 2 && a.tokens.size(0) % 2 == 0, "tokens must be [2 pairs, steps], got shape ", shape_text(a.tokens));
     TORCH_CHECK_VALUE(ref_in.defined(), "ref_logp is required");
     const int64_t P = a.tokens.size(0) / 2, T = a.tokens.size(1);
-    const Tensor ref = f32_like(ref_in, a.times, {2 * P}, "ref_logp"), ws = choice_scratch(a);
+    const Tensor ref = f32_like(ref_in, a.times, {2 * P}, "ref_logp");
+    size_t need = 0;
+    check(lib.snntc_preference_workspace_bytes(P, T, a.J, &need));
+    const Tensor ws = scratch(a.times, need);
     ChoiceOut r{row_floats(a, {P}), row_floats(a, {2 * P}), Tensor(), Tensor(), Tensor()};
     if (want_grad) r.dtimes = empty(a.times, a.times.sizes());
     if (save) { r.stats = row_floats(a, {a.rows, 2}); r.coef = row_floats(a, {a.rows}); }

@@ -215,8 +215,8 @@ choice_row_kernel(const E* __restrict__ times, E* __restrict__ dtimes, RowArgs a
     if (odd >= 0) g[odd] = (E)(grad_of(single, soft, c) - (token == odd ? c : 0.0f));
 }
 
-// Rows longer than a workgroup holds: slices of kSlicePieces pieces, a workgroup each.  One pass leaves (maximum, sum) of every slice, the
-// next joins those of a row in order, the third reads the row again for its gradient.
+// Rows longer than a workgroup holds: slices of slice_pieces() pieces, a workgroup each.  One pass leaves (maximum, sum) of every slice; what
+// follows joins those of a row in order and reads the row again for its gradient.
 constexpr int kSliceThreads = 256;
 template <int VEC>
 constexpr int slice_pieces() { return VEC == 1 ? 4096 : 1024; }          // 16 KiB of float32, 8 or 16 of 16-bit times
@@ -269,36 +269,47 @@ choice_slice_kernel(const E* __restrict__ times, const float* __restrict__ weigh
     partial[r * slices + slice] = all;
 }
 
+// A wavefront joins the slices of row r: its statistics, log-probability, loss and derivative (0 for a row of weight 0).
+struct Joined { float2 soft; float lp, loss, coef; };
+template <typename E, Mode MODE>
+__device__ __forceinline__ Joined join_slices(const E* times, const Soft* partial, const RowArgs& a, int64_t r, int slices, int lane) {
+    Joined out{float2{0.0f, 0.0f}, 0.0f, 0.0f, 0.0f};
+    const float w = MODE == POLICY && !a.weight ? a.policy.mean : row_weight(a.weight, r);
+    if (w == 0.0f) return out;
+    const long long token = a.tokens[r];
+    const float chosen = token >= 0 && token < a.J ? (float)times[(size_t)r * a.J + token] : NAN;
+    Soft all{-INFINITY, 0.0f};
+    for (int i = lane; i < slices; i += kWave) all = join(all, partial[r * slices + i]);
+    const float m = group_max<kWave>(all.m);
+    all = Soft{m, group_sum<kWave>(m == -INFINITY ? all.s : all.s * exp_fast(all.m - m))};
+    out.soft = float2{all.m, logf(all.s)};
+    out.lp = (-chosen - out.soft.x) - out.soft.y;
+    if (MODE == POLICY) {
+        const RowLoss loss = policy_row(a.policy, r, out.lp);
+        out.loss = loss.loss;
+        out.coef = loss.coef * w;
+    }
+    return out;
+}
+template <Mode MODE>
+__device__ __forceinline__ void store_joined(const RowArgs& a, int64_t r, const Joined& j) {
+    if (a.logp) a.logp[r] = j.lp;
+    if (a.stats) a.stats[r] = j.soft;
+    if (MODE == POLICY) a.row_loss[r] = j.loss;
+    if (MODE == POLICY && a.coef) a.coef[r] = j.coef;
+}
+
 template <typename E, Mode MODE>
 __global__ void __launch_bounds__(kWave)
 choice_join_kernel(const E* __restrict__ times, const Soft* __restrict__ partial, RowArgs a, int slices) {
-    const int64_t r = blockIdx.x;
-    const int lane = threadIdx.x;
-    const float w = MODE == POLICY && !a.weight ? a.policy.mean : row_weight(a.weight, r);
-    Soft all{-INFINITY, 0.0f};
-    float2 soft{0.0f, 0.0f};
-    float lp = 0.0f;
-    RowLoss loss{0.0f, 0.0f};
-    if (w != 0.0f) {
-        for (int i = lane; i < slices; i += kWave) all = join(all, partial[r * slices + i]);
-        const float m = group_max<kWave>(all.m);
-        all = Soft{m, group_sum<kWave>(m == -INFINITY ? all.s : all.s * exp_fast(all.m - m))};
-        soft = float2{all.m, logf(all.s)};
-        const long long token = a.tokens[r];
-        const float chosen = token >= 0 && token < a.J ? (float)times[(size_t)r * a.J + token] : NAN;
-        lp = (-chosen - soft.x) - soft.y;
-        if (MODE == POLICY) loss = policy_row(a.policy, r, lp);
-    }
-    if (lane != 0) return;
-    if (a.logp) a.logp[r] = lp;
-    if (a.stats) a.stats[r] = soft;
-    if (MODE == POLICY) a.row_loss[r] = loss.loss;
-    if (MODE == POLICY && a.coef) a.coef[r] = loss.coef * w;
+    const Joined j = join_slices<E, MODE>(times, partial, a, blockIdx.x, slices, threadIdx.x);
+    if (threadIdx.x == 0) store_joined<MODE>(a, blockIdx.x, j);
 }
 
-template <typename E, int VEC>
+// POLICY: every workgroup of a row joins its slices by itself, which is a load per lane, instead of waiting for a kernel that does.
+template <typename E, int VEC, Mode MODE>
 __global__ void __launch_bounds__(kSliceThreads)
-choice_slice_grad_kernel(const E* __restrict__ times, E* __restrict__ dtimes, RowArgs a, int slices) {
+choice_slice_grad_kernel(const E* __restrict__ times, E* __restrict__ dtimes, const Soft* __restrict__ partial, RowArgs a, int slices) {
     using P = Piece<E, VEC>;
     constexpr int kPieces = slice_pieces<VEC>(), kEach = kPieces / kSliceThreads, kBatch = 4;
     const int64_t block = gridDim.x - 1 - blockIdx.x;                    // (what was read last comes first)
@@ -308,10 +319,26 @@ choice_slice_grad_kernel(const E* __restrict__ times, E* __restrict__ dtimes, Ro
     E* __restrict__ g = dtimes + (size_t)r * a.J;
     const Cut cut = cut_row<E, VEC>(t, a.J);
     const int odd = slice == 0 ? odd_element<VEC>(cut, k) : -1;
-    float c = a.coef[r];
+    float c;
+    float2 soft;
+    if (MODE == POLICY) {
+        __shared__ float shared[3];
+        if (k < kWave) {
+            const Joined j = join_slices<E, MODE>(times, partial, a, r, slices, k);
+            if (k == 0) {
+                shared[0] = j.coef; shared[1] = j.soft.x; shared[2] = j.soft.y;
+                if (slice == 0) store_joined<MODE>(a, r, j);
+            }
+        }
+        __syncthreads();
+        c = shared[0];
+        soft = float2{shared[1], shared[2]};
+    } else {
+        c = a.coef[r];
+        soft = a.stats[r];
+    }
     const bool off = c == 0.0f;
-    if (a.upstream) c *= *a.upstream;
-    const float2 soft = off ? float2{0.0f, 0.0f} : a.stats[r];
+    if (MODE == GRAD && a.upstream) c *= *a.upstream;
     const long long token = off ? -1 : a.tokens[r];
 #pragma unroll
     for (int i0 = 0; i0 < kEach; i0 += kBatch) {
@@ -411,11 +438,18 @@ loss_total_kernel(const float* __restrict__ loss, const float* __restrict__ weig
 
 namespace {
 
-// Rows of up to so many pieces are held by a workgroup; longer ones are sliced.  Nothing has to be held for a gradient from
-// statistics: there the slices' smaller workgroups serve from 1024 pieces on.
+// Whether a workgroup holds a row of so many pieces, or it is sliced.  Held with its gradient / sliced, us, 16-bit times: 48000 outputs (6000
+// pieces) 16 rows 10.6 / 12.6, 1024 rows 42 / 51; 96000 outputs (12000 pieces, a CU to a workgroup) 16 rows 16 / 12, 128 rows 20 / 19,
+// 256 rows 24 / 30; 48000 in float32 (12000 pieces) 16 rows 10 / 12, 64 rows 12 / 13, 128 rows 14 / 18; without the gradient 1024 rows
+// 45 / 37.  Nothing has to be held for a gradient from statistics: there the slices'
+// smaller workgroups serve from 1024 pieces on.
 constexpr int kMostPieces = 16 * 1024;
-template <Mode MODE>
-constexpr int held_pieces() { return MODE == GRAD ? 1024 : kMostPieces; }
+template <int VEC, Mode MODE>
+bool held(int pieces, int64_t rows, bool gradient) {
+    if (MODE == GRAD) return pieces <= 1024;
+    if (VEC == 1) return pieces <= kMostPieces;
+    return pieces <= 8192 || (MODE == POLICY && gradient && rows >= (VEC == 4 ? 64 : 192) && pieces <= kMostPieces);
+}
 
 template <typename E, int VEC, Mode MODE>
 int launch_rows(const E* times, E* dtimes, const RowArgs& a, hipStream_t stream) {
@@ -442,7 +476,7 @@ int launch_rows(const E* times, E* dtimes, const RowArgs& a, hipStream_t stream)
             if (pieces <= 2048) return launch(choice_row_kernel<E, VEC, 256, 8, MODE>, 256);
             if (pieces <= 4096) return launch(choice_row_kernel<E, VEC, 512, 8, MODE>, 512);
             if (pieces <= 8192) return launch(choice_row_kernel<E, VEC, 1024, 8, MODE>, 1024);
-            return launch(choice_row_kernel<E, VEC, 1024, 16, MODE>, 1024);
+            if constexpr (MODE == POLICY) return launch(choice_row_kernel<E, VEC, 1024, 16, MODE>, 1024);
         }
     }
     return fail(SNNTC_ERR_UNSUPPORTED, "loss: a row of %d pieces", pieces);
@@ -459,19 +493,23 @@ int launch_slices(const E* times, E* dtimes, const RowArgs& a, Soft* partial, hi
             hipLaunchKernelGGL((choice_slice_kernel<E, VEC>), dim3((unsigned)blocks), dim3(kSliceThreads), 0, stream, times, a.weight,
                                partial, a.J, slices);
         }
-        KernelTimerScope timer_("choice_join", stream);
-        hipLaunchKernelGGL((choice_join_kernel<E, MODE>), dim3((unsigned)a.rows), dim3(kWave), 0, stream, times, partial, a, slices);
+        if (MODE == LOGP || !dtimes) {
+            KernelTimerScope timer_("choice_join", stream);
+            hipLaunchKernelGGL((choice_join_kernel<E, MODE>), dim3((unsigned)a.rows), dim3(kWave), 0, stream, times, partial, a, slices);
+        }
     }
-    if (MODE == GRAD || (MODE == POLICY && dtimes)) {
-        KernelTimerScope timer_("choice_slice_grad", stream);
-        hipLaunchKernelGGL((choice_slice_grad_kernel<E, VEC>), dim3((unsigned)blocks), dim3(kSliceThreads), 0, stream, times, dtimes, a,
-                           slices);
+    if constexpr (MODE != LOGP) {
+        if (dtimes) {
+            KernelTimerScope timer_("choice_slice_grad", stream);
+            hipLaunchKernelGGL((choice_slice_grad_kernel<E, VEC, MODE>), dim3((unsigned)blocks), dim3(kSliceThreads), 0, stream, times,
+                               dtimes, partial, a, slices);
+        }
     }
     SNNTC_HIP_CHECK(hipGetLastError());
     return SNNTC_OK;
 }
 
-// Everything a mode does with the rows.  The statistics and coef that a sliced gradient needs are in `a`.
+// Everything a mode does with the rows.
 template <Mode MODE>
 int launch_choice(const void* times, int type, void* dtimes, const RowArgs& a, Soft* partial, hipStream_t stream) {
     return with_type(type, [&](auto e) -> int {
@@ -482,24 +520,22 @@ int launch_choice(const void* times, int type, void* dtimes, const RowArgs& a, S
         // pieces of 16 bytes where times and dtimes lie alike to 16-byte boundaries (and to their own type's)
         const bool vec = ((uintptr_t)t % sizeof(E)) == 0 && (!g || (((uintptr_t)t ^ (uintptr_t)g) & 15) == 0);
         if (vec)
-            return a.J / VEC <= held_pieces<MODE>() ? launch_rows<E, VEC, MODE>(t, g, a, stream) : launch_slices<E, VEC, MODE>(t, g, a, partial, stream);
-        return a.J <= held_pieces<MODE>() ? launch_rows<E, 1, MODE>(t, g, a, stream) : launch_slices<E, 1, MODE>(t, g, a, partial, stream);
+            return held<VEC, MODE>(a.J / VEC, a.rows, g) ? launch_rows<E, VEC, MODE>(t, g, a, stream) : launch_slices<E, VEC, MODE>(t, g, a, partial, stream);
+        return held<1, MODE>(a.J, a.rows, g) ? launch_rows<E, 1, MODE>(t, g, a, stream) : launch_slices<E, 1, MODE>(t, g, a, partial, stream);
     });
 }
 
-// The workspace: row arrays the caller does not want, and the slices' sums.
+// What the rows of a pair's sequences need between the kernels, where the caller does not want it: in the workspace, before the slices' sums.
 struct RowArrays {
     float *logp, *stats, *coef;
-    Soft* partial;
     size_t bytes;
-    RowArrays(float* logp_, float* stats_, float* coef_, int64_t rows, int64_t J, void* ws) : logp(logp_), stats(stats_), coef(coef_) {
+    RowArrays(float* stats_, float* coef_, int64_t rows, void* ws) : stats(stats_), coef(coef_) {
         char* scratch = static_cast<char*>(ws);
         const size_t piece = align_up((size_t)rows * sizeof(float));
-        if (!coef) coef = reinterpret_cast<float*>(scratch);
-        if (!logp) logp = reinterpret_cast<float*>(scratch + piece);
+        logp = reinterpret_cast<float*>(scratch);
+        if (!coef) coef = reinterpret_cast<float*>(scratch + piece);
         if (!stats) stats = reinterpret_cast<float*>(scratch + 2 * piece);
-        partial = reinterpret_cast<Soft*>(scratch + 4 * piece);
-        bytes = 4 * piece + (J > kMostPieces ? align_up((size_t)rows * (J / 4096 + 1) * sizeof(Soft)) : 0);
+        bytes = 4 * piece;
     }
 };
 
@@ -514,12 +550,13 @@ RowArgs row_args(const int64_t* tokens, const float* weight, float* logp, float*
 
 }  // namespace
 
-size_t choice_workspace(int64_t rows, int64_t J) { return RowArrays(nullptr, nullptr, nullptr, rows, J, nullptr).bytes; }
+// The slices' sums; rows of at most kMostPieces outputs are held whatever their type and alignment.
+size_t choice_workspace(int64_t rows, int64_t J) { return J > kMostPieces ? align_up((size_t)rows * (J / 4096 + 1) * sizeof(Soft)) : 0; }
+size_t preference_workspace(int64_t rows, int64_t J) { return RowArrays(nullptr, nullptr, rows, nullptr).bytes + choice_workspace(rows, J); }
 
 int launch_time_logp(const void* times, int type, const int64_t* tokens, const float* weight, float* logp, float* stats, int64_t rows,
                      int64_t J, void* ws, hipStream_t stream) {
-    const RowArrays ra(logp, stats, nullptr, rows, J, ws);
-    return launch_choice<LOGP>(times, type, nullptr, row_args(tokens, weight, logp, stats, nullptr, rows, J), ra.partial, stream);
+    return launch_choice<LOGP>(times, type, nullptr, row_args(tokens, weight, logp, stats, nullptr, rows, J), static_cast<Soft*>(ws), stream);
 }
 
 int launch_time_logp_backward(const void* times, int type, const int64_t* tokens, const float* stats, const float* coef,
@@ -531,22 +568,20 @@ int launch_time_logp_backward(const void* times, int type, const int64_t* tokens
 
 int launch_policy_loss(const void* times, int type, const int64_t* actions, const PolicyArgs& p, float* row_loss, float* logp, float* stats,
                        float* coef, void* dtimes, int64_t rows, int64_t J, void* ws, hipStream_t stream) {
-    const RowArrays ra(logp, stats, coef, rows, J, ws);
-    // a row that is sliced is read again for its gradient, which then needs these two
-    const bool sliced = dtimes && J > kMostPieces;
-    RowArgs a = row_args(actions, p.weight, logp, sliced ? ra.stats : stats, sliced ? ra.coef : coef, rows, J);
+    RowArgs a = row_args(actions, p.weight, logp, stats, coef, rows, J);
     a.row_loss = row_loss;
     a.policy = p;
-    return launch_choice<POLICY>(times, type, dtimes, a, ra.partial, stream);
+    return launch_choice<POLICY>(times, type, dtimes, a, static_cast<Soft*>(ws), stream);
 }
 
 int launch_preference_loss(const void* times, int type, const int64_t* tokens, const PreferenceArgs& a, float* pair_loss,
                            float* seq_logp, float* stats, float* coef, void* dtimes, int64_t P, int64_t T, int64_t J, void* ws,
                            hipStream_t stream) {
     const int64_t rows = 2 * P * T;
-    const RowArrays ra(nullptr, stats, coef, rows, J, ws);
+    const RowArrays ra(stats, coef, rows, ws);
     int rc = SNNTC_OK;
-    if (rows > 0) rc = launch_time_logp(times, type, tokens, a.weight, ra.logp, ra.stats, rows, J, ws, stream);
+    if (rows > 0)
+        rc = launch_time_logp(times, type, tokens, a.weight, ra.logp, ra.stats, rows, J, static_cast<char*>(ws) + ra.bytes, stream);
     if (rc) return rc;
     {
         KernelTimerScope timer_("preference_pairs", stream);

@@ -312,6 +312,7 @@ struct PreferenceArgs {
     float beta, smoothing;
 };
 size_t choice_workspace(int64_t rows, int64_t J);
+size_t preference_workspace(int64_t rows, int64_t J);
 int launch_time_logp(const void* times, int type, const int64_t* tokens, const float* weight, float* logp, float* stats, int64_t rows,
                      int64_t J, void* ws, hipStream_t stream);
 int launch_time_logp_backward(const void* times, int type, const int64_t* tokens, const float* stats, const float* coef,

@@ -40,7 +40,7 @@ EXPORTS = (
     "snntc_weight_cost_grad", "snntc_recipe_total",
     "snntc_embed_forward", "snntc_embed_backward_workspace_bytes", "snntc_embed_backward",
     "snntc_gated_scan_workspace_bytes", "snntc_gated_scan_forward", "snntc_gated_scan_backward", "snntc_gated_step",
-    "snntc_choice_workspace_bytes", "snntc_time_logp", "snntc_time_logp_backward", "snntc_policy_loss",
+    "snntc_choice_workspace_bytes", "snntc_preference_workspace_bytes", "snntc_time_logp", "snntc_time_logp_backward", "snntc_policy_loss",
     "snntc_preference_loss", "snntc_loss_total",
     "snntc_scan_status", "snntc_debug_set_scan_wait_polls", "snntc_debug_order_tile",
     "snntc_profile_enable", "snntc_profile_collect", "snntc_profile_entry",
@@ -142,6 +142,7 @@ def load():
     lib.snntc_gated_scan_backward.argtypes = [vp, vp, vp, vp, i32, vp, vp, vp, vp, vp, vp, i64, i64, i64, vp, sz, vp]
     lib.snntc_gated_step.argtypes = [vp, vp, i32, vp, vp, i64, vp]
     lib.snntc_choice_workspace_bytes.argtypes = [i64, i64, psz]
+    lib.snntc_preference_workspace_bytes.argtypes = [i64, i64, i64, psz]
     lib.snntc_time_logp.argtypes = [vp, i32, vp, vp, vp, vp, i64, i64, vp, sz, vp]
     lib.snntc_time_logp_backward.argtypes = [vp, i32, vp, vp, vp, vp, vp, i64, i64, vp]
     lib.snntc_policy_loss.argtypes = [vp, i32, vp, vp, vp, vp, vp, f32, f32, f32, vp, vp, vp, vp, vp, i64, i64, vp, sz, vp]

@@ -54,16 +54,19 @@ def test_gated_argument_errors(lib):
 
 def test_choice_argument_errors(lib):
     need = ctypes.c_size_t()
-    assert lib.snntc_choice_workspace_bytes(100, 10, ctypes.byref(need)) == OK and need.value >= 1600
+    assert lib.snntc_choice_workspace_bytes(100, 10, ctypes.byref(need)) == OK and need.value == 0
+    assert lib.snntc_choice_workspace_bytes(100, 200000, ctypes.byref(need)) == OK and need.value >= 100 * 25 * 8
     assert lib.snntc_choice_workspace_bytes(100, 10, None) == BAD
-    f = lambda t=FAKE, ty=0, k=FAKE, lp=FAKE, r=4, j=5, ws=FAKE, have=1 << 20: lib.snntc_time_logp(
+    assert lib.snntc_preference_workspace_bytes(10, 5, 10, ctypes.byref(need)) == OK and need.value >= 1600
+    assert lib.snntc_preference_workspace_bytes(10, 5, 10, None) == lib.snntc_preference_workspace_bytes(-1, 5, 10, ctypes.byref(need)) == BAD
+    f = lambda t=FAKE, ty=0, k=FAKE, lp=FAKE, r=4, j=70000, ws=FAKE, have=1 << 20: lib.snntc_time_logp(
         t, ty, k, None, lp, None, r, j, ws, have, None)
     assert f(t=None) == f(k=None) == f(lp=None) == f(ty=9) == f(r=-1) == f(j=-1) == f(j=0) == BAD
     assert f(r=1 << 24) == f(j=BIG) == TOO_LARGE
     assert f(ws=None) == f(have=16) == WORKSPACE
     assert f(r=0) == f(r=0, j=0) == OK
     p = lambda old=FAKE, adv=FAKE, lo=0.2, hi=0.2, kl=0.0, loss=FAKE, r=4, ws=FAKE: lib.snntc_policy_loss(
-        FAKE, 0, FAKE, old, adv, None, None, lo, hi, kl, loss, None, None, None, None, r, 5, ws, 1 << 20, None)
+        FAKE, 0, FAKE, old, adv, None, None, lo, hi, kl, loss, None, None, None, None, r, 70000, ws, 1 << 20, None)
     assert p(old=None) == p(adv=None) == p(loss=None) == BAD
     nan, inf = float("nan"), float("inf")
     assert p(lo=-0.1) == p(lo=1.5) == p(hi=-0.1) == p(lo=nan) == p(hi=nan) == p(kl=nan) == p(kl=inf) == BAD
