@@ -372,41 +372,53 @@ choice_slice_grad_kernel(const E* __restrict__ times, E* __restrict__ dtimes, co
 }
 
 __device__ __forceinline__ float wave_sum(float v) { return group_sum<kWave>(v); }
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) v += __shfl_xor(v, d, kWave);
+    return v;
+}
 
 // log(1 + exp(v))
-__device__ __forceinline__ float softplus(float v) { return fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v))); }
+__device__ __forceinline__ double softplus(double v) { return fmax(v, 0.0) + log1p(exp(-fabs(v))); }
 
-// One workgroup per pair.
+// One workgroup per pair.  A sequence's log-probability is a sum of hundreds of terms, of which the reference's takes almost all away
+// again: both are held in 64 bits (in 32 the margin of sequences of 512 rows was off by 1e-4 of itself).
 constexpr int kPairThreads = 256;
 __global__ void __launch_bounds__(kPairThreads)
 preference_pairs_kernel(const float* __restrict__ logp, PreferenceArgs a, float* __restrict__ pair_loss, float* __restrict__ seq_logp,
                         float* __restrict__ coef, int64_t P, int T) {
-    __shared__ float part[2][kPairThreads / kWave];
+    __shared__ double part[2][kPairThreads / kWave];
+    __shared__ float shared_slope;
     const int64_t p = blockIdx.x;
     // (logp is 0 where the weight is, so both are requested together)
-    float sum[2] = {0.0f, 0.0f}, seq[2];
+    double sum[2] = {0.0, 0.0};
     for (int t = threadIdx.x; t < T; t += kPairThreads)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const int64_t e = (p + half * P) * T + t;
-            sum[half] = fmaf(row_weight(a.weight, e), logp[e], sum[half]);
+            sum[half] = fma((double)row_weight(a.weight, e), (double)logp[e], sum[half]);
         }
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-        const float s = wave_sum(sum[half]);
+        const double s = wave_sum(sum[half]);
         if (threadIdx.x % kWave == 0) part[half][threadIdx.x / kWave] = s;
     }
     __syncthreads();
+    if (threadIdx.x == 0) {
+        double seq[2];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        seq[half] = part[half][0];
+        for (int half = 0; half < 2; ++half) {
+            seq[half] = part[half][0];
 #pragma unroll
-        for (int i = 1; i < kPairThreads / kWave; ++i) seq[half] += part[half][i];
-        if (threadIdx.x == 0) seq_logp[p + half * P] = seq[half];
+            for (int i = 1; i < kPairThreads / kWave; ++i) seq[half] += part[half][i];
+            seq_logp[p + half * P] = (float)seq[half];
+        }
+        const double e = a.smoothing, m = a.beta * ((seq[0] - a.ref_logp[p]) - (seq[1] - a.ref_logp[p + P]));
+        pair_loss[p] = (float)((1.0 - e) * softplus(-m) + e * softplus(m));
+        shared_slope = (float)(a.beta / (double)P * (e / (1.0 + exp(-m)) - (1.0 - e) / (1.0 + exp(m))));
     }
-    const float m = a.beta * ((seq[0] - a.ref_logp[p]) - (seq[1] - a.ref_logp[p + P]));
-    if (threadIdx.x == 0) pair_loss[p] = (1.0f - a.smoothing) * softplus(-m) + a.smoothing * softplus(m);
-    const float slope = a.beta / (float)P * (a.smoothing / (1.0f + expf(-m)) - (1.0f - a.smoothing) / (1.0f + expf(m)));
+    __syncthreads();
+    const float slope = shared_slope;
     for (int t = threadIdx.x; t < T; t += kPairThreads)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
