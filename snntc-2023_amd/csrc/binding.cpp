@@ -153,6 +153,7 @@ Tensor index_like(const Tensor& t, const Tensor& with, const char* name, bool na
 
 int64_t* i64(const Tensor& t) { return t.defined() ? static_cast<int64_t*>(t.data_ptr()) : nullptr; }
 void* raw(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+size_t bytes_of(const Tensor& t) { return t.defined() ? (size_t)t.numel() : 0; }
 
 void no_gradient(std::initializer_list<std::pair<const Tensor*, const char*>> tensors, const char* who) {
     for (const auto& t : tensors)
@@ -366,9 +367,9 @@ Tensor embed_tokens_grad(const Tensor& grad_in, const EmbedArgs& a) {
     const int64_t N = a.tokens.numel(), V = a.table.size(0), D = a.table.size(1);
     size_t need = 0;
     check(lib.snntc_embed_backward_workspace_bytes(N, V, D, &need));
-    const Tensor ws = scratch(a.table, need), d = empty(a.table, a.table.sizes());
+    const Tensor ws = need ? scratch(a.table, need) : Tensor(), d = empty(a.table, a.table.sizes());
     check(lib.snntc_embed_backward(f32(grad), raw(a.tokens), (int)a.tokens.element_size(), raw(a.table), float_type(a.table), raw(d), N, V,
-                                   D, a.scale, a.encode, ws.data_ptr(), ws.numel(), stream_of(a.table)));
+                                   D, a.scale, a.encode, raw(ws), bytes_of(ws), stream_of(a.table)));
     return d;
 }
 
@@ -397,8 +398,6 @@ Tensor gated_scratch(const GatedArgs& a) {
     check(lib.snntc_gated_scan_workspace_bytes(a.x.size(0), a.x.size(1), a.x.size(2), &need));
     return need ? scratch(a.x, need) : Tensor();
 }
-
-size_t bytes_of(const Tensor& t) { return t.defined() ? (size_t)t.numel() : 0; }
 
 Scanned gated_scan(const GatedArgs& a) {
     const c10::DeviceGuard guard(a.x.device());

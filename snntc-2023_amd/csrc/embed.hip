@@ -37,6 +37,28 @@ __device__ __forceinline__ void load_cols(const E* row, int slice, int lane, int
     }
 }
 
+// The same as they stand in memory.
+template <typename E>
+struct Raw { E v[kCols]; };
+template <typename E, bool VEC>
+__device__ __forceinline__ Raw<E> load_raw(const E* row, int slice, int lane, int D) {
+    Raw<E> r{};
+    if (VEC) {
+        const int d = column<true>(slice, lane, 0);
+        Four<E> f{};
+        if (d < D) f = *reinterpret_cast<const Four<E>*>(row + d);
+#pragma unroll
+        for (int q = 0; q < kCols; ++q) r.v[q] = f.v[q];
+    } else {
+#pragma unroll
+        for (int q = 0; q < kCols; ++q) {
+            const int d = column<false>(slice, lane, q);
+            if (d < D) r.v[q] = row[d];
+        }
+    }
+    return r;
+}
+
 // STREAM: past the caches, for more than they hold.
 template <typename E, bool VEC, bool STREAM = false>
 __device__ __forceinline__ void store_cols(E* row, int slice, int lane, int D, const float (&v)[kCols]) {
@@ -97,9 +119,9 @@ embed_forward_kernel(const I* __restrict__ tokens, const E* __restrict__ table, 
 // ---- gradient ------------------------------------------------------------------------------------
 //
 // 1. The positions are put in the order (token, position).  Up to kRankMost of them by counting, for each, those that come
-//    before it: N^2 compares spread over the whole chip in one launch, 64 in one instruction and one count of its mask (N = 8192:
-//    1.7 us of compares), where a sort that works by passes is several launches.  More go by stable radix passes of at most nine
-//    bits, two launches each.  The same first launch clears dtable: rows of tokens that do not occur stay like that.
+//    before it: N^2 compares spread over the whole chip in one launch, 64 in one instruction and a scalar count of its mask,
+//    where a sort that works by passes is several launches.  8192 positions take 11 us, 16384 33 us.  More go by stable radix
+//    passes of at most nine bits, two launches each: 16384 positions 24 us.  The same first launch clears dtable: rows of tokens that do not occur stay like that.
 // 2. The sorted positions are cut into chunks of equal length, whatever the tokens' frequencies are; a wavefront owns a chunk and
 //    256 columns.  It adds up the rows of each token in order; a token that lies wholly in the chunk is finished there, the
 //    first and last one may reach beyond it and leave partial sums.
@@ -108,7 +130,7 @@ embed_forward_kernel(const I* __restrict__ tokens, const E* __restrict__ table, 
 constexpr int kRankThreads = 1024;
 constexpr int kRankWaves = kRankThreads / kWave;
 constexpr int kRankOwn = 32;                        // positions a workgroup ranks
-constexpr int kRankMost = 16 * kRankThreads;
+constexpr int kRankMost = 12 * kRankThreads;
 
 // Positions whose token lies outside the table count as token V and end up last.
 template <typename I>
@@ -133,8 +155,6 @@ struct ClearArgs {
         if (block == 0 && tail + threadIdx.x < bytes) p[tail + threadIdx.x] = 0;
     }
 };
-__global__ void __launch_bounds__(256) clear_kernel(ClearArgs clear) { clear.run(); }
-
 // A wavefront holds R x 64 tokens, the workgroup all of them; each of its kRankOwn positions is compared with all.  Equal tokens
 // count where their position is lower: a token before the owned positions is held as 2 token, one behind them as 2 token + 1, and
 // both count where they lie below 2 own + 1.  The owned ones among themselves are counted apart.
@@ -145,12 +165,15 @@ token_rank_kernel(const I* __restrict__ tokens, int* __restrict__ sorted_token, 
     __shared__ int part[kRankWaves][kRankOwn];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int n0 = blockIdx.x * kRankOwn;
-    const int own = lane < kRankOwn && n0 + lane < N ? token_key(tokens, n0 + lane, V) : V;
+    const int loaded = token_key(tokens, min(n0 + lane % kRankOwn, N - 1), V);
+    const int own = n0 + lane % kRankOwn < N ? loaded : V;               // (places behind the last position count as behind everything)
     unsigned held[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) held[r] = token_key(tokens, min((wave * R + r) * kWave + lane, N - 1), V);      // all requested together
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const int i = (wave * R + r) * kWave + lane;
-        held[r] = i >= N || (i >= n0 && i < n0 + kRankOwn) ? ~0u : 2u * (unsigned)token_key(tokens, i, V) + (i >= n0);
+        held[r] = i >= N || (i >= n0 && i < n0 + kRankOwn) ? ~0u : 2u * held[r] + (i >= n0);
     }
     int before = 0;
 #pragma unroll 4
@@ -295,20 +318,18 @@ radix_place_kernel(const I* __restrict__ tokens, const int* __restrict__ key, co
 
 constexpr int kBatch = 8;                           // rows requested together
 
-// The finished sum of table row v.
+// The sum s of a table row's gradients becomes the row's own; e: the row's elements, needed where they are encoded.
+__device__ __forceinline__ void finish_row(float scale, bool encode, const float (&e)[kCols], float (&s)[kCols]) {
+#pragma unroll
+    for (int q = 0; q < kCols; ++q) s[q] *= encode ? -scale * expf(1.0f - scale * e[q]) : scale;
+}
 template <typename E, bool VEC>
 __device__ __forceinline__ void store_row(E* dtable, const E* table, int v, int slice, int lane, int D, float scale, bool encode,
-                                          const float (&s)[kCols]) {
-    float g[kCols];
-    if (encode) {
-        load_cols<E, VEC>(table + (size_t)v * D, slice, lane, D, g);
-#pragma unroll
-        for (int q = 0; q < kCols; ++q) g[q] = -scale * expf(1.0f - scale * g[q]) * s[q];
-    } else {
-#pragma unroll
-        for (int q = 0; q < kCols; ++q) g[q] = scale * s[q];
-    }
-    store_cols<E, VEC>(dtable + (size_t)v * D, slice, lane, D, g);
+                                          float (&s)[kCols]) {
+    float e[kCols] = {};
+    if (encode) load_cols<E, VEC>(table + (size_t)v * D, slice, lane, D, e);
+    finish_row(scale, encode, e, s);
+    store_cols<E, VEC>(dtable + (size_t)v * D, slice, lane, D, s);
 }
 
 // partial[chunk][0]: what a chunk adds to the token that began before it; [1]: the token that begins in it and goes on behind it.
@@ -339,10 +360,18 @@ embed_sums_kernel(const float* __restrict__ grad, const int* __restrict__ sorted
         if (rows > 0) request(0);
         for (int k0 = 0; k0 < rows; k0 += kBatch) {
             float v[kBatch][kCols];
+            Raw<E> e[kBatch];
 #pragma unroll
             for (int k = 0; k < kBatch; ++k)
 #pragma unroll
                 for (int q = 0; q < kCols; ++q) v[k][q] = next[k][q];
+            // the table's rows of the tokens that end in this batch, together: one by one, each would cost a trip to memory
+            if (encode) {
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k)
+                    if (k0 + k < rows && (ends >> (k0 + k)) & 1)
+                        e[k] = load_raw<E, VEC>(table + (size_t)__builtin_amdgcn_readlane(token, k0 + k) * D, slice, lane, D);
+            }
             if (k0 + kBatch < rows) request(k0 + kBatch);
 #pragma unroll
             for (int k = 0; k < kBatch; ++k) {
@@ -352,7 +381,13 @@ embed_sums_kernel(const float* __restrict__ grad, const int* __restrict__ sorted
                 tok = __builtin_amdgcn_readlane(token, k0 + k);
                 if ((ends >> (k0 + k)) & 1) {                            // (uniform)
                     if (head) store_cols<float, VEC>(partial + (size_t)c * 2 * D, slice, lane, D, s);
-                    else store_row<E, VEC>(dtable, table, tok, slice, lane, D, scale, encode, s);
+                    else {
+                        float row_of[kCols];
+#pragma unroll
+                        for (int q = 0; q < kCols; ++q) row_of[q] = (float)e[k].v[q];
+                        finish_row(scale, encode, row_of, s);
+                        store_cols<E, VEC>(dtable + (size_t)tok * D, slice, lane, D, s);
+                    }
                     head = false;
                     tok = V;
 #pragma unroll
@@ -414,6 +449,55 @@ embed_join_kernel(const float* __restrict__ partial, const int* __restrict__ sor
             store_row<E, VEC>(dtable, table, tok, slice, lane, D, scale, encode, s);
         }
         __syncthreads();
+    }
+}
+
+// Few positions: no order has to be made, and one launch does it all.  Every wavefront holds all tokens (lane k: positions k, k + 64, ...)
+// and walks over its share of the table's rows: a compare gives the mask of a row's positions, an empty one clears it, else they
+// are added from the lowest on.  (100 rows of 958 columns, 33 positions: 8 us where sorting, adding and joining take 14.)
+constexpr int kFewHeld = 4, kFew = kFewHeld * kWave;
+template <typename E, typename I, bool VEC>
+__global__ void __launch_bounds__(256)
+embed_few_kernel(const float* __restrict__ grad, const I* __restrict__ tokens, const E* __restrict__ table, E* __restrict__ dtable, int N, int V,
+                 int D, int rows, int slices, int64_t units, float scale, bool encode) {
+    const int64_t unit = (int64_t)blockIdx.x * (256 / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    if (unit >= units) return;
+    const int slice = (int)(unit % slices), lane = threadIdx.x % kWave;
+    const int64_t v0 = unit / slices * rows, v1 = min((int64_t)V, v0 + rows);
+    int held[kFewHeld];
+#pragma unroll
+    for (int h = 0; h < kFewHeld; ++h) held[h] = N > 0 ? token_key(tokens, min(h * kWave + lane, N - 1), V) : V;      // (requested together)
+#pragma unroll
+    for (int h = 0; h < kFewHeld; ++h) held[h] = h * kWave + lane < N ? held[h] : V;
+    for (int64_t v = v0; v < v1; ++v) {
+        unsigned long long here[kFewHeld], any = 0;
+#pragma unroll
+        for (int h = 0; h < kFewHeld; ++h) any |= here[h] = __ballot(held[h] == (int)v);
+        float s[kCols] = {0.0f, 0.0f, 0.0f, 0.0f}, e[kCols] = {};
+        if (any) {
+            if (encode) load_cols<E, VEC>(table + (size_t)v * D, slice, lane, D, e);
+#pragma unroll
+            for (int h = 0; h < kFewHeld; ++h) {
+                unsigned long long mask = here[h];
+                while (mask) {
+                    float r[kBatch][kCols];
+                    const int count = min(kBatch, __popcll(mask));
+#pragma unroll
+                    for (int k = 0; k < kBatch; ++k)
+                        if (k < count) {
+                            load_cols<float, VEC>(grad + (size_t)(h * kWave + __ffsll((long long)mask) - 1) * D, slice, lane, D, r[k]);
+                            mask &= mask - 1;
+                        }
+#pragma unroll
+                    for (int k = 0; k < kBatch; ++k)
+                        if (k < count)
+#pragma unroll
+                            for (int q = 0; q < kCols; ++q) s[q] += r[k][q];
+                }
+            }
+            finish_row(scale, encode, e, s);
+        }
+        store_cols<E, VEC>(dtable + (size_t)v * D, slice, lane, D, s);
     }
 }
 
@@ -551,14 +635,33 @@ int launch_embed_forward(const void* tokens, int token_bytes, const void* table,
     return SNNTC_OK;
 }
 
-size_t embed_backward_workspace(int64_t N, int64_t V, int64_t D) { return N > 0 ? SortWs(nullptr, N, V, D).bytes : 0; }
+size_t embed_backward_workspace(int64_t N, int64_t V, int64_t D) { return N > kFew ? SortWs(nullptr, N, V, D).bytes : 0; }
 
 int launch_embed_backward(const float* grad, const void* tokens, int token_bytes, const void* table, int type, void* dtable, int64_t N,
                           int64_t V, int64_t D, float scale, bool encode, void* ws, hipStream_t stream) {
     const int64_t table_bytes = V * D * (int64_t)type_bytes(type);
-    if (N == 0) {
-        KernelTimerScope timer_("embed_clear", stream);
-        hipLaunchKernelGGL(clear_kernel, dim3(1024), dim3(256), 0, stream, ClearArgs{static_cast<char*>(dtable), table_bytes, 0});
+    const size_t element = type_bytes(type);
+    const bool vec = fours(grad, D, sizeof(float)) && fours(dtable, D, element) && (!encode || fours(table, D, element));
+    if (N <= kFew) {
+        // some 8192 wavefronts, each with up to 64 rows
+        const int slices = (int)((D + kSlice - 1) / kSlice);
+        const int rows = (int)std::max<int64_t>(1, std::min<int64_t>(64, V * slices / 8192));
+        const int64_t units = (V + rows - 1) / rows * slices, blocks = (units + 3) / 4;
+        if (blocks > (1 << 24) - 1) return fail(SNNTC_ERR_TOO_LARGE, "embed: too many table elements");
+        with_type(type, [&](auto e) {
+            using E = decltype(e);
+            KernelTimerScope timer_("embed_few", stream);
+            auto launch = [&](auto i) {
+                using I = decltype(i);
+                auto kern = vec ? embed_few_kernel<E, I, true> : embed_few_kernel<E, I, false>;
+                hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), 0, stream, grad, static_cast<const I*>(tokens),
+                                   static_cast<const E*>(table), static_cast<E*>(dtable), (int)N, (int)V, (int)D, rows, slices, units, scale,
+                                   encode);
+            };
+            if (token_bytes == 8) launch(int64_t{});
+            else launch(int32_t{});
+            return 0;
+        });
         SNNTC_HIP_CHECK(hipGetLastError());
         return SNNTC_OK;
     }
@@ -569,8 +672,6 @@ int launch_embed_backward(const float* grad, const void* tokens, int token_bytes
     int rc = token_bytes == 8 ? sort_tokens(static_cast<const int64_t*>(tokens), w, N, V, dtable, table_bytes, stream)
                               : sort_tokens(static_cast<const int32_t*>(tokens), w, N, V, dtable, table_bytes, stream);
     if (rc) return rc;
-    const size_t element = type_bytes(type);
-    const bool vec = fours(grad, D, sizeof(float)) && fours(dtable, D, element) && (!encode || fours(table, D, element));
     with_type(type, [&](auto e) {
         using E = decltype(e);
         {

@@ -46,7 +46,8 @@ def _case(N, V, D, dtype, seed=0, zipf=True, bits=torch.int64):
 
 @pytest.mark.parametrize("bits", [torch.int32, torch.int64])
 @pytest.mark.parametrize("dtype", list(HALF))
-@pytest.mark.parametrize("N,V,D", [(1, 1, 1), (7, 3, 5), (64, 1000, 64), (300, 40, 257), (1025, 2000, 100), (4100, 97, 36)])
+@pytest.mark.parametrize("N,V,D", [(1, 1, 1), (7, 3, 5), (64, 1000, 64), (300, 40, 257), (1025, 2000, 100), (4100, 97, 36), (63, 2, 70), (128, 9, 300),
+                                   (129, 9, 300), (100, 30000, 12), (256, 3, 40), (257, 3, 40)])
 def test_forward_and_gradient(N, V, D, dtype, bits):
     import snntc_amd as snn
     tok, table, grad = _case(N, V, D, dtype, bits=bits)
@@ -59,7 +60,7 @@ def test_forward_and_gradient(N, V, D, dtype, bits):
 
 @pytest.mark.parametrize("N,V,D,dtype", [(20000, 30, 64, torch.float32), (17000, 50000, 33, torch.bfloat16), (40000, 1, 20, torch.float32),
                                          (70001, 300000, 8, torch.float16), (33000, 5000, 300, torch.float32),
-                                         (16384, 700, 12, torch.float32), (16385, 1023, 12, torch.float32), (16385, 1024, 7, torch.float32),
+                                         (12288, 700, 12, torch.float32), (12289, 1023, 12, torch.float32), (16385, 1024, 7, torch.float32),
                                          (20000, 1200000, 4, torch.bfloat16), (600000, 77, 3, torch.float32)])
 def test_many_tokens(N, V, D, dtype):
     """More positions than the short sort takes; tokens that occur tens of thousands of times; tables most of whose rows are unused."""

@@ -23,7 +23,7 @@ def test_embed_argument_errors(lib):
     assert f(v=0) == BAD and b"empty table" in lib.snntc_last_error()
     assert f(n=BIG) == f(v=BIG) == f(d=BIG) == TOO_LARGE
     assert f(n=0) == f(d=0) == f(n=0, v=0) == f(n=0, tok=None, tab=None, z=None) == OK
-    g = lambda gr=FAKE, tok=FAKE, tab=FAKE, out=FAKE, n=4, v=5, d=6, enc=0, ws=FAKE, have=1 << 20: lib.snntc_embed_backward(
+    g = lambda gr=FAKE, tok=FAKE, tab=FAKE, out=FAKE, n=400, v=5, d=6, enc=0, ws=FAKE, have=1 << 20: lib.snntc_embed_backward(
         gr, tok, 8, tab, 0, out, n, v, d, 1.0, enc, ws, have, None)
     assert g(gr=None) == g(tok=None) == g(out=None) == g(tab=None, enc=1) == g(n=-1) == g(v=0) == BAD
     assert g(n=BIG) == TOO_LARGE
