@@ -644,6 +644,8 @@ static int choice_check(int64_t rows, int64_t J, int times_type, const char* who
     return SNNTC_OK;
 }
 
+static bool stats_aligned(const float* stats) { return ((uintptr_t)stats & 7) == 0; }
+
 int snntc_choice_workspace_bytes(int64_t rows, int64_t J, size_t* bytes) {
     const int rc = choice_check(rows, J, SNNTC_F32, "snntc_choice_workspace_bytes");
     if (rc) return rc;
@@ -671,6 +673,7 @@ int snntc_time_logp(const void* times, int times_type, const int64_t* tokens, co
     int rc = choice_check(rows, J, times_type, "snntc_time_logp");
     if (rc || rows == 0) return rc;
     if (!times || !tokens || !logp) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_time_logp: null pointer");
+    if (!stats_aligned(stats)) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_time_logp: stats must be 8-byte aligned");
     rc = check_workspace(workspace, workspace_bytes, choice_workspace(rows, J));
     if (rc) return rc;
     return launch_time_logp(times, times_type, tokens, weight, logp, stats, rows, J, workspace, static_cast<hipStream_t>(stream));
@@ -681,6 +684,7 @@ int snntc_time_logp_backward(const void* times, int times_type, const int64_t* t
     const int rc = choice_check(rows, J, times_type, "snntc_time_logp_backward");
     if (rc || rows == 0) return rc;
     if (!times || !tokens || !stats || !coef || !dtimes) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_time_logp_backward: null pointer");
+    if (!stats_aligned(stats)) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_time_logp_backward: stats must be 8-byte aligned");
     return launch_time_logp_backward(times, times_type, tokens, stats, coef, upstream, dtimes, rows, J, static_cast<hipStream_t>(stream));
 }
 
@@ -696,6 +700,7 @@ int snntc_policy_loss(const void* times, int times_type, const int64_t* actions,
     if (rows == 0) return SNNTC_OK;
     if (!times || !actions || !old_logp || !advantage || !row_loss)
         return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_policy_loss: null pointer");
+    if (!stats_aligned(stats)) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_policy_loss: stats must be 8-byte aligned");
     rc = check_workspace(workspace, workspace_bytes, choice_workspace(rows, J));
     if (rc) return rc;
     const PolicyArgs a{old_logp, advantage, ref_logp, weight, 1.0f - clip_low, 1.0f + clip_high, kl_coef, 1.0f / (float)rows};
@@ -715,6 +720,7 @@ int snntc_preference_loss(const void* times, int times_type, const int64_t* toke
     if (P == 0) return SNNTC_OK;
     if (!ref_logp || !pair_loss || !seq_logp || (rows > 0 && (!times || !tokens)))
         return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_preference_loss: null pointer");
+    if (!stats_aligned(stats)) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_preference_loss: stats must be 8-byte aligned");
     rc = check_workspace(workspace, workspace_bytes, preference_workspace(rows, J));
     if (rc) return rc;
     const PreferenceArgs a{ref_logp, weight, beta, smoothing};

@@ -27,6 +27,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/autograd.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -768,6 +769,15 @@ void sgd_update(const std::vector<Tensor>& ws, const std::vector<Tensor>& gs, fl
 
 // ---- layers and losses over sequences ---------------------------------------------------------------------------------
 
+// Gradients of nodes that can be differentiated once: where a graph of them is built, a pass through it raises.
+variable_list once(variable_list grads, const char* who) {
+    if (!at::GradMode::is_enabled()) return grads;
+    for (Tensor& g : grads)
+        if (g.defined()) g = g.detach().requires_grad_(true);
+    const auto error = std::make_shared<torch::autograd::DelayedError>(std::string(who) + " can be differentiated once only", (int64_t)grads.size());
+    return (*error)(std::move(grads));
+}
+
 struct EmbedNode : public Node {
     SavedVariable tokens, table;
     float scale;
@@ -781,8 +791,12 @@ struct EmbedNode : public Node {
         std::lock_guard<std::mutex> lock(mutex_);
         if (!grads[0].defined() || !task_should_compute_output(0)) return variable_list(1);
         const Tensor tok = tokens.unpack(), tab = table.unpack();
-        at::AutoGradMode no_grad(false);
-        return {embed_tokens_grad(grads[0], embed_args(tok, tab, scale, encode))};
+        variable_list out(1);
+        {
+            at::AutoGradMode no_grad(false);
+            out[0] = embed_tokens_grad(grads[0], embed_args(tok, tab, scale, encode));
+        }
+        return once(std::move(out), "embed_tokens");
     }
 };
 
@@ -814,11 +828,13 @@ struct GatedNode : public Node {
         if (!grads[0].defined() && !grads[1].defined()) return out;
         const Tensor X = x.unpack(), G = gate.unpack(), S = has_state ? state.unpack() : Tensor(),
                      L = has_lengths ? lengths.unpack() : Tensor(), Y = y.unpack();
-        at::AutoGradMode no_grad(false);
-        ScanGrads g = gated_scan_grad(grads[0], grads[1], GatedArgs{X, G, S, L}, Y, task_should_compute_output(0),
-                                      task_should_compute_output(1), has_state && task_should_compute_output(2));
-        out[0] = g.dx; out[1] = g.dgate; out[2] = g.dstate;
-        return out;
+        {
+            at::AutoGradMode no_grad(false);
+            ScanGrads g = gated_scan_grad(grads[0], grads[1], GatedArgs{X, G, S, L}, Y, task_should_compute_output(0),
+                                          task_should_compute_output(1), has_state && task_should_compute_output(2));
+            out[0] = g.dx; out[1] = g.dgate; out[2] = g.dstate;
+        }
+        return once(std::move(out), "gated_scan");
     }
 };
 
@@ -857,12 +873,16 @@ struct ChoiceNode : public Node {
         std::lock_guard<std::mutex> lock(mutex_);
         if (!grads[0].defined() || !task_should_compute_output(0)) return variable_list(1);
         const Tensor t = times.unpack(), k = tokens.unpack(), s = stats.unpack(), c = coef.unpack();
-        at::AutoGradMode no_grad(false);
-        const c10::DeviceGuard guard(t.device());
-        const Tensor up = grads[0].contiguous(), d = empty(t, t.sizes());
-        check(lib.snntc_time_logp_backward(raw(t), float_type(t), i64(k), f32(s), f32(c), f32(up), raw(d), k.numel(), t.size(-1),
-                                           stream_of(t)));
-        return {d};
+        variable_list out(1);
+        {
+            at::AutoGradMode no_grad(false);
+            const c10::DeviceGuard guard(t.device());
+            const Tensor up = grads[0].contiguous();
+            out[0] = empty(t, t.sizes());
+            check(lib.snntc_time_logp_backward(raw(t), float_type(t), i64(k), f32(s), f32(c), f32(up), raw(out[0]), k.numel(), t.size(-1),
+                                               stream_of(t)));
+        }
+        return once(std::move(out), "a loss over choices");
     }
 };
 

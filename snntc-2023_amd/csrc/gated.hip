@@ -361,7 +361,7 @@ int launch_gated_scan_backward(const float* dy, const float* dfinal, const float
 
 int launch_gated_step(const float* x, const void* gate, int type, const float* state, float* out, int64_t n, hipStream_t stream) {
     const int64_t blocks = (n + 255) / 256;
-    if (blocks > 0x7fffffffLL) return fail(SNNTC_ERR_TOO_LARGE, "gated step: too many elements");
+    if (blocks >= (1 << 24)) return fail(SNNTC_ERR_TOO_LARGE, "gated step: 2^32 elements and more");
     with_type(type, [&](auto g) {
         using G = decltype(g);
         KernelTimerScope timer_("gated_step", stream);

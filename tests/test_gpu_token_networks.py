@@ -216,6 +216,19 @@ def test_threads_with_streams_of_their_own():
     assert not failures
 
 
+def test_a_second_derivative_is_refused():
+    import snntc_amd as snn
+    table = torch.rand(9, 4, device=DEV, requires_grad=True)
+    k = torch.tensor([[1, 2], [2, 3]], device=DEV)
+    x = torch.rand(2, 2, 4, device=DEV, requires_grad=True)
+    f = torch.zeros(2, 2, device=DEV)
+    for out, leaf in ((snn.SnnEmbed.apply(k, table), table), (snn.SnnGatedScan.apply(x, x)[0], x),
+                      (snn.policy_loss(x, k, f, f + 1), x), (snn.preference_loss(x, k, f[0]), x)):
+        (g,) = torch.autograd.grad((out * out).sum(), [leaf], create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiated once only"):
+            g.sum().backward()
+
+
 def test_saved_tensor_hooks_inference_mode_and_transforms():
     import snntc_amd as snn
     net = _net()

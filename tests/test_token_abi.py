@@ -49,7 +49,7 @@ def test_gated_argument_errors(lib):
     assert g(dx=None, dg=None, ds=None) == g(ds=None, t=0) == OK
     s = lambda x=FAKE, ga=FAKE, ty=0, out=FAKE, n=4: lib.snntc_gated_step(x, ga, ty, None, out, n, None)
     assert s(x=None) == s(ga=None) == s(ty=3) == s(out=None) == s(n=-1) == BAD
-    assert s(n=0) == OK
+    assert s(n=0) == OK and s(n=BIG) == TOO_LARGE
 
 
 def test_choice_argument_errors(lib):
@@ -78,6 +78,9 @@ def test_choice_argument_errors(lib):
     assert q(P=1 << 20, T=1 << 10) == q(P=BIG, T=0) == q(P=1 << 24, T=0) == TOO_LARGE
     assert q(ws=None) == WORKSPACE and q(P=0) == OK
     b = lambda t=FAKE, s=FAKE, c=FAKE, d=FAKE: lib.snntc_time_logp_backward(t, 0, FAKE, s, c, None, d, 4, 5, None)
+    odd = ctypes.c_void_p(0x1004)
+    assert b(s=odd) == BAD and b"aligned" in lib.snntc_last_error()
+    assert lib.snntc_time_logp(FAKE, 0, FAKE, None, FAKE, odd, 4, 5, None, 0, None) == BAD
     assert b(t=None) == b(s=None) == b(c=None) == b(d=None) == BAD
     assert lib.snntc_loss_total(FAKE, None, None, 3, None) == lib.snntc_loss_total(None, None, FAKE, 3, None) == BAD
     assert lib.snntc_loss_total(FAKE, None, FAKE, -1, None) == BAD
