@@ -87,7 +87,7 @@ inline bool fours(const void* p, int64_t D, size_t element) { return D % kCols =
 // ---- forward -------------------------------------------------------------------------------------
 
 __device__ __forceinline__ float time_of(float e, float scale, bool encode) {
-    return encode ? expf(1.0f - scale * e) : scale * e;
+    return encode ? exp_close(1.0f - scale * e) : scale * e;
 }
 
 // A wavefront owns 256 columns of TOKENS consecutive tokens and requests their rows together.
@@ -321,7 +321,7 @@ constexpr int kBatch = 8;                           // rows requested together
 // The sum s of a table row's gradients becomes the row's own; e: the row's elements, needed where they are encoded.
 __device__ __forceinline__ void finish_row(float scale, bool encode, const float (&e)[kCols], float (&s)[kCols]) {
 #pragma unroll
-    for (int q = 0; q < kCols; ++q) s[q] *= encode ? -scale * expf(1.0f - scale * e[q]) : scale;
+    for (int q = 0; q < kCols; ++q) s[q] *= encode ? -scale * exp_close(1.0f - scale * e[q]) : scale;
 }
 template <typename E, bool VEC>
 __device__ __forceinline__ void store_row(E* dtable, const E* table, int v, int slice, int lane, int D, float scale, bool encode,
@@ -411,9 +411,9 @@ embed_join_kernel(const float* __restrict__ partial, const int* __restrict__ sor
     __shared__ float part[kJoinWaves][kCols][kWave];
     const int c = blockIdx.x, lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int64_t i0 = (int64_t)c * chunk, i1 = i0 + chunk;
-    const int tok = sorted_token[i1];
-    if (tok >= V || sorted_token[i1 - 1] != tok) return;                 // nothing goes on behind this chunk
-    if (i0 > 0 && sorted_token[i0 - 1] == tok) return;                   // it began earlier
+    const int tok = sorted_token[i1], ends = sorted_token[i1 - 1], before = sorted_token[i0 > 0 ? i0 - 1 : 0];
+    if (tok >= V || ends != tok) return;                                 // nothing goes on behind this chunk
+    if (i0 > 0 && before == tok) return;                                 // it began earlier
     int last = c + 1;                                                    // the last chunk that begins with this token
     while (last + 1 < chunks) {
         const int at = last + 1 + lane;
@@ -605,26 +605,26 @@ int sort_tokens(const I* tokens, const SortWs& w, int64_t N, int64_t V, void* dt
 
 }  // namespace
 
-// Outputs above this size are stored past the caches, which hold 256 MB: 131072 x 1024 (537 MB) and its gradient 366 -> 327 us; below
+// Outputs above this size are stored past the caches, which hold 256 MB: 131072 x 1024 (537 MB) and its gradient 366 -> 327 us, 318 with eight rows a wavefront; below
 // it, what follows finds them there.
 constexpr int64_t kStreamBytes = 256ll << 20;
 
 int launch_embed_forward(const void* tokens, int token_bytes, const void* table, int type, float* z, int64_t N, int64_t V, int64_t D,
                          float scale, bool encode, hipStream_t stream) {
     const int slices = (int)((D + kSlice - 1) / kSlice);
-    // four rows in flight a wavefront once that still leaves every SIMD two of them
-    const int each = N * slices >= 8192 ? 4 : 1;
+    // four rows in flight a wavefront once that still leaves every SIMD two of them, eight where they stream past the caches
+    const bool stream_out = N * D * (int64_t)sizeof(float) > kStreamBytes;
+    const bool vec = fours(table, D, type_bytes(type)) && fours(z, D, sizeof(float));
+    const int each = vec && stream_out ? 8 : N * slices >= 8192 ? 4 : 1;
     const int64_t units = (N + each - 1) / each * slices, blocks = (units + 3) / 4;
     if (blocks > (1 << 24) - 1) return fail(SNNTC_ERR_TOO_LARGE, "embed: too many rows");
-    const bool vec = fours(table, D, type_bytes(type)) && fours(z, D, sizeof(float));
-    const bool stream_out = N * D * (int64_t)sizeof(float) > kStreamBytes;
     with_type(type, [&](auto e) {
         using E = decltype(e);
         KernelTimerScope timer_("embed_forward", stream);
         auto launch = [&](auto i) {
             using I = decltype(i);
             auto kern = !vec ? (each == 4 ? embed_forward_kernel<E, I, false, 4, false> : embed_forward_kernel<E, I, false, 1, false>)
-                        : stream_out ? embed_forward_kernel<E, I, true, 4, true>
+                        : each == 8 ? embed_forward_kernel<E, I, true, 8, true>
                         : each == 4 ? embed_forward_kernel<E, I, true, 4, false> : embed_forward_kernel<E, I, true, 1, false>;
             hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), 0, stream, static_cast<const I*>(tokens),
                                static_cast<const E*>(table), z, (int)N, (int)V, (int)D, slices, units, scale, encode);

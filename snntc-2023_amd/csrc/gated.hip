@@ -15,8 +15,8 @@ namespace {
 // is 1 and a below 2e-35, e is held finite.  A NaN stays one.)
 struct Gate { float a, rest; };
 __device__ __forceinline__ Gate gate_of(float g) {
-    const float e = expf(g < -80.0f ? 80.0f : -g);
-    const float a = 1.0f / (1.0f + e);
+    const float e = exp_close(g < -80.0f ? 80.0f : -g);
+    const float a = __builtin_amdgcn_rcpf(1.0f + e);                     // (off by a step at most)
     return Gate{a, e * a};
 }
 
