@@ -89,6 +89,15 @@ __device__ __forceinline__ void forget(P& p) {
         p = __builtin_bit_cast(P, w);
     }
 }
+template <bool STREAM, typename P>
+__device__ __forceinline__ void store_piece(P* to, const P& p) {
+    if constexpr (STREAM) {
+        typedef unsigned Words __attribute__((ext_vector_type(sizeof(P) / sizeof(unsigned))));
+        __builtin_nontemporal_store(__builtin_bit_cast(Words, p), reinterpret_cast<Words*>(to));
+    } else {
+        *to = p;
+    }
+}
 struct Cut { int lead, pieces, tail; };
 template <typename E, int VEC>
 __device__ __forceinline__ Cut cut_row(const E* t, int J) {
@@ -111,7 +120,7 @@ __device__ __forceinline__ float grad_of(float t, const float2& soft, float c) {
 
 // WIDTH threads own a row and hold all of it in registers, so that it is read once: R pieces each, at most WIDTH * R * VEC elements and
 // the odd ones.  Up to 64 threads a row: several rows a workgroup.
-template <typename E, int VEC, int WIDTH, int R, Mode MODE>
+template <typename E, int VEC, int WIDTH, int R, Mode MODE, bool STREAM>
 __global__ void __launch_bounds__(WIDTH < 256 ? 256 : WIDTH)
 choice_row_kernel(const E* __restrict__ times, E* __restrict__ dtimes, RowArgs a) {
     constexpr int kRows = WIDTH < 256 ? 256 / WIDTH : 1, kWaves = WIDTH <= kWave ? 1 : WIDTH / kWave;
@@ -138,7 +147,7 @@ choice_row_kernel(const E* __restrict__ times, E* __restrict__ dtimes, RowArgs a
         if (MODE == LOGP || !dtimes) return;
 #pragma unroll
         for (int i = 0; i < R; ++i)
-            if (i * WIDTH + k < cut.pieces) reinterpret_cast<P*>(g + cut.lead)[i * WIDTH + k] = P{};
+            if (i * WIDTH + k < cut.pieces) store_piece<STREAM>(reinterpret_cast<P*>(g + cut.lead) + i * WIDTH + k, P{});
         if (odd >= 0) g[odd] = (E)0.0f;
         return;
     }
@@ -210,7 +219,7 @@ choice_row_kernel(const E* __restrict__ times, E* __restrict__ dtimes, RowArgs a
         P out;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) out.v[v] = (E)d[v];
-        reinterpret_cast<P*>(g + cut.lead)[i * WIDTH + k] = out;
+        store_piece<STREAM>(reinterpret_cast<P*>(g + cut.lead) + i * WIDTH + k, out);
     }
     if (odd >= 0) g[odd] = (E)(grad_of(single, soft, c) - (token == odd ? c : 0.0f));
 }
@@ -307,7 +316,7 @@ choice_join_kernel(const E* __restrict__ times, const Soft* __restrict__ partial
 }
 
 // POLICY: every workgroup of a row joins its slices by itself, which is a load per lane, instead of waiting for a kernel that does.
-template <typename E, int VEC, Mode MODE>
+template <typename E, int VEC, Mode MODE, bool STREAM>
 __global__ void __launch_bounds__(kSliceThreads)
 choice_slice_grad_kernel(const E* __restrict__ times, E* __restrict__ dtimes, const Soft* __restrict__ partial, RowArgs a, int slices) {
     using P = Piece<E, VEC>;
@@ -365,7 +374,7 @@ choice_slice_grad_kernel(const E* __restrict__ times, E* __restrict__ dtimes, co
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) out.v[v] = (E)d[v];
             }
-            reinterpret_cast<P*>(g + cut.lead)[piece] = out;
+            store_piece<STREAM>(reinterpret_cast<P*>(g + cut.lead) + piece, out);
         }
     }
     if (odd >= 0) g[odd] = off ? (E)0.0f : (E)(grad_of((float)t[odd], soft, c) - (token == odd ? c : 0.0f));
@@ -463,7 +472,7 @@ bool held(int pieces, int64_t rows, bool gradient) {
     return pieces <= 8192 || (MODE == POLICY && gradient && rows >= (VEC == 4 ? 64 : 192) && pieces <= kMostPieces);
 }
 
-template <typename E, int VEC, Mode MODE>
+template <typename E, int VEC, Mode MODE, bool STREAM>
 int launch_rows(const E* times, E* dtimes, const RowArgs& a, hipStream_t stream) {
     const int pieces = VEC == 1 ? a.J : a.J / VEC;
     auto launch = [&](auto kern, int width) -> int {
@@ -476,25 +485,25 @@ int launch_rows(const E* times, E* dtimes, const RowArgs& a, hipStream_t stream)
         SNNTC_HIP_CHECK(hipGetLastError());
         return SNNTC_OK;
     };
-    if (pieces <= 16) return launch(choice_row_kernel<E, VEC, 16, 1, MODE>, 16);
-    if (pieces <= 64) return launch(choice_row_kernel<E, VEC, 64, 1, MODE>, 64);
+    if (pieces <= 16) return launch(choice_row_kernel<E, VEC, 16, 1, MODE, STREAM>, 16);
+    if (pieces <= 64) return launch(choice_row_kernel<E, VEC, 64, 1, MODE, STREAM>, 64);
     if constexpr (VEC == 1) {
-        if (pieces <= 1024) return launch(choice_row_kernel<E, 1, 64, 16, MODE>, 64);
-        if constexpr (MODE != GRAD) return launch(choice_row_kernel<E, 1, 1024, 16, MODE>, 1024);
+        if (pieces <= 1024) return launch(choice_row_kernel<E, 1, 64, 16, MODE, STREAM>, 64);
+        if constexpr (MODE != GRAD) return launch(choice_row_kernel<E, 1, 1024, 16, MODE, STREAM>, 1024);
     } else {
-        if (pieces <= 256) return launch(choice_row_kernel<E, VEC, 64, 4, MODE>, 64);
-        if (pieces <= 1024) return launch(choice_row_kernel<E, VEC, 256, 4, MODE>, 256);
+        if (pieces <= 256) return launch(choice_row_kernel<E, VEC, 64, 4, MODE, STREAM>, 64);
+        if (pieces <= 1024) return launch(choice_row_kernel<E, VEC, 256, 4, MODE, STREAM>, 256);
         if constexpr (MODE != GRAD) {
-            if (pieces <= 2048) return launch(choice_row_kernel<E, VEC, 256, 8, MODE>, 256);
-            if (pieces <= 4096) return launch(choice_row_kernel<E, VEC, 512, 8, MODE>, 512);
-            if (pieces <= 8192) return launch(choice_row_kernel<E, VEC, 1024, 8, MODE>, 1024);
-            if constexpr (MODE == POLICY) return launch(choice_row_kernel<E, VEC, 1024, 16, MODE>, 1024);
+            if (pieces <= 2048) return launch(choice_row_kernel<E, VEC, 256, 8, MODE, STREAM>, 256);
+            if (pieces <= 4096) return launch(choice_row_kernel<E, VEC, 512, 8, MODE, STREAM>, 512);
+            if (pieces <= 8192) return launch(choice_row_kernel<E, VEC, 1024, 8, MODE, STREAM>, 1024);
+            if constexpr (MODE == POLICY) return launch(choice_row_kernel<E, VEC, 1024, 16, MODE, STREAM>, 1024);
         }
     }
     return fail(SNNTC_ERR_UNSUPPORTED, "loss: a row of %d pieces", pieces);
 }
 
-template <typename E, int VEC, Mode MODE>
+template <typename E, int VEC, Mode MODE, bool STREAM>
 int launch_slices(const E* times, E* dtimes, const RowArgs& a, Soft* partial, hipStream_t stream) {
     const int per = slice_pieces<VEC>(), pieces = a.J / VEC, slices = (pieces + per - 1) / per;
     const int64_t blocks = a.rows * slices;
@@ -513,7 +522,7 @@ int launch_slices(const E* times, E* dtimes, const RowArgs& a, Soft* partial, hi
     if constexpr (MODE != LOGP) {
         if (dtimes) {
             KernelTimerScope timer_("choice_slice_grad", stream);
-            hipLaunchKernelGGL((choice_slice_grad_kernel<E, VEC, MODE>), dim3((unsigned)blocks), dim3(kSliceThreads), 0, stream, times,
+            hipLaunchKernelGGL((choice_slice_grad_kernel<E, VEC, MODE, STREAM>), dim3((unsigned)blocks), dim3(kSliceThreads), 0, stream, times,
                                dtimes, partial, a, slices);
         }
     }
@@ -531,9 +540,18 @@ int launch_choice(const void* times, int type, void* dtimes, const RowArgs& a, S
         E* g = static_cast<E*>(dtimes);
         // pieces of 16 bytes where times and dtimes lie alike to 16-byte boundaries (and to their own type's)
         const bool vec = ((uintptr_t)t % sizeof(E)) == 0 && (!g || (((uintptr_t)t ^ (uintptr_t)g) & 15) == 0);
-        if (vec)
-            return held<VEC, MODE>(a.J / VEC, a.rows, g) ? launch_rows<E, VEC, MODE>(t, g, a, stream) : launch_slices<E, VEC, MODE>(t, g, a, partial, stream);
-        return held<1, MODE>(a.J, a.rows, g) ? launch_rows<E, 1, MODE>(t, g, a, stream) : launch_slices<E, 1, MODE>(t, g, a, partial, stream);
+        auto go = [&](auto width, auto past) -> int {
+            constexpr int W = decltype(width)::value;
+            constexpr bool STREAM = decltype(past)::value;
+            return held<W, MODE>(a.J / W, a.rows, g) ? launch_rows<E, W, MODE, STREAM>(t, g, a, stream)
+                                                     : launch_slices<E, W, MODE, STREAM>(t, g, a, partial, stream);
+        };
+        if (!vec) return go(std::integral_constant<int, 1>{}, std::false_type{});
+        if constexpr (MODE != LOGP)
+            // rows of 32000 outputs in 16 bits, times and gradient 300 MB 66 -> 52 us, 500 MB 105 -> 78, 1 GB 199 -> 189; up to 200 MB alike
+            if (g && 2 * a.rows * a.J * (int64_t)sizeof(E) > kStreamBytes)
+                return go(std::integral_constant<int, VEC>{}, std::true_type{});
+        return go(std::integral_constant<int, VEC>{}, std::false_type{});
     });
 }
 

@@ -605,14 +605,11 @@ int sort_tokens(const I* tokens, const SortWs& w, int64_t N, int64_t V, void* dt
 
 }  // namespace
 
-// Outputs above this size are stored past the caches, which hold 256 MB: 131072 x 1024 (537 MB) and its gradient 366 -> 327 us, 318 with eight rows a wavefront; below
-// it, what follows finds them there.
-constexpr int64_t kStreamBytes = 256ll << 20;
-
 int launch_embed_forward(const void* tokens, int token_bytes, const void* table, int type, float* z, int64_t N, int64_t V, int64_t D,
                          float scale, bool encode, hipStream_t stream) {
     const int slices = (int)((D + kSlice - 1) / kSlice);
-    // four rows in flight a wavefront once that still leaves every SIMD two of them, eight where they stream past the caches
+    // four rows in flight a wavefront once that still leaves every SIMD two of them, eight where they stream past the caches (131072 x
+    // 1024 forward and gradient 366 us from the caches, 327 past them, 318 with eight rows)
     const bool stream_out = N * D * (int64_t)sizeof(float) > kStreamBytes;
     const bool vec = fours(table, D, type_bytes(type)) && fours(z, D, sizeof(float));
     const int each = vec && stream_out ? 8 : N * slices >= 8192 ? 4 : 1;

@@ -283,6 +283,10 @@ int with_type(int type, F&& f) {
     }
 }
 
+// Calls that touch more than the caches hold (256 MB, the memory's own included) store their results past them: otherwise what the next
+// kernel reads waits for the write-back of what this one has left.  Smaller calls leave their results where the next kernel finds them.
+constexpr int64_t kStreamBytes = 256ll << 20;
+
 // exp(v) by the hardware's base-2 exponential: v log2(e) is rounded once, and what the rounding and log2(e)'s own have lost is put back to
 // first order, so the result is off by two steps at most (one half-step of t is worth |t| half-steps of 2^t otherwise).  Below 2^-126
 // the result is 0.  About half of the library function's instructions.
