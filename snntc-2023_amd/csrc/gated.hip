@@ -36,8 +36,15 @@ __device__ __forceinline__ int length_of(const int64_t* lengths, int64_t b, int6
 // sizes alone.  Forward + backward in us, sequences whole / cut, 16-bit gates: 4096 steps, 16 groups of 64 channels 104 + 168 / 18 + 24,
 // 128 groups 117 + 190 / 105 + 138, 192 groups 125 + 208 / 157 + 228; 512 steps, 16 groups 16 + 24 / 12 + 14, 128 groups 17 + 25 /
 // 18 + 23; 128 steps, any number 8 + 10 / 12 + 13.
+//
+// Workgroups are dealt to the dies in turn.  Where rows are not whole lines, of the gates either, neighbours go to one die, whose cache then holds the
+// lines that they share: in turn / neighbours together, 24 x 333 x 777 38 / 34 us, 16 x 2530 x 777 258 / 226, 16 x 8434 x 777 941 / 753,
+// 16 x 32768 x 200 1265 / 1128.  Where they do, in turn: 32768 x 1024, cut, 249 / 264, others the same.
+// Calls that touch more than the caches hold store past them, where rows are whole lines (a line stored by two groups has to meet
+// in a cache): 32768 x 1024 270 -> 249, 16 x 1920 x 1024 182 -> 171, 16 x 6400 x 1024 613 -> 600; 16 x 8434 x 777 753 -> 827.
 constexpr int kWaves = 8, kSteps = 8, kTile = kWaves * kSteps;
 constexpr int kThreads = kWaves * kWave;
+constexpr int kDies = 8;
 constexpr int kFill = 160, kShort = 4, kCutFill = 1024;
 
 struct Map { float A, H; };                         // h -> A h + H
@@ -45,21 +52,31 @@ __device__ __forceinline__ Map then(const Map& first, const Map& second) { retur
 
 struct Geometry {
     int B, T, D, groups, parts, part;               // groups of 64 channels, parts of `part` steps (a multiple of kTile)
+    bool shared_lines;                              // between neighbouring groups
 };
+template <bool STREAM, typename E>
+__device__ __forceinline__ void put(E* to, E v) {
+    if constexpr (STREAM) __builtin_nontemporal_store(v, to);
+    else *to = v;
+}
 struct Place {
     int64_t b;
     int d, s, lane, wave;
     bool valid;                                     // lanes behind the last channel repeat it and store nothing
 };
-__device__ __forceinline__ Place place_of(const Geometry& g, int64_t block) {
+__device__ __forceinline__ Place place_of(const Geometry& g) {
+    int block = blockIdx.x;
+    if (g.shared_lines) {
+        const int die = blockIdx.x % kDies, each = gridDim.x / kDies, more = gridDim.x % kDies;
+        block = die * each + min(die, more) + blockIdx.x / kDies;
+    }
     Place p;
     p.lane = threadIdx.x % kWave;
     p.wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int64_t rest = block / g.groups;
-    const int d = (int)(block % g.groups) * kWave + p.lane;
+    const int rest = block / g.groups, d = block % g.groups * kWave + p.lane;
     p.valid = d < g.D;
     p.d = p.valid ? d : g.D - 1;
-    p.s = (int)(rest % g.parts);
+    p.s = rest % g.parts;
     p.b = rest / g.parts;
     return p;
 }
@@ -100,13 +117,13 @@ __device__ __forceinline__ float enter_part(const Map* parts, const Geometry& g,
     return h;
 }
 
-template <typename G>
+template <typename G, bool STREAM>
 __global__ void __launch_bounds__(kThreads)
 gated_scan_forward_kernel(const float* __restrict__ x, const G* __restrict__ gate, const float* __restrict__ state,
                           const int64_t* __restrict__ lengths, float* __restrict__ y, float* __restrict__ final_state,
                           const Map* __restrict__ parts, Geometry g) {
     __shared__ Map maps[2][kWaves][kWave];
-    const Place p = place_of(g, blockIdx.x);
+    const Place p = place_of(g);
     const int t0 = p.s * g.part, t1 = min(g.T, t0 + g.part);
     const int n = min(length_of(lengths, p.b, g.T), t1);                 // steps from n on are not there
     float h = state ? state[p.b * g.D + p.d] : 0.0f;
@@ -130,7 +147,7 @@ gated_scan_forward_kernel(const float* __restrict__ x, const G* __restrict__ gat
         if (tile >= n) {                                                 // (uniform) nothing there any more
 #pragma unroll
             for (int i = 0; i < kSteps; ++i)
-                if (t + i < t1 && p.valid) out[(size_t)(t + i) * g.D] = 0.0f;
+                if (t + i < t1 && p.valid) put<STREAM>(out + (size_t)(t + i) * g.D, 0.0f);
             continue;
         }
         float a[kSteps], b[kSteps];
@@ -152,7 +169,7 @@ gated_scan_forward_kernel(const float* __restrict__ x, const G* __restrict__ gat
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             in = fmaf(a[i], in, b[i]);
-            if (t + i < t1 && p.valid) out[(size_t)(t + i) * g.D] = t + i < n ? in : 0.0f;
+            if (t + i < t1 && p.valid) put<STREAM>(out + (size_t)(t + i) * g.D, t + i < n ? in : 0.0f);
         }
     }
     if (final_state && p.s == g.parts - 1 && p.wave == 0 && p.valid) final_state[p.b * g.D + p.d] = h;
@@ -167,7 +184,7 @@ gated_scan_parts_kernel(const float* __restrict__ x, const G* __restrict__ gate,
     // the grid leaves out the last part on the way: renumbered over parts - 1
     Geometry less = g;
     less.parts = g.parts - 1;
-    Place p = place_of(less, blockIdx.x);
+    Place p = place_of(less);
     if (DOWN) ++p.s;
     const int t0 = p.s * g.part, t1 = min(g.T, t0 + g.part);
     const int n = min(length_of(lengths, p.b, g.T), t1);
@@ -212,14 +229,14 @@ gated_scan_parts_kernel(const float* __restrict__ x, const G* __restrict__ gate,
 }
 
 // The same walk from the end: v_t = a_t u_t, u_t = dy_t + v_{t+1}, v behind the last step = dfinal.
-template <typename G>
+template <typename G, bool STREAM>
 __global__ void __launch_bounds__(kThreads)
 gated_scan_backward_kernel(const float* __restrict__ dy, const float* __restrict__ dfinal, const float* __restrict__ x,
                            const G* __restrict__ gate, const float* __restrict__ y, const float* __restrict__ state,
                            const int64_t* __restrict__ lengths, float* __restrict__ dx, G* __restrict__ dgate, float* __restrict__ dstate,
                            const Map* __restrict__ parts, Geometry g) {
     __shared__ Map maps[2][kWaves][kWave];
-    const Place p = place_of(g, blockIdx.x);
+    const Place p = place_of(g);
     const int t0 = p.s * g.part, t1 = min(g.T, t0 + g.part);
     const int n = min(length_of(lengths, p.b, g.T), t1);
     float v = dfinal ? dfinal[p.b * g.D + p.d] : 0.0f;
@@ -249,8 +266,8 @@ gated_scan_backward_kernel(const float* __restrict__ dy, const float* __restrict
             for (int i = 0; i < kSteps; ++i)
                 if (t + i < t1 && p.valid) {
                     const size_t e = base + (size_t)(t + i) * g.D;
-                    if (dx) dx[e] = 0.0f;
-                    if (dgate) dgate[e] = (G)0.0f;
+                    if (dx) put<STREAM>(dx + e, 0.0f);
+                    if (dgate) put<STREAM>(dgate + e, (G)0.0f);
                 }
             continue;
         }
@@ -282,8 +299,8 @@ gated_scan_backward_kernel(const float* __restrict__ dy, const float* __restrict
             if (t + i < t1 && p.valid) {
                 const bool there = t + i < n;
                 const size_t e = base + (size_t)(t + i) * g.D;
-                if (dx) dx[e] = there ? q[i].rest * u : 0.0f;
-                if (dgate) dgate[e] = (G)(there ? u * lead[i] * (q[i].a * q[i].rest) : 0.0f);
+                if (dx) put<STREAM>(dx + e, there ? q[i].rest * u : 0.0f);
+                if (dgate) put<STREAM>(dgate + e, (G)(there ? u * lead[i] * (q[i].a * q[i].rest) : 0.0f));
             }
         }
     }
@@ -302,8 +319,9 @@ gated_step_kernel(const float* x, const G* gate, const float* state, float* out,
 }  // namespace
 
 namespace {
-Geometry geometry(int64_t B, int64_t T, int64_t D) {
-    Geometry g{(int)B, (int)T, (int)D, (int)((D + kWave - 1) / kWave), 1, 0};
+constexpr int kLine = 128;
+Geometry geometry(int64_t B, int64_t T, int64_t D, int gate_bytes = 4) {
+    Geometry g{(int)B, (int)T, (int)D, (int)((D + kWave - 1) / kWave), 1, 0, D * gate_bytes % kLine != 0};
     const int64_t rows = B * g.groups, tiles = (T + kTile - 1) / kTile;
     if (rows < kFill && tiles > kShort) g.parts = (int)std::min(tiles, (kCutFill + rows - 1) / rows);
     g.part = (int)((tiles + g.parts - 1) / g.parts * kTile);
@@ -319,7 +337,7 @@ size_t gated_scan_workspace(int64_t B, int64_t T, int64_t D) {
 
 int launch_gated_scan_forward(const float* x, const void* gate, int type, const float* state, const int64_t* lengths, float* y,
                               float* final_state, int64_t B, int64_t T, int64_t D, void* ws, hipStream_t stream) {
-    const Geometry g = geometry(B, T, D);
+    const Geometry g = geometry(B, T, D, (int)type_bytes(type));
     const int64_t rows = B * g.groups;
     with_type(type, [&](auto e) {
         using G = decltype(e);
@@ -329,7 +347,8 @@ int launch_gated_scan_forward(const float* x, const void* gate, int type, const 
                                static_cast<const G*>(gate), lengths, static_cast<Map*>(ws), g);
         }
         KernelTimerScope timer_("gated_scan_forward", stream);
-        hipLaunchKernelGGL(gated_scan_forward_kernel<G>, dim3((unsigned)(rows * g.parts)), dim3(kThreads), 0, stream, x,
+        const bool past = B * T * D * (int64_t)(2 * sizeof(float) + sizeof(G)) > kStreamBytes && !g.shared_lines;      // x, y, gates
+        hipLaunchKernelGGL((past ? gated_scan_forward_kernel<G, true> : gated_scan_forward_kernel<G, false>), dim3((unsigned)(rows * g.parts)), dim3(kThreads), 0, stream, x,
                            static_cast<const G*>(gate), state, lengths, y, final_state, static_cast<const Map*>(ws), g);
         return 0;
     });
@@ -340,7 +359,7 @@ int launch_gated_scan_forward(const float* x, const void* gate, int type, const 
 int launch_gated_scan_backward(const float* dy, const float* dfinal, const float* x, const void* gate, int type, const float* y,
                                const float* state, const int64_t* lengths, float* dx, void* dgate, float* dstate, int64_t B, int64_t T,
                                int64_t D, void* ws, hipStream_t stream) {
-    const Geometry g = geometry(B, T, D);
+    const Geometry g = geometry(B, T, D, (int)type_bytes(type));
     const int64_t rows = B * g.groups;
     with_type(type, [&](auto e) {
         using G = decltype(e);
@@ -350,7 +369,8 @@ int launch_gated_scan_backward(const float* dy, const float* dfinal, const float
                                static_cast<const G*>(gate), lengths, static_cast<Map*>(ws), g);
         }
         KernelTimerScope timer_("gated_scan_backward", stream);
-        hipLaunchKernelGGL(gated_scan_backward_kernel<G>, dim3((unsigned)(rows * g.parts)), dim3(kThreads), 0, stream, dy, dfinal, x,
+        const bool past = B * T * D * (int64_t)(4 * sizeof(float) + 2 * sizeof(G)) > kStreamBytes && !g.shared_lines;  // dy, x, y, dx, gates, dgate
+        hipLaunchKernelGGL((past ? gated_scan_backward_kernel<G, true> : gated_scan_backward_kernel<G, false>), dim3((unsigned)(rows * g.parts)), dim3(kThreads), 0, stream, dy, dfinal, x,
                            static_cast<const G*>(gate), y, state, lengths, dx, static_cast<G*>(dgate), dstate, static_cast<const Map*>(ws),
                            g);
         return 0;
