@@ -81,7 +81,8 @@ def _policy_reference(times, tokens, old, adv, ref, weight, kl=KL):
     return (loss * on, lt * on), (logp * on, tol * on), (g, gt), (loss * w).sum()
 
 
-def _check_policy(times, tokens, old, adv, ref, weight):
+def _check_policy(times, tokens, old, adv, ref, weight, same=True):
+    """same: one workgroup owns a row with and without its gradient, or several do, so that the losses are equal to the last digit."""
     import snntc_amd as snn
     dev = [None if v is None else v.to(DEV) for v in (times, tokens, old, adv, ref, weight)]
     loss, logp, grad = snn.policy_time_loss(*dev[:4], ref_logp=dev[4], weight=dev[5], clip=CLIP, kl_coef=KL)
@@ -98,7 +99,11 @@ def _check_policy(times, tokens, old, adv, ref, weight):
     (g2,) = torch.autograd.grad(objective, [leaf], torch.tensor(-0.5, device=DEV))
     _close(g2, -0.5 * wg[0], 0.5 * wg[1] + TINY[times.dtype] + HALF[times.dtype] * wg[0].abs(), "gradient through autograd")
     quiet = snn.policy_time_loss(*dev[:4], ref_logp=dev[4], weight=dev[5], clip=CLIP, kl_coef=KL, want_grad=False)
-    assert quiet[2] is None and torch.equal(quiet[0], loss) and torch.equal(quiet[1], logp)
+    assert quiet[2] is None
+    if same:
+        assert torch.equal(quiet[0], loss) and torch.equal(quiet[1], logp)
+    _close(quiet[1], *wp, "logp without the gradient")
+    _close(quiet[0], *wl, "loss without the gradient")
 
 
 @pytest.mark.parametrize("dtype", list(HALF))
@@ -119,6 +124,50 @@ def test_policy_of_long_rows_and_many_rows(rows, J, dtype):
     times, tokens, gen = _case(rows, J, dtype, spread=20.0)
     old, adv, ref = _policy_inputs(times, tokens, gen)
     _check_policy(times, tokens, old, adv, ref, None)
+
+
+@pytest.mark.parametrize("rows,J,dtype", [((64,), 32801, torch.float32), ((70,), 65536, torch.float32), ((192,), 65551, torch.float16),
+                                          ((200,), 131072, torch.bfloat16)])
+def test_long_rows_held_for_their_gradient(rows, J, dtype):
+    """More than 8192 pieces of 16 bytes, in enough rows that one workgroup keeps each."""
+    times, tokens, gen = _case(rows, J, dtype, spread=20.0)
+    old, adv, ref = _policy_inputs(times, tokens, gen)
+    _check_policy(times, tokens, old, adv, ref, None, same=False)
+
+
+@pytest.mark.parametrize("J", [50, 251, 1003, 4001, 8005, 16001, 32003, 60001, 70001])
+def test_gradients_larger_than_the_caches(J):
+    """Rows do not know how many there are: both halves of a batch whose times and gradient are more than 256 MB, by themselves."""
+    import snntc_amd as snn
+    rows = 2 ** 25 // J + 2
+    gen = torch.Generator(device=DEV).manual_seed(J)
+    times = 1.0 + 8.0 * torch.rand(rows, J, generator=gen, device=DEV)
+    tokens = torch.randint(0, J, (rows,), generator=gen, device=DEV)
+    old, adv = torch.full((rows,), -math.log(J), device=DEV), torch.randn(rows, generator=gen, device=DEV)
+    weight = (torch.rand(rows, generator=gen, device=DEV) - 0.2).clamp(min=0.0)
+    whole = snn.policy_time_loss(times, tokens, old, adv, weight=weight)
+    cut = rows // 8 * 4                                         # (4 J elements are whole pieces of 16 bytes: rows lie to those as they did)
+    for part in (slice(0, cut), slice(cut, rows)):
+        half = snn.policy_time_loss(times[part].clone(), tokens[part], old[part], adv[part], weight=weight[part])
+        assert all(torch.equal(w[part], h) for w, h in zip(whole, half))
+
+
+@pytest.mark.parametrize("J", [50, 251, 1003, 4001, 9001])
+def test_preference_gradients_larger_than_the_caches(J):
+    """Two pairs of long sequences and each by itself, where the mean over pairs makes its gradient twice as large."""
+    import snntc_amd as snn
+    T = 2 ** 23 // J // 4 * 4 + 4
+    gen = torch.Generator(device=DEV).manual_seed(J)
+    times = 1.0 + 8.0 * torch.rand(4, T, J, generator=gen, device=DEV)
+    tokens = torch.randint(0, J, (4, T), generator=gen, device=DEV)
+    ref = snn.time_logp(times, tokens).double().sum(1).float()[[2, 3, 0, 1]]
+    weight = (torch.rand(4, T, generator=gen, device=DEV) < 0.8).float()
+    beta = 1e-3
+    whole = snn.preference_time_loss(times, tokens, ref, weight, beta)
+    for pair in ([0, 2], [1, 3]):
+        one = snn.preference_time_loss(times[pair], tokens[pair], ref[pair], weight[pair], beta)
+        assert torch.equal(2.0 * whole[-1][pair], one[-1])
+        assert torch.equal(whole[0][pair[:1]], one[0])
 
 
 def test_rows_of_weight_zero_are_not_read():

@@ -69,6 +69,18 @@ def test_many_tokens(N, V, D, dtype):
     _close(snn.embed_tokens_grad(grad, tok, table, 0.5, True), *_reference(tok, table, 0.5, True, grad), "dtable")
 
 
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("N,D", [(67111, 1000), (16411, 4100), (67111, 1001)])
+def test_outputs_larger_than_the_caches(N, D, dtype):
+    """Rows do not know how many there are: both halves of an output of more than 256 MB, by themselves."""
+    import snntc_amd as snn
+    tok, table, _ = _case(N, 300, D, dtype)
+    tok[5] = -1
+    z = snn.embed_tokens(tok, table, 0.5, True)
+    for part in (slice(0, N // 2), slice(N // 2, N)):
+        assert torch.equal(z[part].nan_to_num(-1.0), snn.embed_tokens(tok[part], table, 0.5, True).nan_to_num(-1.0))
+
+
 def test_one_token_throughout_and_all_different():
     import snntc_amd as snn
     for tok in (torch.full((5000,), 6), torch.arange(5000), torch.arange(5000).flip(0), torch.arange(5000) // 64, torch.arange(5000) % 2):

@@ -99,6 +99,30 @@ def test_long_sequences(B, T, D, lengths):
     _check(*_case(B, T, D, torch.bfloat16, lengths=lengths))
 
 
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("B,T,D", [(9, 70, 96), (11, 200, 160), (2, 700, 192)])
+def test_rows_of_whole_and_half_lines(B, T, D, dtype):
+    _check(*_case(B, T, D, dtype, lengths="ragged"))
+
+
+@pytest.mark.parametrize("B,T,D", [(1, 24000, 1024), (24, 1000, 1024), (12, 1000, 1024), (3, 4001, 1024), (16, 1600, 992)])
+def test_more_than_the_caches_hold(B, T, D):
+    """Gates of 16-bit values in float32: the same results as from 16 bits, where the call touches less than 256 MB and stores otherwise."""
+    import snntc_amd as snn
+    gen = torch.Generator(device=DEV).manual_seed(T)
+    x = torch.exp(torch.rand(B, T, D, generator=gen, device=DEV))
+    gate = (1.5 + 2.0 * torch.randn(B, T, D, generator=gen, device=DEV)).to(torch.bfloat16)
+    gy = torch.randn(B, T, D, generator=gen, device=DEV)
+    n = torch.full((B,), T - 77, device=DEV)
+    y, final = snn.gated_scan(x, gate, None, n)
+    y32, final32 = snn.gated_scan(x, gate.float(), None, n)
+    assert torch.equal(y, y32) and torch.equal(final, final32)
+    dx, dgate, dstate = snn.gated_scan_grad(gy, None, x, gate, y, None, n)
+    dx32, dgate32, dstate32 = snn.gated_scan_grad(gy, None, x, gate.float(), y, None, n)
+    assert torch.equal(dx, dx32) and torch.equal(dstate, dstate32) and torch.equal(dgate, dgate32.to(torch.bfloat16))
+    assert not y[:, T - 77:].any() and not dx[:, T - 77:].any() and not dgate[:, T - 77:].any()
+
+
 def test_ends_of_the_lengths():
     """Lengths around every place where a sequence may be cut, negative ones and ones beyond T included."""
     x, gate, s, _, gy, gf = _case(40, 600, 8)
