@@ -102,7 +102,7 @@ def policy_step(model, optimizer, inputs, actions, old_logp, advantage, ref_logp
     ref_logp: ops.time_logp of the model that made the choices and of the reference.  Returns the loss."""
     optimizer.zero_grad(set_to_none=True)
     times = model(inputs)
-    loss = policy_loss(times.view(*actions.shape, times.shape[-1]), actions, old_logp, advantage, ref_logp, weight, clip, kl_coef)
+    loss = policy_loss(times.reshape(*actions.shape, times.shape[-1]), actions, old_logp, advantage, ref_logp, weight, clip, kl_coef)
     loss.backward()
     optimizer.step()
     return loss.detach()
@@ -113,7 +113,7 @@ def preference_step(model, optimizer, inputs, tokens, ref_logp, weight=None, bet
     of tokens[2P,T].  ref_logp[2P]: the sequences' log-probabilities under the reference.  Returns the loss."""
     optimizer.zero_grad(set_to_none=True)
     times = model(inputs)
-    loss = preference_loss(times.view(*tokens.shape, times.shape[-1]), tokens, ref_logp, weight, beta, smoothing)
+    loss = preference_loss(times.reshape(*tokens.shape, times.shape[-1]), tokens, ref_logp, weight, beta, smoothing)
     loss.backward()
     optimizer.step()
     return loss.detach()

@@ -77,6 +77,28 @@ def test_preference_training_step_updates_every_weight():
     assert abs(float(loss) + 1.0) < 1e-4                    # ratios of one, advantages of one
 
 
+def test_steps_take_times_of_any_layout():
+    """A model whose times are a view that is no plain block of memory."""
+    from snntc_amd import train
+
+    class Turned(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.times = torch.nn.Parameter(1.0 + torch.rand(20, 6, 30, device=DEV))
+
+        def forward(self, _):
+            return self.times.transpose(0, 1)
+
+    _, act, weight = _batch()
+    for step in (lambda m, o: train.policy_step(m, o, None, act, torch.full((6, 20), -3.0, device=DEV), torch.ones(6, 20, device=DEV)),
+                 lambda m, o: train.preference_step(m, o, None, act, torch.zeros(6, device=DEV), weight)):
+        turned, plain = Turned(), Turned()
+        plain.times = torch.nn.Parameter(turned.times.detach().transpose(0, 1).contiguous())
+        plain.forward = lambda _, m=plain: m.times
+        got, want = (step(m, torch.optim.SGD(m.parameters(), lr=0.1)) for m in (turned, plain))
+        assert torch.equal(got, want) and torch.equal(turned.times.transpose(0, 1), plain.times)
+
+
 def test_sgd_update_takes_the_gradients():
     import snntc_amd as snn
     net = _net()
