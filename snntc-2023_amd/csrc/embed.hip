@@ -90,7 +90,8 @@ __device__ __forceinline__ float time_of(float e, float scale, bool encode) {
     return encode ? exp_close(1.0f - scale * e) : scale * e;
 }
 
-// A wavefront owns 256 columns of TOKENS consecutive tokens and requests their rows together.
+// A wavefront owns 256 columns of TOKENS consecutive tokens and requests their rows together.  Bound by memory: 131072 tokens of 1024
+// columns from a 16-bit table 121 us, 5.35 TB/s; 8192 of 800 from float32 8.8 us, 4.6 TB/s.
 template <typename E, typename I, bool VEC, int TOKENS, bool STREAM>
 __global__ void __launch_bounds__(256)
 embed_forward_kernel(const I* __restrict__ tokens, const E* __restrict__ table, float* __restrict__ z, int N, int V, int D, int slices,
@@ -121,10 +122,11 @@ embed_forward_kernel(const I* __restrict__ tokens, const E* __restrict__ table, 
 // 1. The positions are put in the order (token, position).  Up to kRankMost of them by counting, for each, those that come
 //    before it: N^2 compares spread over the whole chip in one launch, 64 in one instruction and a scalar count of its mask,
 //    where a sort that works by passes is several launches.  8192 positions take 11 us, 16384 33 us.  More go by stable radix
-//    passes of at most nine bits, two launches each: 16384 positions 24 us.  The same first launch clears dtable: rows of tokens that do not occur stay like that.
+//    passes of at most nine bits, two launches each: 16384 positions 24 us.  The same first launch clears dtable (at 6 TB/s): rows of
+//    tokens that do not occur stay like that.
 // 2. The sorted positions are cut into chunks of equal length, whatever the tokens' frequencies are; a wavefront owns a chunk and
 //    256 columns.  It adds up the rows of each token in order; a token that lies wholly in the chunk is finished there, the
-//    first and last one may reach beyond it and leave partial sums.
+//    first and last one may reach beyond it and leave partial sums.  131072 rows of 1024: 624 MB in 151 us, 4.1 TB/s.
 // 3. Partial sums of one token are added in the order of their chunks.
 
 constexpr int kRankThreads = 1024;
