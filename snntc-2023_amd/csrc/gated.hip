@@ -26,7 +26,7 @@ __device__ __forceinline__ int length_of(const int64_t* lengths, int64_t b, int6
     return (int)(n < 0 ? 0 : n > T ? T : n);
 }
 
-// A workgroup owns 64 neighbouring channels of a sequence and walks along it in tiles of kWaves x kSteps steps: each wavefront holds
+// A workgroup owns W (64) neighbouring channels of a sequence and walks along it in tiles of kWaves x kSteps steps: each wavefront holds
 // kSteps of them in registers (lane = channel).  A run of steps maps the state it is given to A h + H, so the wavefronts exchange
 // (A, H) of their runs through LDS, every one composes those before its own, and goes through its steps a second time with the
 // right start.  The next tile's loads are under way meanwhile; every value is read once and written once.  Bound by memory: 32 x 256 x
@@ -36,7 +36,9 @@ __device__ __forceinline__ int length_of(const int64_t* lengths, int64_t b, int6
 // (A, H) of each part, and a workgroup starts from the composition of the parts before its own.  The order of composition depends on
 // sizes alone.  Forward + backward in us, sequences whole / cut, 16-bit gates: 4096 steps, 16 groups of 64 channels 104 + 168 / 18 + 24,
 // 128 groups 117 + 190 / 105 + 138, 192 groups 125 + 208 / 157 + 228; 512 steps, 16 groups 16 + 24 / 12 + 14, 128 groups 17 + 25 /
-// 18 + 23; 128 steps, any number 8 + 10 / 12 + 13.
+// 18 + 23; 128 steps, any number 8 + 10 / 12 + 13.  As few of two to four tiles become groups of 32 channels, each half of a wavefront
+// with eight steps of its own: 256 x 1024 7.6 + 11.3 / 7.1 + 7.8, 8 of them 8.7 + 12.8 / 7.2 + 10.6, 32 x 200 x 200 8.2 + 11.6 / 7.2 + 8.5;
+// 20 x 256 x 500 (160 groups) alike, 32 x 256 x 800 39 / 45.
 //
 // Workgroups are dealt to the dies in turn.  Where rows are not whole lines, of the gates either, neighbours go to one die, whose cache then holds the
 // lines that they share: in turn / neighbours together, 24 x 333 x 777 38 / 34 us, 16 x 2530 x 777 258 / 226, 16 x 8434 x 777 941 / 753,
@@ -46,14 +48,15 @@ __device__ __forceinline__ int length_of(const int64_t* lengths, int64_t b, int6
 constexpr int kWaves = 8, kSteps = 8, kTile = kWaves * kSteps;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kDies = 8;
-constexpr int kFill = 160, kShort = 4, kCutFill = 1024;
+constexpr int kFill = 160, kShort = 4, kCutFill = 1024, kHalf = kWave / 2;
 
 struct Map { float A, H; };                         // h -> A h + H
 __device__ __forceinline__ Map then(const Map& first, const Map& second) { return Map{first.A * second.A, fmaf(second.A, first.H, second.H)}; }
 
 struct Geometry {
-    int B, T, D, groups, parts, part;               // groups of 64 channels, parts of `part` steps (a multiple of kTile)
+    int B, T, D, groups, parts, part;               // groups of 64 (or 32) channels, parts of `part` steps (a multiple of kTile)
     bool shared_lines;                              // between neighbouring groups
+    bool half;                                      // groups of 32
 };
 template <bool STREAM, typename E>
 __device__ __forceinline__ void put(E* to, E v) {
@@ -62,9 +65,10 @@ __device__ __forceinline__ void put(E* to, E v) {
 }
 struct Place {
     int64_t b;
-    int d, s, lane, wave;
+    int d, s, lane, run;                            // run: the wavefront, or half of one where groups are 32 channels
     bool valid;                                     // lanes behind the last channel repeat it and store nothing
 };
+template <int W>
 __device__ __forceinline__ Place place_of(const Geometry& g) {
     int block = blockIdx.x;
     if (g.shared_lines) {
@@ -72,9 +76,9 @@ __device__ __forceinline__ Place place_of(const Geometry& g) {
         block = die * each + min(die, more) + blockIdx.x / kDies;
     }
     Place p;
-    p.lane = threadIdx.x % kWave;
-    p.wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int rest = block / g.groups, d = block % g.groups * kWave + p.lane;
+    p.lane = threadIdx.x % W;
+    p.run = W == kWave ? __builtin_amdgcn_readfirstlane(threadIdx.x / W) : threadIdx.x / W;
+    const int rest = block / g.groups, d = block % g.groups * W + p.lane;
     p.valid = d < g.D;
     p.d = p.valid ? d : g.D - 1;
     p.s = rest % g.parts;
@@ -84,12 +88,13 @@ __device__ __forceinline__ Place place_of(const Geometry& g) {
 
 // Composition of maps[w][lane] over the wavefronts, w ascending (or descending) from the state h: what comes in at wavefront `wave`
 // and what goes out at the end.
-template <bool DOWN>
-__device__ __forceinline__ float through(const Map (*maps)[kWave], const Place& p, float h, float* in) {
+template <bool DOWN, int W>
+__device__ __forceinline__ float through(const Map (*maps)[W], const Place& p, float h, float* in) {
+    constexpr int kRuns = kThreads / W;
 #pragma unroll
-    for (int k = 0; k < kWaves; ++k) {
-        const int w = DOWN ? kWaves - 1 - k : k;
-        if (w == p.wave) *in = h;
+    for (int k = 0; k < kRuns; ++k) {
+        const int w = DOWN ? kRuns - 1 - k : k;
+        if (w == p.run) *in = h;
         const Map m = maps[w][p.lane];
         h = fmaf(m.A, h, m.H);
     }
@@ -102,7 +107,7 @@ __device__ __forceinline__ float enter_part(const Map* parts, const Geometry& g,
     const int count = DOWN ? g.parts - 1 - p.s : p.s;
     if (count == 0) return h;
     const int first = DOWN ? p.s + 1 : 0, per = (count + kWaves - 1) / kWaves;
-    const int r0 = min(count, p.wave * per), r1 = min(count, r0 + per);
+    const int r0 = min(count, p.run * per), r1 = min(count, r0 + per);
     Map m{1.0f, 0.0f};
 #pragma unroll 8
     for (int r = r0; r < r1; ++r) {
@@ -110,25 +115,26 @@ __device__ __forceinline__ float enter_part(const Map* parts, const Geometry& g,
         const Map next = parts[((size_t)p.b * g.parts + first + r) * g.D + p.d];
         m = DOWN ? then(next, m) : then(m, next);
     }
-    maps[p.wave][p.lane] = m;
+    maps[p.run][p.lane] = m;
     __syncthreads();
     float unused;
-    h = through<DOWN>(maps, p, h, &unused);
+    h = through<DOWN, kWave>(maps, p, h, &unused);
     __syncthreads();
     return h;
 }
 
-template <typename G, bool STREAM>
+template <typename G, bool STREAM, int W>
 __global__ void __launch_bounds__(kThreads)
 gated_scan_forward_kernel(const float* __restrict__ x, const G* __restrict__ gate, const float* __restrict__ state,
                           const int64_t* __restrict__ lengths, float* __restrict__ y, float* __restrict__ final_state,
                           const Map* __restrict__ parts, Geometry g) {
-    __shared__ Map maps[2][kWaves][kWave];
-    const Place p = place_of(g);
+    constexpr int kSpan = kThreads / W * kSteps;                         // steps of a tile
+    __shared__ Map maps[2][kThreads / W][W];
+    const Place p = place_of<W>(g);
     const int t0 = p.s * g.part, t1 = min(g.T, t0 + g.part);
     const int n = min(length_of(lengths, p.b, g.T), t1);                 // steps from n on are not there
     float h = state ? state[p.b * g.D + p.d] : 0.0f;
-    h = enter_part<false>(parts, g, p, maps[0], h);
+    if constexpr (W == kWave) h = enter_part<false>(parts, g, p, maps[0], h);
     const size_t base = (size_t)p.b * g.T * g.D + p.d;
     float xn[kSteps];
     G gn[kSteps];
@@ -141,9 +147,9 @@ gated_scan_forward_kernel(const float* __restrict__ x, const G* __restrict__ gat
         }
     };
     int buffer = 0;
-    if (t0 < n) request(t0 + p.wave * kSteps);
-    for (int tile = t0; tile < t1; tile += kTile) {
-        const int t = tile + p.wave * kSteps;
+    if (t0 < n) request(t0 + p.run * kSteps);
+    for (int tile = t0; tile < t1; tile += kSpan) {
+        const int t = tile + p.run * kSteps;
         float* __restrict__ out = y + base;
         if (tile >= n) {                                                 // (uniform) nothing there any more
 #pragma unroll
@@ -161,11 +167,11 @@ gated_scan_forward_kernel(const float* __restrict__ x, const G* __restrict__ gat
             m.H = fmaf(a[i], m.H, b[i]);
             m.A *= a[i];
         }
-        maps[buffer][p.wave][p.lane] = m;
-        if (tile + kTile < n) request(t + kTile);
+        maps[buffer][p.run][p.lane] = m;
+        if (tile + kSpan < n) request(t + kSpan);
         __syncthreads();
         float in = h;
-        h = through<false>(maps[buffer], p, h, &in);
+        h = through<false, W>(maps[buffer], p, h, &in);
         buffer ^= 1;                                                     // (the other half is written behind the next barrier's readers)
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
@@ -173,7 +179,7 @@ gated_scan_forward_kernel(const float* __restrict__ x, const G* __restrict__ gat
             if (t + i < t1 && p.valid) put<STREAM>(out + (size_t)(t + i) * g.D, t + i < n ? in : 0.0f);
         }
     }
-    if (final_state && p.s == g.parts - 1 && p.wave == 0 && p.valid) final_state[p.b * g.D + p.d] = h;
+    if (final_state && p.s == g.parts - 1 && p.run == 0 && p.valid) final_state[p.b * g.D + p.d] = h;
 }
 
 // (A, H) of every part but the last on the way: forward of x and the gates, backward (DOWN) of the gradients v_t = a_t (dy_t + v_{t+1}).
@@ -185,13 +191,13 @@ gated_scan_parts_kernel(const float* __restrict__ x, const G* __restrict__ gate,
     // the grid leaves out the last part on the way: renumbered over parts - 1
     Geometry less = g;
     less.parts = g.parts - 1;
-    Place p = place_of(less);
+    Place p = place_of<kWave>(less);
     if (DOWN) ++p.s;
     const int t0 = p.s * g.part, t1 = min(g.T, t0 + g.part);
     const int n = min(length_of(lengths, p.b, g.T), t1);
     const size_t base = (size_t)p.b * g.T * g.D + p.d;
     // each wavefront composes a consecutive share of the part's steps; shares are joined once
-    const int share = g.part / kWaves, w0 = t0 + p.wave * share, w1 = min(n, w0 + share);
+    const int share = g.part / kWaves, w0 = t0 + p.run * share, w1 = min(n, w0 + share);
     Map m{1.0f, 0.0f};
     float xn[kSteps];
     G gn[kSteps];
@@ -220,9 +226,9 @@ gated_scan_parts_kernel(const float* __restrict__ x, const G* __restrict__ gate,
             m.A *= q.a;
         }
     }
-    maps[p.wave][p.lane] = m;
+    maps[p.run][p.lane] = m;
     __syncthreads();
-    if (p.wave != 0) return;
+    if (p.run != 0) return;
     m = maps[DOWN ? kWaves - 1 : 0][p.lane];
 #pragma unroll
     for (int k = 1; k < kWaves; ++k) m = then(m, maps[DOWN ? kWaves - 1 - k : k][p.lane]);
@@ -230,18 +236,19 @@ gated_scan_parts_kernel(const float* __restrict__ x, const G* __restrict__ gate,
 }
 
 // The same walk from the end: v_t = a_t u_t, u_t = dy_t + v_{t+1}, v behind the last step = dfinal.
-template <typename G, bool STREAM>
+template <typename G, bool STREAM, int W>
 __global__ void __launch_bounds__(kThreads)
 gated_scan_backward_kernel(const float* __restrict__ dy, const float* __restrict__ dfinal, const float* __restrict__ x,
                            const G* __restrict__ gate, const float* __restrict__ y, const float* __restrict__ state,
                            const int64_t* __restrict__ lengths, float* __restrict__ dx, G* __restrict__ dgate, float* __restrict__ dstate,
                            const Map* __restrict__ parts, Geometry g) {
-    __shared__ Map maps[2][kWaves][kWave];
-    const Place p = place_of(g);
+    constexpr int kSpan = kThreads / W * kSteps;                         // steps of a tile
+    __shared__ Map maps[2][kThreads / W][W];
+    const Place p = place_of<W>(g);
     const int t0 = p.s * g.part, t1 = min(g.T, t0 + g.part);
     const int n = min(length_of(lengths, p.b, g.T), t1);
     float v = dfinal ? dfinal[p.b * g.D + p.d] : 0.0f;
-    v = enter_part<true>(parts, g, p, maps[0], v);
+    if constexpr (W == kWave) v = enter_part<true>(parts, g, p, maps[0], v);
     const float start = state ? state[p.b * g.D + p.d] : 0.0f;
     const size_t base = (size_t)p.b * g.T * g.D + p.d;
     float un[kSteps], xn[kSteps], hn[kSteps];
@@ -258,10 +265,10 @@ gated_scan_backward_kernel(const float* __restrict__ dy, const float* __restrict
         }
     };
     int buffer = 0;
-    const int last = t0 + (t1 - t0 - 1) / kTile * kTile;
+    const int last = t0 + (t1 - t0 - 1) / kSpan * kSpan;
     bool asked = false;
-    for (int tile = last; tile >= t0; tile -= kTile) {
-        const int t = tile + p.wave * kSteps;
+    for (int tile = last; tile >= t0; tile -= kSpan) {
+        const int t = tile + p.run * kSteps;
         if (tile >= n) {                                                 // (uniform) nothing there
 #pragma unroll
             for (int i = 0; i < kSteps; ++i)
@@ -287,11 +294,11 @@ gated_scan_backward_kernel(const float* __restrict__ dy, const float* __restrict
             m.H = q[i].a * (m.H + up[i]);
             m.A *= q[i].a;
         }
-        maps[buffer][p.wave][p.lane] = m;
-        if (tile > t0) request(t - kTile);
+        maps[buffer][p.run][p.lane] = m;
+        if (tile > t0) request(t - kSpan);
         __syncthreads();
         float in = v;
-        v = through<true>(maps[buffer], p, v, &in);
+        v = through<true, W>(maps[buffer], p, v, &in);
         buffer ^= 1;
 #pragma unroll
         for (int i = kSteps - 1; i >= 0; --i) {
@@ -305,7 +312,7 @@ gated_scan_backward_kernel(const float* __restrict__ dy, const float* __restrict
             }
         }
     }
-    if (dstate && p.s == 0 && p.wave == 0 && p.valid) dstate[p.b * g.D + p.d] = v;
+    if (dstate && p.s == 0 && p.run == 0 && p.valid) dstate[p.b * g.D + p.d] = v;
 }
 
 template <typename G>
@@ -325,6 +332,8 @@ Geometry geometry(int64_t B, int64_t T, int64_t D, int gate_bytes = 4) {
     Geometry g{(int)B, (int)T, (int)D, (int)((D + kWave - 1) / kWave), 1, 0, D * gate_bytes % kLine != 0};
     const int64_t rows = B * g.groups, tiles = (T + kTile - 1) / kTile;
     if (rows < kFill && tiles > kShort) g.parts = (int)std::min(tiles, (kCutFill + rows - 1) / rows);
+    g.half = rows < kFill && tiles > 1 && tiles <= kShort;
+    if (g.half) g.groups = (int)((D + kHalf - 1) / kHalf);
     g.part = (int)((tiles + g.parts - 1) / g.parts * kTile);
     g.parts = T > 0 ? (int)((T + g.part - 1) / g.part) : 1;
     return g;
@@ -349,7 +358,8 @@ int launch_gated_scan_forward(const float* x, const void* gate, int type, const 
         }
         KernelTimerScope timer_("gated_scan_forward", stream);
         const bool past = B * T * D * (int64_t)(2 * sizeof(float) + sizeof(G)) > kStreamBytes && !g.shared_lines;      // x, y, gates
-        auto kern = past ? gated_scan_forward_kernel<G, true> : gated_scan_forward_kernel<G, false>;
+        auto kern = g.half ? gated_scan_forward_kernel<G, false, kHalf>
+                    : past ? gated_scan_forward_kernel<G, true, kWave> : gated_scan_forward_kernel<G, false, kWave>;
         hipLaunchKernelGGL(kern, dim3((unsigned)(rows * g.parts)), dim3(kThreads), 0, stream, x,
                            static_cast<const G*>(gate), state, lengths, y, final_state, static_cast<const Map*>(ws), g);
         return 0;
@@ -372,7 +382,8 @@ int launch_gated_scan_backward(const float* dy, const float* dfinal, const float
         }
         KernelTimerScope timer_("gated_scan_backward", stream);
         const bool past = B * T * D * (int64_t)(4 * sizeof(float) + 2 * sizeof(G)) > kStreamBytes && !g.shared_lines;  // dy, x, y, dx, gates, dgate
-        auto kern = past ? gated_scan_backward_kernel<G, true> : gated_scan_backward_kernel<G, false>;
+        auto kern = g.half ? gated_scan_backward_kernel<G, false, kHalf>
+                    : past ? gated_scan_backward_kernel<G, true, kWave> : gated_scan_backward_kernel<G, false, kWave>;
         hipLaunchKernelGGL(kern, dim3((unsigned)(rows * g.parts)), dim3(kThreads), 0, stream, dy, dfinal, x,
                            static_cast<const G*>(gate), y, state, lengths, dx, static_cast<G*>(dgate), dstate, static_cast<const Map*>(ws),
                            g);

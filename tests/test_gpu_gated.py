@@ -132,6 +132,21 @@ def test_ends_of_the_lengths():
     _check(x, gate, s, n, gy, gf)
 
 
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("B,T,D", [(3, 65, 31), (2, 128, 32), (2, 129, 33), (5, 255, 100), (4, 256, 64)])
+def test_short_sequences_of_few_channels(B, T, D, dtype):
+    for lengths in (None, "ragged"):
+        _check(*_case(B, T, D, dtype, lengths=lengths))
+
+
+def test_ends_of_the_lengths_of_short_sequences():
+    x, gate, s, _, gy, gf = _case(34, 256, 40, torch.bfloat16)
+    n = torch.tensor([0, 1, 2, 7, 8, 9, 15, 16, 17, 31, 32, 33, 63, 64, 65, 71, 72, 73, 119, 120, 121, 127, 128, 129, 135, 136, 137, 191, 192,
+                      193, 254, 255, 256, 300], device=DEV)
+    n[2] = -1
+    _check(x, gate, s, n, gy, gf)
+
+
 def test_gates_at_their_ends():
     """Gates that keep everything, take everything, or mix: 1 - a keeps its precision where a is close to 1."""
     import snntc_amd as snn
