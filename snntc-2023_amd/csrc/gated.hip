@@ -32,23 +32,26 @@ __device__ __forceinline__ int length_of(const int64_t* lengths, int64_t b, int6
 // right start.  The next tile's loads are under way meanwhile; every value is read once and written once.  Bound by memory: 32 x 256 x
 // 800 13.4 us forward and 24.8 backward, 5.9 and 6.4 TB/s; 32768 x 1024 cut along time 38 + 58 and 33 + 120, 5.3 to 6.1 TB/s.
 //
-// Where that makes fewer than kFill workgroups of more than kShort tiles, sequences are also cut along time: a first kernel composes
+// Where that makes fewer than kFill workgroups, long sequences (more than kShort tiles) are also cut along time: a first kernel composes
 // (A, H) of each part, and a workgroup starts from the composition of the parts before its own.  The order of composition depends on
 // sizes alone.  Forward + backward in us, sequences whole / cut, 16-bit gates: 4096 steps, 16 groups of 64 channels 104 + 168 / 18 + 24,
-// 128 groups 117 + 190 / 105 + 138, 192 groups 125 + 208 / 157 + 228; 512 steps, 16 groups 16 + 24 / 12 + 14, 128 groups 17 + 25 /
-// 18 + 23; 128 steps, any number 8 + 10 / 12 + 13.  As few of two to four tiles become groups of 32 channels, each half of a wavefront
-// with eight steps of its own: 256 x 1024 7.6 + 11.3 / 7.1 + 7.8, 8 of them 8.7 + 12.8 / 7.2 + 10.6, 32 x 200 x 200 8.2 + 11.6 / 7.2 + 8.5;
-// 20 x 256 x 500 (160 groups) alike, 32 x 256 x 800 39 / 45.
+// 192 groups 125 + 208 / 157 + 228.
+// As few that are not cut become groups of 32 channels: each half of a wavefront has eight steps of its own, a tile twice as many.  Groups
+// of 64 / 32, us: 256 x 1024 7.5 + 11.2 / 7.0 + 7.6, 32 x 200 x 200 8.2 + 11.5 / 6.7 + 8.4; 160 groups alike, 32 x 256 x 800 39 / 45.  One
+// workgroup of 32 channels a CU, or a little less (kMany groups of 64 and more), is not cut however long: cut / in groups of 32, us,
+// 2048 steps, 128 groups 44 + 68 / 33 + 64, 96 groups 35 + 53 / 28 + 57, 80 groups 31 + 48 / 27 + 54, 144 groups 48 + 77 / 47 + 112; 8192
+// steps, 128 groups 187 + 330 / 142 + 285; 384 steps, 32 groups 11 + 11 / 7 + 10; 512 steps, 32 groups 11 + 12 / 9 + 12, 16 groups
+// 9 + 10 / 8 + 12.
 //
-// Workgroups are dealt to the dies in turn.  Where rows are not whole lines, of the gates either, neighbours go to one die, whose cache then holds the
-// lines that they share: in turn / neighbours together, 24 x 333 x 777 38 / 34 us, 16 x 2530 x 777 258 / 226, 16 x 8434 x 777 941 / 753,
-// 16 x 32768 x 200 1265 / 1128.  Where they do, in turn: 32768 x 1024, cut, 249 / 264, others the same.
+// Workgroups are dealt to the dies in turn.  Where rows, those of the gates among them, are not whole lines, neighbours go to one die, whose
+// cache then holds the lines that they share: in turn / neighbours together, 24 x 333 x 777 38 / 34 us, 16 x 2530 x 777 258 / 226,
+// 16 x 8434 x 777 941 / 753, 16 x 32768 x 200 1265 / 1128.  Where they are, in turn: 32768 x 1024, cut, 249 / 264, others the same.
 // Calls that touch more than the caches hold store past them, where rows are whole lines (a line stored by two groups has to meet
-// in a cache): 32768 x 1024 270 -> 249, 16 x 1920 x 1024 182 -> 171, 16 x 6400 x 1024 613 -> 600; 16 x 8434 x 777 753 -> 827.
+// in a cache): 32768 x 1024 270 -> 249, 8 x 4096 x 1024 231 -> 215, 16 x 1920 x 1024 182 -> 171, 16 x 6400 x 1024 613 -> 600; 16 x 8434 x 777 753 -> 827.
 constexpr int kWaves = 8, kSteps = 8, kTile = kWaves * kSteps;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kDies = 8;
-constexpr int kFill = 160, kShort = 4, kCutFill = 1024, kHalf = kWave / 2;
+constexpr int kFill = 160, kMany = 96, kUnits = 256, kShort = 6, kCutFill = 1024, kHalf = kWave / 2;
 
 struct Map { float A, H; };                         // h -> A h + H
 __device__ __forceinline__ Map then(const Map& first, const Map& second) { return Map{first.A * second.A, fmaf(second.A, first.H, second.H)}; }
@@ -330,9 +333,9 @@ namespace {
 constexpr int kLine = 128;
 Geometry geometry(int64_t B, int64_t T, int64_t D, int gate_bytes = 4) {
     Geometry g{(int)B, (int)T, (int)D, (int)((D + kWave - 1) / kWave), 1, 0, D * gate_bytes % kLine != 0};
-    const int64_t rows = B * g.groups, tiles = (T + kTile - 1) / kTile;
-    if (rows < kFill && tiles > kShort) g.parts = (int)std::min(tiles, (kCutFill + rows - 1) / rows);
-    g.half = rows < kFill && tiles > 1 && tiles <= kShort;
+    const int64_t rows = B * g.groups, tiles = (T + kTile - 1) / kTile, halves = B * ((D + kHalf - 1) / kHalf);
+    if (rows < kFill && tiles > kShort && (rows < kMany || halves > kUnits)) g.parts = (int)std::min(tiles, (kCutFill + rows - 1) / rows);
+    g.half = rows < kFill && tiles > 1 && g.parts == 1;
     if (g.half) g.groups = (int)((D + kHalf - 1) / kHalf);
     g.part = (int)((tiles + g.parts - 1) / g.parts * kTile);
     g.parts = T > 0 ? (int)((T + g.part - 1) / g.part) : 1;
@@ -358,8 +361,8 @@ int launch_gated_scan_forward(const float* x, const void* gate, int type, const 
         }
         KernelTimerScope timer_("gated_scan_forward", stream);
         const bool past = B * T * D * (int64_t)(2 * sizeof(float) + sizeof(G)) > kStreamBytes && !g.shared_lines;      // x, y, gates
-        auto kern = g.half ? gated_scan_forward_kernel<G, false, kHalf>
-                    : past ? gated_scan_forward_kernel<G, true, kWave> : gated_scan_forward_kernel<G, false, kWave>;
+        auto kern = g.half ? (past ? gated_scan_forward_kernel<G, true, kHalf> : gated_scan_forward_kernel<G, false, kHalf>)
+                           : (past ? gated_scan_forward_kernel<G, true, kWave> : gated_scan_forward_kernel<G, false, kWave>);
         hipLaunchKernelGGL(kern, dim3((unsigned)(rows * g.parts)), dim3(kThreads), 0, stream, x,
                            static_cast<const G*>(gate), state, lengths, y, final_state, static_cast<const Map*>(ws), g);
         return 0;
@@ -382,8 +385,8 @@ int launch_gated_scan_backward(const float* dy, const float* dfinal, const float
         }
         KernelTimerScope timer_("gated_scan_backward", stream);
         const bool past = B * T * D * (int64_t)(4 * sizeof(float) + 2 * sizeof(G)) > kStreamBytes && !g.shared_lines;  // dy, x, y, dx, gates, dgate
-        auto kern = g.half ? gated_scan_backward_kernel<G, false, kHalf>
-                    : past ? gated_scan_backward_kernel<G, true, kWave> : gated_scan_backward_kernel<G, false, kWave>;
+        auto kern = g.half ? (past ? gated_scan_backward_kernel<G, true, kHalf> : gated_scan_backward_kernel<G, false, kHalf>)
+                           : (past ? gated_scan_backward_kernel<G, true, kWave> : gated_scan_backward_kernel<G, false, kWave>);
         hipLaunchKernelGGL(kern, dim3((unsigned)(rows * g.parts)), dim3(kThreads), 0, stream, dy, dfinal, x,
                            static_cast<const G*>(gate), y, state, lengths, dx, static_cast<G*>(dgate), dstate, static_cast<const Map*>(ws),
                            g);

@@ -105,7 +105,8 @@ def test_rows_of_whole_and_half_lines(B, T, D, dtype):
     _check(*_case(B, T, D, dtype, lengths="ragged"))
 
 
-@pytest.mark.parametrize("B,T,D", [(1, 24000, 1024), (24, 1000, 1024), (12, 1000, 1024), (3, 4001, 1024), (16, 1600, 992)])
+@pytest.mark.parametrize("B,T,D", [(1, 24000, 1024), (24, 1000, 1024), (12, 1000, 1024), (3, 4001, 1024), (16, 1600, 992),
+                                   (8, 1500, 1024), (8, 3000, 1024)])
 def test_more_than_the_caches_hold(B, T, D):
     """Gates of 16-bit values in float32: the same results as from 16 bits, where the call touches less than 256 MB and stores otherwise."""
     import snntc_amd as snn
@@ -137,6 +138,12 @@ def test_ends_of_the_lengths():
 def test_short_sequences_of_few_channels(B, T, D, dtype):
     for lengths in (None, "ragged"):
         _check(*_case(B, T, D, dtype, lengths=lengths))
+
+
+@pytest.mark.parametrize("B,T,D,lengths", [(100, 520, 40, "ragged"), (60, 700, 100, None), (125, 450, 33, "ragged"), (130, 400, 70, None),
+                                           (1, 384, 1030, "ragged"), (1, 385, 1030, None)])
+def test_around_the_line_between_cut_and_whole(B, T, D, lengths):
+    _check(*_case(B, T, D, torch.float16, lengths=lengths))
 
 
 def test_ends_of_the_lengths_of_short_sequences():
