@@ -20,19 +20,21 @@ __device__ __forceinline__ int column(int slice, int lane, int q) { return slice
 template <typename E>
 struct alignas(kCols * sizeof(E)) Four { E v[kCols]; };
 
-template <typename E, bool VEC>
+// STREAM: past the caches, for more than they hold.
+template <typename E, bool VEC, bool STREAM = false>
 __device__ __forceinline__ void load_cols(const E* row, int slice, int lane, int D, float (&v)[kCols]) {
     if (VEC) {
         const int d = column<true>(slice, lane, 0);
-        Four<E> f{};
-        if (d < D) f = *reinterpret_cast<const Four<E>*>(row + d);
+        typedef E Words __attribute__((ext_vector_type(kCols)));
+        Words f{};
+        if (d < D) f = STREAM ? __builtin_nontemporal_load(reinterpret_cast<const Words*>(row + d)) : *reinterpret_cast<const Words*>(row + d);
 #pragma unroll
-        for (int q = 0; q < kCols; ++q) v[q] = (float)f.v[q];
+        for (int q = 0; q < kCols; ++q) v[q] = (float)f[q];
     } else {
 #pragma unroll
         for (int q = 0; q < kCols; ++q) {
             const int d = column<false>(slice, lane, q);
-            v[q] = d < D ? (float)row[d] : 0.0f;
+            v[q] = d >= D ? 0.0f : STREAM ? (float)__builtin_nontemporal_load(row + d) : (float)row[d];
         }
     }
 }
@@ -59,7 +61,6 @@ __device__ __forceinline__ Raw<E> load_raw(const E* row, int slice, int lane, in
     return r;
 }
 
-// STREAM: past the caches, for more than they hold.
 template <typename E, bool VEC, bool STREAM = false>
 __device__ __forceinline__ void store_cols(E* row, int slice, int lane, int D, const float (&v)[kCols]) {
     if (VEC) {
@@ -335,7 +336,7 @@ __device__ __forceinline__ void store_row(E* dtable, const E* table, int v, int 
 }
 
 // partial[chunk][0]: what a chunk adds to the token that began before it; [1]: the token that begins in it and goes on behind it.
-template <typename E, bool VEC>
+template <typename E, bool VEC, bool STREAM>
 __global__ void __launch_bounds__(256)
 embed_sums_kernel(const float* __restrict__ grad, const int* __restrict__ sorted_token, const int* __restrict__ sorted_pos,
                   const E* __restrict__ table, E* __restrict__ dtable, float* __restrict__ partial, int N, int V, int D, int chunk,
@@ -357,7 +358,7 @@ embed_sums_kernel(const float* __restrict__ grad, const int* __restrict__ sorted
         auto request = [&](int k0) {
 #pragma unroll
             for (int k = 0; k < kBatch; ++k)
-                load_cols<float, VEC>(grad + (size_t)__builtin_amdgcn_readlane(row, min(k0 + k, kWave - 1)) * D, slice, lane, D, next[k]);
+                load_cols<float, VEC, STREAM>(grad + (size_t)__builtin_amdgcn_readlane(row, min(k0 + k, kWave - 1)) * D, slice, lane, D, next[k]);
         };
         if (rows > 0) request(0);
         for (int k0 = 0; k0 < rows; k0 += kBatch) {
@@ -607,12 +608,16 @@ int sort_tokens(const I* tokens, const SortWs& w, int64_t N, int64_t V, void* dt
 
 }  // namespace
 
+// Whether times and the gradient that comes back for them are more than the caches hold (kStreamBytes): forward and gradient of N x 1024 from
+// 32768 rows of 16 bits, us, through the caches / past them, N = 20000 81 / 83, 33000 127 / 109, 40000 142 / 119, 60000 203 / 159, 131072 366 / 275.
+static bool beyond_caches(int64_t N, int64_t D) { return 2 * N * D * (int64_t)sizeof(float) > kStreamBytes; }
+
 int launch_embed_forward(const void* tokens, int token_bytes, const void* table, int type, float* z, int64_t N, int64_t V, int64_t D,
                          float scale, bool encode, hipStream_t stream) {
     const int slices = (int)((D + kSlice - 1) / kSlice);
     // four rows in flight a wavefront once that still leaves every SIMD two of them, eight where they stream past the caches (131072 x
-    // 1024 forward and gradient 366 us from the caches, 327 past them, 318 with eight rows)
-    const bool stream_out = N * D * (int64_t)sizeof(float) > kStreamBytes;
+    // 1024 136 us with four, 127 with eight)
+    const bool stream_out = beyond_caches(N, D);
     const bool vec = fours(table, D, type_bytes(type)) && fours(z, D, sizeof(float));
     const int each = vec && stream_out ? 8 : N * slices >= 8192 ? 4 : 1;
     const int64_t units = (N + each - 1) / each * slices, blocks = (units + 3) / 4;
@@ -677,7 +682,9 @@ int launch_embed_backward(const float* grad, const void* tokens, int token_bytes
         using E = decltype(e);
         {
             KernelTimerScope timer_("embed_sums", stream);
-            auto kern = vec ? embed_sums_kernel<E, true> : embed_sums_kernel<E, false>;
+            const bool past = beyond_caches(N, D);                       // (131072 x 777 352 -> 306 us)
+            auto kern = vec ? (past ? embed_sums_kernel<E, true, true> : embed_sums_kernel<E, true, false>)
+                            : (past ? embed_sums_kernel<E, false, true> : embed_sums_kernel<E, false, false>);
             hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), 0, stream, grad, w.token, w.pos, static_cast<const E*>(table),
                                static_cast<E*>(dtable), w.partial, (int)N, (int)V, (int)D, p.chunk, p.slices, units, scale, encode);
         }

@@ -48,6 +48,8 @@ __device__ __forceinline__ int length_of(const int64_t* lengths, int64_t b, int6
 // 16 x 8434 x 777 941 / 753, 16 x 32768 x 200 1265 / 1128.  Where they are, in turn: 32768 x 1024, cut, 249 / 264, others the same.
 // Calls that touch more than the caches hold store past them, where rows are whole lines (a line stored by two groups has to meet
 // in a cache): 32768 x 1024 270 -> 249, 8 x 4096 x 1024 231 -> 215, 16 x 1920 x 1024 182 -> 171, 16 x 6400 x 1024 613 -> 600; 16 x 8434 x 777 753 -> 827.
+// Where sequences are cut, they load past them too, in the second and last reading: 32768 x 1024 249 -> 237, 16 x 102400 x 64 820 -> 745,
+// 16 x 30720 x 64 231 -> 224; whole ones gain less (16 x 6400 x 1024 626 -> 612) or lose what a cache still holds (8 x 4096 x 1024 211 -> 243).
 constexpr int kWaves = 8, kSteps = 8, kTile = kWaves * kSteps;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kDies = 8;
@@ -61,9 +63,16 @@ struct Geometry {
     bool shared_lines;                              // between neighbouring groups
     bool half;                                      // groups of 32
 };
-template <bool STREAM, typename E>
+// What goes past the caches.
+enum Past { NONE, STORES, BOTH };
+template <Past PAST, typename E>
+__device__ __forceinline__ E get(const E* from) {
+    if constexpr (PAST == BOTH) return __builtin_nontemporal_load(from);
+    else return *from;
+}
+template <Past PAST, typename E>
 __device__ __forceinline__ void put(E* to, E v) {
-    if constexpr (STREAM) __builtin_nontemporal_store(v, to);
+    if constexpr (PAST != NONE) __builtin_nontemporal_store(v, to);
     else *to = v;
 }
 struct Place {
@@ -126,7 +135,7 @@ __device__ __forceinline__ float enter_part(const Map* parts, const Geometry& g,
     return h;
 }
 
-template <typename G, bool STREAM, int W>
+template <typename G, Past PAST, int W>
 __global__ void __launch_bounds__(kThreads)
 gated_scan_forward_kernel(const float* __restrict__ x, const G* __restrict__ gate, const float* __restrict__ state,
                           const int64_t* __restrict__ lengths, float* __restrict__ y, float* __restrict__ final_state,
@@ -145,8 +154,8 @@ gated_scan_forward_kernel(const float* __restrict__ x, const G* __restrict__ gat
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             const size_t e = base + (size_t)max(0, min(t + i, n - 1)) * g.D;
-            xn[i] = x[e];
-            gn[i] = gate[e];
+            xn[i] = get<PAST>(x + e);
+            gn[i] = get<PAST>(gate + e);
         }
     };
     int buffer = 0;
@@ -157,7 +166,7 @@ gated_scan_forward_kernel(const float* __restrict__ x, const G* __restrict__ gat
         if (tile >= n) {                                                 // (uniform) nothing there any more
 #pragma unroll
             for (int i = 0; i < kSteps; ++i)
-                if (t + i < t1 && p.valid) put<STREAM>(out + (size_t)(t + i) * g.D, 0.0f);
+                if (t + i < t1 && p.valid) put<PAST>(out + (size_t)(t + i) * g.D, 0.0f);
             continue;
         }
         float a[kSteps], b[kSteps];
@@ -179,7 +188,7 @@ gated_scan_forward_kernel(const float* __restrict__ x, const G* __restrict__ gat
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             in = fmaf(a[i], in, b[i]);
-            if (t + i < t1 && p.valid) put<STREAM>(out + (size_t)(t + i) * g.D, t + i < n ? in : 0.0f);
+            if (t + i < t1 && p.valid) put<PAST>(out + (size_t)(t + i) * g.D, t + i < n ? in : 0.0f);
         }
     }
     if (final_state && p.s == g.parts - 1 && p.run == 0 && p.valid) final_state[p.b * g.D + p.d] = h;
@@ -239,7 +248,7 @@ gated_scan_parts_kernel(const float* __restrict__ x, const G* __restrict__ gate,
 }
 
 // The same walk from the end: v_t = a_t u_t, u_t = dy_t + v_{t+1}, v behind the last step = dfinal.
-template <typename G, bool STREAM, int W>
+template <typename G, Past PAST, int W>
 __global__ void __launch_bounds__(kThreads)
 gated_scan_backward_kernel(const float* __restrict__ dy, const float* __restrict__ dfinal, const float* __restrict__ x,
                            const G* __restrict__ gate, const float* __restrict__ y, const float* __restrict__ state,
@@ -261,10 +270,10 @@ gated_scan_backward_kernel(const float* __restrict__ dy, const float* __restrict
         for (int i = 0; i < kSteps; ++i) {
             const int at = max(0, min(t + i, n - 1));
             const size_t e = base + (size_t)at * g.D;
-            gn[i] = gate[e];
-            un[i] = dy ? dy[e] : 0.0f;
-            xn[i] = x[e];
-            hn[i] = y[at > 0 ? e - g.D : e];
+            gn[i] = get<PAST>(gate + e);
+            un[i] = dy ? get<PAST>(dy + e) : 0.0f;
+            xn[i] = get<PAST>(x + e);
+            hn[i] = get<PAST>(y + (at > 0 ? e - g.D : e));
         }
     };
     int buffer = 0;
@@ -277,8 +286,8 @@ gated_scan_backward_kernel(const float* __restrict__ dy, const float* __restrict
             for (int i = 0; i < kSteps; ++i)
                 if (t + i < t1 && p.valid) {
                     const size_t e = base + (size_t)(t + i) * g.D;
-                    if (dx) put<STREAM>(dx + e, 0.0f);
-                    if (dgate) put<STREAM>(dgate + e, (G)0.0f);
+                    if (dx) put<PAST>(dx + e, 0.0f);
+                    if (dgate) put<PAST>(dgate + e, (G)0.0f);
                 }
             continue;
         }
@@ -310,8 +319,8 @@ gated_scan_backward_kernel(const float* __restrict__ dy, const float* __restrict
             if (t + i < t1 && p.valid) {
                 const bool there = t + i < n;
                 const size_t e = base + (size_t)(t + i) * g.D;
-                if (dx) put<STREAM>(dx + e, there ? q[i].rest * u : 0.0f);
-                if (dgate) put<STREAM>(dgate + e, (G)(there ? u * lead[i] * (q[i].a * q[i].rest) : 0.0f));
+                if (dx) put<PAST>(dx + e, there ? q[i].rest * u : 0.0f);
+                if (dgate) put<PAST>(dgate + e, (G)(there ? u * lead[i] * (q[i].a * q[i].rest) : 0.0f));
             }
         }
     }
@@ -361,8 +370,9 @@ int launch_gated_scan_forward(const float* x, const void* gate, int type, const 
         }
         KernelTimerScope timer_("gated_scan_forward", stream);
         const bool past = B * T * D * (int64_t)(2 * sizeof(float) + sizeof(G)) > kStreamBytes && !g.shared_lines;      // x, y, gates
-        auto kern = g.half ? (past ? gated_scan_forward_kernel<G, true, kHalf> : gated_scan_forward_kernel<G, false, kHalf>)
-                           : (past ? gated_scan_forward_kernel<G, true, kWave> : gated_scan_forward_kernel<G, false, kWave>);
+        auto kern = g.half ? (past ? gated_scan_forward_kernel<G, STORES, kHalf> : gated_scan_forward_kernel<G, NONE, kHalf>)
+                    : !past ? gated_scan_forward_kernel<G, NONE, kWave>
+                    : g.parts > 1 ? gated_scan_forward_kernel<G, BOTH, kWave> : gated_scan_forward_kernel<G, STORES, kWave>;
         hipLaunchKernelGGL(kern, dim3((unsigned)(rows * g.parts)), dim3(kThreads), 0, stream, x,
                            static_cast<const G*>(gate), state, lengths, y, final_state, static_cast<const Map*>(ws), g);
         return 0;
@@ -385,8 +395,9 @@ int launch_gated_scan_backward(const float* dy, const float* dfinal, const float
         }
         KernelTimerScope timer_("gated_scan_backward", stream);
         const bool past = B * T * D * (int64_t)(4 * sizeof(float) + 2 * sizeof(G)) > kStreamBytes && !g.shared_lines;  // dy, x, y, dx, gates, dgate
-        auto kern = g.half ? (past ? gated_scan_backward_kernel<G, true, kHalf> : gated_scan_backward_kernel<G, false, kHalf>)
-                           : (past ? gated_scan_backward_kernel<G, true, kWave> : gated_scan_backward_kernel<G, false, kWave>);
+        auto kern = g.half ? (past ? gated_scan_backward_kernel<G, STORES, kHalf> : gated_scan_backward_kernel<G, NONE, kHalf>)
+                    : !past ? gated_scan_backward_kernel<G, NONE, kWave>
+                    : g.parts > 1 ? gated_scan_backward_kernel<G, BOTH, kWave> : gated_scan_backward_kernel<G, STORES, kWave>;
         hipLaunchKernelGGL(kern, dim3((unsigned)(rows * g.parts)), dim3(kThreads), 0, stream, dy, dfinal, x,
                            static_cast<const G*>(gate), y, state, lengths, dx, static_cast<G*>(dgate), dstate, static_cast<const Map*>(ws),
                            g);

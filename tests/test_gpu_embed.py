@@ -72,13 +72,27 @@ def test_many_tokens(N, V, D, dtype):
 @pytest.mark.parametrize("dtype", list(HALF))
 @pytest.mark.parametrize("N,D", [(67111, 1000), (16411, 4100), (67111, 1001)])
 def test_outputs_larger_than_the_caches(N, D, dtype):
-    """Rows do not know how many there are: both halves of an output of more than 256 MB, by themselves."""
+    """Rows do not know how many there are: the quarters of an output of more than 256 MB, by themselves."""
     import snntc_amd as snn
     tok, table, _ = _case(N, 300, D, dtype)
     tok[5] = -1
     z = snn.embed_tokens(tok, table, 0.5, True)
-    for part in (slice(0, N // 2), slice(N // 2, N)):
+    for part in (slice(k * N // 4, (k + 1) * N // 4) for k in range(4)):
         assert torch.equal(z[part].nan_to_num(-1.0), snn.embed_tokens(tok[part], table, 0.5, True).nan_to_num(-1.0))
+
+
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("D", [1100, 1101])
+def test_gradients_larger_than_the_caches(D, dtype):
+    """Of more than 256 MB with the times: the same sums as of the columns by themselves, which are less."""
+    import snntc_amd as snn
+    N = 31007
+    tok, table, grad = _case(N, 700, D, dtype)
+    d = snn.embed_tokens_grad(grad, tok, table, 0.5, True)
+    for part in (slice(0, 512), slice(512, D)):
+        half = snn.embed_tokens_grad(grad[:, part], tok, table[:, part], 0.5, True)
+        # the same terms in chunks of another length: each side is off by its own roundings
+        _close(d[:, part], half.double().cpu(), 2 * _reference(tok, table[:, part], 0.5, True, grad[:, part])[1], "dtable")
 
 
 def test_one_token_throughout_and_all_different():
