@@ -92,7 +92,7 @@ __device__ __forceinline__ float time_of(float e, float scale, bool encode) {
 }
 
 // A wavefront owns 256 columns of TOKENS consecutive tokens and requests their rows together.  Bound by memory: 131072 tokens of 1024
-// columns from a 16-bit table 121 us, 5.35 TB/s; 8192 of 800 from float32 8.8 us, 4.6 TB/s.
+// columns from a 16-bit table 98 us, 6.6 TB/s; 8192 of 800 from float32 8.8 us, 4.6 TB/s.
 template <typename E, typename I, bool VEC, int TOKENS, bool STREAM>
 __global__ void __launch_bounds__(256)
 embed_forward_kernel(const I* __restrict__ tokens, const E* __restrict__ table, float* __restrict__ z, int N, int V, int D, int slices,
@@ -127,7 +127,7 @@ embed_forward_kernel(const I* __restrict__ tokens, const E* __restrict__ table, 
 //    tokens that do not occur stay like that.
 // 2. The sorted positions are cut into chunks of equal length, whatever the tokens' frequencies are; a wavefront owns a chunk and
 //    256 columns.  It adds up the rows of each token in order; a token that lies wholly in the chunk is finished there, the
-//    first and last one may reach beyond it and leave partial sums.  131072 rows of 1024: 624 MB in 151 us, 4.1 TB/s.
+//    first and last one may reach beyond it and leave partial sums.  131072 rows of 1024: 624 MB in 124 us, 5.0 TB/s.
 // 3. Partial sums of one token are added in the order of their chunks.
 
 constexpr int kRankThreads = 1024;
@@ -616,7 +616,7 @@ int launch_embed_forward(const void* tokens, int token_bytes, const void* table,
                          float scale, bool encode, hipStream_t stream) {
     const int slices = (int)((D + kSlice - 1) / kSlice);
     // four rows in flight a wavefront once that still leaves every SIMD two of them, eight where they stream past the caches (131072 x
-    // 1024 136 us with four, 127 with eight)
+    // 1024 with the table thrown out of the caches by gradients 136 us with four, 127 with eight)
     const bool stream_out = beyond_caches(N, D);
     const bool vec = fours(table, D, type_bytes(type)) && fours(z, D, sizeof(float));
     const int each = vec && stream_out ? 8 : N * slices >= 8192 ? 4 : 1;

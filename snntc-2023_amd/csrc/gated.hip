@@ -30,7 +30,7 @@ __device__ __forceinline__ int length_of(const int64_t* lengths, int64_t b, int6
 // kSteps of them in registers (lane = channel).  A run of steps maps the state it is given to A h + H, so the wavefronts exchange
 // (A, H) of their runs through LDS, every one composes those before its own, and goes through its steps a second time with the
 // right start.  The next tile's loads are under way meanwhile; every value is read once and written once.  Bound by memory: 32 x 256 x
-// 800 13.4 us forward and 24.8 backward, 5.9 and 6.4 TB/s; 32768 x 1024 cut along time 38 + 58 and 33 + 120, 5.3 to 6.1 TB/s.
+// 800 13.4 us forward and 24.8 backward, 5.9 and 6.4 TB/s; 32768 x 1024 cut along time 37 + 57 and 35 + 107, 5.4 to 6.3 TB/s.
 //
 // Where that makes fewer than kFill workgroups, long sequences (more than kShort tiles) are also cut along time: a first kernel composes
 // (A, H) of each part, and a workgroup starts from the composition of the parts before its own.  The order of composition depends on
