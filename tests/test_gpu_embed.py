@@ -95,6 +95,18 @@ def test_gradients_larger_than_the_caches(D, dtype):
         _close(d[:, part], half.double().cpu(), 2 * _reference(tok, table[:, part], 0.5, True, grad[:, part])[1], "dtable")
 
 
+def test_more_elements_than_32_bits_count():
+    import snntc_amd as snn
+    N, D = 2300007, 1000
+    tok = torch.arange(N - 1, -1, -1, device=DEV)
+    table = torch.rand(N, D, device=DEV).to(torch.bfloat16)
+    z = snn.embed_tokens(tok, table, 0.5)
+    assert torch.equal(z[-3:], 0.5 * table[:3].float().flip(0)) and torch.equal(z[:3], 0.5 * table[-3:].float().flip(0))
+    d = snn.embed_tokens_grad(z, tok, table, 0.5)
+    for k in range(0, N, 100000):                               # (halves and quarters of bfloat16 are exact)
+        assert torch.equal(d[k:k + 100000], 0.25 * table[k:k + 100000])
+
+
 def test_one_token_throughout_and_all_different():
     import snntc_amd as snn
     for tok in (torch.full((5000,), 6), torch.arange(5000), torch.arange(5000).flip(0), torch.arange(5000) // 64, torch.arange(5000) % 2):

@@ -154,6 +154,28 @@ def test_ends_of_the_lengths_of_short_sequences():
     _check(x, gate, s, n, gy, gf)
 
 
+@pytest.mark.parametrize("B,T", [(12, 190001), (3, 760003)])
+def test_more_elements_than_32_bits_count(B, T):
+    """The first and last sequence are the same, and come out the same."""
+    import snntc_amd as snn
+    gen = torch.Generator(device=DEV).manual_seed(T)
+    x = 1.0 + torch.rand(B, T, 1024, generator=gen, device=DEV)
+    gate = torch.empty(B, T, 1024, dtype=torch.bfloat16, device=DEV).normal_(1.5, 2.0, generator=gen)
+    gy = torch.empty(B, T, 1024, device=DEV).normal_(generator=gen)
+    for v in (x, gate, gy):
+        v[-1] = v[0]
+    y, final = snn.gated_scan(x, gate)
+    assert torch.equal(y[0], y[-1]) and torch.equal(final[0], final[-1])
+    # the last 300 steps by the formula, begun 300 steps earlier: what the state there is off by is multiplied by all gates in between
+    last = slice(T - 600, T)
+    want = _reference(x[-1:, last, :16], gate[-1:, last, :16], y[-1:, T - 601, :16], None)
+    _close(y[-1:, T - 300:, :16], [v[:, 300:] for v in want["y"]], "y")
+    _close(final[-1:, :16], want["final"], "final")             # (made by joining runs of steps, y step by step: each within its bound)
+    dx, dgate, dstate = snn.gated_scan_grad(gy, None, x, gate, y)
+    assert torch.equal(dx[0], dx[-1]) and torch.equal(dgate[0], dgate[-1]) and torch.equal(dstate[0], dstate[-1])
+    assert not torch.equal(dx[0], dx[1]) and bool(torch.isfinite(dx[-1]).all())
+
+
 def test_gates_at_their_ends():
     """Gates that keep everything, take everything, or mix: 1 - a keeps its precision where a is close to 1."""
     import snntc_amd as snn
