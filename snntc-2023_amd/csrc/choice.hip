@@ -434,7 +434,8 @@ preference_pairs_kernel(const float* __restrict__ logp, PreferenceArgs a, float*
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const int64_t e = (p + half * P) * T + t;
-            coef[e] = row_weight(a.weight, e) * (half ? -slope : slope);
+            const float w = row_weight(a.weight, e);
+            coef[e] = w == 0.0f ? 0.0f : w * (half ? -slope : slope);    // (a slope may be NaN: a row of weight 0 has none)
         }
 }
 

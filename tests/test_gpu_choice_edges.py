@@ -1,0 +1,36 @@
+"""Losses over choices where a row, a pair or a limit is out of the ordinary."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("J", [10, 1000, 5001, 9000, 70000])
+def test_rows_of_weight_zero_in_a_pair_without_a_margin(J, dtype):
+    """A choice out of range makes its pair's margin NaN, and the gradient of the pair's rows; its rows of weight 0 are still not
+    read and have none, and the other pair is as it was."""
+    import snntc_amd as snn
+    gen = torch.Generator().manual_seed(J)
+    times = (1.0 + 8.0 * torch.rand(4, 3, J, generator=gen)).to(dtype)
+    tokens = torch.randint(0, J, (4, 3), generator=gen)
+    ref = torch.tensor([-3.0, -4.0, -5.0, -6.0])
+    weight = torch.tensor([[1.0, 0.0, 0.5], [1.0, 1.0, 0.0], [0.0, 2.0, 0.0], [0.0, 1.0, 1.0]])
+    want = snn.preference_time_loss(*(v.to(DEV) for v in (times, tokens, ref, weight)))
+    tokens[0, 2] = J
+    times[weight == 0] = float("nan")
+    tokens[weight == 0] = -7
+    t, k, r, w = (v.to(DEV) for v in (times, tokens, ref, weight))
+    loss, seq, grad = snn.preference_time_loss(t, k, r, w)
+    leaf = t.clone().requires_grad_(True)
+    (through,) = torch.autograd.grad(snn.preference_loss(leaf, k, r, w), [leaf])
+    off = w == 0
+    for g in (grad, through):
+        assert (g[off] == 0).all()
+        assert torch.isnan(g[0, [0, 2]]).all() and torch.isnan(g[2, 1]).all()
+    assert torch.equal(grad[[1, 3]], want[2][[1, 3]])
+    assert torch.equal(torch.isnan(loss), torch.tensor([True, False], device=DEV)) and torch.equal(loss[1], want[0][1])
+    assert torch.equal(torch.isnan(seq), torch.tensor([True, False, False, False], device=DEV)) and torch.equal(seq[1:], want[1][1:])
