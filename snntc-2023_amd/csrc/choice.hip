@@ -425,7 +425,9 @@ preference_pairs_kernel(const float* __restrict__ logp, PreferenceArgs a, float*
             seq_logp[p + half * P] = (float)seq[half];
         }
         const double e = a.smoothing, m = a.beta * ((seq[0] - a.ref_logp[p]) - (seq[1] - a.ref_logp[p + P]));
-        pair_loss[p] = (float)((1.0 - e) * softplus(-m) + e * softplus(m));
+        // (a term of factor 0 is none: at an infinite margin, from a sequence that cannot occur, it would be 0 times infinity)
+        const double towards = e < 1.0 ? (1.0 - e) * softplus(-m) : 0.0, against = e > 0.0 ? e * softplus(m) : 0.0;
+        pair_loss[p] = isnan(m) ? NAN : (float)(towards + against);
         shared_slope = (float)(a.beta / (double)P * (e / (1.0 + exp(-m)) - (1.0 - e) / (1.0 + exp(m))));
     }
     __syncthreads();

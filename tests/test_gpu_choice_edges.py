@@ -34,3 +34,24 @@ def test_rows_of_weight_zero_in_a_pair_without_a_margin(J, dtype):
     assert torch.equal(grad[[1, 3]], want[2][[1, 3]])
     assert torch.equal(torch.isnan(loss), torch.tensor([True, False], device=DEV)) and torch.equal(loss[1], want[0][1])
     assert torch.equal(torch.isnan(seq), torch.tensor([True, False, False, False], device=DEV)) and torch.equal(seq[1:], want[1][1:])
+
+
+@pytest.mark.parametrize("smoothing", [0.0, 0.25, 1.0])
+def test_sequences_that_cannot_occur(smoothing):
+    """A sequence with an output that can never be chosen has log-probability minus infinity.  Where only the rejected one has, the
+    margin is infinite: without smoothing the loss is 0, where only the preferred one has, infinite; a term of factor 0 is none."""
+    import snntc_amd as snn
+    gen = torch.Generator().manual_seed(7)
+    times = 1.0 + 8.0 * torch.rand(4, 3, 6, generator=gen)
+    tokens = torch.zeros(4, 3, dtype=torch.int64)
+    times[2, 1, 0] = math.inf                                   # the rejected one of pair 0
+    times[1, 0, 0] = math.inf                                   # the preferred one of pair 1
+    t, k, ref = times.to(DEV), tokens.to(DEV), torch.full((4,), -5.0, device=DEV)
+    loss, seq, grad = snn.preference_time_loss(t, k, ref, beta=0.5, smoothing=smoothing)
+    assert seq.tolist()[1:3] == [-math.inf, -math.inf]
+    assert loss.tolist() == [0.0 if smoothing == 0.0 else math.inf, 0.0 if smoothing == 1.0 else math.inf]
+    # d loss / d margin is the smoothing at plus infinity, the smoothing - 1 at minus infinity; times beta over the pairs
+    slopes = torch.tensor([smoothing, smoothing - 1.0], dtype=torch.float64) * 0.5 / 2
+    p = torch.softmax(-times.double(), -1)
+    want = torch.cat([slopes, -slopes])[:, None, None] * (p - torch.nn.functional.one_hot(tokens, 6))
+    assert torch.allclose(grad.double().cpu(), want, rtol=1e-5, atol=1e-7)
