@@ -233,6 +233,12 @@ radix_count_kernel(const I* __restrict__ tokens, const int* __restrict__ key, in
     for (int d = threadIdx.x; d < bins; d += kRadixThreads) counts[(size_t)blockIdx.x * bins + d] = hist[d];
 }
 
+// What the lanes of a wavefront have read and written in LDS before comes before what they do after.
+__device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 template <typename I, bool FIRST>
 __global__ void __launch_bounds__(kRadixThreads)
 radix_place_kernel(const I* __restrict__ tokens, const int* __restrict__ key, const int* __restrict__ pos, const int* __restrict__ counts,
@@ -312,8 +318,11 @@ radix_place_kernel(const I* __restrict__ tokens, const int* __restrict__ key, co
             out_key[at] = k;
             out_pos[at] = FIRST ? (int)(i + lane) : pos[i + lane];
         }
-        // the last of equal digits moves the mark on, after all have read it (one wavefront: its LDS accesses are in order)
+        // the last of equal digits moves the mark on, after all have read it and before they read again: one wavefront's LDS accesses are
+        // done in order, and the barriers (no instructions) keep the compiler from changing it
+        wave_order();
         if (there && (same >> lane) == 1) seen[wave][digit] = at + 1;
+        wave_order();
     }
 }
 
