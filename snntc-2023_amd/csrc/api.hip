@@ -11,7 +11,7 @@
 #include <string>
 #include <vector>
 
-#include "snntc_common.h"
+#include "sequences.h"
 
 // Library-owned scratch of snntc_fc_forward_static (the entry point that allocates nothing): held by
 // every GPU the library runs on until the process ends.  Host code never passes this name to a

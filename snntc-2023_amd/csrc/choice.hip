@@ -9,7 +9,7 @@
 // logsumexp is kept as the pair (maximum, log of the sum above it): neurons that never fire sit at MAX_SPIKE_TIME, and in a row of
 // them the one number 10^5 + log J would have lost the logarithm's digits.
 // A row of weight 0 is not read: its loss, logp and gradient are 0.
-#include "snntc_common.h"
+#include "sequences.h"
 
 namespace snntc {
 namespace {

@@ -5,7 +5,7 @@
 // here the tokens are sorted first (by token, then by position), and the rows are added in that order.
 #include <algorithm>
 
-#include "snntc_common.h"
+#include "sequences.h"
 
 namespace snntc {
 namespace {

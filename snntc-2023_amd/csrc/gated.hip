@@ -6,7 +6,7 @@
 // A step mixes two spike times, so what comes out lies between those that went in and is a spike time itself.
 #include <algorithm>
 
-#include "snntc_common.h"
+#include "sequences.h"
 
 namespace snntc {
 namespace {
