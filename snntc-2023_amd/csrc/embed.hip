@@ -97,7 +97,7 @@ template <typename E, typename I, bool VEC, int TOKENS, bool STREAM>
 __global__ void __launch_bounds__(256)
 embed_forward_kernel(const I* __restrict__ tokens, const E* __restrict__ table, float* __restrict__ z, int N, int V, int D, int slices,
                      int64_t units, float scale, bool encode) {
-    const int64_t unit = (int64_t)blockIdx.x * (256 / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int64_t unit = workgroup() * (256 / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     if (unit >= units) return;
     const int64_t n0 = unit / slices * TOKENS;
     const int slice = (int)(unit % slices), lane = threadIdx.x % kWave;
@@ -630,7 +630,6 @@ int launch_embed_forward(const void* tokens, int token_bytes, const void* table,
     const bool vec = fours(table, D, type_bytes(type)) && fours(z, D, sizeof(float));
     const int each = vec && stream_out ? 8 : N * slices >= 8192 ? 4 : 1;
     const int64_t units = (N + each - 1) / each * slices, blocks = (units + 3) / 4;
-    if (blocks > (1 << 24) - 1) return fail(SNNTC_ERR_TOO_LARGE, "embed: too many rows");
     with_type(type, [&](auto e) {
         using E = decltype(e);
         KernelTimerScope timer_("embed_forward", stream);
@@ -639,7 +638,7 @@ int launch_embed_forward(const void* tokens, int token_bytes, const void* table,
             auto kern = !vec ? (each == 4 ? embed_forward_kernel<E, I, false, 4, false> : embed_forward_kernel<E, I, false, 1, false>)
                         : each == 8 ? embed_forward_kernel<E, I, true, 8, true>
                         : each == 4 ? embed_forward_kernel<E, I, true, 4, false> : embed_forward_kernel<E, I, true, 1, false>;
-            hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), 0, stream, static_cast<const I*>(tokens),
+            hipLaunchKernelGGL(kern, wide_grid(blocks, 256), dim3(256), 0, stream, static_cast<const I*>(tokens),
                                static_cast<const E*>(table), z, (int)N, (int)V, (int)D, slices, units, scale, encode);
         };
         if (token_bytes == 8) launch(int64_t{});

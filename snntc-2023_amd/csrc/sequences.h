@@ -18,6 +18,15 @@ int with_type(int type, F&& f) {
     }
 }
 
+// One dimension of a launch holds less than 2^32 threads; more workgroups than that go on in the second one.  A kernel that is launched so
+// counts by workgroup() and leaves out what lies behind its last one (there may be up to kGridRow - 1 too many).
+constexpr int64_t kGridRow = 1 << 20;
+inline dim3 wide_grid(int64_t blocks, int threads) {
+    if (blocks * threads < (1ll << 32)) return dim3((unsigned)blocks);
+    return dim3((unsigned)kGridRow, (unsigned)((blocks + kGridRow - 1) / kGridRow));
+}
+__device__ __forceinline__ int64_t workgroup() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 // Calls that touch more than the caches hold (256 MB, the memory's own included) store their results past them: otherwise what the next
 // kernel reads waits for the write-back of what this one has left.  Smaller calls leave their results where the next kernel finds them.
 constexpr int64_t kStreamBytes = 256ll << 20;

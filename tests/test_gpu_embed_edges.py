@@ -18,3 +18,20 @@ def test_every_position_is_placed_once(N, V, runs):
     grad[:, 3] = 1.0
     want = torch.zeros(V, 4, device=DEV, dtype=torch.float64).index_add_(0, tok, grad.double())
     assert torch.equal(snn.embed_tokens_grad(grad, tok, torch.zeros(V, 4, device=DEV)).double(), want)
+
+
+@pytest.mark.parametrize("N,D", [(2 ** 28 + 5, 3), (2 ** 29 + 9, 4)])
+def test_more_tokens_than_a_grid_dimension_holds(N, D):
+    """Some 2^24 workgroups: rows read element by element, and four elements at a time."""
+    import snntc_amd as snn
+    table = torch.randint(-64, 65, (1000, D), device=DEV).float()
+    tok = torch.randint(0, 1000, (N,), device=DEV, dtype=torch.int32)
+    tok[-2] = -1
+    z = snn.embed_tokens(tok, table, 0.5)
+    for first in range(0, N, 2 ** 24):                          # (an indexing of 2^26 rows of four is refused by PyTorch itself)
+        part = slice(first, min(N, first + 2 ** 24))
+        want = 0.5 * table[tok[part].clamp(min=0).long()]
+        if part.stop == N:
+            assert torch.isnan(z[-2]).all()
+            z[-2], want[-2] = 0.0, 0.0
+        assert torch.equal(z[part], want)
