@@ -131,7 +131,7 @@ choice_row_kernel(const E* __restrict__ times, E* __restrict__ dtimes, RowArgs a
     const int k = threadIdx.x % WIDTH;
     // the gradient pass begins with the rows that were read last: they may still be in a cache (16 x 512 rows of 32768 outputs, a part
     // of them of weight 0: 199 -> 176 us; 1 GB of times, or 30 MB: alike)
-    const int64_t block = MODE == GRAD ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+    const int64_t block = MODE == GRAD ? (int64_t)gridDim.x * gridDim.y - 1 - workgroup() : workgroup();
     const int64_t r = block * kRows + threadIdx.x / WIDTH;
     if (r >= a.rows) return;                                             // (whole rows; no barrier where rows share a workgroup)
     const E* __restrict__ t = times + (size_t)r * a.J;
@@ -234,13 +234,13 @@ constexpr int slice_pieces() { return VEC == 1 ? 4096 : 1024; }          // 16 K
 
 template <typename E, int VEC>
 __global__ void __launch_bounds__(kSliceThreads)
-choice_slice_kernel(const E* __restrict__ times, const float* __restrict__ weight, Soft* __restrict__ partial, int J, int slices) {
+choice_slice_kernel(const E* __restrict__ times, const float* __restrict__ weight, Soft* __restrict__ partial, int64_t rows, int J, int slices) {
     __shared__ Soft part[kSliceThreads / kWave];
     using P = Piece<E, VEC>;
     constexpr int kPieces = slice_pieces<VEC>(), kEach = kPieces / kSliceThreads, kBatch = 4;
-    const int64_t r = blockIdx.x / slices;
-    const int slice = blockIdx.x % slices, k = threadIdx.x;
-    if (row_weight(weight, r) == 0.0f) return;
+    const int64_t block = workgroup(), r = block / slices;
+    const int slice = block % slices, k = threadIdx.x;
+    if (r >= rows || row_weight(weight, r) == 0.0f) return;
     const E* __restrict__ t = times + (size_t)r * J;
     const Cut cut = cut_row<E, VEC>(t, J);
     const int odd = slice == 0 ? odd_element<VEC>(cut, k) : -1;
@@ -323,8 +323,9 @@ __global__ void __launch_bounds__(kSliceThreads)
 choice_slice_grad_kernel(const E* __restrict__ times, E* __restrict__ dtimes, const Soft* __restrict__ partial, RowArgs a, int slices) {
     using P = Piece<E, VEC>;
     constexpr int kPieces = slice_pieces<VEC>(), kEach = kPieces / kSliceThreads, kBatch = 4;
-    const int64_t block = gridDim.x - 1 - blockIdx.x;                    // (what was read last comes first)
+    const int64_t block = (int64_t)gridDim.x * gridDim.y - 1 - workgroup();            // (what was read last comes first)
     const int64_t r = block / slices;
+    if (r >= a.rows) return;
     const int slice = block % slices, k = threadIdx.x;
     const E* __restrict__ t = times + (size_t)r * a.J;
     E* __restrict__ g = dtimes + (size_t)r * a.J;
@@ -481,11 +482,11 @@ template <typename E, int VEC, Mode MODE, bool STREAM>
 int launch_rows(const E* times, E* dtimes, const RowArgs& a, hipStream_t stream) {
     const int pieces = VEC == 1 ? a.J : a.J / VEC;
     auto launch = [&](auto kern, int width) -> int {
-        const int64_t per = width < 256 ? 256 / width : 1, blocks = (a.rows + per - 1) / per, threads = width < 256 ? 256 : width;
-        if (blocks * threads >= (1ll << 32)) return fail(SNNTC_ERR_TOO_LARGE, "loss: too many long rows");
+        const int64_t per = width < 256 ? 256 / width : 1, blocks = (a.rows + per - 1) / per;
+        const int threads = width < 256 ? 256 : width;
         {
             KernelTimerScope timer_(MODE == LOGP ? "time_logp" : MODE == POLICY ? "policy_loss" : "time_logp_backward", stream);
-            hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3((unsigned)threads), 0, stream, times, dtimes, a);
+            hipLaunchKernelGGL(kern, wide_grid(blocks, threads), dim3((unsigned)threads), 0, stream, times, dtimes, a);
         }
         SNNTC_HIP_CHECK(hipGetLastError());
         return SNNTC_OK;
@@ -512,12 +513,11 @@ template <typename E, int VEC, Mode MODE, bool STREAM>
 int launch_slices(const E* times, E* dtimes, const RowArgs& a, Soft* partial, hipStream_t stream) {
     const int per = slice_pieces<VEC>(), pieces = a.J / VEC, slices = (pieces + per - 1) / per;
     const int64_t blocks = a.rows * slices;
-    if (blocks >= (1 << 24)) return fail(SNNTC_ERR_TOO_LARGE, "loss: too many long rows");
     if constexpr (MODE != GRAD) {
         {
             KernelTimerScope timer_("choice_slice", stream);
-            hipLaunchKernelGGL((choice_slice_kernel<E, VEC>), dim3((unsigned)blocks), dim3(kSliceThreads), 0, stream, times, a.weight,
-                               partial, a.J, slices);
+            hipLaunchKernelGGL((choice_slice_kernel<E, VEC>), wide_grid(blocks, kSliceThreads), dim3(kSliceThreads), 0, stream, times, a.weight,
+                               partial, a.rows, a.J, slices);
         }
         if (MODE == LOGP || !dtimes) {
             KernelTimerScope timer_("choice_join", stream);
@@ -527,7 +527,7 @@ int launch_slices(const E* times, E* dtimes, const RowArgs& a, Soft* partial, hi
     if constexpr (MODE != LOGP) {
         if (dtimes) {
             KernelTimerScope timer_("choice_slice_grad", stream);
-            hipLaunchKernelGGL((choice_slice_grad_kernel<E, VEC, MODE, STREAM>), dim3((unsigned)blocks), dim3(kSliceThreads), 0, stream, times,
+            hipLaunchKernelGGL((choice_slice_grad_kernel<E, VEC, MODE, STREAM>), wide_grid(blocks, kSliceThreads), dim3(kSliceThreads), 0, stream, times,
                                dtimes, partial, a, slices);
         }
     }

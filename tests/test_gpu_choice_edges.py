@@ -55,3 +55,55 @@ def test_sequences_that_cannot_occur(smoothing):
     p = torch.softmax(-times.double(), -1)
     want = torch.cat([slopes, -slopes])[:, None, None] * (p - torch.nn.functional.one_hot(tokens, 6))
     assert torch.allclose(grad.double().cpu(), want, rtol=1e-5, atol=1e-7)
+
+
+def _many_rows(rows, J):
+    """Rows of weight 0, which are not read, but for the first and the last three; times that lie differently to 16 bytes than the
+    gradient; None where the card has no room for both."""
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 2 * rows * J * 2 + (4 << 30):
+        return None
+    gen = torch.Generator().manual_seed(J)
+    times = torch.empty(rows * J + 1, dtype=torch.bfloat16, device=DEV)[1:].view(rows, J)
+    some = torch.tensor([0, rows - 3, rows - 2, rows - 1], device=DEV)
+    times[some] = (1.0 + 8.0 * torch.rand(4, J, generator=gen)).to(torch.bfloat16).to(DEV)
+    tokens = torch.full((rows,), 77, device=DEV)
+    weight = torch.zeros(rows, device=DEV)
+    weight[some] = torch.tensor([1.0, 0.5, 0.25, 2.0], device=DEV)
+    old, adv = torch.full((rows,), -8.0, device=DEV), torch.ones(rows, device=DEV)
+    return [times, tokens, old, adv, weight], some
+
+
+# Sums in another order and other pieces of a row: J / 64 + 40 roundings of 2^-24 at most on either side, and bfloat16's step.
+def _like(a, b, dtype=torch.float32):
+    return torch.allclose(a.float(), b.float(), rtol=2.0 ** -7 if dtype == torch.bfloat16 else 2e-5, atol=1e-12 if dtype == torch.bfloat16 else 2e-5)
+
+
+def test_more_rows_than_a_grid_dimension_holds():
+    """2^22 workgroups of 1024 threads."""
+    import snntc_amd as snn
+    made = _many_rows(2 ** 22 + 3, 1025)
+    if made is None:
+        pytest.skip("needs 22 GB of the card's memory")
+    (times, tokens, old, adv, weight), some = made
+    loss, logp, grad = snn.policy_time_loss(times, tokens, old, adv, weight=weight)
+    one = snn.policy_time_loss(times[some], tokens[some], old[some], adv[some], weight=weight[some])
+    assert _like(loss[some], one[0]) and _like(logp[some], one[1]) and _like(grad[some], one[2], torch.bfloat16)
+    for v in (loss, logp, grad):
+        v[some] = 0.0
+        assert not v.any()
+
+
+def test_more_slices_than_a_grid_dimension_holds():
+    """The gradient from statistics of 2^23 rows of two slices each."""
+    import snntc_amd as snn
+    made = _many_rows(2 ** 23 + 3, 4097)
+    if made is None:
+        pytest.skip("needs 142 GB of the card's memory")
+    (times, tokens, old, adv, weight), some = made
+    leaf = times.requires_grad_(True)
+    (grad,) = torch.autograd.grad(snn.policy_loss(leaf, tokens, old, adv, weight=weight), [leaf])
+    one = snn.policy_time_loss(leaf.detach()[some], tokens[some], old[some], adv[some], weight=weight[some])
+    assert _like(grad[some], one[2], torch.bfloat16)
+    grad[some] = 0.0
+    assert not any(part.any() for part in grad.split(2 ** 20))
