@@ -336,7 +336,7 @@ SNNTC_API int snntc_embed_backward(const float* grad, const void* tokens, int to
  * behind a sequence's length, dy there is not read.  One workspace size serves both directions.
  * snntc_gated_step is one step of n independent channels: out = a state + (1 - a) x (state NULL: zeros; out may be state).
  * Errors: a negative size, a gate_type that is none of the above, a NULL required pointer -> BAD_ARGUMENT; B, T or D
- * above 2^30, or B ceil(D / 64) of 2^20 and more -> TOO_LARGE; a workspace below _workspace_bytes -> WORKSPACE.
+ * above 2^30, B ceil(D / 64) of 2^20 and more, or n of 2^32 and more -> TOO_LARGE; a workspace below _workspace_bytes -> WORKSPACE.
  * ------------------------------------------------------------------------------------------- */
 SNNTC_API int snntc_gated_scan_workspace_bytes(int64_t B, int64_t T, int64_t D, size_t* bytes);
 SNNTC_API int snntc_gated_scan_forward(const float* x, const void* gate, int gate_type, const float* state, const int64_t* lengths,

@@ -629,6 +629,7 @@ int snntc_gated_scan_backward(const float* dy, const float* dfinal, const float*
 
 int snntc_gated_step(const float* x, const void* gate, int gate_type, const float* state, float* out, int64_t n, void* stream) {
     if (n < 0) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_gated_step: negative size");
+    if (n >= (1ll << 32)) return fail(SNNTC_ERR_TOO_LARGE, "snntc_gated_step: 2^32 elements and more");
     if (!known_type(gate_type)) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_gated_step: unknown gate type %d", gate_type);
     if (n == 0) return SNNTC_OK;
     if (!x || !gate || !out) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_gated_step: null pointer");

@@ -330,7 +330,7 @@ gated_scan_backward_kernel(const float* __restrict__ dy, const float* __restrict
 template <typename G>
 __global__ void __launch_bounds__(256)
 gated_step_kernel(const float* x, const G* gate, const float* state, float* out, long long n) {
-    const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long e = workgroup() * 256 + threadIdx.x;
     if (e >= n) return;
     const Gate g = gate_of((float)gate[e]);
     out[e] = g.a * (state ? state[e] : 0.0f) + g.rest * x[e];
@@ -409,11 +409,10 @@ int launch_gated_scan_backward(const float* dy, const float* dfinal, const float
 
 int launch_gated_step(const float* x, const void* gate, int type, const float* state, float* out, int64_t n, hipStream_t stream) {
     const int64_t blocks = (n + 255) / 256;
-    if (blocks >= (1 << 24)) return fail(SNNTC_ERR_TOO_LARGE, "gated step: 2^32 elements and more");
     with_type(type, [&](auto g) {
         using G = decltype(g);
         KernelTimerScope timer_("gated_step", stream);
-        hipLaunchKernelGGL(gated_step_kernel<G>, dim3((unsigned)blocks), dim3(256), 0, stream, x, static_cast<const G*>(gate), state, out,
+        hipLaunchKernelGGL(gated_step_kernel<G>, wide_grid(blocks, 256), dim3(256), 0, stream, x, static_cast<const G*>(gate), state, out,
                            (long long)n);
         return 0;
     });
