@@ -3,7 +3,12 @@
 // and its gradient, with u the gradient that reaches h_t:
 //     u_t = dy_t + a_{t+1} u_{t+1}  (the last step of a sequence: dy_t + dfinal)
 //     dx_t = (1 - a_t) u_t,   dgate_t = u_t (h_{t-1} - x_t) a_t (1 - a_t),   dstate = a_1 u_1
-// A step mixes two spike times, so what comes out lies between those that went in and is a spike time itself.
+// A step mixes two spike times, so what comes out lies between those that went in and is a spike time itself.  That needs a and 1 - a
+// to add up to one.  In float32 the half steps of each leave them off, by as much in every step alike where a gate stays, which the
+// 1 / (1 - a) steps of the mean add up: a constant came back 0.05 % off at gates of 10, 0.2 % at 12.  Gates, the state along a sequence and the maps
+// of its runs are therefore held in 64 bits, and a result is rounded to 32 once.  (What that costs, forward + backward in us, 32 bits / 64:
+// 32 x 256 x 800 14.4 + 26.1 / 15.7 + 26.2, 24 x 333 x 777 17.1 + 28.2 / 20.4 + 30.1, 16 x 6400 x 1024 200 + 430 / 201 + 429,
+// 16 x 32768 x 16 56 + 78 / 71 + 90.)
 #include <algorithm>
 
 #include "sequences.h"
@@ -11,14 +16,19 @@
 namespace snntc {
 namespace {
 
-// a = sigmoid(g) and 1 - a, each to its own precision: with e = exp(-g), a = 1 / (1 + e) and 1 - a = e a.  (Below -80, where 1 - a
-// is 1 and a below 2e-35, e is held finite.  A NaN stays one.)
-struct Gate { float a, rest; };
-__device__ __forceinline__ Gate gate_of(float g) {
-    const float e = exp_close(g < -80.0f ? 80.0f : -g);
-    const float a = __builtin_amdgcn_rcpf(1.0f + e);                     // (off by a step at most)
-    return Gate{a, e * a};
-}
+// a = sigmoid(g) and 1 - a: with e = exp(-g), a = 1 / (1 + e) and 1 - a = e a, each to its own precision.  e is a float32 number, off by
+// two steps at most, which moves both together; the reciprocal in 32 bits is off by a step, after a step of Newton's method in 64 by the
+// square of that, 2^-46, and so is a + (1 - a) from one.  (Below -80, where 1 - a is 1 and a below 2e-35, e is held finite.  A NaN stays one.)
+struct Gate {
+    float e, near;                                  // near: a, off by a step
+    __device__ __forceinline__ explicit Gate(float g) : e(exp_close(g < -80.0f ? 80.0f : -g)), near(__builtin_amdgcn_rcpf(1.0f + e)) {}
+    __device__ __forceinline__ double a() const {
+        const double whole = 1.0 + (double)e, r = (double)near;
+        return fma(r, fma(-whole, r, 1.0), r);
+    }
+};
+
+constexpr float kKeep = INFINITY;                   // the gate that leaves the state as it is: a = 1, 1 - a = 0
 
 __device__ __forceinline__ int length_of(const int64_t* lengths, int64_t b, int64_t T) {
     if (!lengths) return (int)T;
@@ -55,8 +65,8 @@ constexpr int kThreads = kWaves * kWave;
 constexpr int kDies = 8;
 constexpr int kFill = 160, kMany = 96, kUnits = 256, kShort = 6, kCutFill = 1024, kHalf = kWave / 2;
 
-struct Map { float A, H; };                         // h -> A h + H
-__device__ __forceinline__ Map then(const Map& first, const Map& second) { return Map{first.A * second.A, fmaf(second.A, first.H, second.H)}; }
+struct Map { double A, H; };                        // h -> A h + H
+__device__ __forceinline__ Map then(const Map& first, const Map& second) { return Map{first.A * second.A, fma(second.A, first.H, second.H)}; }
 
 struct Geometry {
     int B, T, D, groups, parts, part;               // groups of 64 (or 32) channels, parts of `part` steps (a multiple of kTile)
@@ -101,26 +111,26 @@ __device__ __forceinline__ Place place_of(const Geometry& g) {
 // Composition of maps[w][lane] over the wavefronts, w ascending (or descending) from the state h: what comes in at wavefront `wave`
 // and what goes out at the end.
 template <bool DOWN, int W>
-__device__ __forceinline__ float through(const Map (*maps)[W], const Place& p, float h, float* in) {
+__device__ __forceinline__ double through(const Map (*maps)[W], const Place& p, double h, double* in) {
     constexpr int kRuns = kThreads / W;
 #pragma unroll
     for (int k = 0; k < kRuns; ++k) {
         const int w = DOWN ? kRuns - 1 - k : k;
         if (w == p.run) *in = h;
         const Map m = maps[w][p.lane];
-        h = fmaf(m.A, h, m.H);
+        h = fma(m.A, h, m.H);
     }
     return h;
 }
 
 // The state with which part s begins, from the maps of the parts on its way: each wavefront composes a consecutive share of them.
 template <bool DOWN>
-__device__ __forceinline__ float enter_part(const Map* parts, const Geometry& g, const Place& p, Map (*maps)[kWave], float h) {
+__device__ __forceinline__ double enter_part(const Map* parts, const Geometry& g, const Place& p, Map (*maps)[kWave], double h) {
     const int count = DOWN ? g.parts - 1 - p.s : p.s;
     if (count == 0) return h;
     const int first = DOWN ? p.s + 1 : 0, per = (count + kWaves - 1) / kWaves;
     const int r0 = min(count, p.run * per), r1 = min(count, r0 + per);
-    Map m{1.0f, 0.0f};
+    Map m{1.0, 0.0};
 #pragma unroll 8
     for (int r = r0; r < r1; ++r) {
         // ascending in time; going down, the later part acts first
@@ -129,7 +139,7 @@ __device__ __forceinline__ float enter_part(const Map* parts, const Geometry& g,
     }
     maps[p.run][p.lane] = m;
     __syncthreads();
-    float unused;
+    double unused;
     h = through<DOWN, kWave>(maps, p, h, &unused);
     __syncthreads();
     return h;
@@ -145,7 +155,7 @@ gated_scan_forward_kernel(const float* __restrict__ x, const G* __restrict__ gat
     const Place p = place_of<W>(g);
     const int t0 = p.s * g.part, t1 = min(g.T, t0 + g.part);
     const int n = min(length_of(lengths, p.b, g.T), t1);                 // steps from n on are not there
-    float h = state ? state[p.b * g.D + p.d] : 0.0f;
+    double h = state ? (double)state[p.b * g.D + p.d] : 0.0;
     if constexpr (W == kWave) h = enter_part<false>(parts, g, p, maps[0], h);
     const size_t base = (size_t)p.b * g.T * g.D + p.d;
     float xn[kSteps];
@@ -169,29 +179,29 @@ gated_scan_forward_kernel(const float* __restrict__ x, const G* __restrict__ gat
                 if (t + i < t1 && p.valid) put<PAST>(out + (size_t)(t + i) * g.D, 0.0f);
             continue;
         }
-        float a[kSteps], b[kSteps];
-        Map m{1.0f, 0.0f};
+        double a[kSteps], b[kSteps];
+        Map m{1.0, 0.0};
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
-            const Gate q = gate_of((float)gn[i]);
-            a[i] = t + i < n ? q.a : 1.0f;
-            b[i] = t + i < n ? q.rest * xn[i] : 0.0f;
-            m.H = fmaf(a[i], m.H, b[i]);
+            const Gate q(t + i < n ? (float)gn[i] : kKeep);
+            a[i] = q.a();
+            b[i] = (double)q.e * a[i] * (double)(t + i < n ? xn[i] : 0.0f);
+            m.H = fma(a[i], m.H, b[i]);
             m.A *= a[i];
         }
         maps[buffer][p.run][p.lane] = m;
         if (tile + kSpan < n) request(t + kSpan);
         __syncthreads();
-        float in = h;
+        double in = h;
         h = through<false, W>(maps[buffer], p, h, &in);
-        buffer ^= 1;                                                     // (the other half is written behind the next barrier's readers)
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
-            in = fmaf(a[i], in, b[i]);
-            if (t + i < t1 && p.valid) put<PAST>(out + (size_t)(t + i) * g.D, t + i < n ? in : 0.0f);
+            in = fma(a[i], in, b[i]);
+            if (t + i < t1 && p.valid) put<PAST>(out + (size_t)(t + i) * g.D, t + i < n ? (float)in : 0.0f);
         }
+        buffer ^= 1;                                                     // (the other half is written behind the next barrier's readers)
     }
-    if (final_state && p.s == g.parts - 1 && p.run == 0 && p.valid) final_state[p.b * g.D + p.d] = h;
+    if (final_state && p.s == g.parts - 1 && p.run == 0 && p.valid) final_state[p.b * g.D + p.d] = (float)h;
 }
 
 // (A, H) of every part but the last on the way: forward of x and the gates, backward (DOWN) of the gradients v_t = a_t (dy_t + v_{t+1}).
@@ -210,7 +220,7 @@ gated_scan_parts_kernel(const float* __restrict__ x, const G* __restrict__ gate,
     const size_t base = (size_t)p.b * g.T * g.D + p.d;
     // each wavefront composes a consecutive share of the part's steps; shares are joined once
     const int share = g.part / kWaves, w0 = t0 + p.run * share, w1 = min(n, w0 + share);
-    Map m{1.0f, 0.0f};
+    Map m{1.0, 0.0};
     float xn[kSteps];
     G gn[kSteps];
     auto at = [&](int i) { return DOWN ? w1 - 1 - i : w0 + i; };        // the i-th step on the way
@@ -233,9 +243,10 @@ gated_scan_parts_kernel(const float* __restrict__ x, const G* __restrict__ gate,
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             if (i0 + i >= count) break;
-            const Gate q = gate_of((float)gv[i]);
-            m.H = DOWN ? q.a * (m.H + xv[i]) : fmaf(q.a, m.H, q.rest * xv[i]);
-            m.A *= q.a;
+            const Gate q((float)gv[i]);
+            const double a = q.a();
+            m.H = DOWN ? a * (m.H + (double)xv[i]) : fma(a, m.H, (double)q.e * a * (double)xv[i]);
+            m.A *= a;
         }
     }
     maps[p.run][p.lane] = m;
@@ -259,7 +270,7 @@ gated_scan_backward_kernel(const float* __restrict__ dy, const float* __restrict
     const Place p = place_of<W>(g);
     const int t0 = p.s * g.part, t1 = min(g.T, t0 + g.part);
     const int n = min(length_of(lengths, p.b, g.T), t1);
-    float v = dfinal ? dfinal[p.b * g.D + p.d] : 0.0f;
+    double v = dfinal ? (double)dfinal[p.b * g.D + p.d] : 0.0;
     if constexpr (W == kWave) v = enter_part<true>(parts, g, p, maps[0], v);
     const float start = state ? state[p.b * g.D + p.d] : 0.0f;
     const size_t base = (size_t)p.b * g.T * g.D + p.d;
@@ -293,38 +304,38 @@ gated_scan_backward_kernel(const float* __restrict__ dy, const float* __restrict
         }
         if (!asked) request(t);
         asked = true;
-        Gate q[kSteps];
-        float up[kSteps], lead[kSteps];
-        Map m{1.0f, 0.0f};
+        double a[kSteps];
+        float rest[kSteps], up[kSteps], slope[kSteps];               // slope: (h_{t-1} - x_t) a_t (1 - a_t)
+        Map m{1.0, 0.0};
 #pragma unroll
         for (int i = kSteps - 1; i >= 0; --i) {
-            const bool there = t + i < n;
-            q[i] = gate_of((float)gn[i]);
-            if (!there) q[i] = Gate{1.0f, 0.0f};
-            up[i] = there ? un[i] : 0.0f;
-            lead[i] = (t + i > 0 ? hn[i] : start) - xn[i];
-            m.H = q[i].a * (m.H + up[i]);
-            m.A *= q[i].a;
+            const Gate q(t + i < n ? (float)gn[i] : kKeep);
+            a[i] = q.a();
+            rest[i] = q.e * q.near;
+            up[i] = t + i < n ? un[i] : 0.0f;
+            slope[i] = ((t + i > 0 ? hn[i] : start) - xn[i]) * (rest[i] * q.near);
+            m.H = a[i] * (m.H + (double)up[i]);
+            m.A *= a[i];
         }
         maps[buffer][p.run][p.lane] = m;
         if (tile > t0) request(t - kSpan);
         __syncthreads();
-        float in = v;
+        double in = v;
         v = through<true, W>(maps[buffer], p, v, &in);
-        buffer ^= 1;
 #pragma unroll
         for (int i = kSteps - 1; i >= 0; --i) {
-            const float u = up[i] + in;
-            in = q[i].a * u;
+            const double sum = (double)up[i] + in;
+            const float u = (float)sum;
+            in = a[i] * sum;
             if (t + i < t1 && p.valid) {
-                const bool there = t + i < n;
                 const size_t e = base + (size_t)(t + i) * g.D;
-                if (dx) put<PAST>(dx + e, there ? q[i].rest * u : 0.0f);
-                if (dgate) put<PAST>(dgate + e, (G)(there ? u * lead[i] * (q[i].a * q[i].rest) : 0.0f));
+                if (dx) put<PAST>(dx + e, t + i < n ? rest[i] * u : 0.0f);
+                if (dgate) put<PAST>(dgate + e, (G)(t + i < n ? u * slope[i] : 0.0f));
             }
         }
+        buffer ^= 1;
     }
-    if (dstate && p.s == 0 && p.run == 0 && p.valid) dstate[p.b * g.D + p.d] = v;
+    if (dstate && p.s == 0 && p.run == 0 && p.valid) dstate[p.b * g.D + p.d] = (float)v;
 }
 
 template <typename G>
@@ -332,8 +343,9 @@ __global__ void __launch_bounds__(256)
 gated_step_kernel(const float* x, const G* gate, const float* state, float* out, long long n) {
     const long long e = workgroup() * 256 + threadIdx.x;
     if (e >= n) return;
-    const Gate g = gate_of((float)gate[e]);
-    out[e] = g.a * (state ? state[e] : 0.0f) + g.rest * x[e];
+    const Gate g((float)gate[e]);
+    const double a = g.a();
+    out[e] = (float)fma(a, state ? (double)state[e] : 0.0, (double)g.e * a * (double)x[e]);
 }
 
 }  // namespace
