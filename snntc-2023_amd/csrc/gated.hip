@@ -53,11 +53,15 @@ __device__ __forceinline__ int length_of(const int64_t* lengths, int64_t b, int6
 // steps, 128 groups 187 + 330 / 142 + 285; 384 steps, 32 groups 11 + 11 / 7 + 10; 512 steps, 32 groups 11 + 12 / 9 + 12, 16 groups
 // 9 + 10 / 8 + 12.
 //
-// Workgroups are dealt to the dies in turn.  Where rows, those of the gates among them, are not whole lines, neighbours go to one die, whose
-// cache then holds the lines that they share: in turn / neighbours together, 24 x 333 x 777 38 / 34 us, 16 x 2530 x 777 258 / 226,
-// 16 x 8434 x 777 941 / 753, 16 x 32768 x 200 1265 / 1128.  Where they are, in turn: 32768 x 1024, cut, 249 / 264, others the same.
-// Calls that touch more than the caches hold store past them, where rows are whole lines (a line stored by two groups has to meet
-// in a cache): 32768 x 1024 270 -> 249, 8 x 4096 x 1024 231 -> 215, 16 x 1920 x 1024 182 -> 171, 16 x 6400 x 1024 613 -> 600; 16 x 8434 x 777 753 -> 827.
+// Workgroups are dealt to the dies in turn.  Where neighbours share lines they go to one die, whose cache then holds those: where rows, those
+// of the gates among them, are not whole lines (in turn / neighbours together, 24 x 333 x 777 38 / 34 us, 16 x 2530 x 777 258 / 226,
+// 16 x 8434 x 777 941 / 753, 16 x 32768 x 200 1265 / 1128), and where 32 channels of 16-bit gates are half a line (8 x 1024 x 1024
+// 21.4 + 32.8 / 20.2 + 30.2, 8 x 4096 x 1024 66 + 154 / 63 + 155, 2 x 8192 x 4096 146 + 294 / 143 + 287).  Else in turn: 32768 x 1024, cut, 249 / 264,
+// others the same.
+// Calls that touch more than the caches hold store past them, where rows are whole lines (the ends of a row that is none are stored by two groups
+// that need not run at one time): 32768 x 1024 270 -> 249, 8 x 4096 x 1024 231 -> 215, 16 x 1920 x 1024 182 -> 171, 16 x 6400 x 1024 613 -> 600;
+// 16 x 8434 x 777 753 -> 827.  Half lines of 16-bit gates are among them, whose two halves neighbours on one die store together (through the
+// caches 8 x 4096 x 1024 78 + 159, 2 x 2048 x 4096 35 + 75 for 35 + 57).
 // Where sequences are cut, they load past them too, in the second and last reading: 32768 x 1024 249 -> 237, 16 x 102400 x 64 820 -> 745,
 // 16 x 30720 x 64 231 -> 224; whole ones gain less (16 x 6400 x 1024 626 -> 612) or lose what a cache still holds (8 x 4096 x 1024 211 -> 243).
 constexpr int kWaves = 8, kSteps = 8, kTile = kWaves * kSteps;
@@ -70,8 +74,9 @@ __device__ __forceinline__ Map then(const Map& first, const Map& second) { retur
 
 struct Geometry {
     int B, T, D, groups, parts, part;               // groups of 64 (or 32) channels, parts of `part` steps (a multiple of kTile)
-    bool shared_lines;                              // between neighbouring groups
     bool half;                                      // groups of 32
+    bool whole_lines;                               // rows are
+    bool together;                                  // neighbouring groups share lines: they go to one die
 };
 // What goes past the caches.
 enum Past { NONE, STORES, BOTH };
@@ -93,7 +98,7 @@ struct Place {
 template <int W>
 __device__ __forceinline__ Place place_of(const Geometry& g) {
     int block = blockIdx.x;
-    if (g.shared_lines) {
+    if (g.together) {
         const int die = blockIdx.x % kDies, each = gridDim.x / kDies, more = gridDim.x % kDies;
         block = die * each + min(die, more) + blockIdx.x / kDies;
     }
@@ -353,11 +358,12 @@ gated_step_kernel(const float* x, const G* gate, const float* state, float* out,
 namespace {
 constexpr int kLine = 128;
 Geometry geometry(int64_t B, int64_t T, int64_t D, int gate_bytes = 4) {
-    Geometry g{(int)B, (int)T, (int)D, (int)((D + kWave - 1) / kWave), 1, 0, D * gate_bytes % kLine != 0};
+    Geometry g{(int)B, (int)T, (int)D, (int)((D + kWave - 1) / kWave), 1, 0, false, D * gate_bytes % kLine == 0, false};
     const int64_t rows = B * g.groups, tiles = (T + kTile - 1) / kTile, halves = B * ((D + kHalf - 1) / kHalf);
     if (rows < kFill && tiles > kShort && (rows < kMany || halves > kUnits)) g.parts = (int)std::min(tiles, (kCutFill + rows - 1) / rows);
     g.half = rows < kFill && tiles > 1 && g.parts == 1;
     if (g.half) g.groups = (int)((D + kHalf - 1) / kHalf);
+    g.together = !g.whole_lines || (g.half && kHalf * gate_bytes % kLine != 0);
     g.part = (int)((tiles + g.parts - 1) / g.parts * kTile);
     g.parts = T > 0 ? (int)((T + g.part - 1) / g.part) : 1;
     return g;
@@ -381,7 +387,7 @@ int launch_gated_scan_forward(const float* x, const void* gate, int type, const 
                                static_cast<const G*>(gate), lengths, static_cast<Map*>(ws), g);
         }
         KernelTimerScope timer_("gated_scan_forward", stream);
-        const bool past = B * T * D * (int64_t)(2 * sizeof(float) + sizeof(G)) > kStreamBytes && !g.shared_lines;      // x, y, gates
+        const bool past = B * T * D * (int64_t)(2 * sizeof(float) + sizeof(G)) > kStreamBytes && g.whole_lines;      // x, y, gates
         auto kern = g.half ? (past ? gated_scan_forward_kernel<G, STORES, kHalf> : gated_scan_forward_kernel<G, NONE, kHalf>)
                     : !past ? gated_scan_forward_kernel<G, NONE, kWave>
                     : g.parts > 1 ? gated_scan_forward_kernel<G, BOTH, kWave> : gated_scan_forward_kernel<G, STORES, kWave>;
@@ -406,7 +412,7 @@ int launch_gated_scan_backward(const float* dy, const float* dfinal, const float
                                static_cast<const G*>(gate), lengths, static_cast<Map*>(ws), g);
         }
         KernelTimerScope timer_("gated_scan_backward", stream);
-        const bool past = B * T * D * (int64_t)(4 * sizeof(float) + 2 * sizeof(G)) > kStreamBytes && !g.shared_lines;  // dy, x, y, dx, gates, dgate
+        const bool past = B * T * D * (int64_t)(4 * sizeof(float) + 2 * sizeof(G)) > kStreamBytes && g.whole_lines;  // dy, x, y, dx, gates, dgate
         auto kern = g.half ? (past ? gated_scan_backward_kernel<G, STORES, kHalf> : gated_scan_backward_kernel<G, NONE, kHalf>)
                     : !past ? gated_scan_backward_kernel<G, NONE, kWave>
                     : g.parts > 1 ? gated_scan_backward_kernel<G, BOTH, kWave> : gated_scan_backward_kernel<G, STORES, kWave>;
