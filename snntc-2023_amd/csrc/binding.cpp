@@ -780,17 +780,18 @@ variable_list once(variable_list grads, const char* who) {
 
 struct EmbedNode : public Node {
     SavedVariable tokens, table;
+    Tensor shape;                                            // not encoded: in table's place, whose values the gradient does not need
     float scale;
     bool encode;
     std::string name() const override { return "SnnEmbedBackward"; }
     void release_variables() override {
         std::lock_guard<std::mutex> lock(mutex_);
-        tokens.reset_data(); table.reset_data();
+        tokens.reset_data(); table.reset_data(); shape.reset();
     }
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
         if (!grads[0].defined() || !task_should_compute_output(0)) return variable_list(1);
-        const Tensor tok = tokens.unpack(), tab = table.unpack();
+        const Tensor tok = tokens.unpack(), tab = encode ? table.unpack() : shape;
         variable_list out(1);
         {
             at::AutoGradMode no_grad(false);
@@ -810,7 +811,9 @@ Tensor embed_layer(const Tensor& tokens, const Tensor& table, float scale, bool 
     if (!wants_grad(a.table)) return z;
     auto node = make_node<EmbedNode>({a.table});
     node->scale = scale; node->encode = encode;
-    node->tokens = SavedVariable(a.tokens, false); node->table = SavedVariable(a.table, false);
+    node->tokens = SavedVariable(a.tokens, false);
+    if (encode) node->table = SavedVariable(a.table, false);
+    else node->shape = a.table.detach();
     return with_history(z, node);
 }
 

@@ -454,13 +454,15 @@ class SnnEmbed(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, tokens, table, scale, encode):
-        ctx.save_for_backward(tokens, table)
+        ctx.save_for_backward(tokens, table if encode else None)
         ctx.how = (scale, encode)
+        ctx.shape = None if encode else table.detach()        # whose values the gradient does not need
         return embed_tokens(tokens, table, scale, encode)
 
     @staticmethod
     def backward(ctx, grad):
-        return None, embed_tokens_grad(grad, *ctx.saved_tensors, *ctx.how), None, None
+        tokens, table = ctx.saved_tensors
+        return None, embed_tokens_grad(grad, tokens, ctx.shape if table is None else table, *ctx.how), None, None
 
 
 def gated_scan(x, gate, state=None, lengths=None):

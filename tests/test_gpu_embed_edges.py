@@ -35,3 +35,30 @@ def test_more_tokens_than_a_grid_dimension_holds(N, D):
             assert torch.isnan(z[-2]).all()
             z[-2], want[-2] = 0.0, 0.0
         assert torch.equal(z[part], want)
+
+
+def test_a_table_that_is_not_encoded_may_change_before_its_gradient():
+    """scale * table: the gradient does not read the table, so an update in between is no error; encoded, it does and is."""
+    import snntc_amd as snn
+    table = torch.rand(20, 6, device=DEV, requires_grad=True)
+    tok, up = torch.randint(0, 20, (40,), device=DEV), torch.randn(40, 6, device=DEV)
+    want = snn.embed_tokens_grad(up, tok, table.detach(), 0.5)
+    from snntc_amd import ops
+    for f in (snn.SnnEmbed.apply, ops.GENERAL["embed_layer"]):
+        z = f(tok, table, 0.5, False)
+        with torch.no_grad():
+            table.mul_(0.5)
+        (d,) = torch.autograd.grad(z, [table], up, retain_graph=True)
+        assert torch.equal(d, want) and torch.equal(torch.autograd.grad(z, [table], up)[0], want)
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(z, [table], up)
+        z = f(tok, table, 0.5, True)
+        with torch.no_grad():
+            table.mul_(0.5)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(z, [table], up)
+        z = f(tok, table, 0.5, False)
+        with torch.no_grad():
+            tok.clamp_(max=19)                                    # the tokens are read
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(z, [table], up)
