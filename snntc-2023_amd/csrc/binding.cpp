@@ -769,13 +769,22 @@ void sgd_update(const std::vector<Tensor>& ws, const std::vector<Tensor>& gs, fl
 
 // ---- layers and losses over sequences ---------------------------------------------------------------------------------
 
-// Gradients of nodes that can be differentiated once: where a graph of them is built, a pass through it raises.
-variable_list once(variable_list grads, const char* who) {
+// Gradients of a node that can be differentiated once: where a graph of them is built, a pass through it raises.  The node that does leads
+// on to all that the gradients depend on, the node's own inputs and the upstream gradients: a pass that is only to reach some of
+// these runs nothing else, and would leave these terms out.
+variable_list once(variable_list grads, const Node& node, const variable_list& upstream, const char* who) {
     if (!at::GradMode::is_enabled()) return grads;
-    for (Tensor& g : grads)
-        if (g.defined()) g = g.detach().requires_grad_(true);
-    const auto error = std::make_shared<torch::autograd::DelayedError>(std::string(who) + " can be differentiated once only", (int64_t)grads.size());
-    return (*error)(std::move(grads));
+    torch::autograd::edge_list edges = node.next_edges();
+    for (const Tensor& up : upstream)
+        if (up.defined()) edges.push_back(torch::autograd::impl::gradient_edge(up));
+    const std::shared_ptr<Node> error(new torch::autograd::Error(std::string(who) + " can be differentiated once only", std::move(edges)),
+                                      torch::autograd::deleteNode);
+    for (Tensor& g : grads) {
+        if (!g.defined()) continue;
+        g = g.detach();
+        torch::autograd::set_history(g, error);
+    }
+    return grads;
 }
 
 struct EmbedNode : public Node {
@@ -797,7 +806,7 @@ struct EmbedNode : public Node {
             at::AutoGradMode no_grad(false);
             out[0] = embed_tokens_grad(grads[0], embed_args(tok, tab, scale, encode));
         }
-        return once(std::move(out), "embed_tokens");
+        return once(std::move(out), *this, grads, "embed_tokens");
     }
 };
 
@@ -837,7 +846,7 @@ struct GatedNode : public Node {
                                           task_should_compute_output(1), has_state && task_should_compute_output(2));
             out[0] = g.dx; out[1] = g.dgate; out[2] = g.dstate;
         }
-        return once(std::move(out), "gated_scan");
+        return once(std::move(out), *this, grads, "gated_scan");
     }
 };
 
@@ -885,7 +894,7 @@ struct ChoiceNode : public Node {
             check(lib.snntc_time_logp_backward(raw(t), float_type(t), i64(k), f32(s), f32(c), f32(up), raw(out[0]), k.numel(), t.size(-1),
                                                stream_of(t)));
         }
-        return once(std::move(out), "a loss over choices");
+        return once(std::move(out), *this, grads, "a loss over choices");
     }
 };
 
