@@ -432,6 +432,19 @@ class SnnPadTime(torch.autograd.Function):
 # ---- sequences of tokens and choices ----------------------------------------------------------------------------
 
 
+def _once(who, grads, *depends):
+    """The gradients of an operator that can be differentiated once: where a graph of them is built, a pass through it raises, as
+    it does on the native path.  depends: the operator's inputs and the upstream gradients, which the graph leads on to (a pass that is
+    only to reach some of these would run nothing else, and leave these terms out)."""
+    if not torch.is_grad_enabled():
+        return grads
+    there = [g.detach().requires_grad_() for g in grads if g is not None]
+    joined = there + [d for d in depends if isinstance(d, torch.Tensor) and d.requires_grad]
+    marked = torch._C._functions.DelayedError(f"{who} can be differentiated once only", len(joined))(*joined)
+    marked = iter([marked] if isinstance(marked, torch.Tensor) else marked)
+    return tuple(None if g is None else next(marked) for g in grads)
+
+
 def embed_tokens(tokens, table, scale=1.0, encode=False):
     """Rows of table[V,D] as spike times: scale * table[tokens], or exp(1 - scale * table[tokens]) with encode=True,
     the encoding train.encode_input gives pixels.  tokens: int64 or int32 of any shape; table: float32, bfloat16 or
@@ -456,13 +469,16 @@ class SnnEmbed(torch.autograd.Function):
     def forward(ctx, tokens, table, scale, encode):
         ctx.save_for_backward(tokens, table if encode else None)
         ctx.how = (scale, encode)
-        ctx.shape = None if encode else table.detach()        # whose values the gradient does not need
+        ctx.table = None if encode else table                 # whose values the gradient does not need
         return embed_tokens(tokens, table, scale, encode)
 
     @staticmethod
     def backward(ctx, grad):
         tokens, table = ctx.saved_tensors
-        return None, embed_tokens_grad(grad, tokens, ctx.shape if table is None else table, *ctx.how), None, None
+        table = ctx.table if table is None else table
+        with torch.no_grad():
+            d = embed_tokens_grad(grad, tokens, table, *ctx.how)
+        return None, *_once("embed_tokens", [d], table, grad), None, None
 
 
 def gated_scan(x, gate, state=None, lengths=None):
@@ -501,7 +517,9 @@ class SnnGatedScan(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad_y, grad_final):
         want = ctx.needs_input_grad
-        return *gated_scan_grad(grad_y, grad_final, *ctx.saved_tensors, want[0], want[1], want[2]), None
+        with torch.no_grad():
+            grads = gated_scan_grad(grad_y, grad_final, *ctx.saved_tensors, want[0], want[1], want[2])
+        return *_once("gated_scan", grads, *ctx.saved_tensors[:2], ctx.saved_tensors[3], grad_y, grad_final), None
 
 
 def time_logp(times, tokens, weight=None):
@@ -536,12 +554,16 @@ class PolicyTimeLoss(torch.autograd.Function):
     def forward(ctx, times, actions, old_logp, advantage, ref_logp, weight, clip, kl_coef):
         loss, _, grad = policy_time_loss(times, actions, old_logp, advantage, ref_logp, weight, clip, kl_coef,
                                          want_grad=times.requires_grad)
-        ctx.save_for_backward(*[] if grad is None else [grad])
+        if grad is not None:
+            ctx.save_for_backward(times, grad)
         return _weighted_total(loss, weight)
 
     @staticmethod
     def backward(ctx, upstream):
-        return (ctx.saved_tensors[0] * upstream if ctx.saved_tensors else None), None, None, None, None, None, None, None
+        times, grad = ctx.saved_tensors
+        with torch.no_grad():
+            grad = grad * upstream
+        return *_once("a loss over choices", [grad], times, upstream), None, None, None, None, None, None, None
 
 
 def preference_time_loss(times, tokens, ref_logp, weight=None, beta=0.1, smoothing=0.0, want_grad=True):
@@ -564,12 +586,16 @@ class PreferenceTimeLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, times, tokens, ref_logp, weight, beta, smoothing):
         loss, _, grad = preference_time_loss(times, tokens, ref_logp, weight, beta, smoothing, want_grad=times.requires_grad)
-        ctx.save_for_backward(*[] if grad is None else [grad])
+        if grad is not None:
+            ctx.save_for_backward(times, grad)
         return _weighted_total(loss, None)
 
     @staticmethod
     def backward(ctx, upstream):
-        return (ctx.saved_tensors[0] * upstream if ctx.saved_tensors else None), None, None, None, None, None
+        times, grad = ctx.saved_tensors
+        with torch.no_grad():
+            grad = grad * upstream
+        return *_once("a loss over choices", [grad], times, upstream), None, None, None, None, None
 
 
 def _function(cls, *args):

@@ -62,7 +62,7 @@ def _run(f, inputs, watch):
     return f(*args), args
 
 
-@pytest.mark.parametrize("watch", [False])
+@pytest.mark.parametrize("watch", [False, True])
 @pytest.mark.parametrize("name", OPS)
 def test_a_second_derivative_is_refused_on_either_path(name, watch):
     """Whether the upstream gradient depends on the inputs or not: what is differentiated again has to say that it cannot be, where a
