@@ -445,6 +445,13 @@ def _once(who, grads, *depends):
     return tuple(None if g is None else next(marked) for g in grads)
 
 
+def _no_gradient(who, **tensors):
+    """A loss differentiates the times only, on this path as on the native one."""
+    for name, t in tensors.items():
+        if t is not None and t.requires_grad:
+            raise ValueError(f"{who}: {name} must not require a gradient")
+
+
 def embed_tokens(tokens, table, scale=1.0, encode=False):
     """Rows of table[V,D] as spike times: scale * table[tokens], or exp(1 - scale * table[tokens]) with encode=True,
     the encoding train.encode_input gives pixels.  tokens: int64 or int32 of any shape; table: float32, bfloat16 or
@@ -552,6 +559,7 @@ class PolicyTimeLoss(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, times, actions, old_logp, advantage, ref_logp, weight, clip, kl_coef):
+        _no_gradient("policy loss", old_logp=old_logp, advantage=advantage, ref_logp=ref_logp, weight=weight)
         loss, _, grad = policy_time_loss(times, actions, old_logp, advantage, ref_logp, weight, clip, kl_coef,
                                          want_grad=times.requires_grad)
         if grad is not None:
@@ -585,6 +593,7 @@ class PreferenceTimeLoss(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, times, tokens, ref_logp, weight, beta, smoothing):
+        _no_gradient("preference loss", ref_logp=ref_logp, weight=weight)
         loss, _, grad = preference_time_loss(times, tokens, ref_logp, weight, beta, smoothing, want_grad=times.requires_grad)
         if grad is not None:
             ctx.save_for_backward(times, grad)

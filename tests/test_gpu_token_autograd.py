@@ -76,3 +76,24 @@ def test_a_second_derivative_is_refused_on_either_path(name, watch):
         for g in first:
             with pytest.raises(RuntimeError, match="differentiated once only"):
                 torch.autograd.grad((g * g).sum() + sum((a * a).sum() for a in args), args, retain_graph=True)
+
+
+@pytest.mark.parametrize("watch", [False, True])
+def test_losses_refuse_other_inputs_that_require_a_gradient(watch):
+    """Only the times have one: None in its place would leave it out without a word."""
+    import contextlib
+    import snntc_amd as snn
+    times = (4 * _rand(4, 3, 6)).requires_grad_(True)
+    k = torch.zeros(4, 3, dtype=torch.int64, device=DEV)
+    f = -_rand(4, 3)
+    names = ("old_logp", "advantage", "ref_logp", "weight")
+    for name in names:
+        args = {n: f.clone().requires_grad_(n == name) for n in names}
+        with _Watch() if watch else contextlib.nullcontext():
+            with pytest.raises(ValueError, match=f"policy loss: {name} must not require a gradient"):
+                snn.policy_loss(times, k, **args, kl_coef=0.1)
+    for name in ("ref_logp", "weight"):
+        args = {n: t.clone().requires_grad_(n == name) for n, t in (("ref_logp", f[:, 0]), ("weight", f))}
+        with _Watch() if watch else contextlib.nullcontext():
+            with pytest.raises(ValueError, match=f"preference loss: {name} must not require a gradient"):
+                snn.preference_loss(times, k, **args)
