@@ -522,6 +522,32 @@ Tensor loss_total(const Tensor& loss, const Tensor& weight) {
     return total;
 }
 
+// An objective, and what its gradient is made from if that is wanted (`save`).
+struct Objective { Tensor total, stats, coef; };
+
+Objective policy_objective(const ChoiceArgs& a, const PolicyIn& p, bool save) {
+    const ChoiceOut r = policy_loss(a, p, false, save);
+    const c10::DeviceGuard guard(a.times.device());
+    return {loss_total(r.loss, a.weight), r.stats, r.coef};
+}
+
+Objective preference_objective(const ChoiceArgs& a, const Tensor& ref, float beta, float smoothing, bool save) {
+    const ChoiceOut r = preference_loss(a, ref, beta, smoothing, false, save);
+    const c10::DeviceGuard guard(a.times.device());
+    return {loss_total(r.loss, Tensor()), r.stats, r.coef};
+}
+
+// The gradient of an objective by the times, from the row statistics and the derivative by each row's log-probability that it has left.
+Tensor objective_grad(const ChoiceArgs& a, const Tensor& stats_in, const Tensor& coef_in, const Tensor& upstream) {
+    const Tensor stats = f32_like(stats_in, a.times, {a.rows, 2}, "stats"), coef = f32_like(coef_in, a.times, {a.rows}, "coef"),
+                 up = f32_like(upstream, a.times, {}, "upstream");
+    const c10::DeviceGuard guard(a.times.device());
+    const Tensor d = empty(a.times, a.times.sizes());
+    check(lib.snntc_time_logp_backward(raw(a.times), float_type(a.times), i64(a.tokens), f32(stats), f32(coef), f32(up), raw(d), a.rows, a.J,
+                                       stream_of(a.times)));
+    return d;
+}
+
 // ---- autograd nodes ------------------------------------------------------------------------------------------------
 
 template <typename N>
@@ -888,49 +914,39 @@ struct ChoiceNode : public Node {
         variable_list out(1);
         {
             at::AutoGradMode no_grad(false);
-            const c10::DeviceGuard guard(t.device());
-            const Tensor up = grads[0].contiguous();
-            out[0] = empty(t, t.sizes());
-            check(lib.snntc_time_logp_backward(raw(t), float_type(t), i64(k), f32(s), f32(c), f32(up), raw(out[0]), k.numel(), t.size(-1),
-                                               stream_of(t)));
+            out[0] = objective_grad(choice_args(t, k, Tensor(), "tokens"), s, c, grads[0]);
         }
         return once(std::move(out), *this, grads, "a loss over choices");
     }
 };
 
-Tensor choice_history(const Tensor& total, const ChoiceArgs& a, const ChoiceOut& r) {
+Tensor choice_history(const ChoiceArgs& a, const Objective& r) {
     auto node = make_node<ChoiceNode>({a.times});
     node->times = SavedVariable(a.times, false); node->tokens = SavedVariable(a.tokens, false);
     node->stats = SavedVariable(r.stats, false); node->coef = SavedVariable(r.coef, false);
-    return with_history(total, node);
+    return with_history(r.total, node);
 }
 
 Tensor policy_layer(const ChoiceArgs& a, const PolicyIn& p) {
     no_gradient({{&p.old_logp, "old_logp"}, {&p.advantage, "advantage"}, {&p.ref_logp, "ref_logp"}, {&a.weight, "weight"}}, "policy loss");
     const bool grad = wants_grad(a.times);
-    ChoiceOut r;
-    Tensor total;
+    Objective r;
     {
         at::AutoGradMode no_grad(false);
-        r = policy_loss(a, p, false, grad);
-        const c10::DeviceGuard guard(a.times.device());
-        total = loss_total(r.loss, a.weight);
+        r = policy_objective(a, p, grad);
     }
-    return grad ? choice_history(total, a, r) : total;
+    return grad ? choice_history(a, r) : r.total;
 }
 
 Tensor preference_layer(const ChoiceArgs& a, const Tensor& ref, float beta, float smoothing) {
     no_gradient({{&ref, "ref_logp"}, {&a.weight, "weight"}}, "preference loss");
     const bool grad = wants_grad(a.times);
-    ChoiceOut r;
-    Tensor total;
+    Objective r;
     {
         at::AutoGradMode no_grad(false);
-        r = preference_loss(a, ref, beta, smoothing, false, grad);
-        const c10::DeviceGuard guard(a.times.device());
-        total = loss_total(r.loss, Tensor());
+        r = preference_objective(a, ref, beta, smoothing, grad);
     }
-    return grad ? choice_history(total, a, r) : total;
+    return grad ? choice_history(a, r) : r.total;
 }
 
 // ---- the example training recipe -------------------------------------------------------------------------------------
@@ -1677,20 +1693,54 @@ SNNTC_METHOD(py_preference_layer) {
     END_HANDLE_TH_ERRORS
 }
 
-// loss_total(loss, weight) -> sum of weight loss, or the mean
-SNNTC_METHOD(py_loss_total) {
+// policy_objective(times, actions, old_logp, advantage, ref_logp, weight, clip_low, clip_high, kl_coef, save) -> (objective, stats, coef)
+SNNTC_METHOD(py_policy_objective) {
     HANDLE_TH_ERRORS
-    arity(n, 2, "loss_total");
-    const Tensor l = tensor_arg(a[0], "loss"), w = optional_tensor(a[1], "weight");
-    Tensor total;
+    arity(n, 10, "policy_objective");
+    const Tensor t = tensor_arg(a[0], "times"), k = tensor_arg(a[1], "actions"), w = optional_tensor(a[5], "weight");
+    const PolicyIn p = policy_in(a + 2);
+    const bool save = bool_arg(a[9]);
+    Objective r;
     {
         NoGil nogil;
         at::AutoGradMode no_grad(false);
-        const Tensor lc = dev_f32(l, "loss", l.dim());
-        const c10::DeviceGuard guard(lc.device());
-        total = loss_total(lc, f32_like(w, lc, lc.sizes(), "weight"));
+        r = policy_objective(choice_args(t, k, w, "actions"), p, save);
     }
-    return wrap(total);
+    return wrap3(r.total, r.stats, r.coef);
+    END_HANDLE_TH_ERRORS
+}
+
+// preference_objective(times, tokens, ref_logp, weight, beta, smoothing, save) -> (objective, stats, coef)
+SNNTC_METHOD(py_preference_objective) {
+    HANDLE_TH_ERRORS
+    arity(n, 7, "preference_objective");
+    const Tensor t = tensor_arg(a[0], "times"), k = tensor_arg(a[1], "tokens"), ref = tensor_arg(a[2], "ref_logp"),
+                 w = optional_tensor(a[3], "weight");
+    const float beta = float_arg(a[4]), smoothing = float_arg(a[5]);
+    const bool save = bool_arg(a[6]);
+    Objective r;
+    {
+        NoGil nogil;
+        at::AutoGradMode no_grad(false);
+        r = preference_objective(choice_args(t, k, w, "tokens"), ref, beta, smoothing, save);
+    }
+    return wrap3(r.total, r.stats, r.coef);
+    END_HANDLE_TH_ERRORS
+}
+
+// objective_grad(times, tokens, stats, coef, upstream) -> dtimes
+SNNTC_METHOD(py_objective_grad) {
+    HANDLE_TH_ERRORS
+    arity(n, 5, "objective_grad");
+    const Tensor t = tensor_arg(a[0], "times"), k = tensor_arg(a[1], "tokens"), s = tensor_arg(a[2], "stats"), c = tensor_arg(a[3], "coef"),
+                 up = tensor_arg(a[4], "upstream");
+    Tensor d;
+    {
+        NoGil nogil;
+        at::AutoGradMode no_grad(false);
+        d = objective_grad(choice_args(t, k, Tensor(), "tokens"), s, c, up);
+    }
+    return wrap(d);
     END_HANDLE_TH_ERRORS
 }
 
@@ -1726,7 +1776,8 @@ PyMethodDef g_methods[] = {SNNTC_ENTRY(bind), SNNTC_ENTRY(fc_forward), SNNTC_ENT
                            SNNTC_ENTRY(embed_tokens_grad), SNNTC_ENTRY(embed_layer), SNNTC_ENTRY(gated_scan),
                            SNNTC_ENTRY(gated_scan_grad), SNNTC_ENTRY(gated_layer), SNNTC_ENTRY(gated_step), SNNTC_ENTRY(time_logp),
                            SNNTC_ENTRY(policy_loss), SNNTC_ENTRY(policy_layer), SNNTC_ENTRY(preference_loss),
-                           SNNTC_ENTRY(preference_layer), SNNTC_ENTRY(loss_total), {nullptr, nullptr, 0, nullptr}};
+                           SNNTC_ENTRY(preference_layer), SNNTC_ENTRY(policy_objective),
+                           SNNTC_ENTRY(preference_objective), SNNTC_ENTRY(objective_grad), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_binding", "Native host path of the SNN-TC ops.", -1, g_methods,
                         nullptr, nullptr, nullptr, nullptr};

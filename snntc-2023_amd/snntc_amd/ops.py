@@ -445,6 +445,13 @@ def _once(who, grads, *depends):
     return tuple(None if g is None else next(marked) for g in grads)
 
 
+def _objective_grad(ctx, upstream):
+    """From the rows' statistics and the derivatives by their log-probabilities that the forward pass has left."""
+    with torch.no_grad():
+        grad = _lib.native().objective_grad(*ctx.saved_tensors, upstream)
+    return _once("a loss over choices", [grad], ctx.saved_tensors[0], upstream)
+
+
 def _no_gradient(who, **tensors):
     """A loss differentiates the times only, on this path as on the native one."""
     for name, t in tensors.items():
@@ -546,10 +553,6 @@ def policy_time_loss(times, actions, old_logp, advantage, ref_logp=None, weight=
     return _lib.native().policy_loss(times, actions, old_logp, advantage, ref_logp, weight, clip[0], clip[1], kl_coef, want_grad)
 
 
-def _weighted_total(loss, weight):
-    return _lib.native().loss_total(loss, weight)
-
-
 class PolicyTimeLoss(torch.autograd.Function):
     """The objective of policy_time_loss, differentiable in times."""
 
@@ -560,18 +563,14 @@ class PolicyTimeLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, times, actions, old_logp, advantage, ref_logp, weight, clip, kl_coef):
         _no_gradient("policy loss", old_logp=old_logp, advantage=advantage, ref_logp=ref_logp, weight=weight)
-        loss, _, grad = policy_time_loss(times, actions, old_logp, advantage, ref_logp, weight, clip, kl_coef,
-                                         want_grad=times.requires_grad)
-        if grad is not None:
-            ctx.save_for_backward(times, grad)
-        return _weighted_total(loss, weight)
+        total, *rows = _lib.native().policy_objective(times, actions, old_logp, advantage, ref_logp, weight, clip[0], clip[1], kl_coef,
+                                                      times.requires_grad)
+        ctx.save_for_backward(times, actions, *rows)
+        return total
 
     @staticmethod
     def backward(ctx, upstream):
-        times, grad = ctx.saved_tensors
-        with torch.no_grad():
-            grad = grad * upstream
-        return *_once("a loss over choices", [grad], times, upstream), None, None, None, None, None, None, None
+        return *_objective_grad(ctx, upstream), None, None, None, None, None, None, None
 
 
 def preference_time_loss(times, tokens, ref_logp, weight=None, beta=0.1, smoothing=0.0, want_grad=True):
@@ -594,17 +593,13 @@ class PreferenceTimeLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, times, tokens, ref_logp, weight, beta, smoothing):
         _no_gradient("preference loss", ref_logp=ref_logp, weight=weight)
-        loss, _, grad = preference_time_loss(times, tokens, ref_logp, weight, beta, smoothing, want_grad=times.requires_grad)
-        if grad is not None:
-            ctx.save_for_backward(times, grad)
-        return _weighted_total(loss, None)
+        total, *rows = _lib.native().preference_objective(times, tokens, ref_logp, weight, beta, smoothing, times.requires_grad)
+        ctx.save_for_backward(times, tokens, *rows)
+        return total
 
     @staticmethod
     def backward(ctx, upstream):
-        times, grad = ctx.saved_tensors
-        with torch.no_grad():
-            grad = grad * upstream
-        return *_once("a loss over choices", [grad], times, upstream), None, None, None, None, None
+        return *_objective_grad(ctx, upstream), None, None, None, None, None
 
 
 def _function(cls, *args):

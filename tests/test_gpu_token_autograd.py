@@ -97,3 +97,46 @@ def test_losses_refuse_other_inputs_that_require_a_gradient(watch):
         with _Watch() if watch else contextlib.nullcontext():
             with pytest.raises(ValueError, match=f"preference loss: {name} must not require a gradient"):
                 snn.preference_loss(times, k, **args)
+
+
+@pytest.mark.parametrize("name", OPS)
+def test_the_function_and_the_native_node_agree(name):
+    f, inputs = _ops()[name]
+    (a, native), (b, function) = _run(f, inputs, False), _run(f, inputs, True)
+    assert type(a.grad_fn).__name__ != type(b.grad_fn).__name__ and torch.equal(a, b)
+    up = _rand(1, *a.shape, seed=5)[0]
+    for x, y in zip(torch.autograd.grad(a, native, up), torch.autograd.grad(b, function, up)):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_gradients_of_16_bits_are_rounded_once_behind_the_upstream_factor(dtype):
+    """A loss scale keeps float16 gradients above its smallest numbers, 2^-24: they are not rounded before it is in them."""
+    import snntc_amd as snn
+    k = torch.randint(0, 6, (4, 3), generator=torch.Generator().manual_seed(2)).to(DEV)
+    times = (4 * _rand(4, 3, 6)).to(dtype)
+    old, adv = -2.0 - _rand(4, 3), _rand(4, 3, seed=1) - 0.5
+    weight = torch.full((4, 3), 2.0 ** -30, device=DEV)
+    # (ratios that are never clipped: every row has a gradient)
+    for loss in (lambda t: snn.policy_loss(t, k, old, adv, weight=weight, clip=(1.0, 1e9)), lambda t: snn.preference_loss(t, k, old[:, 0].contiguous(), weight)):
+        grads = []
+        for watch in (False, True):
+            out, (leaf,) = _run(loss, (times,), watch)
+            grads += torch.autograd.grad(out * 2.0 ** 30, [leaf])
+        assert torch.equal(*grads) and float((grads[0] != 0).float().mean()) > 0.9
+
+
+def test_nothing_of_the_times_size_but_the_times_is_kept():
+    import snntc_amd as snn
+    times = (4 * _rand(4, 3, 600)).requires_grad_(True)
+    k, f = torch.zeros(4, 3, dtype=torch.int64, device=DEV), -_rand(4, 3)
+    for loss in (lambda: snn.policy_loss(times, k, f, f), lambda: snn.preference_loss(times, k, f[:, 0].contiguous())):
+        for watch in (False, True):
+            kept = []
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
+                if watch:
+                    with _Watch():
+                        loss()
+                else:
+                    loss()
+            assert kept and all(t.data_ptr() == times.data_ptr() or t.numel() <= 2 * k.numel() for t in kept)
