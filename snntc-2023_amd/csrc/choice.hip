@@ -17,12 +17,13 @@ namespace {
 // Running maximum m and sum s of exp(v - m); empty: m = -inf, s = 0.
 struct Soft { float m, s; };
 // exp by the hardware's base-2 exponential: the argument's product with log2(e) adds its own size in half steps to the result's
-// error, of terms that shrink faster than that grows.
+// error, of terms that shrink faster than that grows.  For the terms of sums, and for gradients that are rounded to 16 bits; an element of
+// a float32 gradient is one exponential by itself (off by up to 32 half steps at times of 13 that way, by 5 with what the product loses).
 __device__ __forceinline__ float exp_fast(float v) { return __builtin_amdgcn_exp2f(v * 1.44269504f); }
 __device__ __forceinline__ Soft join(const Soft& a, const Soft& b) {
     const float m = fmaxf(a.m, b.m);
     if (m == -INFINITY) return Soft{m, a.s + b.s};                     // nothing yet (or a NaN sum to keep)
-    return Soft{m, a.s * exp_fast(a.m - m) + b.s * exp_fast(b.m - m)};
+    return Soft{m, a.s * exp_close(a.m - m) + b.s * exp_close(b.m - m)};
 }
 template <int WIDTH>
 __device__ __forceinline__ float group_max(float v) {
@@ -116,7 +117,12 @@ __device__ __forceinline__ int odd_element(const Cut& c, int k) {
     return k >= VEC && k < VEC + c.tail ? c.lead + c.pieces * VEC + k - VEC : -1;
 }
 
-__device__ __forceinline__ float grad_of(float t, const float2& soft, float c) { return c * exp_fast((-t - soft.x) - soft.y); }
+// c p of an element, from the row's maximum and c over its sum.
+template <typename E>
+__device__ __forceinline__ float grad_of(E t, float top, float share) {
+    const float v = -(float)t - top;
+    return share * (sizeof(E) == sizeof(float) ? exp_close(v) : exp_fast(v));
+}
 
 // WIDTH threads own a row and hold all of it in registers, so that it is read once: R pieces each, at most WIDTH * R * VEC elements and
 // the odd ones.  Up to 64 threads a row: several rows a workgroup.
@@ -161,10 +167,11 @@ choice_row_kernel(const E* __restrict__ times, E* __restrict__ dtimes, RowArgs a
     const long long token = a.tokens[r];
     const bool known = token >= 0 && token < a.J;
     float2 soft;
-    float c = w;
+    float c = w, share;
     if (MODE == GRAD) {
         soft = a.stats[r];
         if (a.upstream) c *= *a.upstream;
+        share = c * exp_close(-soft.y);
     } else {
         const float chosen = known ? (float)t[token] : NAN;
         float m = -single;
@@ -205,6 +212,7 @@ choice_row_kernel(const E* __restrict__ times, E* __restrict__ dtimes, RowArgs a
             if (MODE == POLICY && a.coef) a.coef[r] = c;
         }
         if (MODE == LOGP || !dtimes) return;
+        share = c / all.s;
     }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
@@ -213,7 +221,7 @@ choice_row_kernel(const E* __restrict__ times, E* __restrict__ dtimes, RowArgs a
         const int j0 = cut.lead + (i * WIDTH + k) * VEC;
         float d[VEC];
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) d[v] = grad_of((float)held[i].v[v], soft, c);
+        for (int v = 0; v < VEC; ++v) d[v] = grad_of<E>(held[i].v[v], soft.x, share);
         if (token >= j0 && token < j0 + VEC) {
 #pragma unroll
             for (int v = 0; v < VEC; ++v) d[v] -= token == j0 + v ? c : 0.0f;
@@ -223,7 +231,7 @@ choice_row_kernel(const E* __restrict__ times, E* __restrict__ dtimes, RowArgs a
         for (int v = 0; v < VEC; ++v) out.v[v] = (E)d[v];
         store_piece<STREAM>(reinterpret_cast<P*>(g + cut.lead) + i * WIDTH + k, out);
     }
-    if (odd >= 0) g[odd] = (E)(grad_of(single, soft, c) - (token == odd ? c : 0.0f));
+    if (odd >= 0) g[odd] = (E)(grad_of<E>((E)single, soft.x, share) - (token == odd ? c : 0.0f));
 }
 
 // Rows longer than a workgroup holds: slices of slice_pieces() pieces, a workgroup each.  One pass leaves (maximum, sum) of every slice; what
@@ -271,7 +279,7 @@ choice_slice_kernel(const E* __restrict__ times, const float* __restrict__ weigh
         all = join(all, Soft{m, sum});
     }
     const float m = group_max<kWave>(all.m);
-    all = Soft{m, group_sum<kWave>(m == -INFINITY ? all.s : all.s * exp_fast(all.m - m))};
+    all = Soft{m, group_sum<kWave>(m == -INFINITY ? all.s : all.s * exp_close(all.m - m))};
     if (k % kWave == 0) part[k / kWave] = all;
     __syncthreads();
     if (k != 0) return;
@@ -281,10 +289,10 @@ choice_slice_kernel(const E* __restrict__ times, const float* __restrict__ weigh
 }
 
 // A wavefront joins the slices of row r: its statistics, log-probability, loss and derivative (0 for a row of weight 0).
-struct Joined { float2 soft; float lp, loss, coef; };
+struct Joined { float2 soft; float lp, loss, coef, sum; };
 template <typename E, Mode MODE>
 __device__ __forceinline__ Joined join_slices(const E* times, const Soft* partial, const RowArgs& a, int64_t r, int slices, int lane) {
-    Joined out{float2{0.0f, 0.0f}, 0.0f, 0.0f, 0.0f};
+    Joined out{float2{0.0f, 0.0f}, 0.0f, 0.0f, 0.0f, 1.0f};
     const float w = MODE == POLICY && !a.weight ? a.policy.mean : row_weight(a.weight, r);
     if (w == 0.0f) return out;
     const long long token = a.tokens[r];
@@ -292,8 +300,9 @@ __device__ __forceinline__ Joined join_slices(const E* times, const Soft* partia
     Soft all{-INFINITY, 0.0f};
     for (int i = lane; i < slices; i += kWave) all = join(all, partial[r * slices + i]);
     const float m = group_max<kWave>(all.m);
-    all = Soft{m, group_sum<kWave>(m == -INFINITY ? all.s : all.s * exp_fast(all.m - m))};
+    all = Soft{m, group_sum<kWave>(m == -INFINITY ? all.s : all.s * exp_close(all.m - m))};
     out.soft = float2{all.m, logf(all.s)};
+    out.sum = all.s;
     out.lp = (-chosen - out.soft.x) - out.soft.y;
     if (MODE == POLICY) {
         const RowLoss loss = policy_row(a.policy, r, out.lp);
@@ -331,26 +340,28 @@ choice_slice_grad_kernel(const E* __restrict__ times, E* __restrict__ dtimes, co
     E* __restrict__ g = dtimes + (size_t)r * a.J;
     const Cut cut = cut_row<E, VEC>(t, a.J);
     const int odd = slice == 0 ? odd_element<VEC>(cut, k) : -1;
-    float c;
-    float2 soft;
+    float c, top, share;
     if (MODE == POLICY) {
         __shared__ float shared[3];
         if (k < kWave) {
             const Joined j = join_slices<E, MODE>(times, partial, a, r, slices, k);
             if (k == 0) {
-                shared[0] = j.coef; shared[1] = j.soft.x; shared[2] = j.soft.y;
+                shared[0] = j.coef; shared[1] = j.soft.x; shared[2] = j.coef / j.sum;
                 if (slice == 0) store_joined<MODE>(a, r, j);
             }
         }
         __syncthreads();
-        c = shared[0];
-        soft = float2{shared[1], shared[2]};
+        c = shared[0]; top = shared[1]; share = shared[2];
     } else {
         c = a.coef[r];
-        soft = a.stats[r];
     }
     const bool off = c == 0.0f;
-    if (MODE == GRAD && a.upstream) c *= *a.upstream;
+    if (MODE == GRAD) {
+        const float2 soft = a.stats[r];
+        if (a.upstream) c *= *a.upstream;
+        top = soft.x;
+        share = c * exp_close(-soft.y);
+    }
     const long long token = off ? -1 : a.tokens[r];
 #pragma unroll
     for (int i0 = 0; i0 < kEach; i0 += kBatch) {
@@ -369,7 +380,7 @@ choice_slice_grad_kernel(const E* __restrict__ times, E* __restrict__ dtimes, co
             if (!off) {
                 float d[VEC];
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) d[v] = grad_of((float)held[i].v[v], soft, c);
+                for (int v = 0; v < VEC; ++v) d[v] = grad_of<E>(held[i].v[v], top, share);
                 if (token >= j0 && token < j0 + VEC) {
 #pragma unroll
                     for (int v = 0; v < VEC; ++v) d[v] -= token == j0 + v ? c : 0.0f;
@@ -380,7 +391,7 @@ choice_slice_grad_kernel(const E* __restrict__ times, E* __restrict__ dtimes, co
             store_piece<STREAM>(reinterpret_cast<P*>(g + cut.lead) + piece, out);
         }
     }
-    if (odd >= 0) g[odd] = off ? (E)0.0f : (E)(grad_of((float)t[odd], soft, c) - (token == odd ? c : 0.0f));
+    if (odd >= 0) g[odd] = off ? (E)0.0f : (E)(grad_of<E>(t[odd], top, share) - (token == odd ? c : 0.0f));
 }
 
 __device__ __forceinline__ float wave_sum(float v) { return group_sum<kWave>(v); }

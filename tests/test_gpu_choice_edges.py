@@ -107,3 +107,25 @@ def test_more_slices_than_a_grid_dimension_holds():
     assert _like(grad[some], one[2], torch.bfloat16)
     grad[some] = 0.0
     assert not any(part.any() for part in grad.split(2 ** 20))
+
+
+@pytest.mark.parametrize("J", [100, 1000, 9000, 20000, 70000])
+def test_float32_gradients_of_unlikely_outputs(J):
+    """An element is a single exponential, times what its row has in common.  Of times in steps of 2^-10, whose differences are exact, it stands
+    to the row's earliest output, whose exponential is 1, as exp of their difference: but for two steps of the exponential (4 half steps U of
+    float32) and the product's rounding."""
+    import snntc_amd as snn
+    U = 2.0 ** -24
+    gen = torch.Generator().manual_seed(J)
+    times = (1.0 + torch.randint(0, 12 * 1024, (8, J), generator=gen) / 1024.0).float()
+    times[:, :2] = 1.0
+    want = torch.exp(1.0 - times.double())
+    t, k = times.to(DEV), torch.zeros(8, dtype=torch.int64, device=DEV)
+    old, adv = torch.full((8,), -3.0, device=DEV), -torch.ones(8, device=DEV)
+    _, _, direct = snn.policy_time_loss(t, k, old, adv, clip=(1.0, 1e9))          # (never clipped)
+    leaf = t.clone().requires_grad_(True)
+    (saved,) = torch.autograd.grad(snn.policy_loss(leaf, k, old, adv, clip=(1.0, 1e9)), [leaf])
+    for got in (direct, saved):
+        g = got.double().cpu()
+        error = (g[:, 2:] / (g[:, 1:2] * want[:, 2:]) - 1.0).abs().max()
+        assert error <= 5.01 * U, f"{float(error / U):.1f} half steps"
