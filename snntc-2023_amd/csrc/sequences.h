@@ -32,12 +32,13 @@ __device__ __forceinline__ int64_t workgroup() { return (int64_t)blockIdx.y * gr
 constexpr int64_t kStreamBytes = 256ll << 20;
 
 // exp(v) by the hardware's base-2 exponential: v log2(e) is rounded once, and what the rounding and log2(e)'s own have lost is put back to
-// first order, so the result is off by two steps at most (one half-step of t is worth |t| half-steps of 2^t otherwise).  Below 2^-126
-// the result is 0.  About half of the library function's instructions.
+// first order, so the result is off by the hardware's step and half of one (one half-step of t is worth |t| half-steps of 2^t otherwise).
+// The library's function is off by one step; this is about half of its instructions.  Below 2^-126 the result is 0.
 __device__ __forceinline__ float exp_close(float v) {
     const float t = v * 1.44269502f;                                     // float(log2 e)
     const float lost = fmaf(v, 1.44269502f, -t) + v * 1.92596299e-8f;    // log2 e - float(log2 e)
-    return __builtin_amdgcn_exp2f(t) * fmaf(fabsf(t) < 256.0f ? lost : 0.0f, 0.693147181f, 1.0f);
+    const float near = __builtin_amdgcn_exp2f(t);
+    return fabsf(t) < 128.0f ? fmaf(near, lost * 0.693147181f, near) : near;           // (else 0, infinity or NaN)
 }
 
 int launch_embed_forward(const void* tokens, int token_bytes, const void* table, int type, float* z, int64_t N, int64_t V, int64_t D,

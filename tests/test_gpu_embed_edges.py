@@ -62,3 +62,16 @@ def test_a_table_that_is_not_encoded_may_change_before_its_gradient():
             tok.clamp_(max=19)                                    # the tokens are read
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             torch.autograd.grad(z, [table], up)
+
+
+def test_encoded_times_are_off_by_less_than_one_and_a_half_steps():
+    """The hardware's exponential is off by a step, what its argument has lost is put back, and the result is rounded once: of intensities in
+    steps of 2^-12, whose distance from one is exact, 3 half steps at most (and the loss put back has its own roundings: a percent)."""
+    import snntc_amd as snn
+    e = torch.arange(-8192, 8193, device=DEV).float().view(-1, 1) / 4096.0
+    z = snn.embed_tokens(torch.arange(len(e), device=DEV), e, 1.0, True).double()
+    want = torch.exp(1.0 - e.double())
+    step = 2.0 ** (torch.floor(torch.log2(want)) - 23)
+    worst, mean = float(((z - want).abs() / step).max()), float(((z - want).abs() / step).mean())
+    assert worst <= 1.515, f"{worst:.3f} steps, {mean:.3f} in the mean"
+    print(f"{worst:.3f} steps, {mean:.3f} in the mean")
