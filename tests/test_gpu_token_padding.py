@@ -42,3 +42,25 @@ def test_lengths_of_another_kind_are_refused_by_the_op():
         recur(x, None, torch.tensor([5, 4, 1], device=DEV, dtype=torch.int32))
     with pytest.raises(snn.SnntcLibraryError, match="lives on cpu"):
         recur(x, None, torch.tensor([5, 4, 1]))
+
+
+def test_a_padded_training_step_from_tokens_to_the_loss():
+    """The whole path, padding behind the lengths and of weight 0 in the loss: the same loss and the same gradients whatever the padding is."""
+    import snntc_amd as snn
+    from snntc_amd import networks
+    net = networks.build([("embed", 50, 24), ("recur", 24), ("steps",), ("dense", 24, 40), ("dense", 40, 30)],
+                         rng=np.random.default_rng(0)).to(DEV)
+    gen = torch.Generator().manual_seed(4)
+    tok, act = torch.randint(0, 50, (6, 20), generator=gen), torch.randint(0, 30, (6, 20), generator=gen).to(DEV)
+    n = torch.tensor([20, 3, 0, 11, 19, 1])
+    behind = torch.arange(20)[None] >= n[:, None]
+    weight = (~behind).float().to(DEV) / float((~behind).sum())
+    results = []
+    for filler in (0, -1, 1 << 40):
+        x = net[1](net[0](torch.where(behind, filler, tok).to(DEV)), None, n.to(DEV))
+        times = net[4](net[3](net[2](x))).view(6, 20, 30)
+        loss = snn.policy_loss(times, act, torch.full((6, 20), -3.0, device=DEV), torch.ones(6, 20, device=DEV), weight=weight)
+        results.append([loss, *torch.autograd.grad(loss, net.weights())])
+    for other in results[1:]:
+        for a, b in zip(results[0], other):
+            assert torch.isfinite(b).all() and torch.equal(a, b)
