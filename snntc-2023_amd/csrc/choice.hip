@@ -477,16 +477,16 @@ loss_total_kernel(const float* __restrict__ loss, const float* __restrict__ weig
 namespace {
 
 // Whether a workgroup holds a row of so many pieces, or it is sliced.  Held with its gradient / sliced, us, 16-bit times: 48000 outputs (6000
-// pieces) 16 rows 10.6 / 12.6, 1024 rows 42 / 51; 96000 outputs (12000 pieces, a CU to a workgroup) 16 rows 16 / 12, 128 rows 20 / 19,
-// 256 rows 24 / 30; 48000 in float32 (12000 pieces) 16 rows 10 / 12, 64 rows 12 / 13, 128 rows 14 / 18; without the gradient 1024 rows
-// 45 / 37.  Nothing has to be held for a gradient from statistics: there the slices'
-// smaller workgroups serve from 1024 pieces on.
+// pieces) 16 rows 11.0 / 12.6, 1024 rows 42 / 51; 96000 outputs (12000 pieces, a CU to a workgroup) 16 rows 16 / 9.5, 128 rows 19.4 / 16.8,
+// 192 rows 21.1 / 21.4, 256 rows 22.6 / 25.8; float32 times, 48000 outputs (12000 pieces) 16 rows 12.3 / 10.4, 64 rows 13.7 / 11.0, 128 rows
+// 15.4 / 15.1, 192 rows 17.9 / 20.0, 256 rows 19.9 / 24.0; 65536 outputs 128 rows 20.3 / 18.1, 192 rows 23.3 / 24.5; without the gradient 48000 outputs,
+// 1024 rows 45 / 37.  Nothing has to be held for a gradient from statistics: there the slices' smaller workgroups serve from 1024 pieces on.
 constexpr int kMostPieces = 16 * 1024;
 template <int VEC, Mode MODE>
 bool held(int pieces, int64_t rows, bool gradient) {
     if (MODE == GRAD) return pieces <= 1024;
     if (VEC == 1) return pieces <= kMostPieces;
-    return pieces <= 8192 || (MODE == POLICY && gradient && rows >= (VEC == 4 ? 64 : 192) && pieces <= kMostPieces);
+    return pieces <= 8192 || (MODE == POLICY && gradient && rows >= 192 && pieces <= kMostPieces);
 }
 
 template <typename E, int VEC, Mode MODE, bool STREAM>

@@ -129,3 +129,12 @@ def test_float32_gradients_of_unlikely_outputs(J):
         g = got.double().cpu()
         error = (g[:, 2:] / (g[:, 1:2] * want[:, 2:]) - 1.0).abs().max()
         assert error <= 5.01 * U, f"{float(error / U):.1f} half steps"
+
+
+@pytest.mark.parametrize("rows,J", [(191, 32801), (192, 32801), (200, 65536)])
+def test_long_float32_rows_held_for_their_gradient(rows, J):
+    """More than 8192 pieces of 16 bytes of float32, around the number of rows from which one workgroup keeps each."""
+    from test_gpu_choice import _case, _check_policy, _policy_inputs
+    times, tokens, gen = _case((rows,), J, torch.float32, spread=20.0)
+    old, adv, ref = _policy_inputs(times, tokens, gen)
+    _check_policy(times, tokens, old, adv, ref, None, same=False)
