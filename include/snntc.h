@@ -301,7 +301,7 @@ SNNTC_API int snntc_recipe_total(const int64_t* rows, const int64_t* cols, int64
 
 /* ---------------------------------------------------------------------------------------------
  * Element types of the tensors below that need not be float32 (tables, gates, the losses' times and the gradients of
- * each).  Arithmetic is float32 throughout; a result is rounded to its type once, to nearest even.
+ * each).  Arithmetic is float32 or wider; a result is rounded to its type once, to nearest even.
  * ------------------------------------------------------------------------------------------- */
 enum { SNNTC_F32 = 0, SNNTC_BF16 = 1, SNNTC_F16 = 2 };
 
@@ -326,6 +326,8 @@ SNNTC_API int snntc_embed_backward(const float* grad, const void* tokens, int to
 /* ---------------------------------------------------------------------------------------------
  * Gated running mean of spike times along a sequence, x[B,T,D], gate[B,T,D] of gate_type:
  *   a_t = sigmoid(gate_t),  h_t = a_t h_{t-1} + (1 - a_t) x_t,  y_t = h_t,  h_0 = state[B,D] (NULL: zeros)
+ * h is carried in 64 bits: y_t lies between the smallest and the largest of h_0 and x_1 .. x_t, to the last digit in sequences of up
+ * to 10^6 steps and within a step of it in longer ones.
  * lengths[B] (int64, NULL: all T; values outside [0, T] count as the nearer end): steps behind a sequence's length are
  * not read, y there is 0, and final_state[B,D] (may be NULL) is h at the sequence's length (the initial state for
  * length 0).
@@ -355,7 +357,8 @@ SNNTC_API int snntc_gated_step(const float* x, const void* gate, int gate_type, 
  * A row of weight 0 is not read: its logp and loss are 0 and its gradient is 0.
  *   snntc_time_logp           logp[rows] and, for the backward call, stats[rows,2] (8-byte aligned; may be NULL).
  *   snntc_time_logp_backward  dtimes[r,j] = upstream coef[r] (softmax(-times[r])[j] - [j = tokens[r]]), of times' type, the
- *                             gradient where coef[r] is a loss's derivative by logp[r] (upstream: a device scalar, NULL = 1).
+ *                             gradient where coef[r] is a loss's derivative by logp[r] (upstream: a device scalar, NULL = 1).  A row whose
+ *                             coef is 0 is not read.  (coef of a row with a token outside [0, J) is NaN in every loss here.)
  *   snntc_policy_loss         clipped policy loss with a KL term, ratio = exp(logp - old_logp), d = ref_logp - logp:
  *       row_loss = kl_coef (exp(d) - d - 1) - min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A),  A = advantage[r]
  *       (ref_logp NULL: no KL term).  The objective is sum_r weight[r] row_loss[r], weight NULL: the mean.  stats, coef[rows]
@@ -364,7 +367,8 @@ SNNTC_API int snntc_gated_step(const float* x, const void* gate, int gate_type, 
  *       weight[2P,T], ref_logp[2P] = log-probability of each sequence under the reference):
  *       seq_logp[q] = sum_t weight[q,t] logp[q,t],  m = beta ((seq_logp - ref_logp)[p] - (seq_logp - ref_logp)[P + p])
  *       pair_loss[p] = -(1 - smoothing) log sigmoid(m) - smoothing log sigmoid(-m)
- *       The objective is the mean of pair_loss.  weight NULL: all 1.  stats, coef[2P,T], dtimes as above.
+ *       The objective is the mean of pair_loss.  weight NULL: all 1.  stats, coef[2P,T], dtimes as above.  A term of factor 0
+ *       (smoothing 0 or 1) is none, also where a sequence that cannot occur makes m infinite.
  *   snntc_loss_total          total = sum_i weight[i] loss[i] (weight NULL: the mean), added in a fixed order.
  * Errors: a negative size, a times_type that is none of the above, a NULL required pointer, J = 0 with rows, a clip below 0
  * or a clip_low above 1, smoothing outside [0, 1], a beta or kl_coef that is not finite -> BAD_ARGUMENT; more than 2^24 - 1

@@ -41,7 +41,9 @@ __device__ __forceinline__ float group_sum(float v) {
 __device__ __forceinline__ float row_weight(const float* weight, int64_t r) { return weight ? weight[r] : 1.0f; }
 
 struct RowLoss { float loss, coef; };
-// The policy loss of a row, and its derivative by logp.
+// The policy loss of a row, and its derivative by logp.  In float32: logp is one, half a step of which (2^-24 |logp|) goes into the ratio and
+// the distance from the reference whatever is done with it, and what these operations add is no more.  expm1 keeps the digits of a small
+// distance, of which the KL term is half the square.
 __device__ __forceinline__ RowLoss policy_row(const PolicyArgs& a, int64_t r, float lp) {
     const float adv = a.advantage[r];
     const float ratio = expf(lp - a.old_logp[r]);

@@ -92,7 +92,7 @@ __device__ __forceinline__ float time_of(float e, float scale, bool encode) {
 }
 
 // A wavefront owns 256 columns of TOKENS consecutive tokens and requests their rows together.  Bound by memory: 131072 tokens of 1024
-// columns from a 16-bit table 98 us, 6.6 TB/s; 8192 of 800 from float32 8.8 us, 4.6 TB/s.
+// columns from a 16-bit table 95 us, 6.9 TB/s; 8192 of 800 from float32 9.0 us, 4.5 TB/s.
 template <typename E, typename I, bool VEC, int TOKENS, bool STREAM>
 __global__ void __launch_bounds__(256)
 embed_forward_kernel(const I* __restrict__ tokens, const E* __restrict__ table, float* __restrict__ z, int N, int V, int D, int slices,

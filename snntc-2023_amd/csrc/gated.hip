@@ -6,7 +6,8 @@
 // A step mixes two spike times, so what comes out lies between those that went in and is a spike time itself.  That needs a and 1 - a
 // to add up to one.  In float32 the half steps of each leave them off, by as much in every step alike where a gate stays, which the
 // 1 / (1 - a) steps of the mean add up: a constant came back 0.05 % off at gates of 10, 0.2 % at 12.  Gates, the state along a sequence and the maps
-// of its runs are therefore held in 64 bits, and a result is rounded to 32 once.  (What that costs, forward + backward in us, 32 bits / 64:
+// of its runs are therefore held in 64 bits, where they add up to one within 2^-46 (below: half a step of a result after 10^6 steps), and a
+// result is rounded to 32 once.  (What that costs, forward + backward in us, 32 bits / 64:
 // 32 x 256 x 800 14.4 + 26.1 / 15.7 + 26.2, 24 x 333 x 777 17.1 + 28.2 / 20.4 + 30.1, 16 x 6400 x 1024 200 + 430 / 201 + 429,
 // 16 x 32768 x 16 56 + 78 / 71 + 90.)
 #include <algorithm>
@@ -17,7 +18,7 @@ namespace snntc {
 namespace {
 
 // a = sigmoid(g) and 1 - a: with e = exp(-g), a = 1 / (1 + e) and 1 - a = e a, each to its own precision.  e is a float32 number, off by
-// two steps at most, which moves both together; the reciprocal in 32 bits is off by a step, after a step of Newton's method in 64 by the
+// a step and a half at most, which moves both together; the reciprocal in 32 bits is off by a step, after a step of Newton's method in 64 by the
 // square of that, 2^-46, and so is a + (1 - a) from one.  (Below -80, where 1 - a is 1 and a below 2e-35, e is held finite.  A NaN stays one.)
 struct Gate {
     float e, near;                                  // near: a, off by a step
@@ -39,31 +40,34 @@ __device__ __forceinline__ int length_of(const int64_t* lengths, int64_t b, int6
 // A workgroup owns W (64) neighbouring channels of a sequence and walks along it in tiles of kWaves x kSteps steps: each wavefront holds
 // kSteps of them in registers (lane = channel).  A run of steps maps the state it is given to A h + H, so the wavefronts exchange
 // (A, H) of their runs through LDS, every one composes those before its own, and goes through its steps a second time with the
-// right start.  The next tile's loads are under way meanwhile; every value is read once and written once.  Bound by memory: 32 x 256 x
-// 800 13.4 us forward and 24.8 backward, 5.9 and 6.4 TB/s; 32768 x 1024 cut along time 37 + 57 and 35 + 107, 5.4 to 6.3 TB/s.
+// right start.  The next tile's loads are under way meanwhile; every value is read once and written once.  Bound by memory, and in short
+// sequences by the instructions between two tiles' loads: 32 x 256 x 800 17.1 us forward and 28.5 backward, 4.6 and 5.5 TB/s; 32768 x 1024
+// cut along time 40 + 57 and 38 + 104, 5.0 to 6.5 TB/s.
 //
 // Where that makes fewer than kFill workgroups, long sequences (more than kShort tiles) are also cut along time: a first kernel composes
 // (A, H) of each part, and a workgroup starts from the composition of the parts before its own.  The order of composition depends on
-// sizes alone.  Forward + backward in us, sequences whole / cut, 16-bit gates: 4096 steps, 16 groups of 64 channels 104 + 168 / 18 + 24,
-// 192 groups 125 + 208 / 157 + 228.
+// sizes alone.  Forward + backward in us, sequences whole / cut, 16-bit gates: 4096 steps, 16 groups of 64 channels 99 + 155 / 18 + 25,
+// 192 groups 122 + 220 / 145 + 225.
 // As few that are not cut become groups of 32 channels: each half of a wavefront has eight steps of its own, a tile twice as many.  Groups
-// of 64 / 32, us: 256 x 1024 7.5 + 11.2 / 7.0 + 7.6, 32 x 200 x 200 8.2 + 11.5 / 6.7 + 8.4; 160 groups alike, 32 x 256 x 800 39 / 45.  One
-// workgroup of 32 channels a CU, or a little less (kMany groups of 64 and more), is not cut however long: cut / in groups of 32, us,
-// 2048 steps, 128 groups 44 + 68 / 33 + 64, 96 groups 35 + 53 / 28 + 57, 80 groups 31 + 48 / 27 + 54, 144 groups 48 + 77 / 47 + 112; 8192
-// steps, 128 groups 187 + 330 / 142 + 285; 384 steps, 32 groups 11 + 11 / 7 + 10; 512 steps, 32 groups 11 + 12 / 9 + 12, 16 groups
-// 9 + 10 / 8 + 12.
+// of 64 / 32, us: 4 x 256 x 1024 9 + 13 / 7 + 8, 32 x 200 x 200 9 + 13 / 7 + 9; 160 groups alike (10 x 256 x 1024 10 + 15 / 10 + 16),
+// 32 x 256 x 800 14 + 23 / 17 + 33.  One workgroup of 32 channels a CU, or a little less (kMany groups of 64 and more), is not cut however
+// long: cut / in groups of 32, us, 2048 steps, 128 groups 48 + 77 / 34 + 57, 96 groups 40 + 56 / 33 + 48, 80 groups 35 + 51 / 32 + 47, 144 groups
+// 52 + 85 / 51 + 98; 8192 steps, 128 groups 194 + 293 / 147 + 308; 384 steps, 32 groups 11 + 12 / 8 + 11; 512 steps, 32 groups 12 + 12 / 10 + 13,
+// 16 groups 12 + 12 / 10 + 13.
 //
 // Workgroups are dealt to the dies in turn.  Where neighbours share lines they go to one die, whose cache then holds those: where rows, those
-// of the gates among them, are not whole lines (in turn / neighbours together, 24 x 333 x 777 38 / 34 us, 16 x 2530 x 777 258 / 226,
-// 16 x 8434 x 777 941 / 753, 16 x 32768 x 200 1265 / 1128), and where 32 channels of 16-bit gates are half a line (8 x 1024 x 1024
-// 21.4 + 32.8 / 20.2 + 30.2, 8 x 4096 x 1024 66 + 154 / 63 + 155, 2 x 8192 x 4096 146 + 294 / 143 + 287).  Else in turn: 32768 x 1024, cut, 249 / 264,
-// others the same.
+// of the gates among them, are not whole lines (in turn / neighbours together, 24 x 333 x 777 22 + 36 / 19 + 29 us, 16 x 2530 x 777
+// 94 + 180 / 82 + 152, 16 x 8434 x 777 313 + 612 / 269 + 507, 16 x 32768 x 200 464 + 827 / 416 + 712), and where 32 channels of 16-bit gates are
+// half a line (8 x 1024 x 1024 21.4 + 32.8 / 20.2 + 30.2, 8 x 4096 x 1024 66 + 154 / 63 + 155, 2 x 8192 x 4096 146 + 294 / 143 + 287).  Else in turn:
+// 32768 x 1024, cut, 110 + 152 / 111 + 157, others the same.
 // Calls that touch more than the caches hold store past them, where rows are whole lines (the ends of a row that is none are stored by two groups
-// that need not run at one time): 32768 x 1024 270 -> 249, 8 x 4096 x 1024 231 -> 215, 16 x 1920 x 1024 182 -> 171, 16 x 6400 x 1024 613 -> 600;
-// 16 x 8434 x 777 753 -> 827.  Half lines of 16-bit gates are among them, whose two halves neighbours on one die store together (through the
-// caches 8 x 4096 x 1024 78 + 159, 2 x 2048 x 4096 35 + 75 for 35 + 57).
-// Where sequences are cut, they load past them too, in the second and last reading: 32768 x 1024 249 -> 237, 16 x 102400 x 64 820 -> 745,
-// 16 x 30720 x 64 231 -> 224; whole ones gain less (16 x 6400 x 1024 626 -> 612) or lose what a cache still holds (8 x 4096 x 1024 211 -> 243).
+// that need not run at one time): through / past, 8 x 4096 x 1024 76 + 160 / 66 + 157, 16 x 1920 x 1024 61 + 132 / 52 + 125, 16 x 6400 x 1024 alike;
+// 16 x 8434 x 777 269 + 507 / 291 + 586.  Half lines of 16-bit gates are among them, whose two halves neighbours on one die store together
+// (through the caches 8 x 4096 x 1024 78 + 159, 2 x 2048 x 4096 35 + 75 for 35 + 57).
+// Where sequences are cut, they load past them too, in the second and last reading (all through the caches / stores past / loads too,
+// 16 x 102400 x 64 338 + 542 / 321 + 521 / 301 + 471, 16 x 30720 x 64 89 + 154 / 87 + 141 / 94 + 135, 32768 x 1024 101 + 170 / 98 + 159 / 109 + 152);
+// whole ones gain less (16 x 6400 x 1024 202 + 421 / 195 + 414) or lose what a cache still holds for a call that follows (8 x 4096 x 1024, the
+// gradient right after the forward pass, 211 / 243).
 constexpr int kWaves = 8, kSteps = 8, kTile = kWaves * kSteps;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kDies = 8;

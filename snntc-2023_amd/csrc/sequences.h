@@ -6,8 +6,8 @@
 
 namespace snntc {
 
-// Element types of tables, gates and times (SNNTC_F32 / SNNTC_BF16 / SNNTC_F16).  Arithmetic is fp32 throughout; a result is
-// rounded to its type once, to nearest even, when it is stored.
+// Element types of tables, gates and times (SNNTC_F32 / SNNTC_BF16 / SNNTC_F16).  Arithmetic is fp32, in 64 bits where a
+// file says so; a result is rounded to its type once, to nearest even, when it is stored.
 inline size_t type_bytes(int type) { return type == SNNTC_F32 ? 4 : 2; }
 template <typename F>
 int with_type(int type, F&& f) {
