@@ -353,7 +353,7 @@ class SNN_recurrence(torch.nn.Module):
         if x.dim() != 3 or x.shape[2] != self.dim:
             raise ValueError(f"input must be [B,T,{self.dim}], got shape {tuple(x.shape)}")
         known = x
-        if lengths is not None and lengths.shape == x.shape[:1] and lengths.device == x.device:        # (else refused below)
+        if isinstance(lengths, torch.Tensor) and lengths.shape == x.shape[:1] and lengths.device == x.device:  # (else refused below)
             # gates behind a length are not read and have no gradient, but the weights' gradient is a sum over all steps of times by
             # gradients: times that are no numbers (of padding tokens that are in no table) would be in it, times 0
             known = x.masked_fill((torch.arange(x.shape[1], device=x.device) >= lengths[:, None])[..., None], 0.0)

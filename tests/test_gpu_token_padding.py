@@ -42,6 +42,8 @@ def test_lengths_of_another_kind_are_refused_by_the_op():
         recur(x, None, torch.tensor([5, 4, 1], device=DEV, dtype=torch.int32))
     with pytest.raises(snn.SnntcLibraryError, match="lives on cpu"):
         recur(x, None, torch.tensor([5, 4, 1]))
+    with pytest.raises(TypeError, match="lengths must be a torch.Tensor"):
+        recur(x, None, [5, 4, 1])
 
 
 def test_a_padded_training_step_from_tokens_to_the_loss():
