@@ -75,3 +75,22 @@ def test_encoded_times_are_off_by_less_than_one_and_a_half_steps():
     worst, mean = float(((z - want).abs() / step).max()), float(((z - want).abs() / step).mean())
     assert worst <= 1.515, f"{worst:.3f} steps, {mean:.3f} in the mean"
     print(f"{worst:.3f} steps, {mean:.3f} in the mean")
+
+
+def test_gradient_of_half_a_billion_positions():
+    """Small whole numbers, whose sums are exact; some 500000 positions a token, spread over all chunks."""
+    import snntc_amd as snn
+    torch.cuda.empty_cache()
+    N, V = 2 ** 29 + 7, 1009
+    if torch.cuda.mem_get_info()[0] < 24 * N + (8 << 30):
+        pytest.skip("needs 21 GB of the card's memory")
+    tok = torch.randint(0, V, (N,), device=DEV, dtype=torch.int32)
+    grad = torch.randint(-8, 9, (N, 1), device=DEV).float()
+    tok[-3:] = torch.tensor([V, -1, 5], device=DEV)
+    d = snn.embed_tokens_grad(grad, tok, torch.zeros(V, 1, device=DEV))
+    want = torch.zeros(V + 1, device=DEV, dtype=torch.float64)
+    for first in range(0, N, 2 ** 26):
+        part = slice(first, min(N, first + 2 ** 26))
+        t = tok[part].long()
+        want.index_add_(0, torch.where((t >= 0) & (t < V), t, V), grad[part, 0].double())
+    assert torch.equal(d[:, 0].double(), want[:V])
