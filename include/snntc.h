@@ -392,6 +392,93 @@ SNNTC_API int snntc_preference_loss(const void* times, int times_type, const int
 SNNTC_API int snntc_loss_total(const float* loss, const float* weight, float* total, int64_t n, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Choices by rules: what changes a row of spike times times[r,:] before a token is drawn from softmax(-times) or a loss over it is
+ * taken.  history[history_rows, history_len] (int64) are sequences of tokens; row r belongs to sequence r / (rows / history_rows) and
+ * sees its first lengths[r] tokens (NULL: all; values outside count as the nearer end), of which the first prompts[sequence] (NULL: 0)
+ * are a prompt.  c_j: occurrences of j among what the row sees, o_j: those behind the prompt; tokens outside [0, J) are none.
+ *     a_j = times_j repetition (times_j > 0), times_j / repetition (else)    where c_j > 0, times_j elsewhere
+ *     b_j = a_j + (presence + frequency o_j)                                 where o_j > 0, a_j elsewhere
+ *     out_j = b_j + delay_j  where bit j % 32 of allowed[j / 32] is set, +infinity elsewhere
+ * in float32, product by product and sum by sum, rounded to times' type once.  repetition, presence, frequency: device arrays with a
+ * number for each sequence, or NULL and *_all for all.  delay[J] or [rows,J] (delay_rows 1 or rows; NULL: none), allowed[ceil(J/32)] or
+ * [rows,ceil(J/32)] likewise; what a masked element holds, or bits behind J, do not matter.  history NULL: no penalties.
+ *   snntc_rule_times           out[rows,J], of times' type; must not overlap times.
+ *   snntc_rule_times_backward  dtimes_j = grad_j times repetition, over it, or as it is, as times_j was; 0 where not allowed.  times may be
+ *                              NULL where history is, or no sequence's repetition differs from 1.  presence, frequency, prompts and delay are not read.
+ *   snntc_choose               tokens[r] (int64): with p = softmax(-out[r] / T), the first j whose running sum of p exceeds uniform[r] of the
+ *                              whole (uniform below 0 or NaN counts as 0; from 1 on: the last possible j), logp[r] = log p_j.  T = temperature[r], or
+ *                              NULL and temperature_all.  T below 1e-37: the earliest output, the lowest index of equal ones, with its
+ *                              log-probability at T = 1; uniform may be NULL where this holds for temperature_all.  Where nothing is
+ *                              possible (all masked or infinite), a time that is allowed is NaN or -infinity, or T is negative or no finite number:
+ *                              token -1 and logp NaN.  rules may be NULL.
+ * Errors: a negative size, an unknown type, a NULL required pointer, J = 0 with rows, history_rows that do not divide rows, delay_rows or
+ * allowed_rows neither 1 nor rows, a repetition_all that is not positive, penalties or a temperature_all that are not finite or (this) below 0 -> BAD_ARGUMENT;
+ * more than 2^24 - 1 rows, J or history_len above 2^30 -> TOO_LARGE; a workspace below snntc_choose_workspace_bytes -> WORKSPACE.
+ * ------------------------------------------------------------------------------------------- */
+typedef struct snntc_rules {
+    const int64_t* history;
+    int64_t history_rows, history_len;
+    const int64_t* lengths;
+    const int64_t* prompts;
+    const float* repetition;
+    const float* presence;
+    const float* frequency;
+    float repetition_all, presence_all, frequency_all;
+    const float* delay;
+    int64_t delay_rows;
+    const int32_t* allowed;
+    int64_t allowed_rows;
+} snntc_rules;
+SNNTC_API int snntc_rule_times(const void* times, int times_type, const snntc_rules* rules, void* out, int64_t rows, int64_t J, void* stream);
+SNNTC_API int snntc_rule_times_backward(const void* grad, const void* times, int times_type, const snntc_rules* rules, void* dtimes,
+                              int64_t rows, int64_t J, void* stream);
+SNNTC_API int snntc_choose_workspace_bytes(int64_t rows, int64_t J, size_t* bytes);
+SNNTC_API int snntc_choose(const void* times, int times_type, const float* uniform, const float* temperature, float temperature_all,
+                 const snntc_rules* rules, int64_t* tokens, float* logp, int64_t rows, int64_t J, void* workspace, size_t workspace_bytes,
+                 void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * One AdamW step over many tensors, w[t] with gradients dw[t] (both of types[t]) of n[t] elements.  g = dw, scaled down to max_norm where
+ * `norm`, the gradients' norm on the device, is given and larger:
+ *     m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ *     w = w (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps)
+ * A norm that is no finite number leaves w, first and second as they are.  The step's number is `step` (from 1), or, where `steps` is
+ * given, one more than that device number, which the call advances (also of a step that is left out): a captured call counts by itself.
+ * first, second: m and v as float32[n], or, where first_scale and second_scale are given, as uint8[n] with a float32 for every 256
+ * elements (the last may be fewer), ceil(n / 256) of them: its largest magnitude s.  Code c (of m: its low 7 bits, the 8th its sign) stands for
+ *     s value(c) / value(largest code),   value(c) = c (c < 8),  (8 + c % 8) 2^(c / 8 - 1) (else)
+ * A state's zero is code 0 and scale 0.  A value between two codes becomes the upper one with the chance of its place between them, a weight of
+ * 16 bits likewise one of its two neighbours; the random bits follow from seed, step, t and the element alone.
+ *   snntc_grad_norm       norm = sqrt of the sum of squares of all gradients (float32 on the device, the sum in 64 bits, the same on
+ *                         every call).
+ *   snntc_adamw_moments   first_out[t], second_out[t] (float32[n]) = what the codes stand for.
+ * All arrays but `steps` and `norm` are HOST arrays of `count` entries, read before the call returns; tensors of n[t] = 0 are skipped.  No two of
+ * the written tensors may overlap, nor a gradient one of them.  The workspace of snntc_adamw_update (SNNTC_ADAMW_WORKSPACE_BYTES) is needed with `steps` only.
+ * Errors: a negative count or size, an unknown type, a NULL required pointer, one scale array without the other, lr or weight_decay not
+ * finite or negative, a beta outside [0, 1), an eps below the smallest normal float32, a step below 1, a max_norm that is not positive -> BAD_ARGUMENT; n[t] above
+ * 2^34 -> TOO_LARGE; a workspace that is missing or too small -> WORKSPACE.
+ * ------------------------------------------------------------------------------------------- */
+#define SNNTC_STATE_BLOCK 256
+#define SNNTC_ADAMW_WORKSPACE_BYTES 256
+typedef struct snntc_adamw {
+    double lr, beta1, beta2, eps, weight_decay;
+    int64_t step;
+    int64_t* steps;
+    const float* norm;
+    double max_norm;
+    uint64_t seed;
+} snntc_adamw;
+SNNTC_API int snntc_grad_norm_workspace_bytes(const int64_t* n, int64_t count, size_t* bytes);
+SNNTC_API int snntc_grad_norm(const void* const* grads, const int* types, const int64_t* n, int64_t count, float* norm, void* workspace,
+                    size_t workspace_bytes, void* stream);
+SNNTC_API int snntc_adamw_update(void* const* w, const void* const* dw, void* const* first, void* const* second, float* const* first_scale,
+                       float* const* second_scale, const int* types, const int64_t* n, int64_t count, const snntc_adamw* how, void* workspace,
+                       size_t workspace_bytes, void* stream);
+SNNTC_API int snntc_adamw_moments(const uint8_t* const* first, const uint8_t* const* second, const float* const* first_scale,
+                        const float* const* second_scale, float* const* first_out, float* const* second_out, const int64_t* n, int64_t count,
+                        void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Health of the bounded wait described at snntc_fc_forward (no counterpart in the reference, whose scan
  * has one thread per neuron and nothing to wait for).
  *   snntc_scan_status(&giveups, stream)  number of wavefronts, on the current device since the process

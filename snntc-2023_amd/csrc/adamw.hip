@@ -1,0 +1,483 @@
+// One AdamW step over many tensors at once.  With g = share dw, share = min(1, max_norm / norm) where the gradients are clipped (else 1),
+//     m = b1 m + (1 - b1) g,   v = b2 v + (1 - b2) g^2,
+//     w = w - lr decay w - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
+// (the reference hands the update to the framework's optimizer, snntc/snntc-mnist.py:70).  One pass: every element is read once and
+// written once, whatever its state is held in.
+//
+// States in 8 bits.  A block of 256 elements of a tensor has one float32 scale, its largest magnitude, which the largest code stands for;
+// code 8 (E - 1) + k, k = 8 .. 15, is k 2^(E - 1) in units of that, codes below 8 are themselves (m: a sign and 7 bits, E to 15; v: 8 bits, E
+// to 31, since v spans the square of m's range).  Two neighbours lie a 15th to an 8th apart, and a step
+// changes v by 1 - b2 of itself: rounded to the nearest, an element whose gradients shrink while its block's do not would stand still for
+// good.  So a value is rounded to either neighbour with the chance of its place between them, and on average a state moves as it should
+// (4000 steps of gradients of constant variance: sqrt v off by 12 % of itself, by 1 on average).  The random bits are a function of seed, step, tensor
+// and element.
+// A double's upper word with 16 random bits and a half added below its third binary digit is that rounding.  Moments are therefore 64
+// bits wide between the codes: next to a border a sum in 32 bits would leave another code than the definition.
+// 16-bit weights are rounded in the same way and for the same reason: a step of a thousandth of a weight is less than half of what
+// they can tell apart.
+#include "sequences.h"
+
+namespace snntc {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kBlock = SNNTC_STATE_BLOCK;                     // elements that share a scale: four to a lane
+static_assert(kBlock == 4 * kWave, "a wavefront owns a block");
+constexpr double kTopFirst = 15 << 14, kTopSecond = 15.0 * (1 << 30);
+
+// A table of tensors travels in the kernel arguments, which hold 4 KiB.
+constexpr int kMostTensors = 48;
+struct AdamTable {
+    void* w[kMostTensors];
+    const void* g[kMostTensors];
+    void* m[kMostTensors];
+    void* v[kMostTensors];
+    float* m_scale[kMostTensors];
+    float* v_scale[kMostTensors];
+    long long n[kMostTensors];
+    unsigned first_block[kMostTensors + 1];
+    int tensor[kMostTensors];                                 // its place in the caller's list, for the random bits
+    int count;
+};
+
+// What depends on the step's number, from the host or (graphs) from the device.
+struct AdamStep { double rate, second; unsigned step; };     // lr / (1 - b1^t), 1 / (1 - b2^t)
+struct AdamScalars {
+    double b1, b2, keep, eps, max_norm;                      // keep: 1 - lr decay
+    const float* norm;                                        // NULL: not clipped
+    const AdamStep* at;                                       // NULL: `step`
+    AdamStep step;
+    unsigned seed_low, seed_high;
+};
+
+__device__ __forceinline__ unsigned mix(unsigned x) {
+    x = (x ^ (x >> 16)) * 0x6A09E667u;
+    x = (x ^ (x >> 15)) * 0xBB67AE85u;
+    return x ^ (x >> 16);
+}
+__device__ __forceinline__ unsigned key_of(const AdamScalars& s, unsigned step, unsigned tensor) {
+    return mix(s.seed_low + mix(s.seed_high + mix(step + mix(tensor))));
+}
+__device__ __forceinline__ unsigned noise(unsigned key, unsigned element) { return mix(element * 0x9E3779B9u ^ key); }
+
+// A code's integer as a double, from the bits of one: 8 <= code: exponent E + 2 and three digits.
+__device__ __forceinline__ double code_value(unsigned code) {
+    const bool low = code < 8;
+    const double d = __hiloint2double((int)((code + (low ? 8208u : 8200u)) << 17), 0);
+    return d - (low ? 8.0 : 0.0);
+}
+// The code of y >= 0 (in units), raised by (bits + 1/2) / 65536 of a step and cut off.
+__device__ __forceinline__ unsigned code_of(double y, unsigned bits, unsigned most) {
+    const bool low = y < 8.0;
+    const unsigned hi = (unsigned)__double2hiint(low ? y + 8.0 : y) + (bits << 1 | 1u);
+    const unsigned c = (hi >> 17) - (low ? 8208u : 8200u);
+    return c < most ? c : most;
+}
+
+// float32 to a weight's type; 16-bit types to one of the two neighbours, the upper one if the place between them in 65536ths exceeds `bits`.
+__device__ __forceinline__ void round_weight(float x, unsigned, float* to) { *to = x; }
+__device__ __forceinline__ void round_weight(float x, unsigned bits, __bf16* to) {
+    unsigned w = __float_as_uint(x);
+    if (fabsf(x) < INFINITY) w += 0xFFFFu - bits;
+    else if (w & 0xFFFFu) w |= 0x10000u;                      // (a NaN stays one)
+    *to = __builtin_bit_cast(__bf16, (unsigned short)(w >> 16));
+}
+__device__ __forceinline__ void round_weight(float x, unsigned bits, _Float16* to) {
+    if (!(fabsf(x) < 65504.0f)) { *to = (_Float16)x; return; }
+    const int e = max((int)(__float_as_uint(x) >> 23 & 255) - 127, -14);
+    const float y = ldexpf(fabsf(x), 10 - e), low = floorf(y);
+    const float q = low + ((y - low) * 65536.0f > (float)bits ? 1.0f : 0.0f);
+    *to = (_Float16)copysignf(ldexpf(q, e - 10), x);
+}
+
+typedef unsigned Words __attribute__((ext_vector_type(4)));
+typedef unsigned Pair __attribute__((ext_vector_type(2)));
+template <typename E> struct FourWords;
+template <> struct FourWords<float> { typedef Words T; };
+template <> struct FourWords<__bf16> { typedef Pair T; };
+template <> struct FourWords<_Float16> { typedef Pair T; };
+template <> struct FourWords<unsigned char> { typedef unsigned T; };
+// Four elements at any place of their type.
+template <typename E> struct Four { E v[4]; };
+template <typename E> struct __attribute__((packed, aligned(sizeof(E)))) Place { typename FourWords<E>::T w; };
+template <typename E>
+__device__ __forceinline__ Four<E> load4(const E* at, int n) {
+    if (n >= 4) return __builtin_bit_cast(Four<E>, reinterpret_cast<const Place<E>*>(at)->w);
+    Four<E> r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.v[i] = i < n ? at[i] : (E)0;
+    return r;
+}
+template <typename E>
+__device__ __forceinline__ void store4(E* at, const Four<E>& r, int n) {
+    if (n >= 4) {
+        reinterpret_cast<Place<E>*>(at)->w = __builtin_bit_cast(typename FourWords<E>::T, r);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i < n) at[i] = r.v[i];
+}
+
+template <typename T>
+__device__ __forceinline__ int tensor_of(const T& tab, unsigned block) {
+    int low = 0, high = tab.count;
+    while (high - low > 1) {                                  // (uniform)
+        const int mid = (low + high) >> 1;
+        if (tab.first_block[mid] <= block) low = mid; else high = mid;
+    }
+    return low;
+}
+
+// What the gradients are scaled by; a norm that is no finite number: the step is left out.
+__device__ __forceinline__ double share_of(const AdamScalars& s, bool* skip) {
+    *skip = false;
+    if (!s.norm) return 1.0;
+    const float norm = *s.norm;
+    *skip = !(norm < INFINITY);
+    return (double)norm > s.max_norm ? s.max_norm / (double)norm : 1.0;
+}
+
+constexpr int kEach = 4;                                       // elements of a thread at a time
+constexpr int kTimes = 2;
+constexpr int kChunk = kThreads * kEach * kTimes;
+
+__device__ __forceinline__ float stepped(float w, float m, float v, float keep, float rate, float second, float eps) {
+    return fmaf(-rate, m / (sqrtf(v * second) + eps), w * keep);
+}
+
+// States in float32.  Bound by memory.
+template <typename E>
+__global__ void __launch_bounds__(kThreads)
+adamw_kernel(AdamTable tab, AdamScalars s) {
+    const int t = tensor_of(tab, blockIdx.x);
+    const long long n = tab.n[t], e0 = (long long)(blockIdx.x - tab.first_block[t]) * kChunk + threadIdx.x * kEach;
+    E* __restrict__ w = static_cast<E*>(tab.w[t]);
+    const E* __restrict__ g = static_cast<const E*>(tab.g[t]);
+    float* __restrict__ m = static_cast<float*>(tab.m[t]);
+    float* __restrict__ v = static_cast<float*>(tab.v[t]);
+    Four<E> W[kTimes], G[kTimes];
+    Four<float> M[kTimes], V[kTimes];
+#pragma unroll
+    for (int i = 0; i < kTimes; ++i) {
+        const long long e = e0 + i * kThreads * kEach;
+        const int left = (int)min(n - e, 4ll);
+        if (left <= 0) continue;
+        W[i] = load4(w + e, left); G[i] = load4(g + e, left); M[i] = load4(m + e, left); V[i] = load4(v + e, left);
+    }
+    bool skip;
+    const float share = (float)share_of(s, &skip);
+    if (skip) return;
+    const AdamStep at = s.at ? *s.at : s.step;
+    const float b1 = (float)s.b1, b2 = (float)s.b2, new1 = (float)(1.0 - s.b1), new2 = (float)(1.0 - s.b2), keep = (float)s.keep,
+                rate = (float)at.rate, second = (float)at.second, eps = (float)s.eps;
+    const unsigned key = sizeof(E) == 2 ? key_of(s, at.step, tab.tensor[t]) : 0;
+#pragma unroll
+    for (int i = 0; i < kTimes; ++i) {
+        const long long e = e0 + i * kThreads * kEach;
+        const int left = (int)min(n - e, 4ll);
+        if (left <= 0) continue;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float d = (float)G[i].v[k] * share;
+            M[i].v[k] = fmaf(b1, M[i].v[k], new1 * d);
+            V[i].v[k] = fmaf(b2, V[i].v[k], new2 * d * d);
+            const unsigned bits = sizeof(E) == 2 ? noise(key, (unsigned)(e + k)) * 0x9E3779B9u >> 16 : 0;
+            round_weight(stepped((float)W[i].v[k], M[i].v[k], V[i].v[k], keep, rate, second, eps), bits, &W[i].v[k]);
+        }
+        store4(w + e, W[i], left); store4(m + e, M[i], left); store4(v + e, V[i], left);
+    }
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, kWave));
+    return v;
+}
+// States in 8 bits: a wavefront owns kTimes blocks of 256 elements.
+template <typename E>
+__global__ void __launch_bounds__(kThreads)
+adamw8_kernel(AdamTable tab, AdamScalars s) {
+    const int t = tensor_of(tab, blockIdx.x), lane = threadIdx.x % kWave;
+    const long long n = tab.n[t], b0 = ((long long)(blockIdx.x - tab.first_block[t]) * (kThreads / kWave) + threadIdx.x / kWave) * kTimes;
+    E* __restrict__ w = static_cast<E*>(tab.w[t]);
+    const E* __restrict__ g = static_cast<const E*>(tab.g[t]);
+    unsigned char* __restrict__ m = static_cast<unsigned char*>(tab.m[t]);
+    unsigned char* __restrict__ v = static_cast<unsigned char*>(tab.v[t]);
+    float *__restrict__ ms = tab.m_scale[t], *__restrict__ vs = tab.v_scale[t];
+    Four<E> W[kTimes], G[kTimes];
+    Four<unsigned char> M[kTimes], V[kTimes];
+    float m_scale[kTimes], v_scale[kTimes];
+#pragma unroll
+    for (int i = 0; i < kTimes; ++i) {
+        const long long e = (b0 + i) * kBlock + lane * 4;
+        const int left = (int)max(min(n - e, 4ll), 0ll);
+        if ((b0 + i) * kBlock >= n) continue;                 // (a whole wavefront)
+        W[i] = load4(w + e, left); G[i] = load4(g + e, left); M[i] = load4(m + e, left); V[i] = load4(v + e, left);
+        m_scale[i] = ms[b0 + i]; v_scale[i] = vs[b0 + i];
+    }
+    bool skip;
+    const double share = share_of(s, &skip);
+    if (skip) return;
+    const AdamStep at = s.at ? *s.at : s.step;
+    const float keep = (float)s.keep, rate = (float)at.rate, second = (float)at.second, eps = (float)s.eps;
+    const double new1 = (1.0 - s.b1) * share, new2 = (1.0 - s.b2) * share * share;
+    const unsigned key = key_of(s, at.step, tab.tensor[t]);
+#pragma unroll
+    for (int i = 0; i < kTimes; ++i) {
+        const long long e = (b0 + i) * kBlock + lane * 4;
+        const int left = (int)max(min(n - e, 4ll), 0ll);
+        if ((b0 + i) * kBlock >= n) continue;
+        const double old1 = s.b1 * ((double)m_scale[i] / kTopFirst), old2 = s.b2 * ((double)v_scale[i] / kTopSecond);
+        double a[4], q[4];
+        float top1 = 0.0f, top2 = 0.0f;
+        bool bad = false;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const double d = (double)(float)G[i].v[k];
+            const double c = code_value(M[i].v[k] & 127u);
+            a[k] = fma(new1, d, old1 * (M[i].v[k] & 128u ? -c : c));
+            q[k] = fma(new2 * d, d, old2 * code_value(V[i].v[k]));
+            const float fa = (float)a[k], fq = (float)q[k];
+            top1 = fmaxf(top1, fabsf(fa)); top2 = fmaxf(top2, fq);
+            bad |= isnan(fa) || isnan(fq);
+            const unsigned bits = sizeof(E) == 2 ? noise(key, (unsigned)(e + k)) * 0x9E3779B9u >> 16 : 0;
+            round_weight(stepped((float)W[i].v[k], fa, fq, keep, rate, second, eps), bits, &W[i].v[k]);
+        }
+        store4(w + e, W[i], left);
+        top1 = wave_max(top1); top2 = wave_max(top2);
+        if (__any(bad)) top1 = top2 = NAN;                    // (a maximum passes over them)
+        const double unit1 = top1 > 0.0f ? kTopFirst / (double)top1 : 0.0, unit2 = top2 > 0.0f ? kTopSecond / (double)top2 : 0.0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const unsigned bits = noise(key, (unsigned)(e + k));
+            const unsigned c = code_of(fabs(a[k]) * unit1, bits & 0xFFFFu, 127u);
+            M[i].v[k] = (unsigned char)(a[k] < 0.0 ? c | 128u : c);
+            V[i].v[k] = (unsigned char)code_of(q[k] * unit2, bits >> 16, 255u);
+        }
+        store4(m + e, M[i], left); store4(v + e, V[i], left);
+        if (lane == 0) { ms[b0 + i] = top1; vs[b0 + i] = top2; }
+    }
+}
+
+// The number of a step that a graph replays: one more each time, and what follows from it.
+__global__ void adamw_advance_kernel(long long* __restrict__ steps, AdamStep* __restrict__ at, double lr, double b1, double b2) {
+    const long long t = *steps + 1;
+    *steps = t;
+    *at = AdamStep{lr / (1.0 - pow(b1, (double)t)), 1.0 / (1.0 - pow(b2, (double)t)), (unsigned)t};
+}
+
+// Both moments from their codes, float32.
+struct MomentTable {
+    const unsigned char* m[kMostTensors];
+    const unsigned char* v[kMostTensors];
+    const float* m_scale[kMostTensors];
+    const float* v_scale[kMostTensors];
+    float* first[kMostTensors];
+    float* second[kMostTensors];
+    long long n[kMostTensors];
+    unsigned first_block[kMostTensors + 1];
+    int count;
+};
+__global__ void __launch_bounds__(kThreads)
+moments_kernel(MomentTable tab) {
+    const int t = tensor_of(tab, blockIdx.x);
+    const long long n = tab.n[t], e0 = (long long)(blockIdx.x - tab.first_block[t]) * kChunk + threadIdx.x * kEach;
+#pragma unroll
+    for (int i = 0; i < kTimes; ++i) {
+        const long long e = e0 + i * kThreads * kEach;
+        const int left = (int)min(n - e, 4ll);
+        if (left <= 0) continue;
+        const Four<unsigned char> M = load4(tab.m[t] + e, left), V = load4(tab.v[t] + e, left);
+        const double u1 = (double)tab.m_scale[t][e / kBlock] / kTopFirst, u2 = (double)tab.v_scale[t][e / kBlock] / kTopSecond;
+        Four<float> a, q;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const double c = code_value(M.v[k] & 127u) * u1;
+            a.v[k] = (float)(M.v[k] & 128u ? -c : c);
+            q.v[k] = (float)(code_value(V.v[k]) * u2);
+        }
+        store4(tab.first[t] + e, a, left); store4(tab.second[t] + e, q, left);
+    }
+}
+
+// ---- the norm over all gradients -------------------------------------------------------------------------------------------------
+
+constexpr int kMostGrads = 96;
+struct GradTable {
+    const void* g[kMostGrads];
+    long long n[kMostGrads];
+    unsigned first_block[kMostGrads + 1];
+    unsigned char type[kMostGrads];
+    int count;
+    long long chunk;                                          // elements of a workgroup
+};
+
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) v += __shfl_xor(v, d, kWave);
+    return v;
+}
+template <int THREADS>
+__device__ __forceinline__ double block_sum(double v) {
+    __shared__ double part[THREADS / kWave];
+    v = wave_sum(v);
+    if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = v;
+    __syncthreads();
+    v = part[0];
+#pragma unroll
+    for (int i = 1; i < THREADS / kWave; ++i) v += part[i];
+    return v;
+}
+
+// Squares in 64 bits: of 10^8 gradients neither the largest overflow nor the smallest vanish, and the sum's order does not show.
+template <typename E>
+__device__ __forceinline__ double squares(const E* __restrict__ g, long long from, long long to) {
+    double sum[4] = {0.0, 0.0, 0.0, 0.0};
+    for (long long e = from + threadIdx.x * 4; e < to; e += kThreads * 4) {
+        const Four<E> x = load4(g + e, (int)min(to - e, 4ll));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const double d = (double)(float)x.v[k];
+            sum[k] = fma(d, d, sum[k]);
+        }
+    }
+    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+__global__ void __launch_bounds__(kThreads)
+grad_squares_kernel(GradTable tab, double* __restrict__ partial) {
+    const int t = tensor_of(tab, blockIdx.x);
+    const long long from = (long long)(blockIdx.x - tab.first_block[t]) * tab.chunk, to = min(from + tab.chunk, tab.n[t]);
+    double s;
+    if (tab.type[t] == SNNTC_F32) s = squares(static_cast<const float*>(tab.g[t]), from, to);
+    else if (tab.type[t] == SNNTC_BF16) s = squares(static_cast<const __bf16*>(tab.g[t]), from, to);
+    else s = squares(static_cast<const _Float16*>(tab.g[t]), from, to);
+    s = block_sum<kThreads>(s);
+    if (threadIdx.x == 0) partial[blockIdx.x] = s;
+}
+__global__ void __launch_bounds__(1024)
+grad_norm_kernel(const double* __restrict__ partial, float* __restrict__ norm, int n) {
+    double s = 0.0;
+    for (int i = threadIdx.x; i < n; i += 1024) s += partial[i];
+    s = block_sum<1024>(s);
+    if (threadIdx.x == 0) *norm = (float)sqrt(s);
+}
+
+// Workgroups of one launch: 2^32 threads are too many.
+constexpr int64_t kMostBlocks = (1 << 24) - 1;
+
+int64_t norm_chunk(int64_t total) { return 4096 * std::max<int64_t>(1, total / (4096ll * 8192)); }
+
+}  // namespace
+
+size_t grad_norm_workspace(const int64_t* n, int64_t count) {
+    int64_t total = 0, blocks = 0;
+    for (int64_t t = 0; t < count; ++t) total += n[t];
+    const int64_t chunk = norm_chunk(total);
+    for (int64_t t = 0; t < count; ++t) blocks += (n[t] + chunk - 1) / chunk;
+    return align_up((size_t)blocks * sizeof(double));
+}
+
+int launch_grad_norm(const void* const* g, const int* types, const int64_t* n, int count, float* norm, void* ws, hipStream_t stream) {
+    int64_t total = 0;
+    for (int t = 0; t < count; ++t) total += n[t];
+    double* partial = static_cast<double*>(ws);
+    int64_t done = 0;
+    for (int t = 0; t < count;) {
+        GradTable tab;
+        tab.count = 0;
+        tab.chunk = norm_chunk(total);
+        int64_t blocks = 0;
+        for (; t < count && tab.count < kMostGrads; ++t) {
+            if (n[t] == 0) continue;
+            tab.g[tab.count] = g[t];
+            tab.n[tab.count] = n[t];
+            tab.type[tab.count] = (unsigned char)types[t];
+            tab.first_block[tab.count] = (unsigned)blocks;
+            blocks += (n[t] + tab.chunk - 1) / tab.chunk;
+            ++tab.count;
+        }
+        if (tab.count == 0) continue;
+        {
+            KernelTimerScope timer_("grad_squares", stream);
+            hipLaunchKernelGGL(grad_squares_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, stream, tab, partial + done);
+        }
+        done += blocks;
+    }
+    {
+        KernelTimerScope timer_("grad_norm", stream);
+        hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(1024), 0, stream, partial, norm, (int)done);
+    }
+    SNNTC_HIP_CHECK(hipGetLastError());
+    return SNNTC_OK;
+}
+
+int launch_adamw(const AdamTensors& a, int count, const AdamNumbers& p, void* ws, hipStream_t stream) {
+    AdamScalars s{};
+    s.b1 = p.b1; s.b2 = p.b2; s.keep = 1.0 - p.lr * p.decay; s.eps = p.eps; s.max_norm = p.max_norm; s.norm = p.norm;
+    s.seed_low = (unsigned)p.seed; s.seed_high = (unsigned)(p.seed >> 32);
+    if (p.steps) {
+        AdamStep* at = static_cast<AdamStep*>(ws);
+        KernelTimerScope timer_("adamw_advance", stream);
+        hipLaunchKernelGGL(adamw_advance_kernel, dim3(1), dim3(1), 0, stream, reinterpret_cast<long long*>(p.steps), at, p.lr, p.b1, p.b2);
+        SNNTC_HIP_CHECK(hipGetLastError());
+        s.at = at;
+    } else {
+        s.step = AdamStep{p.lr / (1.0 - pow(p.b1, (double)p.step)), 1.0 / (1.0 - pow(p.b2, (double)p.step)), (unsigned)p.step};
+    }
+    for (int type = SNNTC_F32; type <= SNNTC_F16; ++type)
+        for (int t = 0; t < count;) {
+            AdamTable tab;
+            tab.count = 0;
+            int64_t blocks = 0;
+            for (; t < count && tab.count < kMostTensors; ++t) {
+                if (a.n[t] == 0 || a.types[t] != type) continue;
+                const int64_t more = (a.n[t] + kChunk - 1) / kChunk;
+                if (blocks + more > kMostBlocks) break;
+                const int c = tab.count++;
+                tab.w[c] = a.w[t]; tab.g[c] = a.g[t]; tab.m[c] = a.m[t]; tab.v[c] = a.v[t];
+                tab.m_scale[c] = a.m_scale ? a.m_scale[t] : nullptr;
+                tab.v_scale[c] = a.v_scale ? a.v_scale[t] : nullptr;
+                tab.n[c] = a.n[t];
+                tab.tensor[c] = t;
+                tab.first_block[c] = (unsigned)blocks;
+                blocks += more;
+            }
+            if (tab.count == 0) continue;
+            with_type(type, [&](auto e) -> int {
+                using E = decltype(e);
+                KernelTimerScope timer_(a.m_scale ? "adamw8" : "adamw", stream);
+                if (a.m_scale) hipLaunchKernelGGL((adamw8_kernel<E>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, tab, s);
+                else hipLaunchKernelGGL((adamw_kernel<E>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, tab, s);
+                return SNNTC_OK;
+            });
+            SNNTC_HIP_CHECK(hipGetLastError());
+        }
+    return SNNTC_OK;
+}
+
+int launch_adamw_moments(const uint8_t* const* m, const uint8_t* const* v, const float* const* m_scale, const float* const* v_scale,
+                         float* const* first, float* const* second, const int64_t* n, int count, hipStream_t stream) {
+    for (int t = 0; t < count;) {
+        MomentTable tab;
+        tab.count = 0;
+        int64_t blocks = 0;
+        for (; t < count && tab.count < kMostTensors; ++t) {
+            if (n[t] == 0) continue;
+            const int64_t more = (n[t] + kChunk - 1) / kChunk;
+            if (blocks + more > kMostBlocks) break;
+            const int c = tab.count++;
+            tab.m[c] = m[t]; tab.v[c] = v[t]; tab.m_scale[c] = m_scale[t]; tab.v_scale[c] = v_scale[t];
+            tab.first[c] = first[t]; tab.second[c] = second[t]; tab.n[c] = n[t];
+            tab.first_block[c] = (unsigned)blocks;
+            blocks += more;
+        }
+        if (tab.count == 0) continue;
+        KernelTimerScope timer_("adamw_moments", stream);
+        hipLaunchKernelGGL(moments_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, stream, tab);
+        SNNTC_HIP_CHECK(hipGetLastError());
+    }
+    return SNNTC_OK;
+}
+
+}  // namespace snntc

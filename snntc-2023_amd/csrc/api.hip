@@ -735,6 +735,168 @@ int snntc_loss_total(const float* loss, const float* weight, float* total, int64
     return launch_loss_total(loss, weight, total, n, static_cast<hipStream_t>(stream));
 }
 
+// The rules as the kernels take them; rows: of times.
+static int rule_args(const snntc_rules* rules, int64_t rows, int64_t J, const char* who, RuleArgs* a) {
+    *a = RuleArgs{};
+    a->rep = 1.0f;
+    if (!rules) return SNNTC_OK;
+    if (rules->history_len < 0 || rules->history_rows < 0) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: negative size", who);
+    if (rules->history_len > (1 << 30)) return fail(SNNTC_ERR_TOO_LARGE, "%s: a history of more than 2^30 tokens", who);
+    const bool sized = (!rules->delay || rules->delay_rows == 1 || rules->delay_rows == rows) &&
+                       (!rules->allowed || rules->allowed_rows == 1 || rules->allowed_rows == rows);
+    if (!sized) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: delay and allowed have one row, or one for each of %lld", who, (long long)rows);
+    if (rules->history && (rows > 0 ? rules->history_rows < 1 || rows % rules->history_rows != 0 : false))
+        return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: %lld rows do not divide into %lld sequences", who, (long long)rows, (long long)rules->history_rows);
+    if (!(rules->repetition_all > 0.0f && rules->repetition_all < INFINITY) || !isfinite(rules->presence_all) || !isfinite(rules->frequency_all))
+        return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: repetition %g, presence %g or frequency %g outside its range", who,
+                    (double)rules->repetition_all, (double)rules->presence_all, (double)rules->frequency_all);
+    if (rules->history && rules->history_len > 0 && rows > 0) {
+        a->history = rules->history;
+        a->L = rules->history_len;
+        a->rows_per_history = rows / rules->history_rows;
+        a->lengths = rules->lengths; a->prompts = rules->prompts;
+        a->repetition = rules->repetition; a->presence = rules->presence; a->frequency = rules->frequency;
+        a->rep = rules->repetition_all; a->pres = rules->presence_all; a->freq = rules->frequency_all;
+    }
+    a->delay = rules->delay;
+    a->delay_stride = rules->delay_rows == 1 ? 0 : J;
+    a->allowed = reinterpret_cast<const unsigned*>(rules->allowed);
+    a->allowed_stride = rules->allowed_rows == 1 ? 0 : (J + 31) / 32;
+    return SNNTC_OK;
+}
+
+int snntc_rule_times(const void* times, int times_type, const snntc_rules* rules, void* out, int64_t rows, int64_t J, void* stream) {
+    RuleArgs a;
+    int rc = choice_check(rows, J, times_type, "snntc_rule_times");
+    if (!rc) rc = rule_args(rules, rows, J, "snntc_rule_times", &a);
+    if (rc || rows == 0) return rc;
+    if (!times || !out) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_rule_times: null pointer");
+    return launch_rule_times(times, times_type, a, out, rows, J, static_cast<hipStream_t>(stream));
+}
+
+int snntc_rule_times_backward(const void* grad, const void* times, int times_type, const snntc_rules* rules, void* dtimes, int64_t rows,
+                              int64_t J, void* stream) {
+    RuleArgs a;
+    int rc = choice_check(rows, J, times_type, "snntc_rule_times_backward");
+    if (!rc) rc = rule_args(rules, rows, J, "snntc_rule_times_backward", &a);
+    if (rc || rows == 0) return rc;
+    if (!a.repetition && a.rep == 1.0f) a.history = nullptr;
+    if (!grad || !dtimes || (a.history && !times)) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_rule_times_backward: null pointer");
+    return launch_rule_times_backward(grad, times, times_type, a, dtimes, rows, J, static_cast<hipStream_t>(stream));
+}
+
+int snntc_choose_workspace_bytes(int64_t rows, int64_t J, size_t* bytes) {
+    const int rc = choice_check(rows, J, SNNTC_F32, "snntc_choose_workspace_bytes");
+    if (rc) return rc;
+    if (!bytes) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_choose_workspace_bytes: bytes is NULL");
+    *bytes = choose_workspace(rows, J);
+    return SNNTC_OK;
+}
+
+int snntc_choose(const void* times, int times_type, const float* uniform, const float* temperature, float temperature_all,
+                 const snntc_rules* rules, int64_t* tokens, float* logp, int64_t rows, int64_t J, void* workspace, size_t workspace_bytes,
+                 void* stream) {
+    RuleArgs a;
+    int rc = choice_check(rows, J, times_type, "snntc_choose");
+    if (!rc) rc = rule_args(rules, rows, J, "snntc_choose", &a);
+    if (rc) return rc;
+    if (!(temperature_all >= 0.0f && temperature_all < INFINITY))
+        return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_choose: temperature %g outside its range", (double)temperature_all);
+    if (rows == 0) return SNNTC_OK;
+    if (!times || !tokens || !logp || (!uniform && (temperature || temperature_all >= 1e-37f)))
+        return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_choose: null pointer");
+    rc = check_workspace(workspace, workspace_bytes, choose_workspace(rows, J));
+    if (rc) return rc;
+    const ChooseArgs c{uniform, temperature, temperature_all, tokens, logp};
+    return launch_choose(times, times_type, a, c, rows, J, workspace, static_cast<hipStream_t>(stream));
+}
+
+// Sizes and types of a list of tensors; types may be NULL.
+static int tensors_check(const int* types, const int64_t* n, int64_t count, const char* who) {
+    if (count < 0 || count > INT32_MAX) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: bad tensor count", who);
+    if (count > 0 && !n) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: null array", who);
+    for (int64_t t = 0; t < count; ++t) {
+        if (n[t] < 0) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: tensor %lld has a negative size", who, (long long)t);
+        if (n[t] > (1ll << 34)) return fail(SNNTC_ERR_TOO_LARGE, "%s: tensor %lld has more than 2^34 elements", who, (long long)t);
+        if (types && !known_type(types[t])) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: tensor %lld has unknown type %d", who, (long long)t, types[t]);
+    }
+    return SNNTC_OK;
+}
+// An array of `count` device pointers of any type.
+static int pointers_check(const void* array, const int64_t* n, int64_t count, const char* who) {
+    if (count > 0 && !array) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: null array", who);
+    const void* const* p = static_cast<const void* const*>(array);
+    for (int64_t t = 0; t < count; ++t)
+        if (n[t] > 0 && !p[t]) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: tensor %lld is a null pointer", who, (long long)t);
+    return SNNTC_OK;
+}
+
+int snntc_grad_norm_workspace_bytes(const int64_t* n, int64_t count, size_t* bytes) {
+    const int rc = tensors_check(nullptr, n, count, "snntc_grad_norm_workspace_bytes");
+    if (rc) return rc;
+    if (!bytes) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_grad_norm_workspace_bytes: bytes is NULL");
+    *bytes = grad_norm_workspace(n, count);
+    return SNNTC_OK;
+}
+
+int snntc_grad_norm(const void* const* grads, const int* types, const int64_t* n, int64_t count, float* norm, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+    const char* who = "snntc_grad_norm";
+    if (count > 0 && !types) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: null array", who);
+    int rc = tensors_check(types, n, count, who);
+    if (!rc) rc = pointers_check(grads, n, count, who);
+    if (rc) return rc;
+    if (!norm) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: norm is NULL", who);
+    rc = check_workspace(workspace, workspace_bytes, grad_norm_workspace(n, count));
+    if (rc) return rc;
+    return launch_grad_norm(grads, types, n, (int)count, norm, workspace, static_cast<hipStream_t>(stream));
+}
+
+int snntc_adamw_update(void* const* w, const void* const* dw, void* const* first, void* const* second, float* const* first_scale,
+                       float* const* second_scale, const int* types, const int64_t* n, int64_t count, const snntc_adamw* how, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+    const char* who = "snntc_adamw_update";
+    if ((count > 0 && !types) || !how) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: null array", who);
+    int rc = tensors_check(types, n, count, who);
+    if (!rc) rc = pointers_check(w, n, count, who);
+    if (!rc) rc = pointers_check(dw, n, count, who);
+    if (!rc) rc = pointers_check(first, n, count, who);
+    if (!rc) rc = pointers_check(second, n, count, who);
+    if (!rc && !first_scale != !second_scale) rc = fail(SNNTC_ERR_BAD_ARGUMENT, "%s: scales of one moment only", who);
+    if (!rc && first_scale) rc = pointers_check(first_scale, n, count, who);
+    if (!rc && first_scale) rc = pointers_check(second_scale, n, count, who);
+    if (rc) return rc;
+    const auto share = [](double v) { return v >= 0.0 && v < 1.0; };
+    if (!(how->lr >= 0.0 && how->lr < INFINITY) || !(how->weight_decay >= 0.0 && how->weight_decay < INFINITY) || !share(how->beta1) ||
+        !share(how->beta2) || !((float)how->eps >= 1.17549435e-38f && how->eps < INFINITY))
+        return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: lr %g, betas (%g, %g), eps %g or weight_decay %g outside its range", who, how->lr, how->beta1,
+                    how->beta2, how->eps, how->weight_decay);
+    if (!how->steps && how->step < 1) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: steps count from 1, got %lld", who, (long long)how->step);
+    if (how->norm && !(how->max_norm > 0.0)) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: max_norm %g is not positive", who, how->max_norm);
+    if (how->steps) {
+        rc = check_workspace(workspace, workspace_bytes, SNNTC_ADAMW_WORKSPACE_BYTES);
+        if (rc) return rc;
+    }
+    const AdamTensors a{w, dw, first, second, first_scale, second_scale, types, n};
+    const AdamNumbers p{how->lr, how->beta1, how->beta2, how->eps, how->weight_decay, how->max_norm, how->step, how->steps, how->norm, how->seed};
+    return launch_adamw(a, (int)count, p, workspace, static_cast<hipStream_t>(stream));
+}
+
+int snntc_adamw_moments(const uint8_t* const* first, const uint8_t* const* second, const float* const* first_scale,
+                        const float* const* second_scale, float* const* first_out, float* const* second_out, const int64_t* n, int64_t count,
+                        void* stream) {
+    const char* who = "snntc_adamw_moments";
+    int rc = tensors_check(nullptr, n, count, who);
+    if (!rc) rc = pointers_check(first, n, count, who);
+    if (!rc) rc = pointers_check(second, n, count, who);
+    if (!rc) rc = pointers_check(first_scale, n, count, who);
+    if (!rc) rc = pointers_check(second_scale, n, count, who);
+    if (!rc) rc = pointers_check(first_out, n, count, who);
+    if (!rc) rc = pointers_check(second_out, n, count, who);
+    if (rc) return rc;
+    return launch_adamw_moments(first, second, first_scale, second_scale, first_out, second_out, n, (int)count, static_cast<hipStream_t>(stream));
+}
+
 int snntc_scan_status(int64_t* giveups, void* stream) {
     if (!giveups) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_scan_status: giveups is NULL");
     return read_scan_giveups(giveups, static_cast<hipStream_t>(stream));

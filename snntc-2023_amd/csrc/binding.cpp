@@ -33,6 +33,7 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
+#include <algorithm>
 #include <array>
 #include <optional>
 #include <string>
@@ -61,7 +62,9 @@ using torch::autograd::variable_list;
     F(snntc_gated_scan_forward) F(snntc_gated_scan_backward) F(snntc_gated_scan_workspace_bytes)                   \
     F(snntc_gated_step) F(snntc_choice_workspace_bytes) F(snntc_preference_workspace_bytes) F(snntc_time_logp)     \
     F(snntc_time_logp_backward)                                                                                    \
-    F(snntc_policy_loss) F(snntc_preference_loss) F(snntc_loss_total)
+    F(snntc_policy_loss) F(snntc_preference_loss) F(snntc_loss_total) F(snntc_rule_times)                          \
+    F(snntc_rule_times_backward) F(snntc_choose_workspace_bytes) F(snntc_choose) F(snntc_grad_norm_workspace_bytes) \
+    F(snntc_grad_norm) F(snntc_adamw_update) F(snntc_adamw_moments)
 
 struct Library {
 #define SNNTC_FIELD(f) decltype(&::f) f = nullptr;
@@ -548,6 +551,274 @@ Tensor objective_grad(const ChoiceArgs& a, const Tensor& stats_in, const Tensor&
     return d;
 }
 
+// ---- choices by rules --------------------------------------------------------------------------------------------------
+
+// A number for all sequences, or a tensor with one for each.
+struct PerRow { Tensor each; float all; };
+
+struct RuleIn { Tensor history, lengths, prompts; PerRow repetition, presence, frequency; Tensor delay, allowed; };
+
+// times[..., J] and what rules it; `c` points into the tensors.
+struct RuleSet {
+    Tensor times, history, lengths, prompts, repetition, presence, frequency, delay, allowed;
+    int64_t rows = 0, J = 0;
+    snntc_rules c{};
+};
+
+RuleSet rule_set(const Tensor& times, const RuleIn& in) {
+    RuleSet r;
+    r.times = dev_float(times, "times");
+    TORCH_CHECK_VALUE(times.dim() >= 2, "times must have at least 2 dimensions, got shape ", shape_text(times));
+    const at::IntArrayRef lead = times.sizes().slice(0, times.dim() - 1);
+    r.J = times.size(-1);
+    r.rows = 1;
+    for (const int64_t n : lead) r.rows *= n;
+    int64_t sequences = 0;
+    if (in.history.defined()) {
+        r.history = index_like(in.history, r.times, "history", false);
+        TORCH_CHECK_VALUE(r.history.dim() == 2, "history must be [sequences, tokens], got shape ", shape_text(r.history));
+        sequences = r.history.size(0);
+        TORCH_CHECK_VALUE(sequences ? r.rows % sequences == 0 : r.rows == 0, "times ", shape_text(times), " do not divide into the ", sequences,
+                          " sequences of history");
+        if (in.lengths.defined()) {
+            r.lengths = index_like(in.lengths, r.times, "lengths", false);
+            TORCH_CHECK_VALUE(r.lengths.sizes() == lead, "lengths must have one entry per row of times, got shape ", shape_text(r.lengths),
+                              " for times ", shape_text(times));
+        }
+        if (in.prompts.defined()) {
+            r.prompts = index_like(in.prompts, r.times, "prompts", false);
+            TORCH_CHECK_VALUE(r.prompts.dim() == 1 && r.prompts.size(0) == sequences, "prompts must have one entry per sequence of history, got shape ",
+                              shape_text(r.prompts));
+        }
+    } else {
+        TORCH_CHECK_VALUE(!in.lengths.defined() && !in.prompts.defined() && !in.repetition.each.defined() && !in.presence.each.defined() &&
+                              !in.frequency.each.defined(), "lengths, prompts and penalties per sequence need a history");
+    }
+    r.repetition = f32_like(in.repetition.each, r.times, {sequences}, "repetition");
+    r.presence = f32_like(in.presence.each, r.times, {sequences}, "presence");
+    r.frequency = f32_like(in.frequency.each, r.times, {sequences}, "frequency");
+    // one row for all, or one for each row of times
+    const auto one_row = [&](const Tensor& t) { return t.dim() == 1; };
+    std::vector<int64_t> sizes = lead.vec();
+    if (in.delay.defined()) {
+        sizes.push_back(r.J);
+        r.delay = f32_like(in.delay, r.times, one_row(in.delay) ? at::IntArrayRef(r.J) : at::IntArrayRef(sizes), "delay");
+        sizes.pop_back();
+    }
+    if (in.allowed.defined()) {
+        const int64_t words = (r.J + 31) / 32;
+        sizes.push_back(words);
+        same_device(in.allowed, r.times, "allowed");
+        TORCH_CHECK_TYPE(in.allowed.scalar_type() == at::kInt, "allowed must be int32, 32 outputs a word, got ", in.allowed.scalar_type());
+        TORCH_CHECK_VALUE(one_row(in.allowed) ? in.allowed.size(0) == words : in.allowed.sizes() == at::IntArrayRef(sizes), "allowed must have ", words,
+                          " words, or so many per row of times, got shape ", shape_text(in.allowed), " for times ", shape_text(times));
+        r.allowed = in.allowed.contiguous();
+    }
+    snntc_rules& c = r.c;
+    c.history = i64(r.history);
+    c.history_rows = sequences;
+    c.history_len = r.history.defined() ? r.history.size(1) : 0;
+    c.lengths = i64(r.lengths); c.prompts = i64(r.prompts);
+    c.repetition = f32(r.repetition); c.presence = f32(r.presence); c.frequency = f32(r.frequency);
+    c.repetition_all = in.repetition.all; c.presence_all = in.presence.all; c.frequency_all = in.frequency.all;
+    c.delay = f32(r.delay);
+    c.delay_rows = r.delay.defined() && r.delay.dim() > 1 ? r.rows : 1;
+    c.allowed = static_cast<const int32_t*>(raw(r.allowed));
+    c.allowed_rows = r.allowed.defined() && r.allowed.dim() > 1 ? r.rows : 1;
+    return r;
+}
+
+Tensor rule_times(const RuleSet& r) {
+    const c10::DeviceGuard guard(r.times.device());
+    const Tensor out = empty(r.times, r.times.sizes());
+    check(lib.snntc_rule_times(raw(r.times), float_type(r.times), &r.c, raw(out), r.rows, r.J, stream_of(r.times)));
+    return out;
+}
+
+Tensor rule_times_grad(const Tensor& grad_in, const RuleSet& r) {
+    same_device(grad_in, r.times, "grad");
+    TORCH_CHECK_TYPE(grad_in.scalar_type() == r.times.scalar_type(), "grad must be ", r.times.scalar_type(), " as times are, got ",
+                     grad_in.scalar_type());
+    TORCH_CHECK_VALUE(grad_in.sizes() == r.times.sizes(), "grad ", shape_text(grad_in), " does not match times ", shape_text(r.times));
+    const c10::DeviceGuard guard(r.times.device());
+    const Tensor grad = grad_in.contiguous(), d = empty(r.times, r.times.sizes());
+    check(lib.snntc_rule_times_backward(raw(grad), raw(r.times), float_type(r.times), &r.c, raw(d), r.rows, r.J, stream_of(r.times)));
+    return d;
+}
+
+struct Choice { Tensor tokens, logp; };
+
+Choice choose_tokens(const RuleSet& r, const Tensor& uniform_in, const PerRow& temperature) {
+    const at::IntArrayRef lead = r.times.sizes().slice(0, r.times.dim() - 1);
+    const Tensor uniform = f32_like(uniform_in, r.times, lead, "uniform"), heat = f32_like(temperature.each, r.times, lead, "temperature");
+    TORCH_CHECK_VALUE(uniform.defined() || (!heat.defined() && temperature.all == 0.0f), "uniform is required unless temperature is 0");
+    const c10::DeviceGuard guard(r.times.device());
+    size_t need = 0;
+    check(lib.snntc_choose_workspace_bytes(r.rows, r.J, &need));
+    const Tensor ws = need ? scratch(r.times, need) : Tensor();
+    Choice out{at::empty(lead, r.times.options().dtype(at::kLong)), at::empty(lead, r.times.options().dtype(at::kFloat))};
+    check(lib.snntc_choose(raw(r.times), float_type(r.times), f32(uniform), f32(heat), temperature.all, &r.c, i64(out.tokens), f32(out.logp), r.rows,
+                           r.J, raw(ws), bytes_of(ws), stream_of(r.times)));
+    return out;
+}
+
+// ---- the update over many tensors --------------------------------------------------------------------------------------
+
+// Device tensors of one type each on one device, by their addresses.
+struct TensorList {
+    std::vector<Tensor> keep;
+    std::vector<void*> at;
+    std::vector<int> types;
+    std::vector<int64_t> n;
+};
+
+void add_tensor(TensorList& list, const Tensor& t) {
+    list.at.push_back(t.numel() ? t.data_ptr() : nullptr);
+    list.n.push_back(t.numel());
+    list.keep.push_back(t);
+}
+
+void on_device(const Tensor& t, const Tensor& with, const char* who, const char* what, size_t i) {
+    if (!t.is_cuda())
+        raise_class(g_library_error, message_args, 0, std::string(who) + ": " + what + " " + std::to_string(i) + " lives on " + t.device().str() +
+                    ": the SNN-TC ops run on a ROCm GPU only (no CPU fallback)");
+    TORCH_CHECK_VALUE(t.device() == with.device(), who, ": ", what, " ", i, " lives on ", t.device().str(), ", not on ", with.device().str());
+}
+
+bool is_float(const Tensor& t) {
+    return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf;
+}
+
+TensorList gradients(const std::vector<Tensor>& gs, const char* who) {
+    TensorList list;
+    for (size_t i = 0; i < gs.size(); ++i) {
+        on_device(gs[i], gs[0], who, "gradient", i);
+        TORCH_CHECK_TYPE(is_float(gs[i]), who, ": gradient ", i, " must be float32, bfloat16 or float16, got ", gs[i].scalar_type());
+        add_tensor(list, gs[i].contiguous());
+        list.types.push_back(float_type(gs[i]));
+    }
+    return list;
+}
+
+Tensor grad_norm(const std::vector<Tensor>& gs) {
+    TORCH_CHECK_VALUE(!gs.empty(), "grad_norm: no gradients");
+    on_device(gs[0], gs[0], "grad_norm", "gradient", 0);
+    const c10::DeviceGuard guard(gs[0].device());
+    const TensorList g = gradients(gs, "grad_norm");
+    size_t need = 0;
+    check(lib.snntc_grad_norm_workspace_bytes(g.n.data(), (int64_t)g.n.size(), &need));
+    const Tensor ws = scratch(gs[0], need), norm = at::empty({}, gs[0].options().dtype(at::kFloat));
+    check(lib.snntc_grad_norm(g.at.data(), g.types.data(), g.n.data(), (int64_t)g.n.size(), f32(norm), ws.data_ptr(), ws.numel(), stream_of(gs[0])));
+    return norm;
+}
+
+// A tensor that the update writes: contiguous, of the given type and size.
+void add_written(TensorList& list, const Tensor& t, const Tensor& with, at::ScalarType type, int64_t n, const char* what, size_t i) {
+    on_device(t, with, "adamw", what, i);
+    TORCH_CHECK_TYPE(t.scalar_type() == type, "adamw: ", what, " ", i, " must be ", type, ", got ", t.scalar_type());
+    TORCH_CHECK_VALUE(t.is_contiguous() && t.numel() == n, "adamw: ", what, " ", i, " must be contiguous with ", n, " elements, got shape ", shape_text(t));
+    add_tensor(list, t);
+}
+
+int64_t state_blocks(int64_t n) { return (n + SNNTC_STATE_BLOCK - 1) / SNNTC_STATE_BLOCK; }
+
+// No two written tensors may overlap, nor a written one with one that is read.
+struct Span { const char* from; const char* to; bool written; };
+void no_overlap(std::vector<Span>& spans) {
+    std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.from < b.from; });
+    const char *written = nullptr, *any = nullptr;
+    for (const Span& s : spans) {
+        TORCH_CHECK_VALUE(!(s.from < written || (s.written && s.from < any)), "adamw: two of the tensors overlap, of which one is updated");
+        if (s.written) written = std::max(written, s.to);
+        any = std::max(any, s.to);
+    }
+}
+void add_spans(std::vector<Span>& spans, const TensorList& list, bool written) {
+    for (const Tensor& t : list.keep)
+        if (t.numel()) spans.push_back({static_cast<const char*>(t.data_ptr()), static_cast<const char*>(t.data_ptr()) + t.nbytes(), written});
+}
+
+struct Moments { std::vector<Tensor> first, second, first_scale, second_scale; bool coded; };
+
+void moment_lists(const Moments& m, const std::vector<Tensor>& sizes, TensorList (&out)[4]) {
+    const size_t n = sizes.size();
+    TORCH_CHECK_VALUE(m.first.size() == n && m.second.size() == n && (!m.coded || (m.first_scale.size() == n && m.second_scale.size() == n)),
+                      "adamw: as many states and scales are needed as there are tensors (", n, ")");
+    for (size_t i = 0; i < n; ++i) {
+        const int64_t k = sizes[i].numel();
+        add_written(out[0], m.first[i], sizes[0], m.coded ? at::kByte : at::kFloat, k, "first", i);
+        add_written(out[1], m.second[i], sizes[0], m.coded ? at::kByte : at::kFloat, k, "second", i);
+        if (!m.coded) continue;
+        add_written(out[2], m.first_scale[i], sizes[0], at::kFloat, state_blocks(k), "first_scale", i);
+        add_written(out[3], m.second_scale[i], sizes[0], at::kFloat, state_blocks(k), "second_scale", i);
+    }
+}
+
+void adamw_update(const std::vector<Tensor>& ws, const std::vector<Tensor>& gs, const Moments& moments, const Tensor& steps, const Tensor& norm,
+                  snntc_adamw how) {
+    TORCH_CHECK_VALUE(ws.size() == gs.size(), "adamw: ", ws.size(), " weight tensors but ", gs.size(), " gradients");
+    if (ws.empty()) return;
+    on_device(ws[0], ws[0], "adamw", "weight", 0);
+    const c10::DeviceGuard guard(ws[0].device());
+    TensorList w, state[4];
+    const TensorList g = gradients(gs, "adamw");
+    for (size_t i = 0; i < ws.size(); ++i) {
+        TORCH_CHECK_TYPE(is_float(ws[i]), "adamw: weight ", i, " must be float32, bfloat16 or float16, got ", ws[i].scalar_type());
+        TORCH_CHECK_VALUE(gs[i].sizes() == ws[i].sizes() && gs[i].scalar_type() == ws[i].scalar_type() && gs[i].device() == ws[i].device(),
+                          "adamw: gradient ", i, " does not match its weight tensor");
+        add_written(w, ws[i], ws[0], ws[i].scalar_type(), ws[i].numel(), "weight", i);
+    }
+    moment_lists(moments, ws, state);
+    std::vector<Span> spans;
+    spans.reserve(6 * ws.size() + 2);
+    add_spans(spans, w, true); add_spans(spans, g, false);
+    for (const TensorList& s : state) add_spans(spans, s, true);
+    no_overlap(spans);
+    Tensor scratch_ws;
+    if (steps.defined()) {
+        on_device(steps, ws[0], "adamw", "step", 0);
+        TORCH_CHECK_TYPE(steps.scalar_type() == at::kLong && steps.numel() == 1, "adamw: a step on the device is one int64");
+        how.steps = i64(steps);
+        scratch_ws = scratch(ws[0], SNNTC_ADAMW_WORKSPACE_BYTES);
+    }
+    if (norm.defined()) {
+        on_device(norm, ws[0], "adamw", "norm", 0);
+        TORCH_CHECK_TYPE(norm.scalar_type() == at::kFloat && norm.numel() == 1, "adamw: norm is one float32");
+        how.norm = f32(norm);
+    }
+    const auto floats = [](TensorList& l) { return reinterpret_cast<float* const*>(l.at.data()); };
+    check(lib.snntc_adamw_update(w.at.data(), g.at.data(), state[0].at.data(), state[1].at.data(), moments.coded ? floats(state[2]) : nullptr,
+                                 moments.coded ? floats(state[3]) : nullptr, g.types.data(), w.n.data(), (int64_t)w.n.size(), &how, raw(scratch_ws),
+                                 bytes_of(scratch_ws), stream_of(ws[0])));
+    const auto changed = [](const Tensor& t) { if (!t.is_inference()) written_behind_autograd(t); };
+    for (const Tensor& t : ws) changed(t);
+    for (const TensorList& s : state)
+        for (const Tensor& t : s.keep) changed(t);
+    if (steps.defined()) changed(steps);
+}
+
+struct MomentsOut { std::vector<Tensor> first, second; };
+
+MomentsOut adamw_moments(const Moments& m) {
+    MomentsOut out;
+    if (m.first.empty() && m.second.empty()) return out;
+    TORCH_CHECK_VALUE(!m.first.empty(), "adamw: as many states and scales are needed as there are tensors (0)");
+    on_device(m.first[0], m.first[0], "adamw", "first", 0);
+    const c10::DeviceGuard guard(m.first[0].device());
+    TensorList state[4], to[2];
+    moment_lists(m, m.first, state);
+    for (const Tensor& t : m.first) {
+        for (int k = 0; k < 2; ++k) add_tensor(to[k], at::empty(t.sizes(), t.options().dtype(at::kFloat)));
+    }
+    const auto codes = [](TensorList& l) { return reinterpret_cast<const uint8_t* const*>(l.at.data()); };
+    const auto floats = [](TensorList& l) { return reinterpret_cast<float* const*>(l.at.data()); };
+    check(lib.snntc_adamw_moments(codes(state[0]), codes(state[1]), floats(state[2]), floats(state[3]), floats(to[0]), floats(to[1]),
+                                  state[0].n.data(), (int64_t)state[0].n.size(), stream_of(m.first[0])));
+    out.first = std::move(to[0].keep);
+    out.second = std::move(to[1].keep);
+    return out;
+}
+
 // ---- autograd nodes ------------------------------------------------------------------------------------------------
 
 template <typename N>
@@ -947,6 +1218,66 @@ Tensor preference_layer(const ChoiceArgs& a, const Tensor& ref, float beta, floa
         r = preference_objective(a, ref, beta, smoothing, grad);
     }
     return grad ? choice_history(a, r) : r.total;
+}
+
+// Ruled times; the gradient reads the times themselves only where a repetition changed them.
+struct RuleNode : public Node {
+    SavedVariable times, history, lengths, repetition, allowed;
+    bool has_history, has_lengths, has_repetition, has_allowed;
+    Tensor shape;                                            // without penalties: in the times' place, whose values the gradient does not need
+    float repetition_all;
+    std::string name() const override { return "TimeRulesBackward"; }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        times.reset_data(); history.reset_data(); lengths.reset_data(); repetition.reset_data(); allowed.reset_data(); shape.reset();
+    }
+    variable_list apply(variable_list&& grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        if (!grads[0].defined() || !task_should_compute_output(0)) return variable_list(1);
+        RuleIn in{};
+        in.repetition.all = 1.0f;
+        if (has_history) {
+            in.history = history.unpack();
+            in.repetition.all = repetition_all;
+            if (has_lengths) in.lengths = lengths.unpack();
+            if (has_repetition) in.repetition.each = repetition.unpack();
+        }
+        if (has_allowed) in.allowed = allowed.unpack();
+        const Tensor t = has_history ? times.unpack() : shape;
+        variable_list out(1);
+        {
+            at::AutoGradMode no_grad(false);
+            out[0] = rule_times_grad(grads[0], rule_set(t, in));
+        }
+        return once(std::move(out), *this, grads, "rule_times");
+    }
+};
+
+Tensor rule_layer(const RuleSet& r, const RuleIn& in) {
+    no_gradient({{&in.repetition.each, "repetition"}, {&in.presence.each, "presence"}, {&in.frequency.each, "frequency"}, {&in.delay, "delay"}},
+                "rule_times");
+    Tensor out;
+    {
+        at::AutoGradMode no_grad(false);
+        out = rule_times(r);
+    }
+    if (!wants_grad(r.times)) return out;
+    auto node = make_node<RuleNode>({r.times});
+    node->has_history = r.history.defined() && (r.repetition.defined() || in.repetition.all != 1.0f);
+    node->has_lengths = node->has_history && r.lengths.defined();
+    node->has_repetition = node->has_history && r.repetition.defined();
+    node->has_allowed = r.allowed.defined();
+    node->repetition_all = in.repetition.all;
+    if (node->has_history) {
+        node->times = SavedVariable(r.times, false);
+        node->history = SavedVariable(r.history, false);
+    } else {
+        node->shape = r.times.detach();
+    }
+    if (node->has_lengths) node->lengths = SavedVariable(r.lengths, false);
+    if (node->has_repetition) node->repetition = SavedVariable(r.repetition, false);
+    if (node->has_allowed) node->allowed = SavedVariable(r.allowed, false);
+    return with_history(out, node);
 }
 
 // ---- the example training recipe -------------------------------------------------------------------------------------
@@ -1744,6 +2075,171 @@ SNNTC_METHOD(py_objective_grad) {
     END_HANDLE_TH_ERRORS
 }
 
+double double_arg(PyObject* o) {
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) throw python_error();
+    return v;
+}
+
+// A number, or a tensor with one for each row or sequence.
+PerRow per_row_arg(PyObject* o) {
+    if (THPVariable_Check(o)) return PerRow{THPVariable_Unpack(o), 1.0f};
+    return PerRow{Tensor(), float_arg(o)};
+}
+
+// history, lengths, prompts, repetition, presence, frequency, delay, allowed
+RuleIn rule_in(PyObject* const* a) {
+    RuleIn in{optional_tensor(a[0], "history"), optional_tensor(a[1], "lengths"), optional_tensor(a[2], "prompts"), per_row_arg(a[3]),
+              per_row_arg(a[4]), per_row_arg(a[5]), optional_tensor(a[6], "delay"), optional_tensor(a[7], "allowed")};
+    return in;
+}
+
+// rule_layer(times, history, lengths, prompts, repetition, presence, frequency, delay, allowed) -> ruled times, differentiable in times
+SNNTC_METHOD(py_rule_layer) {
+    HANDLE_TH_ERRORS
+    arity(n, 9, "rule_times");
+    const Tensor t = tensor_arg(a[0], "times");
+    const RuleIn in = rule_in(a + 1);
+    if (!plain({t, in.history, in.lengths, in.prompts, in.repetition.each, in.presence.each, in.frequency.each, in.delay, in.allowed}))
+        return general("rule_layer", a, n);
+    Tensor out;
+    {
+        NoGil nogil;
+        out = rule_layer(rule_set(t, in), in);
+    }
+    return wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// rule_times(the same) -> ruled times, without a graph
+SNNTC_METHOD(py_rule_times) {
+    HANDLE_TH_ERRORS
+    arity(n, 9, "rule_times");
+    const Tensor t = tensor_arg(a[0], "times");
+    const RuleIn in = rule_in(a + 1);
+    Tensor out;
+    {
+        NoGil nogil;
+        at::AutoGradMode no_grad(false);
+        out = rule_times(rule_set(t, in));
+    }
+    return wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// rule_times_grad(grad, times, history, lengths, repetition, allowed) -> gradient by the times
+SNNTC_METHOD(py_rule_times_grad) {
+    HANDLE_TH_ERRORS
+    arity(n, 6, "rule_times_grad");
+    const Tensor g = tensor_arg(a[0], "grad"), t = tensor_arg(a[1], "times");
+    RuleIn in{};
+    in.history = optional_tensor(a[2], "history"); in.lengths = optional_tensor(a[3], "lengths");
+    in.repetition = per_row_arg(a[4]); in.allowed = optional_tensor(a[5], "allowed");
+    Tensor d;
+    {
+        NoGil nogil;
+        at::AutoGradMode no_grad(false);
+        d = rule_times_grad(g, rule_set(t, in));
+    }
+    return wrap(d);
+    END_HANDLE_TH_ERRORS
+}
+
+// choose_tokens(times, uniform, temperature, history, lengths, prompts, repetition, presence, frequency, delay, allowed) -> (tokens, logp)
+SNNTC_METHOD(py_choose_tokens) {
+    HANDLE_TH_ERRORS
+    arity(n, 11, "choose_tokens");
+    const Tensor t = tensor_arg(a[0], "times"), u = optional_tensor(a[1], "uniform");
+    const PerRow heat = per_row_arg(a[2]);
+    const RuleIn in = rule_in(a + 3);
+    Choice c;
+    {
+        NoGil nogil;
+        at::AutoGradMode no_grad(false);
+        c = choose_tokens(rule_set(t, in), u, heat);
+    }
+    return wrap2(c.tokens, c.logp);
+    END_HANDLE_TH_ERRORS
+}
+
+// grad_norm(list of gradients) -> norm
+SNNTC_METHOD(py_grad_norm) {
+    HANDLE_TH_ERRORS
+    arity(n, 1, "grad_norm");
+    const std::vector<Tensor> gs = tensor_list(a[0], "gradients");
+    Tensor norm;
+    {
+        NoGil nogil;
+        at::AutoGradMode no_grad(false);
+        norm = grad_norm(gs);
+    }
+    return wrap(norm);
+    END_HANDLE_TH_ERRORS
+}
+
+Moments moments_in(PyObject* const* a) {
+    Moments m{tensor_list(a[0], "first"), tensor_list(a[1], "second"), {}, {}, a[2] != Py_None};
+    TORCH_CHECK_VALUE((a[2] == Py_None) == (a[3] == Py_None), "adamw: first_scale and second_scale go together");
+    if (m.coded) {
+        m.first_scale = tensor_list(a[2], "first_scale");
+        m.second_scale = tensor_list(a[3], "second_scale");
+    }
+    return m;
+}
+
+// adamw_update(weights, gradients, first, second, first_scale, second_scale, step, lr, beta1, beta2, eps, weight_decay, norm, max_norm, seed)
+SNNTC_METHOD(py_adamw_update) {
+    HANDLE_TH_ERRORS
+    arity(n, 15, "adamw_update");
+    const std::vector<Tensor> ws = tensor_list(a[0], "params"), gs = tensor_list(a[1], "grads");
+    const Moments m = moments_in(a + 2);
+    snntc_adamw how{};
+    const Tensor steps = THPVariable_Check(a[6]) ? THPVariable_Unpack(a[6]) : Tensor();
+    if (!steps.defined()) how.step = int_arg(a[6]);
+    how.lr = double_arg(a[7]); how.beta1 = double_arg(a[8]); how.beta2 = double_arg(a[9]); how.eps = double_arg(a[10]);
+    how.weight_decay = double_arg(a[11]);
+    const Tensor norm = optional_tensor(a[12], "norm");
+    how.max_norm = double_arg(a[13]);
+    how.seed = PyLong_AsUnsignedLongLongMask(a[14]);
+    if (PyErr_Occurred()) throw python_error();
+    {
+        NoGil nogil;
+        at::AutoGradMode no_grad(false);
+        adamw_update(ws, gs, m, steps, norm, how);
+    }
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject* wrap_list(const std::vector<Tensor>& v) {
+    PyObject* list = PyList_New((Py_ssize_t)v.size());
+    for (size_t i = 0; list && i < v.size(); ++i) {
+        PyObject* t = wrap(v[i]);
+        if (!t) { Py_DECREF(list); return nullptr; }
+        PyList_SET_ITEM(list, (Py_ssize_t)i, t);
+    }
+    return list;
+}
+
+// adamw_moments(first, second, first_scale, second_scale) -> (list of first moments, list of second moments), float32
+SNNTC_METHOD(py_adamw_moments) {
+    HANDLE_TH_ERRORS
+    arity(n, 4, "adamw_moments");
+    const Moments m = moments_in(a);
+    TORCH_CHECK_VALUE(m.coded, "adamw: moments are read back from codes and scales");
+    MomentsOut out;
+    {
+        NoGil nogil;
+        at::AutoGradMode no_grad(false);
+        out = adamw_moments(m);
+    }
+    PyObject *first = wrap_list(out.first), *second = wrap_list(out.second);
+    PyObject* both = first && second ? PyTuple_Pack(2, first, second) : nullptr;
+    Py_XDECREF(first); Py_XDECREF(second);
+    return both;
+    END_HANDLE_TH_ERRORS
+}
+
 // bind(path, SnntcLibraryError, SnntcError, params_array, general paths): looks the C ABI up in the library loaded from `path`
 SNNTC_METHOD(py_bind) {
     HANDLE_TH_ERRORS
@@ -1777,7 +2273,9 @@ PyMethodDef g_methods[] = {SNNTC_ENTRY(bind), SNNTC_ENTRY(fc_forward), SNNTC_ENT
                            SNNTC_ENTRY(gated_scan_grad), SNNTC_ENTRY(gated_layer), SNNTC_ENTRY(gated_step), SNNTC_ENTRY(time_logp),
                            SNNTC_ENTRY(policy_loss), SNNTC_ENTRY(policy_layer), SNNTC_ENTRY(preference_loss),
                            SNNTC_ENTRY(preference_layer), SNNTC_ENTRY(policy_objective),
-                           SNNTC_ENTRY(preference_objective), SNNTC_ENTRY(objective_grad), {nullptr, nullptr, 0, nullptr}};
+                           SNNTC_ENTRY(preference_objective), SNNTC_ENTRY(objective_grad), SNNTC_ENTRY(rule_layer),
+                           SNNTC_ENTRY(rule_times), SNNTC_ENTRY(rule_times_grad), SNNTC_ENTRY(choose_tokens), SNNTC_ENTRY(grad_norm),
+                           SNNTC_ENTRY(adamw_update), SNNTC_ENTRY(adamw_moments), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_binding", "Native host path of the SNN-TC ops.", -1, g_methods,
                         nullptr, nullptr, nullptr, nullptr};

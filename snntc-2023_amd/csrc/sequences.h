@@ -1,8 +1,10 @@
-// The operators over sequences of tokens and choices (embed.hip, gated.hip, choice.hip): element types, what their kernels share and
+// The operators over sequences of tokens and choices (embed.hip, gated.hip, choice.hip, rules.hip): element types, what their kernels share and
 // their launches.
 #pragma once
 
 #include "snntc_common.h"
+
+#include <algorithm>
 
 namespace snntc {
 
@@ -81,5 +83,56 @@ int launch_preference_loss(const void* times, int type, const int64_t* tokens, c
                            float* seq_logp, float* stats, float* coef, void* dtimes, int64_t P, int64_t T, int64_t J, void* ws,
                            hipStream_t stream);
 int launch_loss_total(const float* loss, const float* weight, float* total, int64_t n, hipStream_t stream);
+
+// Rules on times as the kernels take them (snntc_rules in the public header); history, lengths, prompts, the three penalties, delay and
+// allowed may be NULL.  Strides: from a row to the next, 0 where all rows share one.
+struct RuleArgs {
+    const int64_t* history;
+    const int64_t* lengths;
+    const int64_t* prompts;
+    int64_t L, rows_per_history;
+    const float *repetition, *presence, *frequency;
+    float rep, pres, freq;                 // where the pointers are NULL
+    const float* delay;
+    const unsigned* allowed;
+    int64_t delay_stride, allowed_stride;
+    int most;                              // elements of a slice whose occurrences are counted; set by the launch
+};
+struct ChooseArgs {
+    const float* uniform;
+    const float* temperature;              // NULL: heat for all rows
+    float heat;
+    int64_t* tokens;
+    float* logp;
+};
+size_t choose_workspace(int64_t rows, int64_t J);
+int launch_rule_times(const void* times, int type, const RuleArgs& a, void* out, int64_t rows, int64_t J, hipStream_t stream);
+int launch_rule_times_backward(const void* grad, const void* times, int type, const RuleArgs& a, void* dtimes, int64_t rows, int64_t J,
+                               hipStream_t stream);
+int launch_choose(const void* times, int type, const RuleArgs& a, const ChooseArgs& c, int64_t rows, int64_t J, void* ws, hipStream_t stream);
+
+// One AdamW step (adamw.hip).  Host arrays of `count` entries; scales: NULL where the states are float32.
+struct AdamTensors {
+    void* const* w;
+    const void* const* g;
+    void* const* m;
+    void* const* v;
+    float* const* m_scale;
+    float* const* v_scale;
+    const int* types;
+    const int64_t* n;
+};
+struct AdamNumbers {
+    double lr, b1, b2, eps, decay, max_norm;
+    int64_t step;                          // where steps is NULL
+    int64_t* steps;                        // device: steps done so far
+    const float* norm;                     // device, NULL: gradients are not clipped
+    uint64_t seed;
+};
+size_t grad_norm_workspace(const int64_t* n, int64_t count);
+int launch_grad_norm(const void* const* g, const int* types, const int64_t* n, int count, float* norm, void* ws, hipStream_t stream);
+int launch_adamw(const AdamTensors& a, int count, const AdamNumbers& p, void* ws, hipStream_t stream);
+int launch_adamw_moments(const uint8_t* const* m, const uint8_t* const* v, const float* const* m_scale, const float* const* v_scale,
+                         float* const* first, float* const* second, const int64_t* n, int count, hipStream_t stream);
 
 }  // namespace snntc

@@ -42,6 +42,8 @@ EXPORTS = (
     "snntc_gated_scan_workspace_bytes", "snntc_gated_scan_forward", "snntc_gated_scan_backward", "snntc_gated_step",
     "snntc_choice_workspace_bytes", "snntc_preference_workspace_bytes", "snntc_time_logp", "snntc_time_logp_backward", "snntc_policy_loss",
     "snntc_preference_loss", "snntc_loss_total",
+    "snntc_rule_times", "snntc_rule_times_backward", "snntc_choose_workspace_bytes", "snntc_choose",
+    "snntc_grad_norm_workspace_bytes", "snntc_grad_norm", "snntc_adamw_update", "snntc_adamw_moments",
     "snntc_scan_status", "snntc_debug_set_scan_wait_polls", "snntc_debug_order_tile",
     "snntc_profile_enable", "snntc_profile_collect", "snntc_profile_entry",
 )
@@ -57,6 +59,22 @@ class SnntcError(RuntimeError):
     def __init__(self, status, message):
         super().__init__(f"snntc status {status}: {message}")
         self.status = status
+
+
+class Rules(ctypes.Structure):
+    """snntc_rules: what changes times before a choice."""
+    _fields_ = [("history", ctypes.c_void_p), ("history_rows", ctypes.c_int64), ("history_len", ctypes.c_int64),
+                ("lengths", ctypes.c_void_p), ("prompts", ctypes.c_void_p), ("repetition", ctypes.c_void_p),
+                ("presence", ctypes.c_void_p), ("frequency", ctypes.c_void_p), ("repetition_all", ctypes.c_float),
+                ("presence_all", ctypes.c_float), ("frequency_all", ctypes.c_float), ("delay", ctypes.c_void_p),
+                ("delay_rows", ctypes.c_int64), ("allowed", ctypes.c_void_p), ("allowed_rows", ctypes.c_int64)]
+
+
+class AdamW(ctypes.Structure):
+    """snntc_adamw: the numbers of a step."""
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double),
+                ("weight_decay", ctypes.c_double), ("step", ctypes.c_int64), ("steps", ctypes.c_void_p), ("norm", ctypes.c_void_p),
+                ("max_norm", ctypes.c_double), ("seed", ctypes.c_uint64)]
 
 
 _lib = None
@@ -148,6 +166,15 @@ def load():
     lib.snntc_policy_loss.argtypes = [vp, i32, vp, vp, vp, vp, vp, f32, f32, f32, vp, vp, vp, vp, vp, i64, i64, vp, sz, vp]
     lib.snntc_preference_loss.argtypes = [vp, i32, vp, vp, vp, f32, f32, vp, vp, vp, vp, vp, i64, i64, i64, vp, sz, vp]
     lib.snntc_loss_total.argtypes = [vp, vp, vp, i64, vp]
+    prules, pp, pint = c.POINTER(Rules), c.POINTER(vp), c.POINTER(c.c_int)
+    lib.snntc_rule_times.argtypes = [vp, i32, prules, vp, i64, i64, vp]
+    lib.snntc_rule_times_backward.argtypes = [vp, vp, i32, prules, vp, i64, i64, vp]
+    lib.snntc_choose_workspace_bytes.argtypes = [i64, i64, psz]
+    lib.snntc_choose.argtypes = [vp, i32, vp, vp, f32, prules, vp, vp, i64, i64, vp, sz, vp]
+    lib.snntc_grad_norm_workspace_bytes.argtypes = [pi64, i64, psz]
+    lib.snntc_grad_norm.argtypes = [pp, pint, pi64, i64, vp, vp, sz, vp]
+    lib.snntc_adamw_update.argtypes = [pp, pp, pp, pp, pp, pp, pint, pi64, i64, c.POINTER(AdamW), vp, sz, vp]
+    lib.snntc_adamw_moments.argtypes = [pp, pp, pp, pp, pp, pp, pi64, i64, vp]
     lib.snntc_scan_status.argtypes = [c.POINTER(i64), vp]
     lib.snntc_debug_set_scan_wait_polls.argtypes = [c.c_int]
     lib.snntc_debug_order_tile.argtypes = [i64, i64, i64, i64, fparams, c.c_int, c.POINTER(i64)]

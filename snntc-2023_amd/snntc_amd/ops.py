@@ -8,7 +8,8 @@ Counterparts of the reference's op handles (SNN_TC_Modules.py:29-33, 89-93):
     snncv_grad(grad, Xpad, W, Params, Y)     -> (dXpad, dW, dParams)
 
 Around them: loss, pooling, padding and update of an image network; for networks over sequences of tokens embed_tokens,
-gated_scan / gated_step, policy_time_loss and preference_time_loss.
+gated_scan / gated_step, policy_time_loss and preference_time_loss; rule_times and choose_tokens, which choose what those losses are about,
+and adamw_update with grad_norm, the update after them.
 
 ``SnnFc`` / ``SnnCv`` are the differentiable ops that replace ``@ops.RegisterGradient``.
 Tensors must be float32 on a ROCm device (tables, gates and the last two losses' times may be 16-bit floats); ``Params`` is the host-side float32 vector the layers
@@ -602,6 +603,93 @@ class PreferenceTimeLoss(torch.autograd.Function):
         return *_objective_grad(ctx, upstream), None, None, None, None, None
 
 
+def pack_allowed(mask):
+    """A truth value per output, mask[..., J], as the words that rules take: int32 [..., ceil(J / 32)], output j bit j % 32 of word
+    j // 32.  (Grammars mostly come as such words; this is for those that do not.)"""
+    short = -mask.shape[-1] % 32
+    bits = torch.nn.functional.pad(mask.to(torch.bool), (0, short)).unflatten(-1, (-1, 32)).to(torch.int64)
+    words = (bits << torch.arange(32, device=mask.device)).sum(-1)
+    return torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32)
+
+
+def rule_times(times, history=None, lengths=None, prompts=None, repetition=1.0, presence=0.0, frequency=0.0, delay=None, allowed=None):
+    """Spike times times[..., J] (float32, bfloat16 or float16) after the rules of a choice, of their type and differentiable in them.
+    history[S, L] (int64) holds S sequences of tokens, and every rows / S consecutive rows of times belong to one of them: a
+    row sees its first lengths[...] tokens (None: all; tokens outside the outputs are none), of which the first prompts[S]
+    (None: 0) are a prompt.  With c_j the occurrences of j among them and o_j those behind the prompt
+        a_j = times_j * repetition, or times_j / repetition where times_j <= 0,  if c_j > 0    (an output's chance falls, repetition > 1)
+        b_j = a_j + (presence + frequency * o_j)                                  if o_j > 0
+        result_j = b_j + delay_j                                                  where allowed, +infinity elsewhere
+    repetition, presence, frequency: a number, or float32 [S].  delay: float32 [J] or of times' shape.  allowed: int32 words of 32 outputs
+    each, [ceil(J / 32)] or [..., ceil(J / 32)] (see pack_allowed).  Computed in float32, rounded once."""
+    return TimeRules.apply(times, history, lengths, prompts, repetition, presence, frequency, delay, allowed)
+
+
+def rule_times_grad(grad, times, history=None, lengths=None, repetition=1.0, allowed=None):
+    """Gradient of rule_times with respect to times, of their type; what else it takes is constant."""
+    return _lib.native().rule_times_grad(grad, times, history, lengths, repetition, allowed)
+
+
+class TimeRules(torch.autograd.Function):
+    """rule_times, differentiable in times."""
+
+    @classmethod
+    def apply(cls, times, history=None, lengths=None, prompts=None, repetition=1.0, presence=0.0, frequency=0.0, delay=None, allowed=None):
+        return _lib.native().rule_layer(times, history, lengths, prompts, repetition, presence, frequency, delay, allowed)
+
+    @staticmethod
+    def forward(ctx, times, history, lengths, prompts, repetition, presence, frequency, delay, allowed):
+        each = {"repetition": repetition, "presence": presence, "frequency": frequency, "delay": delay}
+        _no_gradient("rule_times", **{k: v for k, v in each.items() if isinstance(v, torch.Tensor)})
+        ctx.repetition = None if isinstance(repetition, torch.Tensor) else repetition
+        ctx.save_for_backward(times, history, lengths, None if ctx.repetition is not None else repetition, allowed)
+        return _lib.native().rule_times(times, history, lengths, prompts, repetition, presence, frequency, delay, allowed)
+
+    @staticmethod
+    def backward(ctx, grad):
+        times, history, lengths, repetition, allowed = ctx.saved_tensors
+        with torch.no_grad():
+            d = rule_times_grad(grad, times, history, lengths, ctx.repetition if repetition is None else repetition, allowed)
+        return *_once("rule_times", [d], times, grad), None, None, None, None, None, None, None, None
+
+
+def choose_tokens(times, uniform, temperature=1.0, history=None, lengths=None, prompts=None, repetition=1.0, presence=0.0, frequency=0.0,
+                  delay=None, allowed=None):
+    """A token for every row of times[..., J], drawn from p = softmax(-rule_times(times, ...) / temperature), and its logarithm ->
+    (tokens[...] int64, logp[...] float32).  uniform[...] (float32, from [0, 1)) decides: the token is the first whose running sum of p
+    exceeds it.  temperature: a number, or float32 [...]; at 0 the earliest output is taken, the lowest index of equal ones, with its
+    log-probability at temperature 1 (uniform may be None where the number is 0).  A row whose rules leave nothing, or with a NaN
+    among what they leave, gives token -1 and NaN.  The ruled times are not stored.  Not differentiable: see rule_times."""
+    return _lib.native().choose_tokens(times, uniform, temperature, history, lengths, prompts, repetition, presence, frequency, delay, allowed)
+
+
+def grad_norm(grads):
+    """The 2-norm of all gradients together, a float32 scalar on their device (sums in 64 bits, the same on every call)."""
+    return _lib.native().grad_norm(list(grads))
+
+
+def adamw_update(params, grads, first, second, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, norm=None, max_norm=1.0,
+                 first_scale=None, second_scale=None, seed=0):
+    """One AdamW step over all tensors in one launch (48 tensors of a type to a launch), in place:
+        m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,
+        w = w (1 - lr weight_decay) - lr / (1 - b1^step) m / (sqrt(v / (1 - b2^step)) + eps)
+    params: float32, bfloat16 or float16, contiguous, grads of their types; first, second: m and v, float32, or uint8 codes with
+    first_scale, second_scale, float32 [ceil(n / 256)] (zeros to begin with).  step: the number of this step, from 1, or an int64
+    device tensor with the number of steps done, which the call advances (for graphs).  norm: grad_norm(grads); gradients are scaled down
+    to max_norm where it is larger, and nothing is changed where it is no finite number.  Codes and 16-bit weights are rounded up or
+    down by chance, from random bits that follow from seed, the step and the element's place."""
+    params, grads = list(params), list(grads)
+    if params or grads:
+        _lib.native().adamw_update(params, grads, list(first), list(second), None if first_scale is None else list(first_scale),
+                                   None if second_scale is None else list(second_scale), step, lr, betas[0], betas[1], eps, weight_decay,
+                                   norm, max_norm, seed)
+
+
+def adamw_moments(first, second, first_scale, second_scale):
+    """What 8-bit states stand for: (list of m, list of v), float32."""
+    return _lib.native().adamw_moments(list(first), list(second), list(first_scale), list(second_scale))
+
+
 def _function(cls, *args):
     return super(cls, cls).apply(*args)                     # torch.autograd.Function's own
 
@@ -622,4 +710,6 @@ GENERAL = {
         PolicyTimeLoss, times, actions, old, adv, ref, weight, (low, high), kl),
     "preference_layer": lambda times, tokens, ref, weight, beta, smoothing: _function(
         PreferenceTimeLoss, times, tokens, ref, weight, beta, smoothing),
+    "rule_layer": lambda times, history, lengths, prompts, rep, pres, freq, delay, allowed: _function(
+        TimeRules, times, history, lengths, prompts, rep, pres, freq, delay, allowed),
 }

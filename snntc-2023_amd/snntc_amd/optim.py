@@ -1,0 +1,109 @@
+"""AdamW as a ``torch.optim.Optimizer`` over the update kernel, for the steps in train.py and any other loop (the reference takes its
+framework's Adam, snntc-mnist.py:70)."""
+import torch
+
+from .ops import adamw_update, grad_norm
+
+_BLOCK = 256                                             # elements of a state that share a scale
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW over all tensors of a group in one launch (see ops.adamw_update for the formula).
+
+      state_bits  32, or 8: codes with a scale for every 256 elements, a quarter of the memory
+      max_norm    None, or what the norm over all gradients of a step is scaled down to; a step whose norm is no finite number then
+                  changes nothing but its number.  `norm` is the last step's, on the device
+      seed        of the random bits by which codes and 16-bit weights are rounded
+      capturable  the steps are counted on the device, so that a captured step counts by itself when it is replayed; learning
+                  rate and the other numbers stay what they were when it was captured
+
+    Weights: contiguous float32, bfloat16 or float16 tensors on one ROCm device, with gradients of their types."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, max_norm=None, seed=0,
+                 capturable=False):
+        if state_bits not in (8, 32):
+            raise ValueError(f"states are held in 8 or 32 bits, not in {state_bits}")
+        self.state_bits, self.max_norm, self.seed, self.capturable = state_bits, max_norm, int(seed), bool(capturable)
+        self.norm = None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def _begin(self, p, steps):
+        """The state of a tensor that has its first gradient."""
+        zeros = lambda n, dtype: torch.zeros(n, dtype=dtype, device=p.device)                   # noqa: E731
+        if self.state_bits == 8:
+            blocks = -(-p.numel() // _BLOCK)
+            state = {"first": zeros(p.shape, torch.uint8), "second": zeros(p.shape, torch.uint8),
+                     "first_scale": zeros(blocks, torch.float32), "second_scale": zeros(blocks, torch.float32)}
+        else:
+            state = {"first": zeros(p.shape, torch.float32), "second": zeros(p.shape, torch.float32)}
+        if self.capturable:
+            if p.device not in steps:                    # one counter for all that begin in the same step
+                steps[p.device] = zeros((), torch.int64)
+            state["step"] = steps[p.device]
+        else:
+            state["step"] = 0
+        self.state[p] = state
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if not self.capturable and torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: a step that is captured into a graph needs capturable=True")
+        groups = []
+        for group in self.param_groups:
+            params = [p for p in group["params"] if p.grad is not None]
+            if any(p.grad.is_sparse for p in params):
+                raise RuntimeError("AdamW: sparse gradients are not supported")
+            groups.append(params)
+        grads = [p.grad for params in groups for p in params]
+        if not grads:
+            return loss
+        self.norm = None if self.max_norm is None else grad_norm(grads)
+        call = 0
+        for group, params in zip(self.param_groups, groups):
+            steps = {}
+            for p in params:
+                if not self.state[p]:
+                    self._begin(p, steps)
+            together = {}                                # tensors with the same number of steps behind them
+            for p in params:
+                n = self.state[p]["step"]
+                together.setdefault(id(n) if self.capturable else n, []).append(p)
+            for tensors in together.values():
+                states = [self.state[p] for p in tensors]
+                number = states[0]["step"]
+                if not self.capturable:
+                    number += 1
+                    for s in states:
+                        s["step"] = number
+                scales = ([s["first_scale"] for s in states], [s["second_scale"] for s in states]) if self.state_bits == 8 else (None, None)
+                adamw_update([p.detach() for p in tensors], [p.grad for p in tensors], [s["first"] for s in states],
+                             [s["second"] for s in states], number, lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                             weight_decay=group["weight_decay"], norm=self.norm, max_norm=self.max_norm or 1.0, first_scale=scales[0],
+                             second_scale=scales[1], seed=self.seed + (call << 32))
+                call += 1
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """As the base class, but a state keeps the type it was saved with (the base class makes it the weights')."""
+        super().load_state_dict(state_dict)
+        params = [p for group in self.param_groups for p in group["params"]]
+        saved = [i for group in state_dict["param_groups"] for i in group["params"]]
+        counters = {}
+        for i, p in zip(saved, params):
+            if i not in state_dict["state"]:
+                continue
+            old = state_dict["state"][i]
+            if ("first_scale" in old) != (self.state_bits == 8):
+                raise ValueError(f"AdamW: the saved states are not of {self.state_bits} bits")
+            state = {k: v.detach().to(p.device, copy=True) for k, v in old.items() if k != "step"}
+            step = int(old["step"])
+            if self.capturable:
+                if (p.device, step) not in counters:
+                    counters[p.device, step] = torch.tensor(step, dtype=torch.int64, device=p.device)
+                step = counters[p.device, step]
+            state["step"] = step
+            self.state[p] = state

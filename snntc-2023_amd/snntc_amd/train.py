@@ -9,7 +9,8 @@ factors, is stock PyTorch around the gfx950 ops.  Weights are saved and restored
 import torch
 
 from ._lib import native
-from .layers import loss_func, policy_loss, preference_loss
+from .layers import SNN_recurrence, SNN_steps, loss_func, policy_loss, preference_loss
+from .ops import choose_tokens, rule_times
 
 
 def encode_input(images):
@@ -97,23 +98,82 @@ def test_step(model, images, labels, num_classes, weight_k=100.0, weight_k2=1e-2
     return loss, (predictions_to_classes(predictions) == labels).sum()
 
 
-def policy_step(model, optimizer, inputs, actions, old_logp, advantage, ref_logp=None, weight=None, clip=(0.2, 0.2), kl_coef=0.0):
+def _ruled(times, rows, rules):
+    times = times.reshape(*rows, times.shape[-1])
+    return rule_times(times, **rules) if rules else times
+
+
+def policy_step(model, optimizer, inputs, actions, old_logp, advantage, ref_logp=None, weight=None, clip=(0.2, 0.2), kl_coef=0.0, rules=None):
     """One optimisation step of a policy on choices it has made: model(inputs) -> spike times with a row per action.  old_logp,
-    ref_logp: ops.time_logp of the model that made the choices and of the reference.  Returns the loss."""
+    ref_logp: ops.time_logp of the model that made the choices and of the reference.  rules: a dict of ops.rule_times' arguments
+    by which the choices were made, every row with its own part of the history (answer_batch).  Returns the loss."""
     optimizer.zero_grad(set_to_none=True)
-    times = model(inputs)
-    loss = policy_loss(times.reshape(*actions.shape, times.shape[-1]), actions, old_logp, advantage, ref_logp, weight, clip, kl_coef)
+    times = _ruled(model(inputs), actions.shape, rules)
+    loss = policy_loss(times, actions, old_logp, advantage, ref_logp, weight, clip, kl_coef)
     loss.backward()
     optimizer.step()
     return loss.detach()
 
 
-def preference_step(model, optimizer, inputs, tokens, ref_logp, weight=None, beta=0.1, smoothing=0.0):
+def preference_step(model, optimizer, inputs, tokens, ref_logp, weight=None, beta=0.1, smoothing=0.0, rules=None):
     """One optimisation step on pairs of sequences, the preferred ones first: model(inputs) -> spike times with a row per token
-    of tokens[2P,T].  ref_logp[2P]: the sequences' log-probabilities under the reference.  Returns the loss."""
+    of tokens[2P,T].  ref_logp[2P]: the sequences' log-probabilities under the reference.  rules: as in policy_step.  Returns the loss."""
     optimizer.zero_grad(set_to_none=True)
-    times = model(inputs)
-    loss = preference_loss(times.reshape(*tokens.shape, times.shape[-1]), tokens, ref_logp, weight, beta, smoothing)
+    times = _ruled(model(inputs), tokens.shape, rules)
+    loss = preference_loss(times, tokens, ref_logp, weight, beta, smoothing)
     loss.backward()
     optimizer.step()
     return loss.detach()
+
+
+@torch.no_grad()
+def answer(net, prompt, uniform, temperature=1.0, **rules):
+    """Continues the sequences prompt[B,P] (int64, P >= 1) token by token: net is a networks.SnnSequential over tokens with SNN_steps
+    between its recurrences and its dense layers, uniform[B,T] (float32, from [0, 1)) draws T tokens of each sequence, rules are
+    ops.rule_times' repetition, presence, frequency, delay and allowed, the same for every step.  Returns (tokens[B,T], logp[B,T]), logp being
+    the tokens' log-probabilities as they were drawn: at temperature 1 what policy_step takes as old_logp (see answer_batch)."""
+    B, P = prompt.shape
+    T = uniform.shape[1]
+    layers = list(net)
+    cut = next((i for i, layer in enumerate(layers) if isinstance(layer, SNN_steps)), None)
+    if P < 1 or cut is None:
+        raise ValueError("answer continues prompts of at least one token, by a network over tokens with an SNN_steps layer")
+    history = torch.cat([prompt, prompt.new_zeros(B, T)], 1)
+    logp = uniform.new_empty(B, T)
+    states, x = {}, prompt
+    for i, layer in enumerate(layers[:cut]):                        # the prompts at once
+        if isinstance(layer, SNN_recurrence):
+            x, states[i] = layer(x, return_state=True)
+        else:
+            x = layer(x)
+    x = x[:, -1].contiguous()
+    prompts = torch.full((B,), P, dtype=torch.int64, device=prompt.device)
+    for t in range(T):
+        if t:
+            x = history[:, P + t - 1]
+            for i, layer in enumerate(layers[:cut]):
+                if isinstance(layer, SNN_recurrence):
+                    x = states[i] = layer.step(x, states[i])
+                else:
+                    x = layer(x)
+        for layer in layers[cut + 1:]:
+            x = layer(x)
+        token, logp[:, t] = choose_tokens(x, uniform[:, t], temperature, history, prompts + t, prompts, **rules)
+        history[:, P + t] = token
+    return history[:, P:], logp
+
+
+def answer_batch(prompt, tokens, logp, advantage, **rules):
+    """policy_step's arguments for tokens[B,T] and logp[B,T] of answer(net, prompt, ..., **rules) and advantage[B], one for each
+    sequence: a dict of inputs, actions, old_logp, advantage, weight (the mean over the drawn tokens; a prompt's rows have none) and rules."""
+    (B, P), T = prompt.shape, tokens.shape[1]
+    history = torch.cat([prompt, tokens], 1)
+    rows = lambda x: torch.cat([x.new_zeros(B, P - 1), x], 1)                                   # noqa: E731
+    for k in ("delay", "allowed"):                                  # of every sequence: of each of its rows
+        if rules.get(k) is not None and rules[k].dim() == 2:
+            rules[k] = rules[k][:, None].expand(B, P + T - 1, -1)
+    seen = torch.arange(1, P + T, device=prompt.device).expand(B, P + T - 1)
+    drawn = rows((tokens >= 0).float())
+    return dict(inputs=history[:, :-1], actions=history[:, 1:], old_logp=rows(logp), advantage=advantage[:, None].expand(B, P + T - 1),
+                weight=drawn / drawn.sum().clamp(min=1.0),
+                rules=dict(history=history, lengths=seen, prompts=torch.full_like(prompt[:, 0], P), **rules))
