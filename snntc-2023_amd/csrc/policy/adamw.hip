@@ -15,7 +15,7 @@
 // bits wide between the codes: next to a border a sum in 32 bits would leave another code than the definition.
 // 16-bit weights are rounded in the same way and for the same reason: a step of a thousandth of a weight is less than half of what
 // they can tell apart.
-#include "sequences.h"
+#include "../sequences.h"
 
 namespace snntc {
 namespace {

@@ -10,7 +10,7 @@
 // length.  So LDS holds a quarter of a byte for each element, whatever the vocabulary, and an element that no token names costs one bit test.
 // The arithmetic of a ruled time is float32 without contraction: products and sums round one by one, as written above.  A
 // token is drawn from the times as rule_times stores them, rounded to times' type, so that its log-probability is that of the ruled times.
-#include "sequences.h"
+#include "../sequences.h"
 
 namespace snntc {
 namespace {

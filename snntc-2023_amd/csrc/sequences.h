@@ -1,4 +1,4 @@
-// The operators over sequences of tokens and choices (embed.hip, gated.hip, choice.hip, rules.hip): element types, what their kernels share and
+// The operators over sequences of tokens and choices (embed.hip, gated.hip, choice.hip, policy/rules.hip): element types, what their kernels share and
 // their launches.
 #pragma once
 
@@ -111,7 +111,7 @@ int launch_rule_times_backward(const void* grad, const void* times, int type, co
                                hipStream_t stream);
 int launch_choose(const void* times, int type, const RuleArgs& a, const ChooseArgs& c, int64_t rows, int64_t J, void* ws, hipStream_t stream);
 
-// One AdamW step (adamw.hip).  Host arrays of `count` entries; scales: NULL where the states are float32.
+// One AdamW step (policy/adamw.hip).  Host arrays of `count` entries; scales: NULL where the states are float32.
 struct AdamTensors {
     void* const* w;
     const void* const* g;
