@@ -803,7 +803,7 @@ int snntc_choose(const void* times, int times_type, const float* uniform, const 
     if (!(temperature_all >= 0.0f && temperature_all < INFINITY))
         return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_choose: temperature %g outside its range", (double)temperature_all);
     if (rows == 0) return SNNTC_OK;
-    if (!times || !tokens || !logp || (!uniform && (temperature || temperature_all >= 1e-37f)))
+    if (!times || !tokens || !logp || (!uniform && (temperature || temperature_all >= 1e-30f)))
         return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_choose: null pointer");
     rc = check_workspace(workspace, workspace_bytes, choose_workspace(rows, J));
     if (rc) return rc;

@@ -5,9 +5,8 @@
 //     t'_j = b_j + delay_j  where j is allowed, +infinity elsewhere,         dt_j = dt'_j (1, r or 1 / r; 0 where not allowed)
 // and a token is the first j with sum_{i <= j} exp(-(t'_i - min t') / T) > u sum_i exp(-(t'_i - min t') / T).
 //
-// A workgroup owns a slice of a row.  It marks the history's tokens that lie in the slice in a bitmap in LDS, a bit for each element; where
-// occurrences count, the marked elements are numbered by their rank in the bitmap and counted in an array of at most the history's
-// length.  So LDS holds a quarter of a byte for each element, whatever the vocabulary, and an element that no token names costs one bit test.
+// A workgroup owns a slice of a row.  It marks the history's tokens that lie in the slice in a bitmap in LDS, a bit for each element, and
+// counts the occurrences of marked elements: an element that no token names costs one bit test.
 // The arithmetic of a ruled time is float32 without contraction: products and sums round one by one, as written above.  A
 // token is drawn from the times as rule_times stores them, rounded to times' type, so that its log-probability is that of the ruled times.
 #include "../sequences.h"
@@ -16,11 +15,13 @@ namespace snntc {
 namespace {
 
 constexpr float kLog2e = 1.44269504f;
-
+constexpr float kColdest = 1e-30f;                   // temperatures below count as 0: log2(e) / T has to leave room for a time
 // VEC elements, 16 bytes (or, of float32, 32), at any place of their type: the target loads and stores four words at any address.
 template <typename E, int VEC>
 struct Piece { E v[VEC]; };
 typedef unsigned Words __attribute__((ext_vector_type(4)));
+typedef unsigned WordsAt2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned WordsAt4 __attribute__((ext_vector_type(4), aligned(4)));
 template <typename E>
 struct __attribute__((packed, aligned(sizeof(E)))) Place { Words w; };
 template <typename E, int VEC>
@@ -32,6 +33,9 @@ __device__ __forceinline__ Piece<E, VEC> read_piece(const E* at) {
     return __builtin_bit_cast(Piece<E, VEC>, all);
 }
 
+// A launch's workgroup among fewer than 2^32: 2^24 rows, and as many slices as their times' memory has place for.
+__device__ __forceinline__ unsigned place() { return (unsigned)workgroup(); }
+
 // What is the same for a whole row.
 struct RowRules {
     const long long* tokens;
@@ -40,11 +44,11 @@ struct RowRules {
     const float* delay;
     const unsigned* allowed;
 };
-__device__ __forceinline__ RowRules row_rules(const RuleArgs& a, int64_t r) {
+__device__ __forceinline__ RowRules row_rules(const RuleArgs& a, unsigned r) {
     RowRules q{};
     q.rep = 1.0f;
     if (a.history) {
-        const int64_t h = r / a.rows_per_history;
+        const int64_t h = r / (unsigned)a.rows_per_history;
         q.tokens = reinterpret_cast<const long long*>(a.history) + h * a.L;
         const auto inside = [&](int64_t n) { return (int)(n < 0 ? 0 : n > a.L ? a.L : n); };
         q.seen = a.lengths ? inside(a.lengths[r]) : (int)a.L;
@@ -54,64 +58,107 @@ __device__ __forceinline__ RowRules row_rules(const RuleArgs& a, int64_t r) {
         q.freq = a.frequency ? a.frequency[h] : a.freq;
         q.inv = 1.0f / q.rep;
     }
-    q.delay = a.delay ? a.delay + r * a.delay_stride : nullptr;
-    q.allowed = a.allowed ? a.allowed + r * a.allowed_stride : nullptr;
+    q.delay = a.delay ? a.delay + (int64_t)r * a.delay_stride : nullptr;
+    q.allowed = a.allowed ? a.allowed + (int64_t)r * a.allowed_stride : nullptr;
     return q;
 }
 
-extern __shared__ unsigned lds_marks[];
+// The marks of a slice of WIDTH * PER elements in LDS: a bitmap and, for COUNT (16-bit or 32-bit integers), occurrences; only those of
+// marked elements are ever cleared or read.
+template <int SLICE, typename COUNT>
+struct MarkMemory { unsigned bits[SLICE / 32]; COUNT count[SLICE]; };
+// For the gradient: `late` marked elements have a time above 0.
+template <int SLICE>
+struct MarkMemory<SLICE, void> { unsigned bits[SLICE / 32], late[SLICE / 32]; };
 
-// The marks of a slice of WIDTH * PER elements in LDS: a bitmap, the marked elements before each of its words, and their occurrences.
-template <int WIDTH, int PER>
+template <int WIDTH, int PER, typename COUNT>
 struct Marks {
-    static constexpr int kSlice = WIDTH * PER, kWords = kSlice / 32, kWaves = WIDTH / kWave;
-    static_assert(kWords <= WIDTH, "a word for each thread");
-    // (named by their place in LDS: kept as pointers they would be read as generic memory)
-    __device__ __forceinline__ static unsigned& bits(int i) { return lds_marks[i]; }
-    __device__ __forceinline__ static unsigned& before(int i) { return lds_marks[kWords + i]; }
-    __device__ __forceinline__ static unsigned& count(int i) { return lds_marks[2 * kWords + i]; }
+    static constexpr int kSlice = WIDTH * PER, kWords = kSlice / 32, kHeld = 1024 / WIDTH < 2 ? 2 : 1024 / WIDTH > 8 ? 8 : 1024 / WIDTH;
+    static constexpr bool kCounts = !std::is_void<COUNT>::value;
+    using Memory = MarkMemory<kSlice, COUNT>;
+    int held[kHeld];                                 // the thread's first tokens; -1: none
 
-    // Returns whether there are any rules from the history; every thread of the workgroup calls it.
-    __device__ __forceinline__ bool build(const RowRules& q, int64_t first, int J, int most, bool counts) {
-        counts = counts && (q.pres != 0.0f || q.freq != 0.0f) && q.prompt < q.seen;
+    __device__ __forceinline__ static void batch(int (&to)[kHeld], const long long* tokens, int64_t from, int64_t end, int J) {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const int64_t at = from + i * WIDTH + (int)threadIdx.x;
+            const long long token = at < end ? tokens[at] : -1;
+            to[i] = (unsigned long long)token < (unsigned long long)J ? (int)token : -1;
+        }
+    }
+    // Before the row's numbers are known: the two do not wait for each other.
+    __device__ __forceinline__ void request(const RuleArgs& a, const RowRules& q, int J) {
+        if (a.history) batch(held, q.tokens, 0, a.L, J);
+    }
+    // f(elements) of the tokens [from, seen), batch by batch: their places in the slice, -1 where they have none.
+    template <typename F>
+    __device__ __forceinline__ void each(const RowRules& q, int from, int first, int end, int J, F&& f) const {
+        const auto use = [&](const int (&tok)[kHeld], int base) {
+            int j[kHeld];
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) {
+                const int at = base + i * WIDTH + (int)threadIdx.x;
+                j[i] = at >= from && at < q.seen && (unsigned)(tok[i] - first) < (unsigned)end ? tok[i] - first : -1;
+            }
+            f(j);
+        };
+        use(held, 0);
+        for (int base = kHeld * WIDTH; base < q.seen; base += kHeld * WIDTH) {
+            int tok[kHeld];
+            batch(tok, q.tokens, base, q.seen, J);
+            use(tok, base);
+        }
+    }
+    // Returns whether there are any rules from the history; every thread of the workgroup calls it.  times: of the slice, for the signs.
+    template <typename E>
+    __device__ __forceinline__ bool build(Memory& lds, const RowRules& q, int64_t first, int J, const E* times) const {
+        const bool counts = counted(q);
         if (q.seen == 0 || (q.rep == 1.0f && !counts)) return false;                   // (uniform)
-        const int k = threadIdx.x, end = (int)min((int64_t)kSlice, J - first);
-        if (k < kWords) { bits(k) = 0; before(k) = 0; }
-        if (counts) for (int i = k; i < most; i += WIDTH) count(i) = 0;
-        __syncthreads();
-        for (int i = k; i < q.seen; i += WIDTH) {
-            const int64_t j = q.tokens[i] - first;
-            if (j >= 0 && j < end) atomicOr(&bits(j >> 5), 1u << (j & 31));
-        }
-        __syncthreads();
-        if (!counts) return true;
-        __shared__ unsigned total[kWaves];
-        const int mine = k < kWords ? __popc(bits(k)) : 0;
-        int sum = mine;
+        const int end = (int)min((int64_t)kSlice, J - first), k = threadIdx.x;
 #pragma unroll
-        for (int d = 1; d < kWave; d <<= 1) {
-            const int other = __shfl_up(sum, d, kWave);
-            if (k % kWave >= d) sum += other;
-        }
-        if (kWaves > 1) {
-            if (k % kWave == kWave - 1) total[k / kWave] = sum;
+        for (int w = 0; w < (kWords + WIDTH - 1) / WIDTH; ++w)
+            if (w * WIDTH + k < kWords) {
+                lds.bits[w * WIDTH + k] = 0;
+                if constexpr (!kCounts) lds.late[w * WIDTH + k] = 0;
+            }
+        __syncthreads();
+        each(q, 0, (int)first, end, J, [&](const int (&j)[kHeld]) {
+            float t[kHeld];
+            if constexpr (!kCounts) {
+#pragma unroll
+                for (int i = 0; i < kHeld; ++i) t[i] = j[i] >= 0 ? (float)times[j[i]] : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) {
+                if (j[i] < 0) continue;
+                atomicOr(&lds.bits[j[i] >> 5], 1u << (j[i] & 31));
+                if constexpr (kCounts) lds.count[j[i]] = 0;
+                else if (t[i] > 0.0f) atomicOr(&lds.late[j[i] >> 5], 1u << (j[i] & 31));
+            }
+        });
+        __syncthreads();
+        if constexpr (kCounts) {
+            if (!counts) return true;
+            each(q, q.prompt, (int)first, end, J, [&](const int (&j)[kHeld]) {
+#pragma unroll
+                for (int i = 0; i < kHeld; ++i) {
+                    if (j[i] < 0) continue;
+                    const unsigned at = j[i];
+                    if constexpr (sizeof(COUNT) == 2)                                  // (at most 2^16 - 1 of a token: no carry to the neighbour)
+                        atomicAdd(reinterpret_cast<unsigned*>(&lds.count[at & ~1u]), at & 1 ? 1u << 16 : 1u);
+                    else
+                        atomicAdd(&lds.count[at], (COUNT)1);
+                }
+            });
             __syncthreads();
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w)
-                if (w < k / kWave) sum += total[w];
         }
-        if (k < kWords) before(k) = sum - mine;
-        __syncthreads();
-        for (int i = q.prompt + k; i < q.seen; i += WIDTH) {
-            const int64_t j = q.tokens[i] - first;
-            if (j >= 0 && j < end) atomicAdd(&count(slot((int)j)), 1u);
-        }
-        __syncthreads();
         return true;
     }
-    __device__ __forceinline__ int slot(int j) const { return before(j >> 5) + __popc(bits(j >> 5) & ((1u << (j & 31)) - 1)); }
-    __device__ __forceinline__ unsigned marked(int j, int vec) const { return bits(j >> 5) >> (j & 31) & ((1u << vec) - 1); }
-    __device__ __forceinline__ bool counted(const RowRules& q) const { return (q.pres != 0.0f || q.freq != 0.0f) && q.prompt < q.seen; }
+    __device__ __forceinline__ static unsigned marked(const Memory& lds, int j, int vec) { return lds.bits[j >> 5] >> (j & 31) & ((1u << vec) - 1); }
+    __device__ __forceinline__ static unsigned late(const Memory& lds, int j) { return lds.late[j >> 5] >> (j & 31); }
+    __device__ __forceinline__ static bool counted(const RowRules& q) {
+        return kCounts && (q.pres != 0.0f || q.freq != 0.0f) && q.prompt < q.seen;
+    }
 };
 
 // A marked element's time before the delay.
@@ -128,35 +175,65 @@ __device__ __forceinline__ float ruled(float t, unsigned occurrences, const RowR
     return t;
 }
 
-// The ruled times of one piece: VEC elements from j on, of which n are in the row.
-template <typename E, int VEC, typename M>
-__device__ __forceinline__ void rule_piece(float (&t)[VEC], const M& marks, bool from_history, const RowRules& q, int64_t first, int local, int n) {
-    const int64_t j = first + local;
-    if (from_history) {
-        const unsigned m = marks.marked(local, VEC);
-        if (m) {
-            const bool counted = marks.counted(q);
+// t where bit `at` of a mask is set, `other` elsewhere: a sign-extended bit selects.
+__device__ __forceinline__ float where_bit(unsigned mask, int at, float t, float other) {
+    const unsigned m = (unsigned)__builtin_amdgcn_sbfe((int)mask, at, 1);
+    return __uint_as_float((__float_as_uint(t) & m) | (__float_as_uint(other) & ~m));
+}
+
+// Keeps the compiler from carrying a piece's elements in float32 from one use to the next, which takes half of the wavefronts' registers.
+template <typename P>
+__device__ __forceinline__ void forget(P& p) {
+    Words w = __builtin_bit_cast(Words, p);
+    asm volatile("" : "+v"(w));
+    p = __builtin_bit_cast(P, w);
+}
+
+// What a piece needs besides its times, requested before the history is gone through: the two do not wait for each other.
+template <int VEC>
+struct Extras { Piece<float, VEC> delay; unsigned allowed; };
+template <int VEC>
+__device__ __forceinline__ void request_delay(Extras<VEC>& x, const RowRules& q, int64_t j, int n) {
+    if (!q.delay || n <= 0) return;
+    if (n >= VEC) {
+        x.delay = read_piece<float, VEC>(q.delay + j);
+    } else {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v)
-                if (m >> v & 1) t[v] = ruled(t[v], counted ? marks.count(marks.slot(local + v)) : 0, q);
-        }
+        for (int v = 0; v < VEC; ++v) x.delay.v[v] = v < n ? q.delay[j + v] : 0.0f;
+    }
+}
+__device__ __forceinline__ unsigned request_allowed(const RowRules& q, int64_t j, int n) { return q.allowed && n > 0 ? q.allowed[j >> 5] >> (j & 31) : 0u; }
+
+// The ruled times of one piece.  Marked elements are few: one at a time and lane, instead of a test for each.
+template <typename E, int VEC, typename M>
+__device__ __forceinline__ void rule_piece(Piece<E, VEC>& p, const typename M::Memory& lds, bool from_history, const RowRules& q,
+                                           const Extras<VEC>& x, int local) {
+    unsigned m = from_history ? M::marked(lds, local, VEC) : 0;
+    if (!m && !q.delay && !q.allowed) return;
+    float t[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) t[v] = (float)p.v[v];
+    const bool counted = M::counted(q);
+    while (m) {
+        const int at = __ffs(m) - 1;
+        m &= m - 1;
+        float y = t[0];
+#pragma unroll
+        for (int v = 1; v < VEC; ++v) y = at == v ? t[v] : y;
+        y = ruled(y, counted ? (unsigned)lds.count[local + at] : 0, q);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) t[v] = at == v ? y : t[v];
     }
     if (q.delay) {
-        if (n == VEC) {
-            const Piece<float, VEC> d = read_piece<float, VEC>(q.delay + j);
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) t[v] += d.v[v];
-        } else {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v)
-                if (v < n) t[v] += q.delay[j + v];
-        }
+        for (int v = 0; v < VEC; ++v) t[v] += x.delay.v[v];
     }
     if (q.allowed) {
-        const unsigned a = q.allowed[j >> 5] >> (j & 31);
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) t[v] = a >> v & 1 ? t[v] : INFINITY;
+        for (int v = 0; v < VEC; ++v) t[v] = where_bit(x.allowed, v, t[v], INFINITY);
     }
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) p.v[v] = (E)t[v];
 }
 
 template <typename E, int VEC>
@@ -167,10 +244,13 @@ __device__ __forceinline__ Piece<E, VEC> load_piece(const E* t, int n, E fill) {
     for (int v = 0; v < VEC; ++v) p.v[v] = v < n ? t[v] : fill;
     return p;
 }
-template <typename E, int VEC>
+template <bool STREAM, typename E, int VEC>
 __device__ __forceinline__ void store_piece(E* t, const Piece<E, VEC>& p, int n) {
     if (n == VEC) {
-        reinterpret_cast<Place<E>*>(t)->w = __builtin_bit_cast(Words, p);
+        if constexpr (STREAM)
+            __builtin_nontemporal_store(__builtin_bit_cast(Words, p), reinterpret_cast<typename std::conditional<sizeof(E) == 2, WordsAt2, WordsAt4>::type*>(t));
+        else
+            reinterpret_cast<Place<E>*>(t)->w = __builtin_bit_cast(Words, p);
         return;
     }
 #pragma unroll
@@ -180,149 +260,173 @@ __device__ __forceinline__ void store_piece(E* t, const Piece<E, VEC>& p, int n)
 
 // Ruled times, or (GRAD) the gradient by the times: in = times or the upstream gradient.  The gradient reads times where a token
 // repeats only: their sign is all it needs.
-template <typename E, int VEC, int WIDTH, int R, bool GRAD>
+template <typename E, int VEC, int WIDTH, int R, typename COUNT, bool STREAM>
 __global__ void __launch_bounds__(WIDTH)
 rule_kernel(const E* __restrict__ in, const E* __restrict__ times, E* __restrict__ out, RuleArgs a, int64_t rows, int J, int slices) {
-    using M = Marks<WIDTH, VEC * R>;
-    const int64_t block = workgroup(), r = block / slices;
+    using M = Marks<WIDTH, VEC * R, COUNT>;
+    constexpr bool GRAD = !M::kCounts;
+    __shared__ typename M::Memory lds;
+    const unsigned block = place(), r = block / (unsigned)slices;
     if (r >= rows) return;
-    const int64_t first = (block % slices) * (int64_t)M::kSlice;
+    const int64_t first = (int64_t)(block - r * (unsigned)slices) * M::kSlice, row = (int64_t)r * J;
     const int end = (int)min((int64_t)M::kSlice, J - first);
-    const E* __restrict__ x = in + r * J + first;
-    E* __restrict__ y = out + r * J + first;
-    Piece<E, VEC> held[R];
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int local = (i * WIDTH + (int)threadIdx.x) * VEC;
-        if (local < end) held[i] = load_piece<E, VEC>(x + local, min(VEC, end - local), (E)0.0f);
-    }
+    const E* __restrict__ x = in + row + first;
+    E* __restrict__ y = out + row + first;
     const RowRules q = row_rules(a, r);
     M marks;
-    const bool from_history = marks.build(q, first, J, a.most, !GRAD);
+    marks.request(a, q, J);
+    const auto at = [&](int i) { return (i * WIDTH + (int)threadIdx.x) * VEC; };
+    Piece<E, VEC> held[R];
+    unsigned allowed[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        const int local = (i * WIDTH + (int)threadIdx.x) * VEC;
-        if (local >= end) continue;
-        const int n = min(VEC, end - local);
-        float t[VEC];
+        if (at(i) < end) held[i] = load_piece<E, VEC>(x + at(i), min(VEC, end - at(i)), (E)0.0f);
+        allowed[i] = request_allowed(q, first + at(i), end - at(i));
+    }
+    Extras<VEC> extras;
+    if constexpr (!GRAD) request_delay(extras, q, first + at(0), end - at(0));
+    const bool from_history = marks.build(lds, q, first, J, GRAD ? times + row + first : nullptr);
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) t[v] = (float)held[i].v[v];
+    for (int i = 0; i < R; ++i) {
         if constexpr (GRAD) {
-            const unsigned m = from_history ? marks.marked(local, VEC) : 0;
+            if (at(i) >= end) continue;
+            const unsigned m = from_history ? M::marked(lds, at(i), VEC) : 0;
             if (m) {
-                const E* __restrict__ at = times + r * J + first + local;
+                const unsigned late = M::late(lds, at(i));
 #pragma unroll
-                for (int v = 0; v < VEC; ++v)
-                    if (m >> v & 1) t[v] *= (float)at[v] > 0.0f ? q.rep : q.inv;
+                for (int v = 0; v < VEC; ++v) {
+                    const float t = (float)held[i].v[v] * where_bit(late, v, q.rep, q.inv);
+                    held[i].v[v] = m >> v & 1 ? (E)t : held[i].v[v];
+                }
             }
             if (q.allowed) {
-                const int64_t j = first + local;
-                const unsigned w = q.allowed[j >> 5] >> (j & 31);
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) t[v] = w >> v & 1 ? t[v] : 0.0f;
+                for (int v = 0; v < VEC; ++v) held[i].v[v] = allowed[i] >> v & 1 ? held[i].v[v] : (E)0.0f;
             }
         } else {
-            rule_piece<E, VEC>(t, marks, from_history, q, first, local, n);
+            Extras<VEC> next;
+            if (i + 1 < R) request_delay(next, q, first + at(i + 1), end - at(i + 1));
+            if (at(i) >= end) continue;
+            extras.allowed = allowed[i];
+            rule_piece<E, VEC, M>(held[i], lds, from_history, q, extras, at(i));
+            extras = next;
         }
-        Piece<E, VEC> p;
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) p.v[v] = (E)t[v];
-        store_piece<E, VEC>(y + local, p, n);
+        store_piece<STREAM, E, VEC>(y + at(i), held[i], min(VEC, end - at(i)));
     }
 }
 
-// A part of a row: the largest negated time m, sum of exp((-t' - m) / T), and the first index that attains m.
-struct Part { double s; float m; int arg; };
+// A wavefront's run of a row: the largest negated time m, the sum of exp((-t' - m) / T), and the first index in the run that attains m (where
+// it is asked for).
+struct Part { float s, m; int arg, unused; };
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int d = kWave / 2; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, kWave));
-    return v;
+// v of the lane that CTRL names, `none` where MASK leaves a row of 16 out.
+template <int CTRL, int MASK, typename T>
+__device__ __forceinline__ T from_lane(T none, T v) {
+    static_assert(sizeof(T) == 4, "one register");
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v), CTRL, MASK, 0xF, false));
 }
-__device__ __forceinline__ float wave_sum(float v) {
+// All of a wavefront's values joined, in the registers' own network: pairs, quads, eights and sixteens by exchange, then lane 15 of a row to
+// the next one and lane 31 to the upper half; the last lane has them all.
+template <typename T, typename F>
+__device__ __forceinline__ T wave_join(T v, T none, F&& f) {
+    v = f(v, from_lane<0xB1, 0xF>(v, v));
+    v = f(v, from_lane<0x4E, 0xF>(v, v));
+    v = f(v, from_lane<0x141, 0xF>(v, v));
+    v = f(v, from_lane<0x140, 0xF>(v, v));
+    v = f(v, from_lane<0x142, 0xA>(none, v));
+    v = f(v, from_lane<0x143, 0xC>(none, v));
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), kWave - 1));
+}
+__device__ __forceinline__ float wave_max(float v) { return wave_join(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); }); }
+__device__ __forceinline__ float wave_sum(float v) { return wave_join(v, 0.0f, [](float a, float b) { return a + b; }); }
+__device__ __forceinline__ int wave_min(int v) { return wave_join(v, INT32_MAX, [](int a, int b) { return min(a, b); }); }
+__device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
     for (int d = kWave / 2; d > 0; d >>= 1) v += __shfl_xor(v, d, kWave);
     return v;
 }
-__device__ __forceinline__ int wave_min(int v) {
-#pragma unroll
-    for (int d = kWave / 2; d > 0; d >>= 1) v = min(v, __shfl_xor(v, d, kWave));
-    return v;
-}
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.0f : m; }
-// exp(v / T), k = log2(e) / T.  The argument is a difference from a maximum: what its rounding loses is its own size in half
-// steps, of a term that shrinks faster than that grows.
-__device__ __forceinline__ float soft(float v, float k) { return __builtin_amdgcn_exp2f(v * k); }
-__device__ __forceinline__ double weight_of(const Part& p, float m, float k) { return p.s * (double)soft(p.m - base_of(m), k); }
-
-// Where a part of a list begins, and the list's maximum and sum.  Parts in order; k: log2(e) / T.
-struct Chosen { int part; double rest; float m; double total; };
+// exp(d / T), k = log2(e) / T, of a difference from a maximum: what the argument's rounding loses is its own size in half steps, of a
+// term that shrinks faster than that grows, and equal times have terms of exactly 1.
+__device__ __forceinline__ float term(float d, float k) { return __builtin_amdgcn_exp2f(d * k); }
+__device__ __forceinline__ double weight_of(const Part& p, float m, float k) { return (double)p.s * (double)term(p.m - base_of(m), k); }
 
 // A row's elements as a wavefront holds them: R pieces, WIDTH / 64 wavefronts one behind the other, so that each has a run of the slice.
-template <typename E, int VEC, int WIDTH, int R>
+template <typename E, int VEC, int WIDTH, int R, typename COUNT>
 struct Run {
-    float v[R][VEC];                                 // negated ruled times; -infinity: not allowed, or behind the row
-    __device__ __forceinline__ static int local(int i) {
-        return (((int)threadIdx.x / kWave * R + i) * kWave + (int)threadIdx.x % kWave) * VEC;
-    }
-    __device__ __forceinline__ void load(const E* times, const RuleArgs& a, const RowRules& q, int64_t first, int J) {
+    static constexpr int kLength = kWave * VEC * R;
+    using M = Marks<WIDTH, VEC * R, COUNT>;
+    Piece<E, VEC> t[R];                              // ruled times; +infinity: not allowed, or behind the row
+    __device__ __forceinline__ static int in_run(int i) { return (i * kWave + (int)threadIdx.x % kWave) * VEC; }
+    __device__ __forceinline__ static int local(int i) { return (int)threadIdx.x / kWave * kLength + in_run(i); }
+    __device__ __forceinline__ float v(int i, int e) const { return -(float)t[i].v[e]; }
+    __device__ __forceinline__ void load(const E* times, const RuleArgs& a, const RowRules& q, int64_t first, int J, typename M::Memory& lds) {
         const int end = (int)min((int64_t)WIDTH * VEC * R, J - first);
-        Piece<E, VEC> held[R];
-#pragma unroll
-        for (int i = 0; i < R; ++i)
-            if (local(i) < end) held[i] = load_piece<E, VEC>(times + first + local(i), min(VEC, end - local(i)), (E)0.0f);
-        Marks<WIDTH, VEC * R> marks;
-        const bool from_history = marks.build(q, first, J, a.most, true);
+        M marks;
+        marks.request(a, q, J);
+        unsigned allowed[R];
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            if (local(i) >= end) {
+            if (local(i) < end) {
+                t[i] = load_piece<E, VEC>(times + first + local(i), min(VEC, end - local(i)), (E)INFINITY);
+            } else {
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) v[i][e] = -INFINITY;
-                continue;
+                for (int e = 0; e < VEC; ++e) t[i].v[e] = (E)INFINITY;
             }
-            const int n = min(VEC, end - local(i));
-            float t[VEC];
+            allowed[i] = request_allowed(q, first + local(i), end - local(i));
+        }
+        Extras<VEC> extras;
+        request_delay(extras, q, first + local(0), end - local(0));
+        const bool from_history = marks.build(lds, q, first, J, times);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) t[e] = (float)held[i].v[e];
-            rule_piece<E, VEC>(t, marks, from_history, q, first, local(i), n);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) v[i][e] = e < n ? -(float)(E)t[e] : -INFINITY;
+        for (int i = 0; i < R; ++i) {
+            Extras<VEC> next;
+            if (i + 1 < R) request_delay(next, q, first + local(i + 1), end - local(i + 1));
+            extras.allowed = allowed[i];
+            if (local(i) < end) rule_piece<E, VEC, M>(t[i], lds, from_history, q, extras, local(i));
+            extras = next;
         }
     }
-    __device__ __forceinline__ Part part(float k, bool greedy) const {
+    __device__ __forceinline__ Part part(float k, bool greedy) {
         float m = -INFINITY;
 #pragma unroll
         for (int i = 0; i < R; ++i)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) m = fmaxf(m, v[i][e]);
+            for (int e = 0; e < VEC; ++e) m = fmaxf(m, v(i, e));
         m = wave_max(m);
         const float base = base_of(m);
         float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < R; ++i)
+        for (int i = 0; i < R; ++i) {
+            forget(t[i]);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) sum += soft(v[i][e] - base, k);
-        Part p{(double)wave_sum(sum), m, 0};
+            for (int e = 0; e < VEC; ++e) sum += term(v(i, e) - base, k);
+        }
+        Part p{wave_sum(sum), m, 0, 0};
         if (greedy) {                                                  // (uniform)
             int at = INT32_MAX;
 #pragma unroll
-            for (int i = R - 1; i >= 0; --i)
+            for (int i = R - 1; i >= 0; --i) {
+                forget(t[i]);
 #pragma unroll
                 for (int e = VEC - 1; e >= 0; --e)
-                    if (v[i][e] == m) at = local(i) + e;
+                    if (v(i, e) == m) at = in_run(i) + e;
+            }
             p.arg = wave_min(at);
         }
         return p;
     }
-    // The first element whose running sum exceeds `rest`, the last possible one where rounding leaves none; -1 in a run without any.
-    __device__ __forceinline__ int pick(double rest, float m, float k, float* value) const {
+    // The first element of the run whose running sum exceeds `rest`, the last possible one where rounding leaves none; -1 in
+    // a run without any.
+    __device__ __forceinline__ int pick(double rest, float m, float k, float* value) {
         const float base = base_of(m);
         const int lane = threadIdx.x % kWave;
 #pragma unroll
         for (int i = 0; i < R; ++i) {
+            forget(t[i]);
             float e[VEC], sum = 0.0f;
 #pragma unroll
-            for (int x = 0; x < VEC; ++x) sum += e[x] = soft(v[i][x] - base, k);
+            for (int x = 0; x < VEC; ++x) sum += e[x] = term(v(i, x) - base, k);
             float run = sum;
 #pragma unroll
             for (int d = 1; d < kWave; d <<= 1) {
@@ -341,19 +445,20 @@ struct Run {
                 if (at < 0) { if ((double)e[x] > left) at = x; else left -= e[x]; }
             }
             at = at < 0 ? last : at;
-            float mine = v[i][0];
+            float mine = v(i, 0);
 #pragma unroll
-            for (int x = 1; x < VEC; ++x) mine = at == x ? v[i][x] : mine;
+            for (int x = 1; x < VEC; ++x) mine = at == x ? v(i, x) : mine;
             *value = __shfl(mine, owner, kWave);
-            return __shfl(local(i) + at, owner, kWave);
+            return __shfl(in_run(i) + at, owner, kWave);
         }
 #pragma unroll
         for (int i = R - 1; i >= 0; --i) {
+            forget(t[i]);
             int last = -1;
             float mine = 0.0f;
 #pragma unroll
             for (int x = 0; x < VEC; ++x)
-                if (soft(v[i][x] - base, k) > 0.0f) { last = local(i) + x; mine = v[i][x]; }
+                if (term(v(i, x) - base, k) > 0.0f) { last = in_run(i) + x; mine = v(i, x); }
             const unsigned long long any = __ballot(last >= 0);
             if (!any) continue;
             const int owner = 63 - __clzll(any);
@@ -365,122 +470,43 @@ struct Run {
 };
 
 struct Heat { float k; bool greedy, valid; double t; };
-// Temperatures below 1e-37 count as 0: log2(e) / T has to be a number.
 __device__ __forceinline__ Heat heat_of(const ChooseArgs& a, int64_t r) {
     const float t = a.temperature ? a.temperature[r] : a.heat;
     Heat h;
     h.valid = t >= 0.0f && t < INFINITY;
-    h.greedy = t < 1e-37f;
+    h.greedy = t < kColdest;
     h.k = h.greedy || !h.valid ? kLog2e : kLog2e / t;
     h.t = h.greedy || !h.valid ? 1.0 : (double)t;
     return h;
 }
-__device__ __forceinline__ void store_choice(const ChooseArgs& a, int64_t r, const Heat& h, int64_t token, float value, float m, double total) {
-    a.tokens[r] = token;
-    a.logp[r] = token < 0 ? NAN : (float)(((double)value - (double)m) / h.t - log(total));
-}
 
-// One slice of a row: its part to `parts`, or (WHOLE: the slice is the row) the row's token.
-// Bound by memory and, in a call of few rows, by the way from the history's tokens through LDS to the sums.
-template <typename E, int VEC, int WIDTH, int R, bool WHOLE>
-__global__ void __launch_bounds__(WIDTH)
-choose_slice_kernel(const E* __restrict__ times, RuleArgs a, ChooseArgs c, Part* __restrict__ parts, int64_t rows, int J, int slices) {
-    constexpr int kWaves = WIDTH / kWave;
-    const int64_t block = workgroup(), r = WHOLE ? block : block / slices;
-    if (r >= rows) return;
-    const int slice = WHOLE ? 0 : block % slices;
-    const int64_t first = (int64_t)slice * (WIDTH * VEC * R);
-    const RowRules q = row_rules(a, r);
-    const Heat h = heat_of(c, r);
-    Run<E, VEC, WIDTH, R> run;
-    run.load(times + r * J, a, q, first, J);
-    Part mine = run.part(h.k, h.greedy);
-    __shared__ Part part[kWaves];
-    if (kWaves > 1) {
-        if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = mine;
-        __syncthreads();
-    }
-    float m = mine.m;
-    double total = mine.s;
-    int arg = mine.arg;
-    if (kWaves > 1) {
-        m = part[0].m;
-#pragma unroll
-        for (int w = 1; w < kWaves; ++w) m = fmaxf(m, part[w].m);
-        total = 0.0;
-        arg = INT32_MAX;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            total += weight_of(part[w], m, h.k);
-            if (part[w].m == m) arg = min(arg, part[w].arg);
-        }
-    }
-    if constexpr (!WHOLE) {
-        if (threadIdx.x == 0) parts[r * slices + slice] = Part{total, m, arg};
-        return;
-    }
-    if (!(total > 0.0) || !h.valid) {                                   // nothing possible, or no numbers
-        if (threadIdx.x == 0) store_choice(c, r, h, -1, 0.0f, m, total);
-        return;
-    }
-    if (h.greedy) {
-        if (threadIdx.x == 0) store_choice(c, r, h, arg, m, m, total);
-        return;
-    }
-    const float u = c.uniform[r];
-    double rest = total * (double)(u > 0.0f ? u : 0.0f);
-    int owner = -1, last = 0;
-    if (kWaves > 1) {
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            const double s = weight_of(part[w], m, h.k);
-            if (s > 0.0) last = w;
-            if (owner < 0) { if (s > rest) owner = w; else rest -= s; }
-        }
-        if (owner < 0) { owner = last; rest = INFINITY; }
-        if ((int)threadIdx.x / kWave != owner) return;
-        rest /= (double)soft(mine.m - base_of(m), h.k);
-    }
-    float value = 0.0f;
-    const int at = run.pick(rest, mine.m, h.k, &value);
-    if (threadIdx.x % kWave == 0) store_choice(c, r, h, at, value, m, total);
-}
-
-// A row's slices joined in order, and the token found in the one that it lies in: that slice is read once more.
-template <typename E, int VEC, int WIDTH, int R>
-__global__ void __launch_bounds__(WIDTH)
-choose_join_kernel(const E* __restrict__ times, RuleArgs a, ChooseArgs c, const Part* __restrict__ parts, int J, int slices) {
-    constexpr int kWaves = WIDTH / kWave;
-    const int64_t r = blockIdx.x;
-    const Heat h = heat_of(c, r);
-    const Part* __restrict__ p = parts + r * slices;
+// A row's n parts joined by a wavefront, and the part that the row's token lies in: part -1: there is none.
+struct Found { int part; double rest, total; float m; };
+template <typename P>
+__device__ __forceinline__ Found find_part(P&& parts, int n, const Heat& h, const float* uniform, int64_t r) {
     const int lane = threadIdx.x % kWave;
-    // every wavefront joins the slices by itself
     float m = -INFINITY;
-    for (int i = lane; i < slices; i += kWave) m = fmaxf(m, p[i].m);
+    for (int i = lane; i < n; i += kWave) m = fmaxf(m, parts(i).m);
     m = wave_max(m);
     double total = 0.0;
     int best = INT32_MAX;
-    for (int i = lane; i < slices; i += kWave) {
-        total += weight_of(p[i], m, h.k);
-        if (p[i].m == m) best = min(best, i);
+    for (int i = lane; i < n; i += kWave) {
+        const Part p = parts(i);
+        total += weight_of(p, m, h.k);
+        if (p.m == m) best = min(best, i);
     }
-#pragma unroll
-    for (int d = kWave / 2; d > 0; d >>= 1) total += __shfl_xor(total, d, kWave);
-    best = wave_min(best);
-    if (!(total > 0.0) || !h.valid) {
-        if (threadIdx.x == 0) store_choice(c, r, h, -1, 0.0f, m, total);
-        return;
-    }
+    total = wave_sum(total);
+    Found f{-1, 0.0, total, m};
+    if (!(total > 0.0) || !h.valid) return f;                           // nothing possible, or no numbers
     if (h.greedy) {
-        if (threadIdx.x == 0) store_choice(c, r, h, (int64_t)best * (WIDTH * VEC * R) + p[best].arg, m, m, total);
-        return;
+        f.part = wave_min(best);
+        return f;
     }
-    const float u = c.uniform[r];
+    const float u = uniform[r];
     double rest = total * (double)(u > 0.0f ? u : 0.0f);
-    int slice = -1, last = 0;
-    for (int i0 = 0; i0 < slices && slice < 0; i0 += kWave) {
-        const double s = i0 + lane < slices ? weight_of(p[i0 + lane], m, h.k) : 0.0;
+    int last = 0;
+    for (int i0 = 0; i0 < n && f.part < 0; i0 += kWave) {
+        const double s = i0 + lane < n ? weight_of(parts(i0 + lane), m, h.k) : 0.0;
         double run = s;
 #pragma unroll
         for (int d = 1; d < kWave; d <<= 1) {
@@ -491,120 +517,177 @@ choose_join_kernel(const E* __restrict__ times, RuleArgs a, ChooseArgs c, const 
         if (any) last = i0 + 63 - __clzll(any);
         if (over) {
             const int owner = __ffsll(over) - 1;
-            slice = i0 + owner;
+            f.part = i0 + owner;
             rest -= __shfl(run - s, owner, kWave);
         } else {
             rest -= __shfl(run, kWave - 1, kWave);
         }
     }
-    if (slice < 0) { slice = last; rest = INFINITY; }
-    rest = fmax(rest, 0.0);
-    const Part part = p[slice];
-    rest /= (double)soft(part.m - base_of(m), h.k);
-    const int64_t first = (int64_t)slice * (WIDTH * VEC * R);
+    if (f.part < 0) { f.part = last; rest = INFINITY; }
+    // (in units of the part's own sum, which the choice of the part keeps above 0)
+    f.rest = fmax(rest, 0.0) / (double)term(parts(f.part).m - base_of(m), h.k);
+    return f;
+}
+
+__device__ __forceinline__ void store_choice(const ChooseArgs& a, int64_t r, const Heat& h, int64_t token, float value, const Found& f) {
+    a.tokens[r] = token;
+    a.logp[r] = token < 0 ? NAN : (float)(((double)value - (double)f.m) / h.t - log(f.total));
+}
+
+// A slice of a row.  WHOLE: the slice is the row, and the row's token is found; else its wavefronts' parts go to `parts`.
+template <typename E, int VEC, int WIDTH, int R, typename COUNT, bool WHOLE>
+__global__ void __launch_bounds__(WIDTH)
+choose_slice_kernel(const E* __restrict__ times, RuleArgs a, ChooseArgs c, Part* __restrict__ parts, int64_t rows, int J, int slices) {
+    using Mine = Run<E, VEC, WIDTH, R, COUNT>;
+    constexpr int kWaves = WIDTH / kWave;
+    __shared__ typename Mine::M::Memory lds;
+    __shared__ Part part[kWaves];
+    const unsigned block = place(), r = WHOLE ? block : block / (unsigned)slices;
+    if (r >= rows) return;
+    const int slice = WHOLE ? 0 : block - r * (unsigned)slices, wave = threadIdx.x / kWave;
     const RowRules q = row_rules(a, r);
-    Run<E, VEC, WIDTH, R> run;
-    run.load(times + r * J, a, q, first, J);
-    const Part mine = run.part(h.k, false);
-    float base = mine.m;
-    if (kWaves > 1) {
-        __shared__ Part wave[kWaves];
-        if (lane == 0) wave[threadIdx.x / kWave] = mine;
-        __syncthreads();
-        int owner = -1, back = 0;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            const double s = weight_of(wave[w], part.m, h.k);
-            if (s > 0.0) back = w;
-            if (owner < 0) { if (s > rest) owner = w; else rest -= s; }
-        }
-        if (owner < 0) { owner = back; rest = INFINITY; }
-        if ((int)threadIdx.x / kWave != owner) return;
-        rest /= (double)soft(mine.m - base_of(part.m), h.k);
+    const Heat h = heat_of(c, r);
+    Mine run;
+    run.load(times + (int64_t)r * J, a, q, (int64_t)slice * (WIDTH * VEC * R), J, lds);
+    const Part mine = run.part(h.k, h.greedy);
+    if constexpr (!WHOLE) {
+        if (threadIdx.x % kWave == 0) parts[((int64_t)r * slices + slice) * kWaves + wave] = mine;
+        return;
     }
+    if (threadIdx.x % kWave == 0) part[wave] = mine;
+    __syncthreads();
+    const Found f = find_part([&](int i) { return part[i]; }, kWaves, h, c.uniform, r);
+    if (wave != (f.part < 0 ? 0 : f.part)) return;
+    int at = -1;
     float value = 0.0f;
-    const int at = run.pick(rest, base, h.k, &value);
-    if (lane == 0) store_choice(c, r, h, at < 0 ? -1 : first + at, value, m, total);
+    if (f.part >= 0 && h.greedy) { at = mine.arg; value = mine.m; }
+    else if (f.part >= 0) at = run.pick(f.rest, mine.m, h.k, &value);
+    if (threadIdx.x % kWave == 0) store_choice(c, r, h, at < 0 ? -1 : wave * Mine::kLength + at, value, f);
+}
+
+// A row's parts joined in order by a wavefront, which reads the run that the token lies in once more.
+template <typename E, int VEC, int R, typename COUNT>
+__global__ void __launch_bounds__(kWave)
+choose_join_kernel(const E* __restrict__ times, RuleArgs a, ChooseArgs c, const Part* __restrict__ parts, int J, int count) {
+    using Mine = Run<E, VEC, kWave, R, COUNT>;
+    __shared__ typename Mine::M::Memory lds;
+    const int64_t r = blockIdx.x;
+    const Heat h = heat_of(c, r);
+    const Part* __restrict__ p = parts + r * count;
+    const Found f = find_part([&](int i) { return p[i]; }, count, h, c.uniform, r);
+    int64_t token = -1;
+    float value = 0.0f;
+    if (f.part >= 0) {
+        const int64_t first = (int64_t)f.part * Mine::kLength;
+        if (h.greedy) {
+            token = first + p[f.part].arg;
+            value = p[f.part].m;
+        } else {
+            Mine run;
+            run.load(times + r * J, a, row_rules(a, r), first, J, lds);
+            const int at = run.pick(f.rest, p[f.part].m, h.k, &value);
+            token = at < 0 ? -1 : first + at;
+        }
+    }
+    if (threadIdx.x == 0) store_choice(c, r, h, token, value, f);
 }
 
 // ---- launches --------------------------------------------------------------------------------------------------------------------
 
-// Bytes of LDS of a slice's marks; a slice counts at most min(slice, L) elements.
-template <int SLICE>
-size_t marks_bytes(const RuleArgs& a) { return a.history ? (size_t)SLICE / 4 + 4 * (size_t)a.most : 0; }
-
-template <typename E, int WIDTH, int R, bool GRAD>
-int launch_rule_slices(const void* in, const void* times, void* out, RuleArgs a, int64_t rows, int64_t J, hipStream_t stream) {
+template <typename E, int WIDTH, int R, typename COUNT, bool STREAM>
+int launch_rule_slices(const void* in, const void* times, void* out, const RuleArgs& a, int64_t rows, int64_t J, hipStream_t stream) {
     constexpr int VEC = 16 / sizeof(E), kSlice = WIDTH * VEC * R;
     const int slices = (int)((J + kSlice - 1) / kSlice);
-    a.most = a.history && !GRAD ? (int)std::min<int64_t>(a.L, kSlice) : 0;
     {
-        KernelTimerScope timer_(GRAD ? "rule_times_backward" : "rule_times", stream);
-        hipLaunchKernelGGL((rule_kernel<E, VEC, WIDTH, R, GRAD>), wide_grid(rows * slices, WIDTH), dim3(WIDTH), marks_bytes<kSlice>(a), stream,
+        KernelTimerScope timer_(std::is_void<COUNT>::value ? "rule_times_backward" : "rule_times", stream);
+        hipLaunchKernelGGL((rule_kernel<E, VEC, WIDTH, R, COUNT, STREAM>), wide_grid(rows * slices, WIDTH), dim3(WIDTH), 0, stream,
                            static_cast<const E*>(in), static_cast<const E*>(times), static_cast<E*>(out), a, rows, (int)J, slices);
     }
     SNNTC_HIP_CHECK(hipGetLastError());
     return SNNTC_OK;
 }
 
-template <bool GRAD>
+// Slices of 4096 elements, of 2048 and a wavefront each in rows of up to 8192 elements (rows of 5003 f16 times with their gradient, 2328 of
+// them: 38 and 33 us; of 32000 bf16 times, 4096 of them: 256 and 310 us).
+template <typename COUNT>
 int launch_rules(const void* in, const void* times, int type, const RuleArgs& a, void* out, int64_t rows, int64_t J, hipStream_t stream) {
     return with_type(type, [&](auto e) -> int {
         using E = decltype(e);
         constexpr int VEC = 16 / sizeof(E);
-        if (J <= 64 * VEC) return launch_rule_slices<E, 64, 1, GRAD>(in, times, out, a, rows, J, stream);
-        return launch_rule_slices<E, 256, 4, GRAD>(in, times, out, a, rows, J, stream);
+        if (J <= 64 * VEC) return launch_rule_slices<E, 64, 1, COUNT, false>(in, times, out, a, rows, J, stream);
+        if (J <= 8192) return launch_rule_slices<E, 64, 32 / VEC, COUNT, false>(in, times, out, a, rows, J, stream);
+        // (4096 rows of 32000 bf16 times without rules: 96 and 89 us)
+        if (2 * rows * J * (int64_t)sizeof(E) > kStreamBytes) return launch_rule_slices<E, 256, 16 / VEC, COUNT, true>(in, times, out, a, rows, J, stream);
+        return launch_rule_slices<E, 256, 16 / VEC, COUNT, false>(in, times, out, a, rows, J, stream);
     });
 }
 
-template <typename E, int WIDTH, int R>
-int launch_choose_slices(const void* times, RuleArgs a, const ChooseArgs& c, int64_t rows, int64_t J, void* ws, hipStream_t stream) {
-    constexpr int VEC = 16 / sizeof(E), kSlice = WIDTH * VEC * R;
-    const int slices = (int)((J + kSlice - 1) / kSlice);
-    const E* t = static_cast<const E*>(times);
-    Part* parts = static_cast<Part*>(ws);
-    a.most = a.history ? (int)std::min<int64_t>(a.L, kSlice) : 0;
-    if (slices == 1) {
+template <typename E, int WIDTH, int R, typename COUNT>
+int launch_choose_whole(const void* times, const RuleArgs& a, const ChooseArgs& c, int64_t rows, int64_t J, hipStream_t stream) {
+    constexpr int VEC = 16 / sizeof(E);
+    {
         KernelTimerScope timer_("choose", stream);
-        hipLaunchKernelGGL((choose_slice_kernel<E, VEC, WIDTH, R, true>), wide_grid(rows, WIDTH), dim3(WIDTH), marks_bytes<kSlice>(a), stream, t, a, c,
-                           nullptr, rows, (int)J, 1);
-    } else {
-        {
-            KernelTimerScope timer_("choose_slice", stream);
-            hipLaunchKernelGGL((choose_slice_kernel<E, VEC, WIDTH, R, false>), wide_grid(rows * slices, WIDTH), dim3(WIDTH), marks_bytes<kSlice>(a),
-                               stream, t, a, c, parts, rows, (int)J, slices);
-        }
-        KernelTimerScope timer_("choose_join", stream);
-        hipLaunchKernelGGL((choose_join_kernel<E, VEC, WIDTH, R>), dim3((unsigned)rows), dim3(WIDTH), marks_bytes<kSlice>(a), stream, t, a, c, parts,
-                           (int)J, slices);
+        hipLaunchKernelGGL((choose_slice_kernel<E, VEC, WIDTH, R, COUNT, true>), wide_grid(rows, WIDTH), dim3(WIDTH), 0, stream,
+                           static_cast<const E*>(times), a, c, nullptr, rows, (int)J, 1);
     }
     SNNTC_HIP_CHECK(hipGetLastError());
     return SNNTC_OK;
 }
 
-constexpr int kChooseSlice = 256 * 32;
+template <typename E, int WIDTH, int R, typename COUNT>
+int launch_choose_slices(const void* times, const RuleArgs& a, const ChooseArgs& c, int64_t rows, int64_t J, Part* parts, hipStream_t stream) {
+    constexpr int VEC = 16 / sizeof(E), kSlice = WIDTH * VEC * R, kWaves = WIDTH / kWave;
+    const int slices = (int)((J + kSlice - 1) / kSlice);
+    {
+        KernelTimerScope timer_("choose_slice", stream);
+        hipLaunchKernelGGL((choose_slice_kernel<E, VEC, WIDTH, R, COUNT, false>), wide_grid(rows * slices, WIDTH), dim3(WIDTH), 0, stream,
+                           static_cast<const E*>(times), a, c, parts, rows, (int)J, slices);
+    }
+    {
+        KernelTimerScope timer_("choose_join", stream);
+        hipLaunchKernelGGL((choose_join_kernel<E, VEC, R, COUNT>), dim3((unsigned)rows), dim3(kWave), 0, stream, static_cast<const E*>(times), a, c,
+                           parts, (int)J, slices * kWaves);
+    }
+    SNNTC_HIP_CHECK(hipGetLastError());
+    return SNNTC_OK;
+}
+
+// Occurrences are counted in 16 bits where no token can have more.
+bool narrow(const RuleArgs& a) { return !a.history || a.L < (1 << 16); }
 
 }  // namespace
 
-size_t choose_workspace(int64_t rows, int64_t J) {
-    return J > kChooseSlice ? align_up((size_t)rows * (size_t)((J + kChooseSlice - 1) / kChooseSlice) * sizeof(Part)) : 0;
-}
+// Every wavefront of a row's slices leaves a part; the shortest slices are of 4096 elements and four wavefronts.
+size_t choose_workspace(int64_t rows, int64_t J) { return J > 4096 ? align_up((size_t)rows * (size_t)((J + 4095) / 4096 * 4) * sizeof(Part)) : 0; }
 
 int launch_rule_times(const void* times, int type, const RuleArgs& a, void* out, int64_t rows, int64_t J, hipStream_t stream) {
-    return launch_rules<false>(times, nullptr, type, a, out, rows, J, stream);
+    return narrow(a) ? launch_rules<unsigned short>(times, nullptr, type, a, out, rows, J, stream)
+                     : launch_rules<unsigned>(times, nullptr, type, a, out, rows, J, stream);
 }
 
 int launch_rule_times_backward(const void* grad, const void* times, int type, const RuleArgs& a, void* dtimes, int64_t rows, int64_t J,
                                hipStream_t stream) {
-    return launch_rules<true>(grad, times, type, a, dtimes, rows, J, stream);
+    return launch_rules<void>(grad, times, type, a, dtimes, rows, J, stream);
 }
 
 int launch_choose(const void* times, int type, const RuleArgs& a, const ChooseArgs& c, int64_t rows, int64_t J, void* ws, hipStream_t stream) {
+    Part* parts = static_cast<Part*>(ws);
     return with_type(type, [&](auto e) -> int {
         using E = decltype(e);
-        constexpr int VEC = 16 / sizeof(E);
-        if (J <= 64 * VEC) return launch_choose_slices<E, 64, 1>(times, a, c, rows, J, ws, stream);
-        return launch_choose_slices<E, 256, 32 / VEC>(times, a, c, rows, J, ws, stream);
+        constexpr int VEC = 16 / sizeof(E), R = 32 / VEC;
+        if (!narrow(a)) {
+            if (J <= 256 * 16) return launch_choose_whole<E, 256, R / 2, unsigned>(times, a, c, rows, J, stream);
+            return launch_choose_slices<E, 256, R / 2, unsigned>(times, a, c, rows, J, parts, stream);
+        }
+        using C = unsigned short;
+        if (J <= 64 * VEC) return launch_choose_whole<E, 64, 1, C>(times, a, c, rows, J, stream);
+        if (J <= 64 * 32) return launch_choose_whole<E, 64, R, C>(times, a, c, rows, J, stream);
+        if (J <= 256 * 32) return launch_choose_whole<E, 256, R, C>(times, a, c, rows, J, stream);
+        // one launch, or slices that overlap better where there are many: 1 row of 32000 float32 times 13 and 20 us, 256 rows of bf16 ones
+        // 16 and 24, 512 of float32 ones 31 and 40, 4096 of bf16 ones 118 and 106
+        if (J <= 1024 * 32 && rows < 2048) return launch_choose_whole<E, 1024, R, C>(times, a, c, rows, J, stream);
+        if (J <= 1024 * 32) return launch_choose_slices<E, 512, R, C>(times, a, c, rows, J, parts, stream);
+        return launch_choose_slices<E, 256, R, C>(times, a, c, rows, J, parts, stream);
     });
 }
 

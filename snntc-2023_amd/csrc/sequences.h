@@ -5,6 +5,7 @@
 #include "snntc_common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace snntc {
 
@@ -96,7 +97,6 @@ struct RuleArgs {
     const float* delay;
     const unsigned* allowed;
     int64_t delay_stride, allowed_stride;
-    int most;                              // elements of a slice whose occurrences are counted; set by the launch
 };
 struct ChooseArgs {
     const float* uniform;
