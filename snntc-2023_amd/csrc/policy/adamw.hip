@@ -58,20 +58,30 @@ __device__ __forceinline__ unsigned mix(unsigned x) {
 __device__ __forceinline__ unsigned key_of(const AdamScalars& s, unsigned step, unsigned tensor) {
     return mix(s.seed_low + mix(s.seed_high + mix(step + mix(tensor))));
 }
-__device__ __forceinline__ unsigned noise(unsigned key, unsigned element) { return mix(element * 0x9E3779B9u ^ key); }
+constexpr unsigned kElement = 0x9E3779B9u;
+// place: the element's number times kElement.
+__device__ __forceinline__ unsigned noise(unsigned key, unsigned place) { return mix(place ^ key); }
+__device__ __forceinline__ unsigned third_noise(unsigned bits) { return bits * kElement >> 16; }
 
-// A code's integer as a double, from the bits of one: 8 <= code: exponent E + 2 and three digits.
-__device__ __forceinline__ double code_value(unsigned code) {
-    const bool low = code < 8;
-    const double d = __hiloint2double((int)((code + (low ? 8208u : 8200u)) << 17), 0);
-    return d - (low ? 8.0 : 0.0);
-}
-// The code of y >= 0 (in units), raised by (bits + 1/2) / 65536 of a step and cut off.
+// Codes are the upper bits of numbers that begin to lose digits at 8: a code's bits below the sign of a float32 are value(code) 2^-129, codes
+// below 8 being such that have fewer digits; and the upper word of y 2^-1025 as a double holds, from its 17th bit on, the code
+// at or below y.
+__device__ __forceinline__ double first_value(unsigned code) { return (double)__uint_as_float((code & 127u) << 20 | (code & 128u) << 24); }
+__device__ __forceinline__ double second_value(unsigned code) { return (double)__uint_as_float(code << 20); }
+constexpr double kFirstUnit = 0x1p129 / kTopFirst, kSecondUnit = 0x1p129 / kTopSecond;        // of a scale
+// The code of y >= 0 (value(largest) for the largest magnitude), raised by (bits + 1/2) / 65536 of a step and cut off.
 __device__ __forceinline__ unsigned code_of(double y, unsigned bits, unsigned most) {
-    const bool low = y < 8.0;
-    const unsigned hi = (unsigned)__double2hiint(low ? y + 8.0 : y) + (bits << 1 | 1u);
-    const unsigned c = (hi >> 17) - (low ? 8208u : 8200u);
+    const unsigned c = ((unsigned)__double2hiint(ldexp(y, -1025)) + (bits << 1 | 1u)) >> 17;
     return c < most ? c : most;
+}
+// top / s for a scale s, 0 for a scale that is none: the hardware's reciprocal of 64 bits made exact by two steps (no such number is near
+// the ends of the doubles).
+__device__ __forceinline__ double per_scale(double top, float s) {
+    const double d = (double)s;
+    double r = __builtin_amdgcn_rcp(d);
+    r = fma(fma(-d, r, 1.0), r, r);
+    r = fma(fma(-d, r, 1.0), r, r);
+    return s > 0.0f && s < INFINITY ? top * r : 0.0;
 }
 
 // float32 to a weight's type; 16-bit types to one of the two neighbours, the upper one if the place between them in 65536ths exceeds `bits`.
@@ -142,8 +152,15 @@ constexpr int kEach = 4;                                       // elements of a 
 constexpr int kTimes = 2;
 constexpr int kChunk = kThreads * kEach * kTimes;
 
+// The hardware's root, off by a step; it takes no number below 2^-126, which a power of four brings up.
+__device__ __forceinline__ float root(float x) {
+    const bool small = x < 0x1p-96f;
+    const float r = __builtin_amdgcn_sqrtf(small ? x * 0x1p96f : x);
+    return small ? r * 0x1p-48f : r;
+}
+// A weight after the step.  Root and reciprocal are the hardware's, two steps of a change that is a small part of the weight.
 __device__ __forceinline__ float stepped(float w, float m, float v, float keep, float rate, float second, float eps) {
-    return fmaf(-rate, m / (sqrtf(v * second) + eps), w * keep);
+    return fmaf(-rate * m, __builtin_amdgcn_rcpf(root(v * second) + eps), w * keep);
 }
 
 // States in float32.  Bound by memory.
@@ -182,18 +199,30 @@ adamw_kernel(AdamTable tab, AdamScalars s) {
             const float d = (float)G[i].v[k] * share;
             M[i].v[k] = fmaf(b1, M[i].v[k], new1 * d);
             V[i].v[k] = fmaf(b2, V[i].v[k], new2 * d * d);
-            const unsigned bits = sizeof(E) == 2 ? noise(key, (unsigned)(e + k)) * 0x9E3779B9u >> 16 : 0;
+            const unsigned bits = sizeof(E) == 2 ? third_noise(noise(key, (unsigned)e * kElement + k * kElement)) : 0;
             round_weight(stepped((float)W[i].v[k], M[i].v[k], V[i].v[k], keep, rate, second, eps), bits, &W[i].v[k]);
         }
         store4(w + e, W[i], left); store4(m + e, M[i], left); store4(v + e, V[i], left);
     }
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int d = kWave / 2; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, kWave));
-    return v;
+// The largest of all lanes' numbers, in the registers' own network (lanes 15 and 31 hand on what their rows have).
+template <int CTRL, int MASK>
+__device__ __forceinline__ unsigned larger(unsigned v) {
+    return max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, MASK, 0xF, false));
 }
+__device__ __forceinline__ unsigned wave_max(unsigned v) {
+    v = larger<0xB1, 0xF>(v);
+    v = larger<0x4E, 0xF>(v);
+    v = larger<0x141, 0xF>(v);
+    v = larger<0x140, 0xF>(v);
+    v = larger<0x142, 0xA>(v);
+    v = larger<0x143, 0xC>(v);
+    return (unsigned)__builtin_amdgcn_readlane((int)v, kWave - 1);
+}
+// A magnitude's bits: ordered as magnitudes are, NaN above all.
+__device__ __forceinline__ unsigned magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
 // States in 8 bits: a wavefront owns kTimes blocks of 256 elements.
 template <typename E>
 __global__ void __launch_bounds__(kThreads)
@@ -228,35 +257,31 @@ adamw8_kernel(AdamTable tab, AdamScalars s) {
         const long long e = (b0 + i) * kBlock + lane * 4;
         const int left = (int)max(min(n - e, 4ll), 0ll);
         if ((b0 + i) * kBlock >= n) continue;
-        const double old1 = s.b1 * ((double)m_scale[i] / kTopFirst), old2 = s.b2 * ((double)v_scale[i] / kTopSecond);
+        const double old1 = s.b1 * kFirstUnit * (double)m_scale[i], old2 = s.b2 * kSecondUnit * (double)v_scale[i];
+        const unsigned place = (unsigned)e * kElement;
         double a[4], q[4];
-        float top1 = 0.0f, top2 = 0.0f;
-        bool bad = false;
+        unsigned top1 = 0, top2 = 0, bits[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const double d = (double)(float)G[i].v[k];
-            const double c = code_value(M[i].v[k] & 127u);
-            a[k] = fma(new1, d, old1 * (M[i].v[k] & 128u ? -c : c));
-            q[k] = fma(new2 * d, d, old2 * code_value(V[i].v[k]));
+            a[k] = fma(new1, d, old1 * first_value(M[i].v[k]));
+            q[k] = fma(new2 * d, d, old2 * second_value(V[i].v[k]));
             const float fa = (float)a[k], fq = (float)q[k];
-            top1 = fmaxf(top1, fabsf(fa)); top2 = fmaxf(top2, fq);
-            bad |= isnan(fa) || isnan(fq);
-            const unsigned bits = sizeof(E) == 2 ? noise(key, (unsigned)(e + k)) * 0x9E3779B9u >> 16 : 0;
-            round_weight(stepped((float)W[i].v[k], fa, fq, keep, rate, second, eps), bits, &W[i].v[k]);
+            top1 = max(top1, magnitude(fa)); top2 = max(top2, magnitude(fq));
+            bits[k] = noise(key, place + k * kElement);
+            round_weight(stepped((float)W[i].v[k], fa, fq, keep, rate, second, eps), sizeof(E) == 2 ? third_noise(bits[k]) : 0, &W[i].v[k]);
         }
         store4(w + e, W[i], left);
-        top1 = wave_max(top1); top2 = wave_max(top2);
-        if (__any(bad)) top1 = top2 = NAN;                    // (a maximum passes over them)
-        const double unit1 = top1 > 0.0f ? kTopFirst / (double)top1 : 0.0, unit2 = top2 > 0.0f ? kTopSecond / (double)top2 : 0.0;
+        const float scale1 = __uint_as_float(wave_max(top1)), scale2 = __uint_as_float(wave_max(top2));
+        const double unit1 = per_scale(kTopFirst, scale1), unit2 = per_scale(kTopSecond, scale2);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const unsigned bits = noise(key, (unsigned)(e + k));
-            const unsigned c = code_of(fabs(a[k]) * unit1, bits & 0xFFFFu, 127u);
-            M[i].v[k] = (unsigned char)(a[k] < 0.0 ? c | 128u : c);
-            V[i].v[k] = (unsigned char)code_of(q[k] * unit2, bits >> 16, 255u);
+            const unsigned c = code_of(fabs(a[k]) * unit1, bits[k] & 0xFFFFu, 127u);
+            M[i].v[k] = (unsigned char)(c | ((unsigned)__double2hiint(a[k]) >> 24 & 128u));
+            V[i].v[k] = (unsigned char)code_of(q[k] * unit2, bits[k] >> 16, 255u);
         }
         store4(m + e, M[i], left); store4(v + e, V[i], left);
-        if (lane == 0) { ms[b0 + i] = top1; vs[b0 + i] = top2; }
+        if (lane == 0) { ms[b0 + i] = scale1; vs[b0 + i] = scale2; }
     }
 }
 
@@ -289,13 +314,12 @@ moments_kernel(MomentTable tab) {
         const int left = (int)min(n - e, 4ll);
         if (left <= 0) continue;
         const Four<unsigned char> M = load4(tab.m[t] + e, left), V = load4(tab.v[t] + e, left);
-        const double u1 = (double)tab.m_scale[t][e / kBlock] / kTopFirst, u2 = (double)tab.v_scale[t][e / kBlock] / kTopSecond;
+        const double u1 = kFirstUnit * (double)tab.m_scale[t][e / kBlock], u2 = kSecondUnit * (double)tab.v_scale[t][e / kBlock];
         Four<float> a, q;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const double c = code_value(M.v[k] & 127u) * u1;
-            a.v[k] = (float)(M.v[k] & 128u ? -c : c);
-            q.v[k] = (float)(code_value(V.v[k]) * u2);
+            a.v[k] = (float)(first_value(M.v[k]) * u1);
+            q.v[k] = (float)(second_value(V.v[k]) * u2);
         }
         store4(tab.first[t] + e, a, left); store4(tab.second[t] + e, q, left);
     }
@@ -331,17 +355,27 @@ __device__ __forceinline__ double block_sum(double v) {
 }
 
 // Squares in 64 bits: of 10^8 gradients neither the largest overflow nor the smallest vanish, and the sum's order does not show.
+// Eight pieces of four elements are requested together.
+constexpr int kPieces = 8;
 template <typename E>
 __device__ __forceinline__ double squares(const E* __restrict__ g, long long from, long long to) {
     double sum[4] = {0.0, 0.0, 0.0, 0.0};
-    for (long long e = from + threadIdx.x * 4; e < to; e += kThreads * 4) {
-        const Four<E> x = load4(g + e, (int)min(to - e, 4ll));
+    const auto add = [&](const Four<E>& x) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const double d = (double)(float)x.v[k];
             sum[k] = fma(d, d, sum[k]);
         }
+    };
+    long long e = from + threadIdx.x * 4;
+    for (; from + kPieces * kThreads * 4 <= to; from += kPieces * kThreads * 4, e += kPieces * kThreads * 4) {
+        Four<E> x[kPieces];
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) x[i] = load4(g + e + i * kThreads * 4, 4);
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) add(x[i]);
     }
+    for (; e < to; e += kThreads * 4) add(load4(g + e, (int)min(to - e, 4ll)));
     return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 __global__ void __launch_bounds__(kThreads)
@@ -366,7 +400,7 @@ grad_norm_kernel(const double* __restrict__ partial, float* __restrict__ norm, i
 // Workgroups of one launch: 2^32 threads are too many.
 constexpr int64_t kMostBlocks = (1 << 24) - 1;
 
-int64_t norm_chunk(int64_t total) { return 4096 * std::max<int64_t>(1, total / (4096ll * 8192)); }
+int64_t norm_chunk(int64_t total) { return 8192 * std::max<int64_t>(1, total / (8192ll * 4096)); }
 
 }  // namespace
 

@@ -319,11 +319,24 @@ rule_kernel(const E* __restrict__ in, const E* __restrict__ times, E* __restrict
 // it is asked for).
 struct Part { float s, m; int arg, unused; };
 
-// v of the lane that CTRL names, `none` where MASK leaves a row of 16 out.
+// v of the lane that CTRL names; `none` where there is no such lane, or MASK leaves a row of 16 out.
 template <int CTRL, int MASK, typename T>
 __device__ __forceinline__ T from_lane(T none, T v) {
-    static_assert(sizeof(T) == 4, "one register");
-    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v), CTRL, MASK, 0xF, false));
+    struct Halves { int h[sizeof(T) / 4]; };
+    const Halves n = __builtin_bit_cast(Halves, none);
+    Halves x = __builtin_bit_cast(Halves, v);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 4); ++i) x.h[i] = __builtin_amdgcn_update_dpp(n.h[i], x.h[i], CTRL, MASK, 0xF, false);
+    return __builtin_bit_cast(T, x);
+}
+// A lane's value for all; the lane is the same for all.
+template <typename T>
+__device__ __forceinline__ T of_lane(T v, int lane) {
+    struct Halves { int h[sizeof(T) / 4]; };
+    Halves x = __builtin_bit_cast(Halves, v);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 4); ++i) x.h[i] = __builtin_amdgcn_readlane(x.h[i], lane);
+    return __builtin_bit_cast(T, x);
 }
 // All of a wavefront's values joined, in the registers' own network: pairs, quads, eights and sixteens by exchange, then lane 15 of a row to
 // the next one and lane 31 to the upper half; the last lane has them all.
@@ -335,14 +348,21 @@ __device__ __forceinline__ T wave_join(T v, T none, F&& f) {
     v = f(v, from_lane<0x140, 0xF>(v, v));
     v = f(v, from_lane<0x142, 0xA>(none, v));
     v = f(v, from_lane<0x143, 0xC>(none, v));
-    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), kWave - 1));
+    return of_lane(v, kWave - 1);
 }
 __device__ __forceinline__ float wave_max(float v) { return wave_join(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); }); }
-__device__ __forceinline__ float wave_sum(float v) { return wave_join(v, 0.0f, [](float a, float b) { return a + b; }); }
+template <typename T>
+__device__ __forceinline__ T wave_sum(T v) { return wave_join(v, (T)0, [](T a, T b) { return a + b; }); }
 __device__ __forceinline__ int wave_min(int v) { return wave_join(v, INT32_MAX, [](int a, int b) { return min(a, b); }); }
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int d = kWave / 2; d > 0; d >>= 1) v += __shfl_xor(v, d, kWave);
+// The sum of the lanes up to and with each.
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {
+    v += from_lane<0x111, 0xF>((T)0, v);
+    v += from_lane<0x112, 0xF>((T)0, v);
+    v += from_lane<0x114, 0xF>((T)0, v);
+    v += from_lane<0x118, 0xF>((T)0, v);
+    v += from_lane<0x142, 0xA>((T)0, v);
+    v += from_lane<0x143, 0xC>((T)0, v);
     return v;
 }
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.0f : m; }
@@ -352,19 +372,16 @@ __device__ __forceinline__ float term(float d, float k) { return __builtin_amdgc
 __device__ __forceinline__ double weight_of(const Part& p, float m, float k) { return (double)p.s * (double)term(p.m - base_of(m), k); }
 
 // A row's elements as a wavefront holds them: R pieces, WIDTH / 64 wavefronts one behind the other, so that each has a run of the slice.
-template <typename E, int VEC, int WIDTH, int R, typename COUNT>
+template <typename E, int VEC, int R>
 struct Run {
     static constexpr int kLength = kWave * VEC * R;
-    using M = Marks<WIDTH, VEC * R, COUNT>;
     Piece<E, VEC> t[R];                              // ruled times; +infinity: not allowed, or behind the row
     __device__ __forceinline__ static int in_run(int i) { return (i * kWave + (int)threadIdx.x % kWave) * VEC; }
     __device__ __forceinline__ static int local(int i) { return (int)threadIdx.x / kWave * kLength + in_run(i); }
     __device__ __forceinline__ float v(int i, int e) const { return -(float)t[i].v[e]; }
-    __device__ __forceinline__ void load(const E* times, const RuleArgs& a, const RowRules& q, int64_t first, int J, typename M::Memory& lds) {
-        const int end = (int)min((int64_t)WIDTH * VEC * R, J - first);
-        M marks;
-        marks.request(a, q, J);
-        unsigned allowed[R];
+    unsigned allowed[R];
+    Extras<VEC> extras;
+    __device__ __forceinline__ void request(const E* times, const RowRules& q, int64_t first, int end) {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             if (local(i) < end) {
@@ -375,9 +392,11 @@ struct Run {
             }
             allowed[i] = request_allowed(q, first + local(i), end - local(i));
         }
-        Extras<VEC> extras;
         request_delay(extras, q, first + local(0), end - local(0));
-        const bool from_history = marks.build(lds, q, first, J, times);
+    }
+    // M: the marks of the slice
+    template <typename M>
+    __device__ __forceinline__ void rule(const typename M::Memory& lds, bool from_history, const RowRules& q, int64_t first, int end) {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             Extras<VEC> next;
@@ -420,20 +439,13 @@ struct Run {
     // a run without any.
     __device__ __forceinline__ int pick(double rest, float m, float k, float* value) {
         const float base = base_of(m);
-        const int lane = threadIdx.x % kWave;
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             forget(t[i]);
             float e[VEC], sum = 0.0f;
 #pragma unroll
             for (int x = 0; x < VEC; ++x) sum += e[x] = term(v(i, x) - base, k);
-            float run = sum;
-#pragma unroll
-            for (int d = 1; d < kWave; d <<= 1) {
-                const float other = __shfl_up(run, d, kWave);
-                if (lane >= d) run += other;
-            }
-            const float all = __shfl(run, kWave - 1, kWave);
+            const float run = wave_scan(sum), all = of_lane(run, kWave - 1);
             if (!((double)all > rest)) { rest -= all; continue; }
             const unsigned long long over = __ballot((double)run > rest);
             const int owner = __ffsll(over) - 1;
@@ -448,8 +460,8 @@ struct Run {
             float mine = v(i, 0);
 #pragma unroll
             for (int x = 1; x < VEC; ++x) mine = at == x ? v(i, x) : mine;
-            *value = __shfl(mine, owner, kWave);
-            return __shfl(in_run(i) + at, owner, kWave);
+            *value = of_lane(mine, owner);
+            return of_lane(in_run(i) + at, owner);
         }
 #pragma unroll
         for (int i = R - 1; i >= 0; --i) {
@@ -462,15 +474,15 @@ struct Run {
             const unsigned long long any = __ballot(last >= 0);
             if (!any) continue;
             const int owner = 63 - __clzll(any);
-            *value = __shfl(mine, owner, kWave);
-            return __shfl(last, owner, kWave);
+            *value = of_lane(mine, owner);
+            return of_lane(last, owner);
         }
         return -1;
     }
 };
 
 struct Heat { float k; bool greedy, valid; double t; };
-__device__ __forceinline__ Heat heat_of(const ChooseArgs& a, int64_t r) {
+__device__ __forceinline__ Heat heat_of(const ChooseArgs& a, unsigned r) {
     const float t = a.temperature ? a.temperature[r] : a.heat;
     Heat h;
     h.valid = t >= 0.0f && t < INFINITY;
@@ -481,55 +493,52 @@ __device__ __forceinline__ Heat heat_of(const ChooseArgs& a, int64_t r) {
 }
 
 // A row's n parts joined by a wavefront, and the part that the row's token lies in: part -1: there is none.
-struct Found { int part; double rest, total; float m; };
-template <typename P>
-__device__ __forceinline__ Found find_part(P&& parts, int n, const Heat& h, const float* uniform, int64_t r) {
+struct Found { int part; double rest, total; float m; Part at; };
+__device__ __forceinline__ Found find_part(const Part* parts, int n, const Heat& h, const float* uniform, unsigned r) {
     const int lane = threadIdx.x % kWave;
+    const Part none{0.0f, -INFINITY, 0, 0}, mine = lane < n ? parts[lane] : none;       // (mostly all there are)
+    const auto get = [&](int i0) { return i0 == 0 ? mine : i0 + lane < n ? parts[i0 + lane] : none; };
+    const float u = h.greedy || !h.valid ? 0.0f : uniform[r];
     float m = -INFINITY;
-    for (int i = lane; i < n; i += kWave) m = fmaxf(m, parts(i).m);
+    for (int i0 = 0; i0 < n; i0 += kWave) m = fmaxf(m, get(i0).m);
     m = wave_max(m);
     double total = 0.0;
     int best = INT32_MAX;
-    for (int i = lane; i < n; i += kWave) {
-        const Part p = parts(i);
+    for (int i0 = 0; i0 < n; i0 += kWave) {
+        const Part p = get(i0);
         total += weight_of(p, m, h.k);
-        if (p.m == m) best = min(best, i);
+        if (p.m == m) best = min(best, i0 + lane);
     }
     total = wave_sum(total);
-    Found f{-1, 0.0, total, m};
+    Found f{-1, 0.0, total, m, none};
     if (!(total > 0.0) || !h.valid) return f;                           // nothing possible, or no numbers
     if (h.greedy) {
         f.part = wave_min(best);
+        f.at = parts[f.part];
         return f;
     }
-    const float u = uniform[r];
     double rest = total * (double)(u > 0.0f ? u : 0.0f);
     int last = 0;
     for (int i0 = 0; i0 < n && f.part < 0; i0 += kWave) {
-        const double s = i0 + lane < n ? weight_of(parts(i0 + lane), m, h.k) : 0.0;
-        double run = s;
-#pragma unroll
-        for (int d = 1; d < kWave; d <<= 1) {
-            const double other = __shfl_up(run, d, kWave);
-            if (lane >= d) run += other;
-        }
+        const double s = weight_of(get(i0), m, h.k), run = wave_scan(s);
         const unsigned long long any = __ballot(s > 0.0), over = __ballot(run > rest && s > 0.0);
         if (any) last = i0 + 63 - __clzll(any);
         if (over) {
             const int owner = __ffsll(over) - 1;
             f.part = i0 + owner;
-            rest -= __shfl(run - s, owner, kWave);
+            rest -= of_lane(run - s, owner);
         } else {
-            rest -= __shfl(run, kWave - 1, kWave);
+            rest -= of_lane(run, kWave - 1);
         }
     }
     if (f.part < 0) { f.part = last; rest = INFINITY; }
+    f.at = parts[f.part];
     // (in units of the part's own sum, which the choice of the part keeps above 0)
-    f.rest = fmax(rest, 0.0) / (double)term(parts(f.part).m - base_of(m), h.k);
+    f.rest = fmax(rest, 0.0) / (double)term(f.at.m - base_of(m), h.k);
     return f;
 }
 
-__device__ __forceinline__ void store_choice(const ChooseArgs& a, int64_t r, const Heat& h, int64_t token, float value, const Found& f) {
+__device__ __forceinline__ void store_choice(const ChooseArgs& a, unsigned r, const Heat& h, int64_t token, float value, const Found& f) {
     a.tokens[r] = token;
     a.logp[r] = token < 0 ? NAN : (float)(((double)value - (double)f.m) / h.t - log(f.total));
 }
@@ -538,17 +547,25 @@ __device__ __forceinline__ void store_choice(const ChooseArgs& a, int64_t r, con
 template <typename E, int VEC, int WIDTH, int R, typename COUNT, bool WHOLE>
 __global__ void __launch_bounds__(WIDTH)
 choose_slice_kernel(const E* __restrict__ times, RuleArgs a, ChooseArgs c, Part* __restrict__ parts, int64_t rows, int J, int slices) {
-    using Mine = Run<E, VEC, WIDTH, R, COUNT>;
+    using M = Marks<WIDTH, VEC * R, COUNT>;
+    using Mine = Run<E, VEC, R>;
     constexpr int kWaves = WIDTH / kWave;
-    __shared__ typename Mine::M::Memory lds;
+    __shared__ typename M::Memory lds;
     __shared__ Part part[kWaves];
     const unsigned block = place(), r = WHOLE ? block : block / (unsigned)slices;
     if (r >= rows) return;
     const int slice = WHOLE ? 0 : block - r * (unsigned)slices, wave = threadIdx.x / kWave;
+    const int64_t first = (int64_t)slice * M::kSlice;
+    const int end = (int)min((int64_t)M::kSlice, J - first);
+    const E* __restrict__ row = times + (int64_t)r * J;
     const RowRules q = row_rules(a, r);
-    const Heat h = heat_of(c, r);
+    M marks;
+    marks.request(a, q, J);
     Mine run;
-    run.load(times + (int64_t)r * J, a, q, (int64_t)slice * (WIDTH * VEC * R), J, lds);
+    run.request(row, q, first, end);
+    const Heat h = heat_of(c, r);
+    const bool from_history = marks.build(lds, q, first, J, row);
+    run.template rule<M>(lds, from_history, q, first, end);
     const Part mine = run.part(h.k, h.greedy);
     if constexpr (!WHOLE) {
         if (threadIdx.x % kWave == 0) parts[((int64_t)r * slices + slice) * kWaves + wave] = mine;
@@ -556,7 +573,7 @@ choose_slice_kernel(const E* __restrict__ times, RuleArgs a, ChooseArgs c, Part*
     }
     if (threadIdx.x % kWave == 0) part[wave] = mine;
     __syncthreads();
-    const Found f = find_part([&](int i) { return part[i]; }, kWaves, h, c.uniform, r);
+    const Found f = find_part(part, kWaves, h, c.uniform, r);
     if (wave != (f.part < 0 ? 0 : f.part)) return;
     int at = -1;
     float value = 0.0f;
@@ -565,29 +582,38 @@ choose_slice_kernel(const E* __restrict__ times, RuleArgs a, ChooseArgs c, Part*
     if (threadIdx.x % kWave == 0) store_choice(c, r, h, at < 0 ? -1 : wave * Mine::kLength + at, value, f);
 }
 
-// A row's parts joined in order by a wavefront, which reads the run that the token lies in once more.
+// A row's parts joined in order, and the run that the token lies in read once more: by the first wavefront, while all go through
+// the history, which was requested before the run was known.
+constexpr int kJoinThreads = 256;
 template <typename E, int VEC, int R, typename COUNT>
-__global__ void __launch_bounds__(kWave)
-choose_join_kernel(const E* __restrict__ times, RuleArgs a, ChooseArgs c, const Part* __restrict__ parts, int J, int count) {
-    using Mine = Run<E, VEC, kWave, R, COUNT>;
-    __shared__ typename Mine::M::Memory lds;
-    const int64_t r = blockIdx.x;
+__global__ void __launch_bounds__(kJoinThreads)
+choose_join_kernel(const E* __restrict__ times, RuleArgs a, ChooseArgs c, const Part* __restrict__ parts, int64_t rows, int J, int count) {
+    using Mine = Run<E, VEC, R>;
+    using M = Marks<kJoinThreads, Mine::kLength / kJoinThreads, COUNT>;
+    __shared__ typename M::Memory lds;
+    const unsigned r = place();
+    if (r >= rows) return;
+    const RowRules q = row_rules(a, r);
     const Heat h = heat_of(c, r);
-    const Part* __restrict__ p = parts + r * count;
-    const Found f = find_part([&](int i) { return p[i]; }, count, h, c.uniform, r);
+    M marks;
+    if (!h.greedy) marks.request(a, q, J);
+    const Found f = find_part(parts + (int64_t)r * count, count, h, c.uniform, r);
+    const int64_t first = (int64_t)f.part * Mine::kLength;
     int64_t token = -1;
     float value = 0.0f;
-    if (f.part >= 0) {
-        const int64_t first = (int64_t)f.part * Mine::kLength;
-        if (h.greedy) {
-            token = first + p[f.part].arg;
-            value = p[f.part].m;
-        } else {
-            Mine run;
-            run.load(times + r * J, a, row_rules(a, r), first, J, lds);
-            const int at = run.pick(f.rest, p[f.part].m, h.k, &value);
-            token = at < 0 ? -1 : first + at;
-        }
+    if (f.part >= 0 && h.greedy) {
+        token = first + f.at.arg;
+        value = f.at.m;
+    } else if (f.part >= 0) {
+        const E* __restrict__ row = times + (int64_t)r * J;
+        const int end = (int)min((int64_t)Mine::kLength, J - first);
+        Mine run;
+        if (threadIdx.x < kWave) run.request(row, q, first, end);
+        const bool from_history = marks.build(lds, q, first, J, row);
+        if (threadIdx.x >= kWave) return;
+        run.template rule<M>(lds, from_history, q, first, end);
+        const int at = run.pick(f.rest, f.at.m, h.k, &value);
+        token = at < 0 ? -1 : first + at;
     }
     if (threadIdx.x == 0) store_choice(c, r, h, token, value, f);
 }
@@ -645,8 +671,8 @@ int launch_choose_slices(const void* times, const RuleArgs& a, const ChooseArgs&
     }
     {
         KernelTimerScope timer_("choose_join", stream);
-        hipLaunchKernelGGL((choose_join_kernel<E, VEC, R, COUNT>), dim3((unsigned)rows), dim3(kWave), 0, stream, static_cast<const E*>(times), a, c,
-                           parts, (int)J, slices * kWaves);
+        hipLaunchKernelGGL((choose_join_kernel<E, VEC, R, COUNT>), wide_grid(rows, kJoinThreads), dim3(kJoinThreads), 0, stream,
+                           static_cast<const E*>(times), a, c, parts, rows, (int)J, slices * kWaves);
     }
     SNNTC_HIP_CHECK(hipGetLastError());
     return SNNTC_OK;
