@@ -10,6 +10,7 @@
 // The arithmetic of a ruled time is float32 without contraction: products and sums round one by one, as written above.  A
 // token is drawn from the times as rule_times stores them, rounded to times' type, so that its log-probability is that of the ruled times.
 #include "../sequences.h"
+#include "wave.h"
 
 namespace snntc {
 namespace {
@@ -23,13 +24,13 @@ typedef unsigned Words __attribute__((ext_vector_type(4)));
 typedef unsigned WordsAt2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef unsigned WordsAt4 __attribute__((ext_vector_type(4), aligned(4)));
 template <typename E>
-struct __attribute__((packed, aligned(sizeof(E)))) Place { Words w; };
+using Place = typename std::conditional<sizeof(E) == 2, WordsAt2, WordsAt4>::type;
 template <typename E, int VEC>
 __device__ __forceinline__ Piece<E, VEC> read_piece(const E* at) {
     constexpr int N = VEC * sizeof(E) / sizeof(Words);
     struct All { Words w[N]; } all;
 #pragma unroll
-    for (int i = 0; i < N; ++i) all.w[i] = reinterpret_cast<const Place<E>*>(at)[i].w;
+    for (int i = 0; i < N; ++i) all.w[i] = reinterpret_cast<const Place<E>*>(at)[i];
     return __builtin_bit_cast(Piece<E, VEC>, all);
 }
 
@@ -247,10 +248,8 @@ __device__ __forceinline__ Piece<E, VEC> load_piece(const E* t, int n, E fill) {
 template <bool STREAM, typename E, int VEC>
 __device__ __forceinline__ void store_piece(E* t, const Piece<E, VEC>& p, int n) {
     if (n == VEC) {
-        if constexpr (STREAM)
-            __builtin_nontemporal_store(__builtin_bit_cast(Words, p), reinterpret_cast<typename std::conditional<sizeof(E) == 2, WordsAt2, WordsAt4>::type*>(t));
-        else
-            reinterpret_cast<Place<E>*>(t)->w = __builtin_bit_cast(Words, p);
+        if constexpr (STREAM) __builtin_nontemporal_store(__builtin_bit_cast(Words, p), reinterpret_cast<Place<E>*>(t));
+        else *reinterpret_cast<Place<E>*>(t) = __builtin_bit_cast(Words, p);
         return;
     }
 #pragma unroll
@@ -319,52 +318,8 @@ rule_kernel(const E* __restrict__ in, const E* __restrict__ times, E* __restrict
 // it is asked for).
 struct Part { float s, m; int arg, unused; };
 
-// v of the lane that CTRL names; `none` where there is no such lane, or MASK leaves a row of 16 out.
-template <int CTRL, int MASK, typename T>
-__device__ __forceinline__ T from_lane(T none, T v) {
-    struct Halves { int h[sizeof(T) / 4]; };
-    const Halves n = __builtin_bit_cast(Halves, none);
-    Halves x = __builtin_bit_cast(Halves, v);
-#pragma unroll
-    for (int i = 0; i < (int)(sizeof(T) / 4); ++i) x.h[i] = __builtin_amdgcn_update_dpp(n.h[i], x.h[i], CTRL, MASK, 0xF, false);
-    return __builtin_bit_cast(T, x);
-}
-// A lane's value for all; the lane is the same for all.
-template <typename T>
-__device__ __forceinline__ T of_lane(T v, int lane) {
-    struct Halves { int h[sizeof(T) / 4]; };
-    Halves x = __builtin_bit_cast(Halves, v);
-#pragma unroll
-    for (int i = 0; i < (int)(sizeof(T) / 4); ++i) x.h[i] = __builtin_amdgcn_readlane(x.h[i], lane);
-    return __builtin_bit_cast(T, x);
-}
-// All of a wavefront's values joined, in the registers' own network: pairs, quads, eights and sixteens by exchange, then lane 15 of a row to
-// the next one and lane 31 to the upper half; the last lane has them all.
-template <typename T, typename F>
-__device__ __forceinline__ T wave_join(T v, T none, F&& f) {
-    v = f(v, from_lane<0xB1, 0xF>(v, v));
-    v = f(v, from_lane<0x4E, 0xF>(v, v));
-    v = f(v, from_lane<0x141, 0xF>(v, v));
-    v = f(v, from_lane<0x140, 0xF>(v, v));
-    v = f(v, from_lane<0x142, 0xA>(none, v));
-    v = f(v, from_lane<0x143, 0xC>(none, v));
-    return of_lane(v, kWave - 1);
-}
 __device__ __forceinline__ float wave_max(float v) { return wave_join(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); }); }
-template <typename T>
-__device__ __forceinline__ T wave_sum(T v) { return wave_join(v, (T)0, [](T a, T b) { return a + b; }); }
 __device__ __forceinline__ int wave_min(int v) { return wave_join(v, INT32_MAX, [](int a, int b) { return min(a, b); }); }
-// The sum of the lanes up to and with each.
-template <typename T>
-__device__ __forceinline__ T wave_scan(T v) {
-    v += from_lane<0x111, 0xF>((T)0, v);
-    v += from_lane<0x112, 0xF>((T)0, v);
-    v += from_lane<0x114, 0xF>((T)0, v);
-    v += from_lane<0x118, 0xF>((T)0, v);
-    v += from_lane<0x142, 0xA>((T)0, v);
-    v += from_lane<0x143, 0xC>((T)0, v);
-    return v;
-}
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.0f : m; }
 // exp(d / T), k = log2(e) / T, of a difference from a maximum: what the argument's rounding loses is its own size in half steps, of a
 // term that shrinks faster than that grows, and equal times have terms of exactly 1.

@@ -462,3 +462,49 @@ def test_optimizer_in_a_captured_step(bits):
     with pytest.raises(RuntimeError, match="capturable"):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             uncounted.step()
+
+
+def test_moments_are_tensors_of_their_own():
+    import snntc_amd as snn
+    m, v, ms, vs = _coded(5, SIZES)
+    first, second = snn.adamw_moments(m, v, ms, vs)
+    kept = [x.clone() for x in first + second]
+    assert all(x.shape == y.shape and x.is_contiguous() for x, y in zip(first + second, m + v))
+    first[5].fill_(7.0)
+    first[5].requires_grad_()
+    (first[5] * 2).sum().backward()
+    assert bool((first[5].grad == 2).all()) and not first[4].requires_grad
+    for x, y in zip(first[:5] + first[6:] + second, kept[:5] + kept[6:]):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("coded", [False, True])
+def test_calls_larger_than_the_caches(coded):
+    """The form that goes past the caches, against the other one on parts of the same tensors."""
+    import snntc_amd as snn
+    n = (1 << 24) + 1234                                      # 28 or 16 bytes an element: above 2^28 bytes in all
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    r = lambda: torch.randn(n, generator=gen, device=DEV)                             # noqa: E731
+    w, g = r(), r()
+    if coded:
+        states = [torch.randint(0, 256, (n,), generator=gen, device=DEV).to(torch.uint8) for _ in range(2)]
+        states += [torch.rand(-(-n // 256), generator=gen, device=DEV) for _ in range(2)]
+    else:
+        states = [r(), r().square()]
+    before = [x.clone() for x in (w, *states)]
+    more = lambda s: dict(first_scale=[s[2]], second_scale=[s[3]]) if coded else {}   # noqa: E731
+    snn.adamw_update([w], [g], [states[0]], [states[1]], 3, seed=1, **more(states))
+    size = 1 << 20                                            # a multiple of 256; the first part has the same places of its elements
+    part = [x[:size].clone() if i < 3 else x[:size // 256].clone() for i, x in enumerate(before)]
+    snn.adamw_update([part[0]], [g[:size].clone()], [part[1]], [part[2]], 3, seed=1, **more(part[1:]))
+    assert torch.equal(w[:size], part[0])
+    for x, y in zip(states, part[1:]):
+        assert torch.equal(x[:y.numel()], y)
+    if coded:
+        first, _ = snn.adamw_moments([states[0]] * 2, [states[1]] * 2, [states[2]] * 2, [states[3]] * 2)
+        assert torch.equal(first[0], first[1])
+        assert torch.equal(first[0][:size], snn.adamw_moments([part[1]], [part[2]], [part[3]], [part[4]])[0][0])
+    # the rest, by the formula in 64 bits
+    if not coded:
+        m = 0.9 * before[1].double() + 0.1 * g.double()
+        assert bool(((states[0] - m).abs() <= 5 * HALF * (before[1].abs() + g.abs())).all())
