@@ -27,11 +27,36 @@ template <typename E>
 using Place = typename std::conditional<sizeof(E) == 2, WordsAt2, WordsAt4>::type;
 template <typename E, int VEC>
 __device__ __forceinline__ Piece<E, VEC> read_piece(const E* at) {
-    constexpr int N = VEC * sizeof(E) / sizeof(Words);
+    if constexpr (VEC == 1) return Piece<E, 1>{{*at}};
+    constexpr int N = VEC * sizeof(E) / sizeof(Words) + (VEC == 1);
     struct All { Words w[N]; } all;
 #pragma unroll
     for (int i = 0; i < N; ++i) all.w[i] = reinterpret_cast<const Place<E>*>(at)[i];
-    return __builtin_bit_cast(Piece<E, VEC>, all);
+    if constexpr (VEC > 1) return __builtin_bit_cast(Piece<E, VEC>, all);
+}
+template <bool STREAM, typename E, int VEC>
+__device__ __forceinline__ void store_piece(E* at, const Piece<E, VEC>& p) {
+    if constexpr (VEC == 1) *at = p.v[0];
+    else if constexpr (STREAM) __builtin_nontemporal_store(__builtin_bit_cast(Words, p), reinterpret_cast<Place<E>*>(at));
+    else *reinterpret_cast<Place<E>*>(at) = __builtin_bit_cast(Words, p);
+}
+// VEC numbers rounded to E, two by one instruction.
+template <typename E, int VEC>
+__device__ __forceinline__ Piece<E, VEC> round_piece(const float (&t)[VEC]) {
+    Piece<E, VEC> p;
+    if constexpr (VEC == 1 || sizeof(E) == 4) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) p.v[v] = (E)t[v];
+    } else {
+        typedef float Pair __attribute__((ext_vector_type(2)));
+        typedef E Two __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int v = 0; v < VEC; v += 2) {
+            const Two two = __builtin_convertvector((Pair{t[v], t[v + 1]}), Two);
+            p.v[v] = two.x; p.v[v + 1] = two.y;
+        }
+    }
+    return p;
 }
 
 // A launch's workgroup among fewer than 2^32: 2^24 rows, and as many slices as their times' memory has place for.
@@ -67,55 +92,52 @@ __device__ __forceinline__ RowRules row_rules(const RuleArgs& a, unsigned r) {
 // The marks of a slice of WIDTH * PER elements in LDS: a bitmap and, for COUNT (16-bit or 32-bit integers), occurrences; only those of
 // marked elements are ever cleared or read.
 template <int SLICE, typename COUNT>
-struct MarkMemory { unsigned bits[SLICE / 32]; COUNT count[SLICE]; };
+struct MarkMemory { unsigned bits[SLICE / 32 + 1]; COUNT count[SLICE]; };
 // For the gradient: `late` marked elements have a time above 0.
 template <int SLICE>
-struct MarkMemory<SLICE, void> { unsigned bits[SLICE / 32], late[SLICE / 32]; };
+struct MarkMemory<SLICE, void> { unsigned bits[SLICE / 32 + 1], late[SLICE / 32 + 1]; };
 
 template <int WIDTH, int PER, typename COUNT>
 struct Marks {
     static constexpr int kSlice = WIDTH * PER, kWords = kSlice / 32, kHeld = 1024 / WIDTH < 2 ? 2 : 1024 / WIDTH > 8 ? 8 : 1024 / WIDTH;
     static constexpr bool kCounts = !std::is_void<COUNT>::value;
     using Memory = MarkMemory<kSlice, COUNT>;
-    int held[kHeld];                                 // the thread's first tokens; -1: none
+    long long held[kHeld];                           // the thread's first tokens, as they come: what is done with them waits for them
 
-    __device__ __forceinline__ static void batch(int (&to)[kHeld], const long long* tokens, int64_t from, int64_t end, int J) {
+    __device__ __forceinline__ static void batch(long long (&to)[kHeld], const long long* tokens, int64_t from, int64_t end) {
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
-            const int64_t at = from + i * WIDTH + (int)threadIdx.x;
-            const long long token = at < end ? tokens[at] : -1;
-            to[i] = (unsigned long long)token < (unsigned long long)J ? (int)token : -1;
-        }
+        for (int i = 0; i < kHeld; ++i) to[i] = tokens[min(from + i * WIDTH + (int)threadIdx.x, end - 1)];
     }
     // Before the row's numbers are known: the two do not wait for each other.
-    __device__ __forceinline__ void request(const RuleArgs& a, const RowRules& q, int J) {
-        if (a.history) batch(held, q.tokens, 0, a.L, J);
+    __device__ __forceinline__ void request(const RuleArgs& a, const RowRules& q) {
+        if (a.history) batch(held, q.tokens, 0, a.L);
     }
     // f(elements) of the tokens [from, seen), batch by batch: their places in the slice, -1 where they have none.
     template <typename F>
-    __device__ __forceinline__ void each(const RowRules& q, int from, int first, int end, int J, F&& f) const {
-        const auto use = [&](const int (&tok)[kHeld], int base) {
+    __device__ __forceinline__ void each(const RowRules& q, int from, int first, int end, F&& f) const {
+        const auto use = [&](const long long (&tok)[kHeld], int base) {
             int j[kHeld];
 #pragma unroll
             for (int i = 0; i < kHeld; ++i) {
                 const int at = base + i * WIDTH + (int)threadIdx.x;
-                j[i] = at >= from && at < q.seen && (unsigned)(tok[i] - first) < (unsigned)end ? tok[i] - first : -1;
+                const unsigned long long to = (unsigned long long)tok[i] - (unsigned)first;
+                j[i] = at >= from && at < q.seen && to < (unsigned)end ? (int)to : -1;
             }
             f(j);
         };
         use(held, 0);
         for (int base = kHeld * WIDTH; base < q.seen; base += kHeld * WIDTH) {
-            int tok[kHeld];
-            batch(tok, q.tokens, base, q.seen, J);
+            long long tok[kHeld];
+            batch(tok, q.tokens, base, q.seen);
             use(tok, base);
         }
     }
     // Returns whether there are any rules from the history; every thread of the workgroup calls it.  times: of the slice, for the signs.
     template <typename E>
-    __device__ __forceinline__ bool build(Memory& lds, const RowRules& q, int64_t first, int J, const E* times) const {
+    __device__ __forceinline__ bool build(Memory& lds, const RowRules& q, int64_t first, int end, const E* times) const {
         const bool counts = counted(q);
         if (q.seen == 0 || (q.rep == 1.0f && !counts)) return false;                   // (uniform)
-        const int end = (int)min((int64_t)kSlice, J - first), k = threadIdx.x;
+        const int k = threadIdx.x;
 #pragma unroll
         for (int w = 0; w < (kWords + WIDTH - 1) / WIDTH; ++w)
             if (w * WIDTH + k < kWords) {
@@ -123,7 +145,7 @@ struct Marks {
                 if constexpr (!kCounts) lds.late[w * WIDTH + k] = 0;
             }
         __syncthreads();
-        each(q, 0, (int)first, end, J, [&](const int (&j)[kHeld]) {
+        each(q, 0, (int)first, end, [&](const int (&j)[kHeld]) {
             float t[kHeld];
             if constexpr (!kCounts) {
 #pragma unroll
@@ -140,7 +162,7 @@ struct Marks {
         __syncthreads();
         if constexpr (kCounts) {
             if (!counts) return true;
-            each(q, q.prompt, (int)first, end, J, [&](const int (&j)[kHeld]) {
+            each(q, q.prompt, (int)first, end, [&](const int (&j)[kHeld]) {
 #pragma unroll
                 for (int i = 0; i < kHeld; ++i) {
                     if (j[i] < 0) continue;
@@ -155,8 +177,10 @@ struct Marks {
         }
         return true;
     }
-    __device__ __forceinline__ static unsigned marked(const Memory& lds, int j, int vec) { return lds.bits[j >> 5] >> (j & 31) & ((1u << vec) - 1); }
-    __device__ __forceinline__ static unsigned late(const Memory& lds, int j) { return lds.late[j >> 5] >> (j & 31); }
+    // Bits of the elements from j on, at any place in their words (there is a word behind the last one).
+    __device__ __forceinline__ static unsigned from(const unsigned* bits, int j) { return __builtin_amdgcn_alignbit(bits[(j >> 5) + 1], bits[j >> 5], j & 31); }
+    __device__ __forceinline__ static unsigned marked(const Memory& lds, int j, int vec) { return from(lds.bits, j) & ((1u << vec) - 1); }
+    __device__ __forceinline__ static unsigned late(const Memory& lds, int j) { return from(lds.late, j); }
     __device__ __forceinline__ static bool counted(const RowRules& q) {
         return kCounts && (q.pres != 0.0f || q.freq != 0.0f) && q.prompt < q.seen;
     }
@@ -185,30 +209,50 @@ __device__ __forceinline__ float where_bit(unsigned mask, int at, float t, float
 // Keeps the compiler from carrying a piece's elements in float32 from one use to the next, which takes half of the wavefronts' registers.
 template <typename P>
 __device__ __forceinline__ void forget(P& p) {
-    Words w = __builtin_bit_cast(Words, p);
-    asm volatile("" : "+v"(w));
-    p = __builtin_bit_cast(P, w);
-}
-
-// What a piece needs besides its times, requested before the history is gone through: the two do not wait for each other.
-template <int VEC>
-struct Extras { Piece<float, VEC> delay; unsigned allowed; };
-template <int VEC>
-__device__ __forceinline__ void request_delay(Extras<VEC>& x, const RowRules& q, int64_t j, int n) {
-    if (!q.delay || n <= 0) return;
-    if (n >= VEC) {
-        x.delay = read_piece<float, VEC>(q.delay + j);
-    } else {
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) x.delay.v[v] = v < n ? q.delay[j + v] : 0.0f;
+    if constexpr (sizeof(P) == sizeof(Words)) {
+        Words w = __builtin_bit_cast(Words, p);
+        asm volatile("" : "+v"(w));
+        p = __builtin_bit_cast(P, w);
     }
 }
-__device__ __forceinline__ unsigned request_allowed(const RowRules& q, int64_t j, int n) { return q.allowed && n > 0 ? q.allowed[j >> 5] >> (j & 31) : 0u; }
+
+// Loads return in order, and the compiler counts on how many are behind the one it waits for: only where none of them is in a branch.
+// So every lane loads whole pieces: behind the end of a slice its last VEC elements once more (a slice that would have fewer begins earlier),
+// and where a row has no delays or mask, these.
+__device__ const float kNoDelay[8] = {};
+__device__ const unsigned kAllAllowed[1] = {~0u};
+
+// (named as device memory: a choice between two pointers would be read as generic memory)
+template <typename T>
+using Device = const T __attribute__((address_space(1)))*;
+
+// A slice of a row: elements [first, first + end).
+struct Slice { int64_t first; int end; };
+template <int SLICE, int VEC>
+__device__ __forceinline__ Slice slice_of(unsigned slice, int J) {
+    const int64_t latest = J > VEC ? (J - VEC) & ~31 : 0;
+    Slice s;
+    s.first = min((int64_t)slice * SLICE, latest);
+    s.end = (int)min((int64_t)SLICE, J - s.first);
+    return s;
+}
+template <int VEC>
+__device__ __forceinline__ Piece<float, VEC> request_delay(const RowRules& q, int64_t j) {
+    const Device<float> d = q.delay ? (Device<float>)q.delay : (Device<float>)kNoDelay;
+    return read_piece<float, VEC>((const float*)(d + (q.delay ? j : 0)));
+}
+struct Allowed { unsigned low, high; };
+__device__ __forceinline__ Allowed request_allowed(const RowRules& q, int64_t j, int J) {
+    const Device<unsigned> w = q.allowed ? (Device<unsigned>)q.allowed : (Device<unsigned>)kAllAllowed;
+    const int at = q.allowed ? (int)(j >> 5) : 0, last = q.allowed ? (J - 1) >> 5 : 0;
+    return Allowed{w[at], w[min(at + 1, last)]};
+}
+__device__ __forceinline__ unsigned allowed_from(const Allowed& w, int64_t j) { return __builtin_amdgcn_alignbit(w.high, w.low, (unsigned)j & 31); }
 
 // The ruled times of one piece.  Marked elements are few: one at a time and lane, instead of a test for each.
 template <typename E, int VEC, typename M>
 __device__ __forceinline__ void rule_piece(Piece<E, VEC>& p, const typename M::Memory& lds, bool from_history, const RowRules& q,
-                                           const Extras<VEC>& x, int local) {
+                                           const Piece<float, VEC>& delay, unsigned allowed, int local) {
     unsigned m = from_history ? M::marked(lds, local, VEC) : 0;
     if (!m && !q.delay && !q.allowed) return;
     float t[VEC];
@@ -227,34 +271,13 @@ __device__ __forceinline__ void rule_piece(Piece<E, VEC>& p, const typename M::M
     }
     if (q.delay) {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) t[v] += x.delay.v[v];
+        for (int v = 0; v < VEC; ++v) t[v] += delay.v[v];
     }
     if (q.allowed) {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) t[v] = where_bit(x.allowed, v, t[v], INFINITY);
+        for (int v = 0; v < VEC; ++v) t[v] = where_bit(allowed, v, t[v], INFINITY);
     }
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) p.v[v] = (E)t[v];
-}
-
-template <typename E, int VEC>
-__device__ __forceinline__ Piece<E, VEC> load_piece(const E* t, int n, E fill) {
-    Piece<E, VEC> p;
-    if (n == VEC) return read_piece<E, VEC>(t);
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) p.v[v] = v < n ? t[v] : fill;
-    return p;
-}
-template <bool STREAM, typename E, int VEC>
-__device__ __forceinline__ void store_piece(E* t, const Piece<E, VEC>& p, int n) {
-    if (n == VEC) {
-        if constexpr (STREAM) __builtin_nontemporal_store(__builtin_bit_cast(Words, p), reinterpret_cast<Place<E>*>(t));
-        else *reinterpret_cast<Place<E>*>(t) = __builtin_bit_cast(Words, p);
-        return;
-    }
-#pragma unroll
-    for (int v = 0; v < VEC; ++v)
-        if (v < n) t[v] = p.v[v];
+    p = round_piece<E, VEC>(t);
 }
 
 // Ruled times, or (GRAD) the gradient by the times: in = times or the upstream gradient.  The gradient reads times where a token
@@ -267,31 +290,29 @@ rule_kernel(const E* __restrict__ in, const E* __restrict__ times, E* __restrict
     __shared__ typename M::Memory lds;
     const unsigned block = place(), r = block / (unsigned)slices;
     if (r >= rows) return;
-    const int64_t first = (int64_t)(block - r * (unsigned)slices) * M::kSlice, row = (int64_t)r * J;
-    const int end = (int)min((int64_t)M::kSlice, J - first);
-    const E* __restrict__ x = in + row + first;
-    E* __restrict__ y = out + row + first;
+    const Slice s = slice_of<M::kSlice, VEC>(block - r * (unsigned)slices, J);
+    const int64_t at = (int64_t)r * J + s.first;
     const RowRules q = row_rules(a, r);
     M marks;
-    marks.request(a, q, J);
-    const auto at = [&](int i) { return (i * WIDTH + (int)threadIdx.x) * VEC; };
+    marks.request(a, q);
+    const auto local = [&](int i) { return min((i * WIDTH + (int)threadIdx.x) * VEC, s.end - VEC); };
     Piece<E, VEC> held[R];
-    unsigned allowed[R];
+    Allowed allowed[R];
+    Piece<float, VEC> delay[2];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        if (at(i) < end) held[i] = load_piece<E, VEC>(x + at(i), min(VEC, end - at(i)), (E)0.0f);
-        allowed[i] = request_allowed(q, first + at(i), end - at(i));
+        held[i] = read_piece<E, VEC>(in + at + local(i));
+        allowed[i] = request_allowed(q, s.first + local(i), J);
     }
-    Extras<VEC> extras;
-    if constexpr (!GRAD) request_delay(extras, q, first + at(0), end - at(0));
-    const bool from_history = marks.build(lds, q, first, J, GRAD ? times + row + first : nullptr);
+    if constexpr (!GRAD) delay[0] = request_delay<VEC>(q, s.first + local(0));
+    const bool from_history = marks.build(lds, q, s.first, s.end, GRAD ? times + at : nullptr);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
+        if ((i * WIDTH + ((int)threadIdx.x & -kWave)) * VEC >= s.end) break;              // (a whole wavefront)
         if constexpr (GRAD) {
-            if (at(i) >= end) continue;
-            const unsigned m = from_history ? M::marked(lds, at(i), VEC) : 0;
+            const unsigned m = from_history ? M::marked(lds, local(i), VEC) : 0;
             if (m) {
-                const unsigned late = M::late(lds, at(i));
+                const unsigned late = M::late(lds, local(i));
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
                     const float t = (float)held[i].v[v] * where_bit(late, v, q.rep, q.inv);
@@ -299,18 +320,15 @@ rule_kernel(const E* __restrict__ in, const E* __restrict__ times, E* __restrict
                 }
             }
             if (q.allowed) {
+                const unsigned w = allowed_from(allowed[i], s.first + local(i));
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) held[i].v[v] = allowed[i] >> v & 1 ? held[i].v[v] : (E)0.0f;
+                for (int v = 0; v < VEC; ++v) held[i].v[v] = w >> v & 1 ? held[i].v[v] : (E)0.0f;
             }
         } else {
-            Extras<VEC> next;
-            if (i + 1 < R) request_delay(next, q, first + at(i + 1), end - at(i + 1));
-            if (at(i) >= end) continue;
-            extras.allowed = allowed[i];
-            rule_piece<E, VEC, M>(held[i], lds, from_history, q, extras, at(i));
-            extras = next;
+            if (i + 1 < R) delay[(i + 1) % 2] = request_delay<VEC>(q, s.first + local(i + 1));
+            rule_piece<E, VEC, M>(held[i], lds, from_history, q, delay[i % 2], allowed_from(allowed[i], s.first + local(i)), local(i));
         }
-        store_piece<STREAM, E, VEC>(y + at(i), held[i], min(VEC, end - at(i)));
+        store_piece<STREAM, E, VEC>(out + at + local(i), held[i]);
     }
 }
 
@@ -331,34 +349,35 @@ template <typename E, int VEC, int R>
 struct Run {
     static constexpr int kLength = kWave * VEC * R;
     Piece<E, VEC> t[R];                              // ruled times; +infinity: not allowed, or behind the row
-    __device__ __forceinline__ static int in_run(int i) { return (i * kWave + (int)threadIdx.x % kWave) * VEC; }
-    __device__ __forceinline__ static int local(int i) { return (int)threadIdx.x / kWave * kLength + in_run(i); }
+    Allowed allowed[R];
+    Piece<float, VEC> delay[2];
+    int end;                                         // of the slice
+    __device__ __forceinline__ int origin() const { return (int)threadIdx.x / kWave * kLength; }      // of the wavefront's run in the slice
+    __device__ __forceinline__ int proper(int i) const { return origin() + (i * kWave + (int)threadIdx.x % kWave) * VEC; }
+    __device__ __forceinline__ int local(int i) const { return min(proper(i), end - VEC); }
+    __device__ __forceinline__ int in_run(int i) const { return local(i) - origin(); }
     __device__ __forceinline__ float v(int i, int e) const { return -(float)t[i].v[e]; }
-    unsigned allowed[R];
-    Extras<VEC> extras;
-    __device__ __forceinline__ void request(const E* times, const RowRules& q, int64_t first, int end) {
+    __device__ __forceinline__ void request(const E* row, const RowRules& q, const Slice& s, int J) {
+        end = s.end;
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            if (local(i) < end) {
-                t[i] = load_piece<E, VEC>(times + first + local(i), min(VEC, end - local(i)), (E)INFINITY);
-            } else {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) t[i].v[e] = (E)INFINITY;
-            }
-            allowed[i] = request_allowed(q, first + local(i), end - local(i));
+            t[i] = read_piece<E, VEC>(row + s.first + local(i));
+            allowed[i] = request_allowed(q, s.first + local(i), J);
         }
-        request_delay(extras, q, first + local(0), end - local(0));
+        delay[0] = request_delay<VEC>(q, s.first + local(0));
     }
-    // M: the marks of the slice
+    // M: the marks of the slice.  own: elements of the slice before this one have been the last slice's.
     template <typename M>
-    __device__ __forceinline__ void rule(const typename M::Memory& lds, bool from_history, const RowRules& q, int64_t first, int end) {
+    __device__ __forceinline__ void rule(const typename M::Memory& lds, bool from_history, const RowRules& q, const Slice& s, int own) {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            Extras<VEC> next;
-            if (i + 1 < R) request_delay(next, q, first + local(i + 1), end - local(i + 1));
-            extras.allowed = allowed[i];
-            if (local(i) < end) rule_piece<E, VEC, M>(t[i], lds, from_history, q, extras, local(i));
-            extras = next;
+            if (i + 1 < R) delay[(i + 1) % 2] = request_delay<VEC>(q, s.first + local(i + 1));
+            rule_piece<E, VEC, M>(t[i], lds, from_history, q, delay[i % 2], allowed_from(allowed[i], s.first + local(i)), local(i));
+            const int skip = max(proper(i), own) - local(i);
+            if (skip > 0) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) t[i].v[e] = e < skip ? (E)INFINITY : t[i].v[e];
+            }
         }
     }
     __device__ __forceinline__ Part part(float k, bool greedy) {
@@ -509,38 +528,38 @@ choose_slice_kernel(const E* __restrict__ times, RuleArgs a, ChooseArgs c, Part*
     __shared__ Part part[kWaves];
     const unsigned block = place(), r = WHOLE ? block : block / (unsigned)slices;
     if (r >= rows) return;
-    const int slice = WHOLE ? 0 : block - r * (unsigned)slices, wave = threadIdx.x / kWave;
-    const int64_t first = (int64_t)slice * M::kSlice;
-    const int end = (int)min((int64_t)M::kSlice, J - first);
+    const unsigned slice = WHOLE ? 0 : block - r * (unsigned)slices, wave = threadIdx.x / kWave;
+    const Slice s = slice_of<M::kSlice, VEC>(slice, J);
     const E* __restrict__ row = times + (int64_t)r * J;
     const RowRules q = row_rules(a, r);
     M marks;
-    marks.request(a, q, J);
+    marks.request(a, q);
     Mine run;
-    run.request(row, q, first, end);
+    run.request(row, q, s, J);
     const Heat h = heat_of(c, r);
-    const bool from_history = marks.build(lds, q, first, J, row);
-    run.template rule<M>(lds, from_history, q, first, end);
+    const bool from_history = marks.build(lds, q, s.first, s.end, row);
+    run.template rule<M>(lds, from_history, q, s, (int)((int64_t)slice * M::kSlice - s.first));
     const Part mine = run.part(h.k, h.greedy);
     if constexpr (!WHOLE) {
-        if (threadIdx.x % kWave == 0) parts[((int64_t)r * slices + slice) * kWaves + wave] = mine;
+        // (an index from where the run has its place, wherever the slice begins)
+        if (threadIdx.x % kWave == 0)
+            parts[((int64_t)r * slices + slice) * kWaves + wave] = Part{mine.s, mine.m, mine.arg - (int)((int64_t)slice * M::kSlice - s.first), 0};
         return;
     }
     if (threadIdx.x % kWave == 0) part[wave] = mine;
     __syncthreads();
     const Found f = find_part(part, kWaves, h, c.uniform, r);
-    if (wave != (f.part < 0 ? 0 : f.part)) return;
+    if (wave != (f.part < 0 ? 0u : (unsigned)f.part)) return;
     int at = -1;
     float value = 0.0f;
     if (f.part >= 0 && h.greedy) { at = mine.arg; value = mine.m; }
     else if (f.part >= 0) at = run.pick(f.rest, mine.m, h.k, &value);
-    if (threadIdx.x % kWave == 0) store_choice(c, r, h, at < 0 ? -1 : wave * Mine::kLength + at, value, f);
+    if (threadIdx.x % kWave == 0) store_choice(c, r, h, at < 0 ? -1 : run.origin() + at, value, f);
 }
 
 // A row's parts joined in order, and the run that the token lies in read once more: by the first wavefront, while all go through
 // the history, which was requested before the run was known.
-constexpr int kJoinThreads = 256;
-template <typename E, int VEC, int R, typename COUNT>
+template <typename E, int VEC, int R, typename COUNT, int kJoinThreads>
 __global__ void __launch_bounds__(kJoinThreads)
 choose_join_kernel(const E* __restrict__ times, RuleArgs a, ChooseArgs c, const Part* __restrict__ parts, int64_t rows, int J, int count) {
     using Mine = Run<E, VEC, R>;
@@ -551,33 +570,33 @@ choose_join_kernel(const E* __restrict__ times, RuleArgs a, ChooseArgs c, const 
     const RowRules q = row_rules(a, r);
     const Heat h = heat_of(c, r);
     M marks;
-    if (!h.greedy) marks.request(a, q, J);
+    if (!h.greedy) marks.request(a, q);
     const Found f = find_part(parts + (int64_t)r * count, count, h, c.uniform, r);
-    const int64_t first = (int64_t)f.part * Mine::kLength;
+    const int64_t begin = (int64_t)f.part * Mine::kLength;
     int64_t token = -1;
     float value = 0.0f;
     if (f.part >= 0 && h.greedy) {
-        token = first + f.at.arg;
+        token = begin + f.at.arg;
         value = f.at.m;
     } else if (f.part >= 0) {
         const E* __restrict__ row = times + (int64_t)r * J;
-        const int end = (int)min((int64_t)Mine::kLength, J - first);
+        const Slice s = slice_of<Mine::kLength, VEC>(f.part, J);
         Mine run;
-        if (threadIdx.x < kWave) run.request(row, q, first, end);
-        const bool from_history = marks.build(lds, q, first, J, row);
+        if (threadIdx.x < kWave) run.request(row, q, s, J);
+        const bool from_history = marks.build(lds, q, s.first, s.end, row);
         if (threadIdx.x >= kWave) return;
-        run.template rule<M>(lds, from_history, q, first, end);
+        run.template rule<M>(lds, from_history, q, s, (int)(begin - s.first));
         const int at = run.pick(f.rest, f.at.m, h.k, &value);
-        token = at < 0 ? -1 : first + at;
+        token = at < 0 ? -1 : s.first + at;
     }
     if (threadIdx.x == 0) store_choice(c, r, h, token, value, f);
 }
 
 // ---- launches --------------------------------------------------------------------------------------------------------------------
 
-template <typename E, int WIDTH, int R, typename COUNT, bool STREAM>
+template <typename E, int WIDTH, int R, typename COUNT, bool STREAM, int VEC = 16 / sizeof(E)>
 int launch_rule_slices(const void* in, const void* times, void* out, const RuleArgs& a, int64_t rows, int64_t J, hipStream_t stream) {
-    constexpr int VEC = 16 / sizeof(E), kSlice = WIDTH * VEC * R;
+    constexpr int kSlice = WIDTH * VEC * R;
     const int slices = (int)((J + kSlice - 1) / kSlice);
     {
         KernelTimerScope timer_(std::is_void<COUNT>::value ? "rule_times_backward" : "rule_times", stream);
@@ -588,13 +607,16 @@ int launch_rule_slices(const void* in, const void* times, void* out, const RuleA
     return SNNTC_OK;
 }
 
-// Slices of 4096 elements, of 2048 and a wavefront each in rows of up to 8192 elements (rows of 5003 f16 times with their gradient, 2328 of
-// them: 38 and 33 us; of 32000 bf16 times, 4096 of them: 256 and 310 us).
+// Slices of 4096 elements, four wavefronts each, and of 2048 by one in rows of up to 8192 elements.  Rows with their gradient:
+//     slices                        2048, 1 wavefront   4096, 4   8192, 4   8192, 8
+//     2328 rows of 5003 f16 times         31.4 us         36.1
+//     4096 rows of 32000 bf16 times      233             220       224       220
 template <typename COUNT>
 int launch_rules(const void* in, const void* times, int type, const RuleArgs& a, void* out, int64_t rows, int64_t J, hipStream_t stream) {
     return with_type(type, [&](auto e) -> int {
         using E = decltype(e);
         constexpr int VEC = 16 / sizeof(E);
+        if (J < VEC) return launch_rule_slices<E, 64, 1, COUNT, false, 1>(in, times, out, a, rows, J, stream);
         if (J <= 64 * VEC) return launch_rule_slices<E, 64, 1, COUNT, false>(in, times, out, a, rows, J, stream);
         if (J <= 8192) return launch_rule_slices<E, 64, 32 / VEC, COUNT, false>(in, times, out, a, rows, J, stream);
         // (4096 rows of 32000 bf16 times without rules: 96 and 89 us)
@@ -603,9 +625,8 @@ int launch_rules(const void* in, const void* times, int type, const RuleArgs& a,
     });
 }
 
-template <typename E, int WIDTH, int R, typename COUNT>
+template <typename E, int WIDTH, int R, typename COUNT, int VEC = 16 / sizeof(E)>
 int launch_choose_whole(const void* times, const RuleArgs& a, const ChooseArgs& c, int64_t rows, int64_t J, hipStream_t stream) {
-    constexpr int VEC = 16 / sizeof(E);
     {
         KernelTimerScope timer_("choose", stream);
         hipLaunchKernelGGL((choose_slice_kernel<E, VEC, WIDTH, R, COUNT, true>), wide_grid(rows, WIDTH), dim3(WIDTH), 0, stream,
@@ -626,8 +647,12 @@ int launch_choose_slices(const void* times, const RuleArgs& a, const ChooseArgs&
     }
     {
         KernelTimerScope timer_("choose_join", stream);
-        hipLaunchKernelGGL((choose_join_kernel<E, VEC, R, COUNT>), wide_grid(rows, kJoinThreads), dim3(kJoinThreads), 0, stream,
-                           static_cast<const E*>(times), a, c, parts, rows, (int)J, slices * kWaves);
+        if (rows >= 256)                                               // (a call on 4096 rows of 32000: 91 us with a wavefront each, 96 with four; 64 of 131072, 2048 tokens: 23.6 and 21.0)
+            hipLaunchKernelGGL((choose_join_kernel<E, VEC, R, COUNT, 64>), wide_grid(rows, 64), dim3(64), 0, stream,
+                               static_cast<const E*>(times), a, c, parts, rows, (int)J, slices * kWaves);
+        else
+            hipLaunchKernelGGL((choose_join_kernel<E, VEC, R, COUNT, 256>), wide_grid(rows, 256), dim3(256), 0, stream,
+                               static_cast<const E*>(times), a, c, parts, rows, (int)J, slices * kWaves);
     }
     SNNTC_HIP_CHECK(hipGetLastError());
     return SNNTC_OK;
@@ -657,16 +682,21 @@ int launch_choose(const void* times, int type, const RuleArgs& a, const ChooseAr
         using E = decltype(e);
         constexpr int VEC = 16 / sizeof(E), R = 32 / VEC;
         if (!narrow(a)) {
+            if (J < VEC) return launch_choose_whole<E, 64, 1, unsigned, 1>(times, a, c, rows, J, stream);
             if (J <= 256 * 16) return launch_choose_whole<E, 256, R / 2, unsigned>(times, a, c, rows, J, stream);
             return launch_choose_slices<E, 256, R / 2, unsigned>(times, a, c, rows, J, parts, stream);
         }
         using C = unsigned short;
+        if (J < VEC) return launch_choose_whole<E, 64, 1, C, 1>(times, a, c, rows, J, stream);
         if (J <= 64 * VEC) return launch_choose_whole<E, 64, 1, C>(times, a, c, rows, J, stream);
         if (J <= 64 * 32) return launch_choose_whole<E, 64, R, C>(times, a, c, rows, J, stream);
         if (J <= 256 * 32) return launch_choose_whole<E, 256, R, C>(times, a, c, rows, J, stream);
-        // one launch, or slices that overlap better where there are many: 1 row of 32000 float32 times 13 and 20 us, 256 rows of bf16 ones
-        // 16 and 24, 512 of float32 ones 31 and 40, 4096 of bf16 ones 118 and 106
-        if (J <= 1024 * 32 && rows < 2048) return launch_choose_whole<E, 1024, R, C>(times, a, c, rows, J, stream);
+        // One launch of a workgroup for each row, or shorter workgroups that overlap better where there are many.  Of bf16 times, in us:
+        //     rows         256 of 10000   256 of 32000   512 of 10000   512 of 32000   1024 of 32000   4096 of 32000
+        //     one launch        11.0           11.6           19.3           20.9            37.3           139.5
+        //     slices            14.6           16.8           16.9           22.9            32.3            91.8
+        if (J <= 1024 * 32 && (rows <= 256 || (rows <= 512 && J > 1024 * 16)))
+            return launch_choose_whole<E, 1024, R, C>(times, a, c, rows, J, stream);
         if (J <= 1024 * 32) return launch_choose_slices<E, 512, R, C>(times, a, c, rows, J, parts, stream);
         return launch_choose_slices<E, 256, R, C>(times, a, c, rows, J, parts, stream);
     });
