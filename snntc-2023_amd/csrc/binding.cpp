@@ -670,6 +670,7 @@ struct TensorList {
     std::vector<void*> at;
     std::vector<int> types;
     std::vector<int64_t> n;
+    void reserve(size_t tensors) { keep.reserve(tensors); at.reserve(tensors); types.reserve(tensors); n.reserve(tensors); }
 };
 
 void add_tensor(TensorList& list, const Tensor& t) {
@@ -691,6 +692,7 @@ bool is_float(const Tensor& t) {
 
 TensorList gradients(const std::vector<Tensor>& gs, const char* who) {
     TensorList list;
+    list.reserve(gs.size());
     for (size_t i = 0; i < gs.size(); ++i) {
         on_device(gs[i], gs[0], who, "gradient", i);
         TORCH_CHECK_TYPE(is_float(gs[i]), who, ": gradient ", i, " must be float32, bfloat16 or float16, got ", gs[i].scalar_type());
@@ -744,6 +746,7 @@ void moment_lists(const Moments& m, const std::vector<Tensor>& sizes, TensorList
     const size_t n = sizes.size();
     TORCH_CHECK_VALUE(m.first.size() == n && m.second.size() == n && (!m.coded || (m.first_scale.size() == n && m.second_scale.size() == n)),
                       "adamw: as many states and scales are needed as there are tensors (", n, ")");
+    for (TensorList& list : out) list.reserve(n);
     for (size_t i = 0; i < n; ++i) {
         const int64_t k = sizes[i].numel();
         add_written(out[0], m.first[i], sizes[0], m.coded ? at::kByte : at::kFloat, k, "first", i);
@@ -762,6 +765,7 @@ void adamw_update(const std::vector<Tensor>& ws, const std::vector<Tensor>& gs, 
     const c10::DeviceGuard guard(ws[0].device());
     TensorList w, state[4];
     const TensorList g = gradients(gs, "adamw");
+    w.reserve(ws.size());
     for (size_t i = 0; i < ws.size(); ++i) {
         TORCH_CHECK_TYPE(is_float(ws[i]), "adamw: weight ", i, " must be float32, bfloat16 or float16, got ", ws[i].scalar_type());
         TORCH_CHECK_VALUE(gs[i].sizes() == ws[i].sizes() && gs[i].scalar_type() == ws[i].scalar_type() && gs[i].device() == ws[i].device(),
@@ -820,6 +824,7 @@ MomentsOut adamw_moments(const Moments& m) {
     for (const Tensor& t : m.first) total += (t.numel() + 63) / 64 * 128;
     const Tensor all = at::empty({total}, m.first[0].options().dtype(at::kFloat));
     int64_t used = 0;
+    for (TensorList& list : to) list.reserve(m.first.size());
     for (const Tensor& t : m.first)
         for (int k = 0; k < 2; ++k) {
             add_tensor(to[k], part_of(all, used, t.sizes()));

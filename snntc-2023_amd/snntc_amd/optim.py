@@ -13,9 +13,10 @@ class AdamW(torch.optim.Optimizer):
       state_bits  32, or 8: codes with a scale for every 256 elements, a quarter of the memory
       max_norm    None, or what the norm over all gradients of a step is scaled down to; a step whose norm is no finite number then
                   changes nothing but its number.  `norm` is the last step's, on the device
-      seed        of the random bits by which codes and 16-bit weights are rounded
+      seed        of the random bits by which codes and 16-bit weights are rounded, from [0, 2^32)
       capturable  the steps are counted on the device, so that a captured step counts by itself when it is replayed; learning
-                  rate and the other numbers stay what they were when it was captured
+                  rate and the other numbers stay what they were when it was captured.  The step before has to have had the same
+                  tensors' gradients, or there is no state yet that a replay could go on from
 
     Weights: contiguous float32, bfloat16 or float16 tensors on one ROCm device, with gradients of their types."""
 
@@ -23,6 +24,10 @@ class AdamW(torch.optim.Optimizer):
                  capturable=False):
         if state_bits not in (8, 32):
             raise ValueError(f"states are held in 8 or 32 bits, not in {state_bits}")
+        if max_norm is not None and not max_norm > 0:
+            raise ValueError(f"max_norm must be positive, or None: {max_norm}")
+        if not 0 <= int(seed) < 1 << 32:
+            raise ValueError(f"a seed is a number of 32 bits, not {seed}")
         self.state_bits, self.max_norm, self.seed, self.capturable = state_bits, max_norm, int(seed), bool(capturable)
         self.norm = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
@@ -44,13 +49,26 @@ class AdamW(torch.optim.Optimizer):
             state["step"] = 0
         self.state[p] = state
 
+    def _parting(self, group, params):
+        """Tensors with a gradient that share their counter with one that has none in this step: lists of them, by counter."""
+        stepping, waiting = {}, set()
+        with_gradient = {id(p) for p in params}
+        for p in group["params"]:
+            state = self.state.get(p)
+            if state and id(p) in with_gradient:
+                stepping.setdefault(id(state["step"]), []).append(p)
+            elif state:
+                waiting.add(id(state["step"]))
+        return [tensors for counter, tensors in stepping.items() if counter in waiting]
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        if not self.capturable and torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        captured = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
+        if captured and not self.capturable:
             raise RuntimeError("AdamW: a step that is captured into a graph needs capturable=True")
         groups = []
         for group in self.param_groups:
@@ -61,9 +79,16 @@ class AdamW(torch.optim.Optimizer):
         grads = [p.grad for params in groups for p in params]
         if not grads:
             return loss
+        parting = [self._parting(group, params) if self.capturable else [] for group, params in zip(self.param_groups, groups)]
+        if captured and (any(parting) or any(not self.state.get(p) for params in groups for p in params)):
+            raise RuntimeError("AdamW: before a step is captured, take one with gradients for the same tensors")
         self.norm = None if self.max_norm is None else grad_norm(grads)
         call = 0
-        for group, params in zip(self.param_groups, groups):
+        for group, params, apart in zip(self.param_groups, groups, parting):
+            for tensors in apart:
+                counter = self.state[tensors[0]]["step"].clone()
+                for p in tensors:
+                    self.state[p]["step"] = counter
             steps = {}
             for p in params:
                 if not self.state[p]:
@@ -74,26 +99,25 @@ class AdamW(torch.optim.Optimizer):
                 together.setdefault(id(n) if self.capturable else n, []).append(p)
             for tensors in together.values():
                 states = [self.state[p] for p in tensors]
-                number = states[0]["step"]
-                if not self.capturable:
-                    number += 1
-                    for s in states:
-                        s["step"] = number
+                number = states[0]["step"] if self.capturable else states[0]["step"] + 1
                 scales = ([s["first_scale"] for s in states], [s["second_scale"] for s in states]) if self.state_bits == 8 else (None, None)
                 adamw_update([p.detach() for p in tensors], [p.grad for p in tensors], [s["first"] for s in states],
                              [s["second"] for s in states], number, lr=group["lr"], betas=group["betas"], eps=group["eps"],
-                             weight_decay=group["weight_decay"], norm=self.norm, max_norm=self.max_norm or 1.0, first_scale=scales[0],
-                             second_scale=scales[1], seed=self.seed + (call << 32))
+                             weight_decay=group["weight_decay"], norm=self.norm, max_norm=1.0 if self.max_norm is None else self.max_norm,
+                             first_scale=scales[0], second_scale=scales[1], seed=self.seed + (call << 32))
+                if not self.capturable:
+                    for s in states:
+                        s["step"] = number
                 call += 1
         return loss
 
     def load_state_dict(self, state_dict):
         """As the base class, but a state keeps the type it was saved with (the base class makes it the weights')."""
         super().load_state_dict(state_dict)
-        params = [p for group in self.param_groups for p in group["params"]]
+        params = [(g, p) for g, group in enumerate(self.param_groups) for p in group["params"]]
         saved = [i for group in state_dict["param_groups"] for i in group["params"]]
-        counters = {}
-        for i, p in zip(saved, params):
+        counters = {}                                    # of a group: every group is a call of its own
+        for i, (g, p) in zip(saved, params):
             if i not in state_dict["state"]:
                 continue
             old = state_dict["state"][i]
@@ -102,8 +126,8 @@ class AdamW(torch.optim.Optimizer):
             state = {k: v.detach().to(p.device, copy=True) for k, v in old.items() if k != "step"}
             step = int(old["step"])
             if self.capturable:
-                if (p.device, step) not in counters:
-                    counters[p.device, step] = torch.tensor(step, dtype=torch.int64, device=p.device)
-                step = counters[p.device, step]
+                if (g, p.device, step) not in counters:
+                    counters[g, p.device, step] = torch.tensor(step, dtype=torch.int64, device=p.device)
+                step = counters[g, p.device, step]
             state["step"] = step
             self.state[p] = state

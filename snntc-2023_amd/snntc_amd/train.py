@@ -131,7 +131,8 @@ def answer(net, prompt, uniform, temperature=1.0, **rules):
     """Continues the sequences prompt[B,P] (int64, P >= 1) token by token: net is a networks.SnnSequential over tokens with SNN_steps
     between its recurrences and its dense layers, uniform[B,T] (float32, from [0, 1)) draws T tokens of each sequence, rules are
     ops.rule_times' repetition, presence, frequency, delay and allowed, the same for every step.  Returns (tokens[B,T], logp[B,T]), logp being
-    the tokens' log-probabilities as they were drawn: at temperature 1 what policy_step takes as old_logp (see answer_batch)."""
+    the tokens' log-probabilities as they were drawn: at temperature 1 what policy_step takes as old_logp (see answer_batch).  A sequence
+    that nothing is allowed for has tokens of -1 and logp NaN from there on."""
     B, P = prompt.shape
     T = uniform.shape[1]
     layers = list(net)
@@ -165,15 +166,18 @@ def answer(net, prompt, uniform, temperature=1.0, **rules):
 
 def answer_batch(prompt, tokens, logp, advantage, **rules):
     """policy_step's arguments for tokens[B,T] and logp[B,T] of answer(net, prompt, ..., **rules) and advantage[B], one for each
-    sequence: a dict of inputs, actions, old_logp, advantage, weight (the mean over the drawn tokens; a prompt's rows have none) and rules."""
+    sequence: a dict of inputs, actions, old_logp, advantage, weight (the mean over the drawn tokens; a prompt's rows have none, nor has
+    any from a sequence's first token of -1 on) and rules."""
     (B, P), T = prompt.shape, tokens.shape[1]
+    there = (tokens >= 0).long().cumprod(1) > 0
+    tokens, logp = torch.where(there, tokens, 0), torch.where(there, logp, 0.0)
     history = torch.cat([prompt, tokens], 1)
     rows = lambda x: torch.cat([x.new_zeros(B, P - 1), x], 1)                                   # noqa: E731
     for k in ("delay", "allowed"):                                  # of every sequence: of each of its rows
         if rules.get(k) is not None and rules[k].dim() == 2:
             rules[k] = rules[k][:, None].expand(B, P + T - 1, -1)
     seen = torch.arange(1, P + T, device=prompt.device).expand(B, P + T - 1)
-    drawn = rows((tokens >= 0).float())
+    drawn = rows(there.float())
     return dict(inputs=history[:, :-1], actions=history[:, 1:], old_logp=rows(logp), advantage=advantage[:, None].expand(B, P + T - 1),
                 weight=drawn / drawn.sum().clamp(min=1.0),
                 rules=dict(history=history, lengths=seen, prompts=torch.full_like(prompt[:, 0], P), **rules))

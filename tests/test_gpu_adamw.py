@@ -508,3 +508,79 @@ def test_calls_larger_than_the_caches(coded):
     if not coded:
         m = 0.9 * before[1].double() + 0.1 * g.double()
         assert bool(((states[0] - m).abs() <= 5 * HALF * (before[1].abs() + g.abs())).all())
+
+
+def _two_groups(n=4):
+    return [torch.nn.Parameter(torch.randn(50, generator=torch.Generator().manual_seed(i)).to(DEV)) for i in range(n)]
+
+
+def _give(ps, k, skip=()):
+    for i, p in enumerate(ps):
+        p.grad = None if i in skip else torch.randn(50, generator=torch.Generator().manual_seed(10 * k + i)).to(DEV)
+
+
+def test_groups_that_resume_count_for_themselves():
+    import snntc_amd as snn
+    ps, qs = _two_groups(), _two_groups()
+    make = lambda a, **how: snn.optim.AdamW([{"params": a[:2], "lr": 0.1}, {"params": a[2:]}], 0.01, **how)                # noqa: E731
+    plain, counted = make(ps), make(qs, capturable=True)
+    for k in range(2):
+        _give(ps, k)
+        _give(qs, k)
+        plain.step()
+        counted.step()
+    again = make(qs, capturable=True)
+    again.load_state_dict(counted.state_dict())
+    for k in range(2, 5):
+        _give(ps, k)
+        _give(qs, k)
+        plain.step()
+        again.step()
+        assert [int(again.state[q]["step"]) for q in qs] == [k + 1] * 4
+    for p, q in zip(ps, qs):
+        assert torch.allclose(p, q, rtol=1e-6, atol=1e-6)
+
+
+def test_a_tensor_without_a_gradient_does_not_count():
+    """Tensors that began together share a counter on the device until one of them sits a step out."""
+    import snntc_amd as snn
+    ps, qs = _two_groups(), _two_groups()
+    plain, counted = snn.optim.AdamW(ps, 0.01), snn.optim.AdamW(qs, 0.01, capturable=True)
+    for k, skip in enumerate(((), (1,), (1, 2), (), (3,))):
+        _give(ps, k, skip)
+        _give(qs, k, skip)
+        plain.step()
+        counted.step()
+    assert [int(counted.state[q]["step"]) for q in qs] == [plain.state[p]["step"] for p in ps] == [5, 3, 4, 4]
+    for p, q in zip(ps, qs):
+        assert torch.allclose(p, q, rtol=1e-6, atol=1e-6)
+
+
+def test_a_captured_step_has_its_states_already():
+    import snntc_amd as snn
+    ps = _two_groups()
+    _give(ps, 0)
+    opt = snn.optim.AdamW(ps, 0.01, capturable=True)
+    before = [p.detach().clone() for p in ps]
+    with pytest.raises(RuntimeError, match="before"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    opt.step()
+    assert all(bool((p != b).any()) for p, b in zip(ps, before))
+    _give(ps, 1, (1,))
+    with pytest.raises(RuntimeError, match="before"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+
+
+def test_a_refused_step_does_not_count():
+    import snntc_amd as snn
+    ps = _two_groups()
+    opt = snn.optim.AdamW(ps, 0.01)
+    _give(ps, 0)
+    opt.step()
+    _give(ps, 1)
+    opt.state[ps[1]]["first"] = opt.state[ps[1]]["first"][:-1]
+    with pytest.raises(ValueError):
+        opt.step()
+    assert [opt.state[p]["step"] for p in ps] == [1] * 4

@@ -213,3 +213,29 @@ def test_tangents_and_transforms_are_refused():
             snn.rule_times(fwad.make_dual(t, t), h, repetition=2.0)
     with pytest.raises((NotImplementedError, RuntimeError)):
         torch.func.grad(lambda x: snn.rule_times(x, h, repetition=2.0).sum())(t)
+
+
+def test_a_sequence_that_nothing_is_allowed_for_has_no_weight():
+    """A sequence that runs out of tokens neither counts nor spoils the step of the others."""
+    import snntc_amd as snn
+    net, prompt, uniform, mask, rules, _ = _drawn(6)
+    mask[2] = False
+    rules["allowed"] = snn.pack_allowed(mask)
+    tokens, logp = snn.train.answer(net, prompt, uniform, **rules)
+    assert bool((tokens[2] == -1).all() and logp[2].isnan().all()) and bool((tokens[[0, 1, 3, 4, 5]] >= 0).all())
+    tokens[4, 5:], logp[4, 5:] = -1, float("nan")                       # (and one that ended)
+    advantage = torch.randn(6, generator=torch.Generator().manual_seed(5)).to(DEV)
+    batch = snn.train.answer_batch(prompt, tokens, logp, advantage, **rules)
+    drawn = torch.zeros(6, 12, dtype=torch.bool, device=DEV)
+    drawn[:, 3:] = tokens >= 0
+    assert torch.equal(batch["weight"] > 0, drawn) and abs(float(batch["weight"].sum()) - 1) < 1e-5
+    loss = snn.train.policy_step(net, torch.optim.SGD(net.parameters(), lr=0.1), **batch)
+    others, rest = _net(6), [0, 1, 3, 4, 5]
+    kept = dict(rules, allowed=snn.pack_allowed(mask[rest]))
+    batch = snn.train.answer_batch(prompt[rest], tokens[rest].clamp(min=0), logp[rest].nan_to_num(0.0), advantage[rest], **kept)
+    batch["weight"] = drawn[rest].float() / drawn.sum()
+    want = snn.train.policy_step(others, torch.optim.SGD(others.parameters(), lr=0.1), **batch)
+    assert bool(torch.isfinite(loss)) and torch.allclose(loss, want, rtol=1e-5, atol=1e-6)
+    for a, b in zip(net.weights(), others.weights()):
+        # (the sums over rows are in another order: at most 72 terms, each half a step off, of a gradient of a tenth the step's size)
+        assert torch.allclose(a, b, rtol=1e-5, atol=1e-5)

@@ -134,3 +134,12 @@ def test_packed_masks(J):
     assert words.dtype == torch.int32 and words.shape == (3, 2, (J + 31) // 32)
     for j in range(J):
         assert torch.equal((words[..., j // 32] >> (j % 32) & 1).bool(), mask[..., j])
+
+
+def test_the_optimizer_refuses_numbers_that_mean_nothing():
+    import torch
+    import snntc_amd as snn
+    w = [torch.nn.Parameter(torch.ones(3))]
+    for wrong in ({"max_norm": 0}, {"max_norm": -1.0}, {"max_norm": float("nan")}, {"seed": -1}, {"seed": 1 << 32}, {"state_bits": 16}):
+        with pytest.raises(ValueError):
+            snn.optim.AdamW(w, **wrong)
