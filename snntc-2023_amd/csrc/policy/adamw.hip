@@ -112,29 +112,31 @@ using Place = typename std::conditional<sizeof(E) == 4, FourFloats, typename std
 // PAST: past the caches.  A call that touches more than they hold reads and writes weights and states so: what the norm has left of
 // the gradients stays there, and the next call's gradients do not wait for this one's results (68 M float32 weights, 404 -> 335 us with
 // the norm; the norm by itself 85 -> 47).
-template <bool PAST, typename E>
-__device__ __forceinline__ Four<E> load4(const E* at, int n) {
-    if (n >= 4) {
-        const Place<E>* p = reinterpret_cast<const Place<E>*>(at);
+// WHOLE: there are four elements from e on; else those at or behind n are the last one once more.  Not one load stands in a branch: the
+// compiler waits for all that are under way where branches meet.
+template <bool PAST, bool WHOLE, typename E>
+__device__ __forceinline__ Four<E> load4(const E* from, long long e, long long n) {
+    if constexpr (WHOLE) {
+        const Place<E>* p = reinterpret_cast<const Place<E>*>(from + e);
         if constexpr (PAST) return __builtin_bit_cast(Four<E>, __builtin_nontemporal_load(p));
         return __builtin_bit_cast(Four<E>, *p);
     }
     Four<E> r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r.v[i] = i < n ? at[i] : (E)0;
+    for (int i = 0; i < 4; ++i) r.v[i] = from[min(e + i, n - 1)];
     return r;
 }
-template <bool PAST, typename E>
-__device__ __forceinline__ void store4(E* at, const Four<E>& r, int n) {
-    if (n >= 4) {
-        Place<E>* p = reinterpret_cast<Place<E>*>(at);
+template <bool PAST, bool WHOLE, typename E>
+__device__ __forceinline__ void store4(E* to, long long e, long long n, const Four<E>& r) {
+    if constexpr (WHOLE) {
+        Place<E>* p = reinterpret_cast<Place<E>*>(to + e);
         if constexpr (PAST) __builtin_nontemporal_store(__builtin_bit_cast(Place<E>, r), p);
         else *p = __builtin_bit_cast(Place<E>, r);
-        return;
-    }
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (i < n) at[i] = r.v[i];
+        for (int i = 0; i < 4; ++i)
+            if (e + i < n) to[e + i] = r.v[i];
+    }
 }
 
 template <typename T>
@@ -156,9 +158,10 @@ __device__ __forceinline__ double share_of(const AdamScalars& s, bool* skip) {
     return (double)norm > s.max_norm ? s.max_norm / (double)norm : 1.0;
 }
 
-constexpr int kEach = 4;                                       // elements of a thread at a time
-constexpr int kTimes = 2;
-constexpr int kChunk = kThreads * kEach * kTimes;
+constexpr int kTimes = 2;                                      // blocks of 256 elements that a wavefront holds
+constexpr int kChunk = kThreads * 4 * kTimes;
+// A wavefront's first element in a tensor, of workgroup `block` of the tensor's.
+__device__ __forceinline__ long long wave_begin(unsigned block) { return ((long long)block * (kThreads / kWave) + threadIdx.x / kWave) * (kBlock * kTimes); }
 
 // The hardware's root, off by a step; it takes no number below 2^-126, which a power of four brings up.
 __device__ __forceinline__ float root(float x) {
@@ -172,12 +175,9 @@ __device__ __forceinline__ float stepped(float w, float m, float v, float keep, 
 }
 
 // States in float32.  Bound by memory.
-template <typename E, bool PAST>
-__global__ void __launch_bounds__(kThreads)
-adamw_kernel(AdamTable tab, AdamScalars s) {
-    const unsigned block = gridDim.x - 1 - blockIdx.x;                      // (the gradients that the norm has read last come first)
-    const int t = tensor_of(tab, block);
-    const long long n = tab.n[t], e0 = (long long)(block - tab.first_block[t]) * kChunk + threadIdx.x * kEach;
+template <bool WHOLE, typename E, bool PAST>
+__device__ __forceinline__ void adamw_run(const AdamTable& tab, const AdamScalars& s, int t, long long begin) {
+    const long long n = tab.n[t], e0 = begin + threadIdx.x % kWave * 4;
     E* __restrict__ w = static_cast<E*>(tab.w[t]);
     const E* __restrict__ g = static_cast<const E*>(tab.g[t]);
     float* __restrict__ m = static_cast<float*>(tab.m[t]);
@@ -186,10 +186,8 @@ adamw_kernel(AdamTable tab, AdamScalars s) {
     Four<float> M[kTimes], V[kTimes];
 #pragma unroll
     for (int i = 0; i < kTimes; ++i) {
-        const long long e = e0 + i * kThreads * kEach;
-        const int left = (int)min(n - e, 4ll);
-        if (left <= 0) continue;
-        W[i] = load4<PAST>(w + e, left); G[i] = load4<false>(g + e, left); M[i] = load4<PAST>(m + e, left); V[i] = load4<PAST>(v + e, left);
+        const long long e = e0 + i * kBlock;
+        W[i] = load4<PAST, WHOLE>(w, e, n); G[i] = load4<false, WHOLE>(g, e, n); M[i] = load4<PAST, WHOLE>(m, e, n); V[i] = load4<PAST, WHOLE>(v, e, n);
     }
     bool skip;
     const float share = (float)share_of(s, &skip);
@@ -200,9 +198,7 @@ adamw_kernel(AdamTable tab, AdamScalars s) {
     const unsigned key = sizeof(E) == 2 ? key_of(s, at.step, tab.tensor[t]) : 0;
 #pragma unroll
     for (int i = 0; i < kTimes; ++i) {
-        const long long e = e0 + i * kThreads * kEach;
-        const int left = (int)min(n - e, 4ll);
-        if (left <= 0) continue;
+        const long long e = e0 + i * kBlock;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const float d = (float)G[i].v[k] * share;
@@ -211,21 +207,27 @@ adamw_kernel(AdamTable tab, AdamScalars s) {
             const unsigned bits = sizeof(E) == 2 ? third_noise(noise(key, (unsigned)e * kElement + k * kElement)) : 0;
             round_weight(stepped((float)W[i].v[k], M[i].v[k], V[i].v[k], keep, rate, second, eps), bits, &W[i].v[k]);
         }
-        store4<PAST>(w + e, W[i], left); store4<PAST>(m + e, M[i], left); store4<PAST>(v + e, V[i], left);
+        store4<PAST, WHOLE>(w, e, n, W[i]); store4<PAST, WHOLE>(m, e, n, M[i]); store4<PAST, WHOLE>(v, e, n, V[i]);
     }
+}
+template <typename E, bool PAST>
+__global__ void __launch_bounds__(kThreads)
+adamw_kernel(AdamTable tab, AdamScalars s) {
+    const unsigned block = gridDim.x - 1 - blockIdx.x;                      // (the gradients that the norm has read last come first)
+    const int t = tensor_of(tab, block);
+    const long long begin = wave_begin(block - tab.first_block[t]), n = tab.n[t];
+    if (begin + kBlock * kTimes <= n) adamw_run<true, E, PAST>(tab, s, t, begin);
+    else if (begin < n) adamw_run<false, E, PAST>(tab, s, t, begin);
 }
 
 __device__ __forceinline__ unsigned wave_max(unsigned v) { return wave_join(v, 0u, [](unsigned a, unsigned b) { return max(a, b); }); }
 // A magnitude's bits: ordered as magnitudes are, NaN above all.
 __device__ __forceinline__ unsigned magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
-// States in 8 bits: a wavefront owns kTimes blocks of 256 elements.
-template <typename E, bool PAST>
-__global__ void __launch_bounds__(kThreads)
-adamw8_kernel(AdamTable tab, AdamScalars s) {
-    const unsigned block = gridDim.x - 1 - blockIdx.x;
-    const int t = tensor_of(tab, block), lane = threadIdx.x % kWave;
-    const long long n = tab.n[t], b0 = ((long long)(block - tab.first_block[t]) * (kThreads / kWave) + threadIdx.x / kWave) * kTimes;
+// States in 8 bits: a wavefront owns kTimes blocks of 256 elements.  (Copies of a tensor's last element leave a block's maxima as they are.)
+template <bool WHOLE, typename E, bool PAST>
+__device__ __forceinline__ void adamw8_run(const AdamTable& tab, const AdamScalars& s, int t, long long begin) {
+    const long long n = tab.n[t], e0 = begin + threadIdx.x % kWave * 4, b0 = begin / kBlock, last = (n - 1) / kBlock;
     E* __restrict__ w = static_cast<E*>(tab.w[t]);
     const E* __restrict__ g = static_cast<const E*>(tab.g[t]);
     unsigned char* __restrict__ m = static_cast<unsigned char*>(tab.m[t]);
@@ -236,11 +238,9 @@ adamw8_kernel(AdamTable tab, AdamScalars s) {
     float m_scale[kTimes], v_scale[kTimes];
 #pragma unroll
     for (int i = 0; i < kTimes; ++i) {
-        const long long e = (b0 + i) * kBlock + lane * 4;
-        const int left = (int)max(min(n - e, 4ll), 0ll);
-        if ((b0 + i) * kBlock >= n) continue;                 // (a whole wavefront)
-        W[i] = load4<PAST>(w + e, left); G[i] = load4<false>(g + e, left); M[i] = load4<PAST>(m + e, left); V[i] = load4<PAST>(v + e, left);
-        m_scale[i] = ms[b0 + i]; v_scale[i] = vs[b0 + i];
+        const long long e = e0 + i * kBlock, b = WHOLE ? b0 + i : min(b0 + i, last);
+        W[i] = load4<PAST, WHOLE>(w, e, n); G[i] = load4<false, WHOLE>(g, e, n); M[i] = load4<PAST, WHOLE>(m, e, n); V[i] = load4<PAST, WHOLE>(v, e, n);
+        m_scale[i] = ms[b]; v_scale[i] = vs[b];
     }
     bool skip;
     const double share = share_of(s, &skip);
@@ -251,9 +251,8 @@ adamw8_kernel(AdamTable tab, AdamScalars s) {
     const unsigned key = key_of(s, at.step, tab.tensor[t]);
 #pragma unroll
     for (int i = 0; i < kTimes; ++i) {
-        const long long e = (b0 + i) * kBlock + lane * 4;
-        const int left = (int)max(min(n - e, 4ll), 0ll);
-        if ((b0 + i) * kBlock >= n) continue;
+        const long long e = e0 + i * kBlock;
+        if (!WHOLE && begin + i * kBlock >= n) return;        // (a whole wavefront)
         const double old1 = s.b1 * kFirstUnit * (double)m_scale[i], old2 = s.b2 * kSecondUnit * (double)v_scale[i];
         const unsigned place = (unsigned)e * kElement;
         double a[4], q[4];
@@ -268,7 +267,7 @@ adamw8_kernel(AdamTable tab, AdamScalars s) {
             bits[k] = noise(key, place + k * kElement);
             round_weight(stepped((float)W[i].v[k], fa, fq, keep, rate, second, eps), sizeof(E) == 2 ? third_noise(bits[k]) : 0, &W[i].v[k]);
         }
-        store4<PAST>(w + e, W[i], left);
+        store4<PAST, WHOLE>(w, e, n, W[i]);
         const float scale1 = __uint_as_float(wave_max(top1)), scale2 = __uint_as_float(wave_max(top2));
         const double unit1 = per_scale(kTopFirst, scale1), unit2 = per_scale(kTopSecond, scale2);
 #pragma unroll
@@ -277,9 +276,18 @@ adamw8_kernel(AdamTable tab, AdamScalars s) {
             M[i].v[k] = (unsigned char)(c | ((unsigned)__double2hiint(a[k]) >> 24 & 128u));
             V[i].v[k] = (unsigned char)code_of(q[k] * unit2, bits[k] >> 16, 255u);
         }
-        store4<PAST>(m + e, M[i], left); store4<PAST>(v + e, V[i], left);
-        if (lane == 0) { ms[b0 + i] = scale1; vs[b0 + i] = scale2; }
+        store4<PAST, WHOLE>(m, e, n, M[i]); store4<PAST, WHOLE>(v, e, n, V[i]);
+        if (threadIdx.x % kWave == 0) { ms[b0 + i] = scale1; vs[b0 + i] = scale2; }
     }
+}
+template <typename E, bool PAST>
+__global__ void __launch_bounds__(kThreads)
+adamw8_kernel(AdamTable tab, AdamScalars s) {
+    const unsigned block = gridDim.x - 1 - blockIdx.x;
+    const int t = tensor_of(tab, block);
+    const long long begin = wave_begin(block - tab.first_block[t]), n = tab.n[t];
+    if (begin + kBlock * kTimes <= n) adamw8_run<true, E, PAST>(tab, s, t, begin);
+    else if (begin < n) adamw8_run<false, E, PAST>(tab, s, t, begin);
 }
 
 // The number of a step that a graph replays: one more each time, and what follows from it.
@@ -301,26 +309,37 @@ struct MomentTable {
     unsigned first_block[kMostTensors + 1];
     int count;
 };
+template <bool WHOLE, bool PAST>
+__device__ __forceinline__ void moments_run(const MomentTable& tab, int t, long long begin) {
+    const long long n = tab.n[t], e0 = begin + threadIdx.x % kWave * 4, b0 = begin / kBlock, last = (n - 1) / kBlock;
+    Four<unsigned char> M[kTimes], V[kTimes];
+    float m_scale[kTimes], v_scale[kTimes];
+#pragma unroll
+    for (int i = 0; i < kTimes; ++i) {
+        const long long e = e0 + i * kBlock, b = WHOLE ? b0 + i : min(b0 + i, last);
+        M[i] = load4<false, WHOLE>(tab.m[t], e, n); V[i] = load4<false, WHOLE>(tab.v[t], e, n);
+        m_scale[i] = tab.m_scale[t][b]; v_scale[i] = tab.v_scale[t][b];
+    }
+#pragma unroll
+    for (int i = 0; i < kTimes; ++i) {
+        const long long e = e0 + i * kBlock;
+        const double u1 = kFirstUnit * (double)m_scale[i], u2 = kSecondUnit * (double)v_scale[i];
+        Four<float> a, q;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            a.v[k] = (float)(first_value(M[i].v[k]) * u1);
+            q.v[k] = (float)(second_value(V[i].v[k]) * u2);
+        }
+        store4<PAST, WHOLE>(tab.first[t], e, n, a); store4<PAST, WHOLE>(tab.second[t], e, n, q);
+    }
+}
 template <bool PAST>
 __global__ void __launch_bounds__(kThreads)
 moments_kernel(MomentTable tab) {
     const int t = tensor_of(tab, blockIdx.x);
-    const long long n = tab.n[t], e0 = (long long)(blockIdx.x - tab.first_block[t]) * kChunk + threadIdx.x * kEach;
-#pragma unroll
-    for (int i = 0; i < kTimes; ++i) {
-        const long long e = e0 + i * kThreads * kEach;
-        const int left = (int)min(n - e, 4ll);
-        if (left <= 0) continue;
-        const Four<unsigned char> M = load4<false>(tab.m[t] + e, left), V = load4<false>(tab.v[t] + e, left);
-        const double u1 = kFirstUnit * (double)tab.m_scale[t][e / kBlock], u2 = kSecondUnit * (double)tab.v_scale[t][e / kBlock];
-        Four<float> a, q;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            a.v[k] = (float)(first_value(M.v[k]) * u1);
-            q.v[k] = (float)(second_value(V.v[k]) * u2);
-        }
-        store4<PAST>(tab.first[t] + e, a, left); store4<PAST>(tab.second[t] + e, q, left);
-    }
+    const long long begin = wave_begin(blockIdx.x - tab.first_block[t]), n = tab.n[t];
+    if (begin + kBlock * kTimes <= n) moments_run<true, PAST>(tab, t, begin);
+    else if (begin < n) moments_run<false, PAST>(tab, t, begin);
 }
 
 // ---- the norm over all gradients -------------------------------------------------------------------------------------------------
@@ -360,15 +379,24 @@ __device__ __forceinline__ double squares(const E* __restrict__ g, long long fro
             sum[k] = fma(d, d, sum[k]);
         }
     };
-    long long e = from + threadIdx.x * 4;
-    for (; from + kPieces * kThreads * 4 <= to; from += kPieces * kThreads * 4, e += kPieces * kThreads * 4) {
-        Four<E> x[kPieces];
+    const auto pieces = [&](auto many) {
+        constexpr int N = decltype(many)::value;
+        for (; from + N * kThreads * 4 <= to; from += N * kThreads * 4) {
+            Four<E> x[N];
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) x[i] = load4<false>(g + e + i * kThreads * 4, 4);
+            for (int i = 0; i < N; ++i) x[i] = load4<false, true>(g, from + (i * kThreads + threadIdx.x) * 4, to);
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) add(x[i]);
+            for (int i = 0; i < N; ++i) add(x[i]);
+        }
+    };
+    pieces(std::integral_constant<int, kPieces>());
+    pieces(std::integral_constant<int, 2>());
+    for (long long e = from + threadIdx.x * 4; e < to; e += kThreads * 4) {
+        Four<E> x = load4<false, false>(g, e, to);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x.v[k] = e + k < to ? x.v[k] : (E)0.0f;
+        add(x);
     }
-    for (; e < to; e += kThreads * 4) add(load4<false>(g + e, (int)min(to - e, 4ll)));
     return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 __global__ void __launch_bounds__(kThreads)
