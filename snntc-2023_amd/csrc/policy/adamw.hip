@@ -139,14 +139,19 @@ __device__ __forceinline__ void store4(E* to, long long e, long long n, const Fo
     }
 }
 
+// The tensor that a workgroup belongs to: all of the table's first workgroups are compared at once.
 template <typename T>
 __device__ __forceinline__ int tensor_of(const T& tab, unsigned block) {
-    int low = 0, high = tab.count;
-    while (high - low > 1) {                                  // (uniform)
-        const int mid = (low + high) >> 1;
-        if (tab.first_block[mid] <= block) low = mid; else high = mid;
+    constexpr int kEntries = sizeof(tab.first_block) / sizeof(unsigned);
+    const int lane = threadIdx.x % kWave;
+    int t = -1;
+#pragma unroll
+    for (int i = 0; i < (kEntries + kWave - 1) / kWave; ++i) {
+        const int at = i * kWave + lane;
+        const unsigned first = tab.first_block[min(at, kEntries - 1)];
+        t += __popcll(__ballot(at < tab.count && first <= block));
     }
-    return low;
+    return t;
 }
 
 // What the gradients are scaled by; a norm that is no finite number: the step is left out.
@@ -161,7 +166,10 @@ __device__ __forceinline__ double share_of(const AdamScalars& s, bool* skip) {
 constexpr int kTimes = 2;                                      // blocks of 256 elements that a wavefront holds
 constexpr int kChunk = kThreads * 4 * kTimes;
 // A wavefront's first element in a tensor, of workgroup `block` of the tensor's.
-__device__ __forceinline__ long long wave_begin(unsigned block) { return ((long long)block * (kThreads / kWave) + threadIdx.x / kWave) * (kBlock * kTimes); }
+__device__ __forceinline__ long long wave_begin(unsigned block) {
+    return ((long long)block * (kThreads / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave)) *
+           (kBlock * kTimes);
+}
 
 // The hardware's root, off by a step; it takes no number below 2^-126, which a power of four brings up.
 __device__ __forceinline__ float root(float x) {

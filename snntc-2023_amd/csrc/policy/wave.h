@@ -16,6 +16,15 @@ __device__ __forceinline__ T from_lane(T none, T v) {
     for (int i = 0; i < (int)(sizeof(T) / 4); ++i) x.h[i] = __builtin_amdgcn_update_dpp(n.h[i], x.h[i], CTRL, MASK, 0xF, false);
     return __builtin_bit_cast(T, x);
 }
+// The same where every lane has one: part of the instruction that uses it.
+template <int CTRL, typename T>
+__device__ __forceinline__ T exchanged(T v) {
+    struct Halves { int h[sizeof(T) / 4]; };
+    Halves x = __builtin_bit_cast(Halves, v);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 4); ++i) x.h[i] = __builtin_amdgcn_mov_dpp(x.h[i], CTRL, 0xF, 0xF, true);
+    return __builtin_bit_cast(T, x);
+}
 // A lane's value for all; the lane is the same for all.
 template <typename T>
 __device__ __forceinline__ T of_lane(T v, int lane) {
@@ -29,10 +38,10 @@ __device__ __forceinline__ T of_lane(T v, int lane) {
 // the next one and lane 31 to the upper half; the last lane has them all.
 template <typename T, typename F>
 __device__ __forceinline__ T wave_join(T v, T none, F&& f) {
-    v = f(v, from_lane<0xB1, 0xF>(v, v));
-    v = f(v, from_lane<0x4E, 0xF>(v, v));
-    v = f(v, from_lane<0x141, 0xF>(v, v));
-    v = f(v, from_lane<0x140, 0xF>(v, v));
+    v = f(v, exchanged<0xB1>(v));
+    v = f(v, exchanged<0x4E>(v));
+    v = f(v, exchanged<0x141>(v));
+    v = f(v, exchanged<0x140>(v));
     v = f(v, from_lane<0x142, 0xA>(none, v));
     v = f(v, from_lane<0x143, 0xC>(none, v));
     return of_lane(v, kWave - 1);
