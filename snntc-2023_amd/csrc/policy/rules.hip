@@ -226,6 +226,9 @@ __device__ const unsigned kAllAllowed[1] = {~0u};
 template <typename T>
 using Device = const T __attribute__((address_space(1)))*;
 
+// Words of a mask that hold a piece's bits.
+struct Allowed { unsigned low, high; };
+
 // A slice of a row: elements [first, first + end).
 struct Slice { int64_t first; int end; };
 template <int SLICE, int VEC>
@@ -236,18 +239,30 @@ __device__ __forceinline__ Slice slice_of(unsigned slice, int J) {
     s.end = (int)min((int64_t)SLICE, J - s.first);
     return s;
 }
-template <int VEC>
-__device__ __forceinline__ Piece<float, VEC> request_delay(const RowRules& q, int64_t j) {
-    const Device<float> d = q.delay ? (Device<float>)q.delay : (Device<float>)kNoDelay;
-    return read_piece<float, VEC>((const float*)(d + (q.delay ? j : 0)));
+// An element of an array by its offset in 32 bits, which the instructions add to a common address.
+template <typename T>
+__device__ __forceinline__ Device<T> place_in(Device<T> array, unsigned i) {
+    return (Device<T>)((Device<char>)array + (unsigned)(i * sizeof(T)));
 }
-struct Allowed { unsigned low, high; };
-__device__ __forceinline__ Allowed request_allowed(const RowRules& q, int64_t j, int J) {
-    const Device<unsigned> w = q.allowed ? (Device<unsigned>)q.allowed : (Device<unsigned>)kAllAllowed;
-    const int at = q.allowed ? (int)(j >> 5) : 0, last = q.allowed ? (J - 1) >> 5 : 0;
-    return Allowed{w[at], w[min(at + 1, last)]};
-}
-__device__ __forceinline__ unsigned allowed_from(const Allowed& w, int64_t j) { return __builtin_amdgcn_alignbit(w.high, w.low, (unsigned)j & 31); }
+// What there is of a slice, by elements of the slice; its first element has the lowest bit of a word of `allowed`.
+template <typename E, int VEC>
+struct Reader {
+    Device<E> times;
+    Device<float> delay;
+    Device<unsigned> allowed;
+    unsigned any_delay, last_word;                   // (0: where there is no array)
+    __device__ __forceinline__ Reader(const E* row, const RowRules& q, const Slice& s)
+        : times((Device<E>)row + s.first), delay(q.delay ? (Device<float>)q.delay + s.first : (Device<float>)kNoDelay),
+          allowed(q.allowed ? (Device<unsigned>)q.allowed + (s.first >> 5) : (Device<unsigned>)kAllAllowed),
+          any_delay(q.delay ? ~0u : 0), last_word(q.allowed ? (unsigned)(s.end - 1) >> 5 : 0) {}
+    __device__ __forceinline__ Piece<E, VEC> piece(int j) const { return read_piece<E, VEC>((const E*)place_in(times, j)); }
+    __device__ __forceinline__ Piece<float, VEC> delays(int j) const { return read_piece<float, VEC>((const float*)place_in(delay, j & any_delay)); }
+    __device__ __forceinline__ Allowed words(int j) const {
+        const unsigned at = (unsigned)j >> 5;
+        return Allowed{*place_in(allowed, min(at, last_word)), *place_in(allowed, min(at + 1, last_word))};
+    }
+};
+__device__ __forceinline__ unsigned allowed_from(const Allowed& w, int j) { return __builtin_amdgcn_alignbit(w.high, w.low, (unsigned)j & 31); }
 
 // The ruled times of one piece.  Marked elements are few: one at a time and lane, instead of a test for each.
 template <typename E, int VEC, typename M>
@@ -293,6 +308,7 @@ rule_kernel(const E* __restrict__ in, const E* __restrict__ times, E* __restrict
     const Slice s = slice_of<M::kSlice, VEC>(block - r * (unsigned)slices, J);
     const int64_t at = (int64_t)r * J + s.first;
     const RowRules q = row_rules(a, r);
+    const Reader<E, VEC> from(in + (int64_t)r * J, q, s);
     M marks;
     marks.request(a, q);
     const auto local = [&](int i) { return min((i * WIDTH + (int)threadIdx.x) * VEC, s.end - VEC); };
@@ -301,10 +317,10 @@ rule_kernel(const E* __restrict__ in, const E* __restrict__ times, E* __restrict
     Piece<float, VEC> delay[2];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        held[i] = read_piece<E, VEC>(in + at + local(i));
-        allowed[i] = request_allowed(q, s.first + local(i), J);
+        held[i] = from.piece(local(i));
+        allowed[i] = from.words(local(i));
     }
-    if constexpr (!GRAD) delay[0] = request_delay<VEC>(q, s.first + local(0));
+    if constexpr (!GRAD) delay[0] = from.delays(local(0));
     const bool from_history = marks.build(lds, q, s.first, s.end, GRAD ? times + at : nullptr);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
@@ -320,13 +336,13 @@ rule_kernel(const E* __restrict__ in, const E* __restrict__ times, E* __restrict
                 }
             }
             if (q.allowed) {
-                const unsigned w = allowed_from(allowed[i], s.first + local(i));
+                const unsigned w = allowed_from(allowed[i], local(i));
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) held[i].v[v] = w >> v & 1 ? held[i].v[v] : (E)0.0f;
             }
         } else {
-            if (i + 1 < R) delay[(i + 1) % 2] = request_delay<VEC>(q, s.first + local(i + 1));
-            rule_piece<E, VEC, M>(held[i], lds, from_history, q, delay[i % 2], allowed_from(allowed[i], s.first + local(i)), local(i));
+            if (i + 1 < R) delay[(i + 1) % 2] = from.delays(local(i + 1));
+            rule_piece<E, VEC, M>(held[i], lds, from_history, q, delay[i % 2], allowed_from(allowed[i], local(i)), local(i));
         }
         store_piece<STREAM, E, VEC>(out + at + local(i), held[i]);
     }
@@ -357,22 +373,22 @@ struct Run {
     __device__ __forceinline__ int local(int i) const { return min(proper(i), end - VEC); }
     __device__ __forceinline__ int in_run(int i) const { return local(i) - origin(); }
     __device__ __forceinline__ float v(int i, int e) const { return -(float)t[i].v[e]; }
-    __device__ __forceinline__ void request(const E* row, const RowRules& q, const Slice& s, int J) {
+    __device__ __forceinline__ void request(const Reader<E, VEC>& from, const Slice& s) {
         end = s.end;
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            t[i] = read_piece<E, VEC>(row + s.first + local(i));
-            allowed[i] = request_allowed(q, s.first + local(i), J);
+            t[i] = from.piece(local(i));
+            allowed[i] = from.words(local(i));
         }
-        delay[0] = request_delay<VEC>(q, s.first + local(0));
+        delay[0] = from.delays(local(0));
     }
     // M: the marks of the slice.  own: elements of the slice before this one have been the last slice's.
     template <typename M>
-    __device__ __forceinline__ void rule(const typename M::Memory& lds, bool from_history, const RowRules& q, const Slice& s, int own) {
+    __device__ __forceinline__ void rule(const typename M::Memory& lds, bool from_history, const RowRules& q, const Reader<E, VEC>& from, int own) {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            if (i + 1 < R) delay[(i + 1) % 2] = request_delay<VEC>(q, s.first + local(i + 1));
-            rule_piece<E, VEC, M>(t[i], lds, from_history, q, delay[i % 2], allowed_from(allowed[i], s.first + local(i)), local(i));
+            if (i + 1 < R) delay[(i + 1) % 2] = from.delays(local(i + 1));
+            rule_piece<E, VEC, M>(t[i], lds, from_history, q, delay[i % 2], allowed_from(allowed[i], local(i)), local(i));
             const int skip = max(proper(i), own) - local(i);
             if (skip > 0) {
 #pragma unroll
@@ -534,11 +550,12 @@ choose_slice_kernel(const E* __restrict__ times, RuleArgs a, ChooseArgs c, Part*
     const RowRules q = row_rules(a, r);
     M marks;
     marks.request(a, q);
+    const Reader<E, VEC> from(row, q, s);
     Mine run;
-    run.request(row, q, s, J);
+    run.request(from, s);
     const Heat h = heat_of(c, r);
     const bool from_history = marks.build(lds, q, s.first, s.end, row);
-    run.template rule<M>(lds, from_history, q, s, (int)((int64_t)slice * M::kSlice - s.first));
+    run.template rule<M>(lds, from_history, q, from, (int)((int64_t)slice * M::kSlice - s.first));
     const Part mine = run.part(h.k, h.greedy);
     if constexpr (!WHOLE) {
         // (an index from where the run has its place, wherever the slice begins)
@@ -581,11 +598,12 @@ choose_join_kernel(const E* __restrict__ times, RuleArgs a, ChooseArgs c, const 
     } else if (f.part >= 0) {
         const E* __restrict__ row = times + (int64_t)r * J;
         const Slice s = slice_of<Mine::kLength, VEC>(f.part, J);
+        const Reader<E, VEC> from(row, q, s);
         Mine run;
-        if (threadIdx.x < kWave) run.request(row, q, s, J);
+        if (threadIdx.x < kWave) run.request(from, s);
         const bool from_history = marks.build(lds, q, s.first, s.end, row);
         if (threadIdx.x >= kWave) return;
-        run.template rule<M>(lds, from_history, q, s, (int)(begin - s.first));
+        run.template rule<M>(lds, from_history, q, from, (int)(begin - s.first));
         const int at = run.pick(f.rest, f.at.m, h.k, &value);
         token = at < 0 ? -1 : s.first + at;
     }
