@@ -405,3 +405,62 @@ def test_more_elements_than_31_bits_count(rows, J):
     if J > 64:
         times[r[:, 0], at] = -60.0
         assert torch.equal(snn.choose_tokens(times, torch.full((rows,), 0.5, device=DEV))[0], at)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("J", [65, 67, 513, 8193, 8197, 12295, 16387, 20481])
+def test_ends_of_rows_under_rules(J, dtype):
+    """Rows that end one element or a few into what a workgroup or a wavefront takes."""
+    import snntc_amd as snn
+    times, k = _inputs(J, 2, 2, J, 40, dtype, signed=True)
+    k["history"][:, ::3] = torch.arange(J - 14, J, device=DEV)
+    want, size, slope = _plain(times, **k)
+    _check(snn.rule_times(times, **k), want, size, dtype)
+    g = torch.randn(2, 2, J, generator=torch.Generator().manual_seed(1)).to(dtype).to(DEV)
+    d = g.double().cpu() * slope
+    _check(snn.rule_times_grad(g, times, k["history"], k["lengths"], k["repetition"], k["allowed"]), d, d.abs(), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,J", [(3, 65), (5, 2049), (3, 8195), (530, 9001), (600, 16387), (260, 16389), (3, 32769), (3, 40961), (300, 40967), (1100, 33000)])
+def test_tokens_from_the_ends_of_rows(rows, J, dtype):
+    """Nearly all of the chance lies with the last seven elements, under every rule."""
+    import snntc_amd as snn
+    gen = torch.Generator().manual_seed(J)
+    times = 20.0 + torch.rand(rows, J, generator=gen)
+    times[:, -7:] = torch.rand(rows, 7, generator=gen) - 5.0
+    times = times.to(dtype).to(DEV)
+    words = torch.randint(-(1 << 31), 1 << 31, (rows, (J + 31) // 32), generator=gen).to(torch.int32)
+    words[:, (J - 4) // 32] |= torch.tensor((1 << (J - 4) % 32), dtype=torch.int64).to(torch.int32)          # one of them is allowed
+    how = dict(history=torch.randint(J - 9, J, (rows, 11), generator=gen).to(DEV), prompts=torch.full((rows,), 3, device=DEV), repetition=1.2,
+               presence=0.3, frequency=0.1, delay=torch.randn(J, generator=gen).to(DEV), allowed=words.to(DEV))
+    ruled = snn.rule_times(times, **how).double()
+    lp = torch.log_softmax(-ruled / 0.9, -1)
+    cum = lp[:, -40:].exp().cumsum(-1)                                # what lies before the last forty has a chance of e^-20 40000 at most
+    seen = set()
+    for u in (0.02, 0.3, 0.6, 0.99):
+        tokens, logp = snn.choose_tokens(times, torch.full((rows,), u, device=DEV), 0.9, **how)
+        at = torch.searchsorted(cum, torch.full((rows, 1), u, dtype=torch.float64, device=DEV))[:, 0]
+        edges = torch.cat([torch.zeros_like(cum[:, :1]), cum], 1)
+        clear = ((edges - u).abs() > 1e-3).all(1)
+        assert torch.equal(tokens[clear], (J - 40 + at)[clear]) and bool(clear.float().mean() > 0.5)
+        ref = lp.gather(-1, tokens[:, None])[:, 0]
+        assert bool(((logp.double() - ref).abs() <= 2.0 ** -20 + 2.0 ** -23 * ref.abs()).all())
+        seen |= set((J - tokens).tolist())
+    assert seen <= set(range(1, 8))
+    assert torch.equal(snn.choose_tokens(times, None, 0.0, **how)[0], ruled.argmin(-1))
+
+
+@pytest.mark.parametrize("L", [65535, 65536, 70000])
+def test_occurrences_past_16_bits(L):
+    import snntc_amd as snn
+    times = 1.0 + torch.rand(1, 5000, device=DEV)
+    history = torch.full((1, L), 4321, device=DEV)
+    history[0, 17], history[0, 300] = 12, 13
+    got = snn.rule_times(times, history, frequency=2.0 ** -10)
+    want = times.clone()
+    want[0, 4321] += 2.0 ** -10 * (L - 2)
+    want[0, 12] += 2.0 ** -10
+    want[0, 13] += 2.0 ** -10
+    assert torch.equal(got, want)
+    assert int(snn.choose_tokens(times, None, 0.0, history, frequency=-1.0)[0]) == 4321
