@@ -659,7 +659,7 @@ def choose_tokens(times, uniform, temperature=1.0, history=None, lengths=None, p
     (tokens[...] int64, logp[...] float32).  uniform[...] (float32, from [0, 1)) decides: the token is the first whose running sum of p
     exceeds it.  temperature: a number, or float32 [...]; at 0 the earliest output is taken, the lowest index of equal ones, with its
     log-probability at temperature 1 (uniform may be None where the number is 0).  A row whose rules leave nothing, or with a NaN
-    among what they leave, gives token -1 and NaN.  The ruled times are not stored.  Not differentiable: see rule_times."""
+    or -infinity among what they leave, gives token -1 and NaN.  The ruled times are not stored.  Not differentiable: see rule_times."""
     return _lib.native().choose_tokens(times, uniform, temperature, history, lengths, prompts, repetition, presence, frequency, delay, allowed)
 
 
