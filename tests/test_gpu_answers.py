@@ -239,3 +239,24 @@ def test_a_sequence_that_nothing_is_allowed_for_has_no_weight():
     for a, b in zip(net.weights(), others.weights()):
         # (the sums over rows are in another order: at most 72 terms, each half a step off, of a gradient of a tenth the step's size)
         assert torch.allclose(a, b, rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_classifier_step_with_the_optimizer(bits):
+    """The recipe's step on images, whose gradients come from its own kernels, updated by this optimizer."""
+    import snntc_amd as snn
+    rng = np.random.default_rng(3)
+    layers = [snn.SNN_dense(12, 30, weight=(4.0 / 12 + rng.standard_normal((13, 30)) / 12 ** 0.5).astype(np.float32)),
+              snn.SNN_dense(30, 7, weight=(4.0 / 30 + rng.standard_normal((31, 7)) / 30 ** 0.5).astype(np.float32))]
+    net = torch.nn.Sequential(*layers).to(DEV)
+    opt = snn.optim.AdamW(net.parameters(), 1e-2, state_bits=bits, weight_decay=0.1, seed=2)
+    images, labels = torch.rand(64, 12, device=DEV), torch.randint(0, 7, (64,), device=DEV)
+    before = [p.detach().double() for p in net.parameters()]
+    loss, _ = snn.train.train_step(net, opt, images, labels, 7)
+    assert bool(torch.isfinite(loss))
+    for p, w in zip(net.parameters(), before):
+        # the first step: m / (1 - b1) is g and v / (1 - b2) its square; the change of at most lr is off by some steps of float32
+        g = p.grad.double()
+        want = w * (1 - 1e-3) - 1e-2 * g / (g.abs() + 1e-8)
+        assert float((p.detach().double() - want).abs().max()) <= 1e-2 * 2.0 ** -20 + 2.0 ** -23 * float(w.abs().max())
+    assert float(snn.train.train_step(net, opt, images, labels, 7)[0]) != float(loss)
