@@ -312,8 +312,8 @@ __device__ __forceinline__ void rule_piece(Piece<E, VEC>& p, const typename M::M
 }
 
 // Ruled times, or (GRAD) the gradient by the times: in = times or the upstream gradient.  The gradient reads times where a token
-// repeats only: their sign is all it needs.  Bound by memory: 4096 rows of 32000 bf16 times forward 112 us (545 MB, 4.9 TB/s; a copy of the times takes 98),
-// gradient 112 us (636 MB, 5.7 TB/s: lines of scattered times for their signs are 91 MB of it).
+// repeats only: their sign is all it needs.  Bound by memory: 4096 rows of 32000 bf16 times forward 110 us (545 MB, 4.9 TB/s; a copy of the times takes 98),
+// gradient 109 us (636 MB, 5.8 TB/s: lines of scattered times for their signs are 91 MB of it).
 template <typename E, int VEC, int WIDTH, int R, typename COUNT, bool STREAM>
 __global__ void __launch_bounds__(WIDTH)
 rule_kernel(const E* __restrict__ in, const E* __restrict__ times, E* __restrict__ out, RuleArgs a, int64_t rows, int J, int slices) {
@@ -551,7 +551,7 @@ __device__ __forceinline__ void store_choice(const ChooseArgs& a, unsigned r, co
 }
 
 // A slice of a row.  WHOLE: the slice is the row, and the row's token is found; else its wavefronts' parts go to `parts`.  Bound by vector instructions:
-// 4096 rows of 32000 bf16 times with delays and 256 tokens each take 79 us (281 MB, 3.6 TB/s, 83 % of the issue slots and the exponentials besides),
+// 4096 rows of 32000 bf16 times with delays and 256 tokens each take 77 us (281 MB, 3.7 TB/s, 84 % of the issue slots and the exponentials besides),
 // without rules 58 with the join.
 template <typename E, int VEC, int WIDTH, int R, typename COUNT, bool WHOLE>
 __global__ void __launch_bounds__(WIDTH)
@@ -646,8 +646,8 @@ int launch_rule_slices(const void* in, const void* times, void* out, const RuleA
 
 // Slices of 4096 elements, four wavefronts each, and of 2048 by one in rows of up to 8192 elements.  Rows with their gradient:
 //     slices                        2048, 1 wavefront   4096, 4   8192, 4   8192, 8
-//     2328 rows of 5003 f16 times         31.4 us         36.1
-//     4096 rows of 32000 bf16 times      233             220       224       220
+//     2328 rows of 5003 f16 times         29.1 us         35.3
+//     4096 rows of 32000 bf16 times      230             219       224       218
 template <typename COUNT>
 int launch_rules(const void* in, const void* times, int type, const RuleArgs& a, void* out, int64_t rows, int64_t J, hipStream_t stream) {
     return with_type(type, [&](auto e) -> int {
@@ -684,7 +684,7 @@ int launch_choose_slices(const void* times, const RuleArgs& a, const ChooseArgs&
     }
     {
         KernelTimerScope timer_("choose_join", stream);
-        // (a call on 4096 rows of 32000: 91 us with a wavefront for each, 96 with four; on 64 of 131072 with 2048 tokens: 23.6 and 21.0)
+        // (a call on 4096 rows of 32000: 89 us with a wavefront for each, 93 with four; on 64 of 131072 with 2048 tokens: 23.2 and 20.4)
         if (rows >= 256)
             hipLaunchKernelGGL((choose_join_kernel<E, VEC, R, COUNT, 64>), wide_grid(rows, 64), dim3(64), 0, stream,
                                static_cast<const E*>(times), a, c, parts, rows, (int)J, slices * kWaves);
@@ -731,8 +731,8 @@ int launch_choose(const void* times, int type, const RuleArgs& a, const ChooseAr
         if (J <= 256 * 32) return launch_choose_whole<E, 256, R, C>(times, a, c, rows, J, stream);
         // One launch of a workgroup for each row, or shorter workgroups that overlap better where there are many.  Of bf16 times, in us:
         //     rows         256 of 10000   256 of 32000   512 of 10000   512 of 32000   1024 of 32000   4096 of 32000
-        //     one launch        11.0           11.6           19.3           20.9            37.3           139.5
-        //     slices            14.6           16.8           16.9           22.9            32.3            91.8
+        //     one launch        11.2           12.2           19.8           20.8            36.7           138
+        //     slices            14.4           17.1           17.2           22.2            31.7            89
         if (J <= 1024 * 32 && (rows <= 256 || (rows <= 512 && J > 1024 * 16)))
             return launch_choose_whole<E, 1024, R, C>(times, a, c, rows, J, stream);
         if (J <= 1024 * 32) return launch_choose_slices<E, 512, R, C>(times, a, c, rows, J, parts, stream);
