@@ -443,7 +443,8 @@ struct Run {
         return p;
     }
     // The first element of the run whose running sum exceeds `rest`, the last possible one where rounding leaves none; -1 in
-    // a run without any.
+    // a run without any.  Sums over lanes are rounded in an order of their own: `run` may rise at a lane without a term, and run - sum need not
+    // be the lane before's `run`.  So only lanes and elements with a term are asked, and what is left in a lane is no less than 0.
     __device__ __forceinline__ int pick(double rest, float m, float k, float* value) {
         const float base = base_of(m);
 #pragma unroll
@@ -454,9 +455,9 @@ struct Run {
             for (int x = 0; x < VEC; ++x) sum += e[x] = term(v(i, x) - base, k);
             const float run = wave_scan(sum), all = of_lane(run, kWave - 1);
             if (!((double)all > rest)) { rest -= all; continue; }
-            const unsigned long long over = __ballot((double)run > rest);
-            const int owner = __ffsll(over) - 1;
-            double left = rest - (double)(run - sum);
+            const unsigned long long any = __ballot(sum > 0.0f), over = __ballot(sum > 0.0f && (double)run > rest);
+            const int owner = over ? __ffsll(over) - 1 : 63 - __clzll(any);
+            double left = fmax(rest - (double)(run - sum), 0.0);
             int at = -1, last = 0;
 #pragma unroll
             for (int x = 0; x < VEC; ++x) {
