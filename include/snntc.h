@@ -448,7 +448,9 @@ SNNTC_API int snntc_choose(const void* times, int times_type, const float* unifo
  * elements (the last may be fewer), ceil(n / 256) of them: its largest magnitude s.  Code c (of m: its low 7 bits, the 8th its sign) stands for
  *     s value(c) / value(largest code),   value(c) = c (c < 8),  (8 + c % 8) 2^(c / 8 - 1) (else)
  * A state's zero is code 0 and scale 0.  A value between two codes becomes the upper one with the chance of its place between them, a weight of
- * 16 bits likewise one of its two neighbours; the random bits follow from seed, step, t and the element alone.
+ * 16 bits likewise one of its two neighbours; the random bits follow from seed, step, t and the element alone.  paired: 0, or (any other) a first
+ * moment whose second moment's code is 0 is held as 0 too.  Rounded apart, each moment is right on average but not their quotient: an element
+ * far below its block's largest that has kept a first moment and lost its second moves by lr first / eps, hundreds of lr, once its gradient is 0.
  *   snntc_grad_norm       norm = sqrt of the sum of squares of all gradients (float32 on the device, the sum in 64 bits, the same on
  *                         every call).
  *   snntc_adamw_moments   first_out[t], second_out[t] (float32[n]) = what the codes stand for.
@@ -467,6 +469,7 @@ typedef struct snntc_adamw {
     const float* norm;
     double max_norm;
     uint64_t seed;
+    int paired;
 } snntc_adamw;
 SNNTC_API int snntc_grad_norm_workspace_bytes(const int64_t* n, int64_t count, size_t* bytes);
 SNNTC_API int snntc_grad_norm(const void* const* grads, const int* types, const int64_t* n, int64_t count, float* norm, void* workspace,

@@ -878,7 +878,8 @@ int snntc_adamw_update(void* const* w, const void* const* dw, void* const* first
         if (rc) return rc;
     }
     const AdamTensors a{w, dw, first, second, first_scale, second_scale, types, n};
-    const AdamNumbers p{how->lr, how->beta1, how->beta2, how->eps, how->weight_decay, how->max_norm, how->step, how->steps, how->norm, how->seed};
+    const AdamNumbers p{how->lr, how->beta1, how->beta2, how->eps, how->weight_decay, how->max_norm, how->step, how->steps, how->norm, how->seed,
+                        how->paired != 0};
     return launch_adamw(a, (int)count, p, workspace, static_cast<hipStream_t>(stream));
 }
 

@@ -2207,10 +2207,10 @@ Moments moments_in(PyObject* const* a) {
     return m;
 }
 
-// adamw_update(weights, gradients, first, second, first_scale, second_scale, step, lr, beta1, beta2, eps, weight_decay, norm, max_norm, seed)
+// adamw_update(weights, gradients, first, second, first_scale, second_scale, step, lr, beta1, beta2, eps, weight_decay, norm, max_norm, seed, paired)
 SNNTC_METHOD(py_adamw_update) {
     HANDLE_TH_ERRORS
-    arity(n, 15, "adamw_update");
+    arity(n, 16, "adamw_update");
     const std::vector<Tensor> ws = tensor_list(a[0], "params"), gs = tensor_list(a[1], "grads");
     const Moments m = moments_in(a + 2);
     snntc_adamw how{};
@@ -2222,6 +2222,8 @@ SNNTC_METHOD(py_adamw_update) {
     how.max_norm = double_arg(a[13]);
     how.seed = PyLong_AsUnsignedLongLongMask(a[14]);
     if (PyErr_Occurred()) throw python_error();
+    how.paired = PyObject_IsTrue(a[15]);
+    if (how.paired < 0) throw python_error();
     {
         NoGil nogil;
         at::AutoGradMode no_grad(false);

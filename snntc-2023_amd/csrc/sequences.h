@@ -128,6 +128,7 @@ struct AdamNumbers {
     int64_t* steps;                        // device: steps done so far
     const float* norm;                     // device, NULL: gradients are not clipped
     uint64_t seed;
+    bool paired;                           // 8 bits: no first moment beside a second of 0
 };
 size_t grad_norm_workspace(const int64_t* n, int64_t count);
 int launch_grad_norm(const void* const* g, const int* types, const int64_t* n, int count, float* norm, void* ws, hipStream_t stream);

@@ -74,7 +74,7 @@ class AdamW(ctypes.Structure):
     """snntc_adamw: the numbers of a step."""
     _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double),
                 ("weight_decay", ctypes.c_double), ("step", ctypes.c_int64), ("steps", ctypes.c_void_p), ("norm", ctypes.c_void_p),
-                ("max_norm", ctypes.c_double), ("seed", ctypes.c_uint64)]
+                ("max_norm", ctypes.c_double), ("seed", ctypes.c_uint64), ("paired", ctypes.c_int)]
 
 
 _lib = None

@@ -669,7 +669,7 @@ def grad_norm(grads):
 
 
 def adamw_update(params, grads, first, second, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, norm=None, max_norm=1.0,
-                 first_scale=None, second_scale=None, seed=0):
+                 first_scale=None, second_scale=None, seed=0, paired=False):
     """One AdamW step over all tensors in one launch (48 tensors of a type to a launch), in place:
         m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,
         w = w (1 - lr weight_decay) - lr / (1 - b1^step) m / (sqrt(v / (1 - b2^step)) + eps)
@@ -677,12 +677,14 @@ def adamw_update(params, grads, first, second, step, lr=1e-3, betas=(0.9, 0.999)
     first_scale, second_scale, float32 [ceil(n / 256)] (zeros to begin with).  step: the number of this step, from 1, or an int64
     device tensor with the number of steps done, which the call advances (for graphs).  norm: grad_norm(grads); gradients are scaled down
     to max_norm where it is larger, and nothing is changed where it is no finite number.  Codes and 16-bit weights are rounded up or
-    down by chance, from random bits that follow from seed, the step and the element's place."""
+    down by chance, from random bits that follow from seed, the step and the element's place.  paired: a first moment whose second moment's code
+    is 0 is held as 0 too.  Without it the two codes' quotient has no bound: where a block's gradients lie more than a hundredfold apart and
+    some are 0, an element can keep its first moment alone and move by lr m / eps, hundreds of lr (optim.AdamW pairs them)."""
     params, grads = list(params), list(grads)
     if params or grads:
         _lib.native().adamw_update(params, grads, list(first), list(second), None if first_scale is None else list(first_scale),
                                    None if second_scale is None else list(second_scale), step, lr, betas[0], betas[1], eps, weight_decay,
-                                   norm, max_norm, seed)
+                                   norm, max_norm, seed, paired)
 
 
 def adamw_moments(first, second, first_scale, second_scale):

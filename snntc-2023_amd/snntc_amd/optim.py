@@ -10,7 +10,8 @@ _BLOCK = 256                                             # elements of a state t
 class AdamW(torch.optim.Optimizer):
     """AdamW over all tensors of a group in one launch (see ops.adamw_update for the formula).
 
-      state_bits  32, or 8: codes with a scale for every 256 elements, a quarter of the memory
+      state_bits  32, or 8: codes with a scale for every 256 elements, a quarter of the memory.  An element whose second moment is too
+                  small for its block (2^-34 of the largest) has no first moment either, so that steps stay those of 32 bits in size
       max_norm    None, or what the norm over all gradients of a step is scaled down to; a step whose norm is no finite number then
                   changes nothing but its number.  `norm` is the last step's, on the device
       seed        of the random bits by which codes and 16-bit weights are rounded, from [0, 2^32)
@@ -104,7 +105,7 @@ class AdamW(torch.optim.Optimizer):
                 adamw_update([p.detach() for p in tensors], [p.grad for p in tensors], [s["first"] for s in states],
                              [s["second"] for s in states], number, lr=group["lr"], betas=group["betas"], eps=group["eps"],
                              weight_decay=group["weight_decay"], norm=self.norm, max_norm=1.0 if self.max_norm is None else self.max_norm,
-                             first_scale=scales[0], second_scale=scales[1], seed=self.seed + (call << 32))
+                             first_scale=scales[0], second_scale=scales[1], seed=self.seed + (call << 32), paired=self.state_bits == 8)
                 if not self.capturable:
                     for s in states:
                         s["step"] = number
@@ -124,6 +125,8 @@ class AdamW(torch.optim.Optimizer):
             if ("first_scale" in old) != (self.state_bits == 8):
                 raise ValueError(f"AdamW: the saved states are not of {self.state_bits} bits")
             state = {k: v.detach().to(p.device, copy=True) for k, v in old.items() if k != "step"}
+            if self.state_bits == 8:
+                state["first"].mul_(state["second"] != 0)           # (as the update leaves them; codes from elsewhere need not be so)
             step = int(old["step"])
             if self.capturable:
                 if (g, p.device, step) not in counters:

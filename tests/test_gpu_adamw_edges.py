@@ -1,0 +1,86 @@
+"""The optimizer with states in 8 bits where gradients of a block lie far apart."""
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_adamw import SIZES, _bits, _coded, _encode, _f64, _decode, _tensors, _expected, LR, B1, B2, EPS, DECAY
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def _steps(bits, r, rare, count, blocks=64):
+    """The largest single change of a weight, in learning rates, of blocks with one gradient of 1 and others of r, some of them 0."""
+    import snntc_amd as snn
+    gen = torch.Generator().manual_seed(3)
+    p = torch.nn.Parameter(torch.zeros(blocks * 256, device=DEV))
+    opt = snn.optim.AdamW([p], 1e-3, weight_decay=0.0, state_bits=bits, seed=5)
+    largest = 0.0
+    for _ in range(count):
+        g = r * torch.randn(p.numel(), generator=gen) * (torch.rand(p.numel(), generator=gen) >= rare)
+        g[::256] = 1.0
+        p.grad = g.to(DEV)
+        before = p.detach().clone()
+        opt.step()
+        largest = max(largest, float((p.detach() - before).abs().max()) / 1e-3)
+    return largest, p.detach().clone()
+
+
+@pytest.mark.parametrize("r", [1e-1, 1e-2, 1e-3, 1e-4, 1e-5, 1e-6])
+@pytest.mark.parametrize("rare,count", [(0.5, 200), (0.97, 200)])
+def test_steps_of_8_bit_states_are_bounded(r, rare, count):
+    """Of any gradients m <= (1 - b1) / sqrt((1 - b2) (1 - b1^2 / b2)) sqrt(v), 7.3 sqrt(v).  A rounding at most doubles what is held of m
+    and halves what is held of v: 7.3 x 2 sqrt 2, and (1 - b1) / sqrt(1 - b2) = 3.2 of the newest gradient, 24 learning rates."""
+    eight, moved = _steps(8, r, rare, count)
+    full, whole = _steps(32, r, rare, count)
+    assert full <= 7.3 and eight <= 24.0, (eight, full)
+    # no weight drifts further than it would if each of its steps were the largest that 32 bits took
+    assert float(moved.abs().max()) <= 1e-3 * count * full
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_codes_of_paired_states(dtype):
+    """Blocks in which half of the second moments are too small for their block: the definition's codes, first ones with their second."""
+    import snntc_amd as snn
+    ws, gs, _, _ = _tensors(2, dtype)
+    m, v, ms, vs = _coded(3, SIZES)
+    gen = torch.Generator().manual_seed(8)
+    for g, second in zip(gs, v):
+        small = (torch.rand(g.shape, generator=gen) < 0.5).to(DEV)
+        g.mul_(torch.where(small, 2e-5, 1.0))
+        second.mul_(~small)
+    before = [(_f64(w), _f64(g), _decode(a, c, "m"), _decode(b, d, "v")) for w, g, a, b, c, d in zip(ws, gs, m, v, ms, vs)]
+    apart = [[x.clone() for x in t] for t in (ws, m, v, ms, vs)]
+    snn.adamw_update(ws, gs, m, v, 4, LR, (B1, B2), EPS, DECAY, None, 1.0, ms, vs, 6, True)
+    snn.adamw_update(apart[0], gs, apart[1], apart[2], 4, LR, (B1, B2), EPS, DECAY, None, 1.0, apart[3], apart[4], 6)
+    dropped = 0
+    for i, (w, g, a, b) in enumerate(before):
+        assert all(torch.equal(x[i], y[i]) for x, y in zip((ws, v, ms, vs), (apart[0], *apart[2:])))
+        assert torch.equal(m[i], torch.where(v[i] == 0, 0, apart[1][i]))
+        if not len(w):
+            continue
+        _, m1, v1, _, _ = _expected(w, g, a, b, 4)
+        bits = _bits(len(w), 6, 4, i)
+        second, _ = _encode(v1, (bits >> np.uint32(16)).astype(np.float64), "v")
+        first, _ = _encode(m1, (bits & np.uint32(0xFFFF)).astype(np.float64), "m")
+        got = m[i].cpu().numpy().reshape(-1)
+        assert np.array_equal(v[i].cpu().numpy().reshape(-1), second)
+        assert np.array_equal(np.where(got == 128, 0, got), np.where((second == 0) | (first == 128), 0, first))
+        dropped += int(((second == 0) & (first % 128 != 0)).sum())
+    assert dropped > 1000
+
+
+def test_states_from_elsewhere_are_paired_when_they_are_loaded():
+    import snntc_amd as snn
+    p = torch.nn.Parameter(torch.ones(700, device=DEV))
+    opt = snn.optim.AdamW([p], 1e-3, weight_decay=0.0, state_bits=8)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    saved = opt.state_dict()
+    saved["state"][0]["second"][10:20] = 0                       # as an update that rounds them apart can leave them
+    again = snn.optim.AdamW([p], 1e-3, weight_decay=0.0, state_bits=8)
+    again.load_state_dict(saved)
+    before = p.detach().clone()
+    p.grad = torch.zeros_like(p)
+    again.step()
+    assert float((p.detach() - before).abs().max()) <= 1e-3 and bool((p.detach() == before)[10:20].all())
