@@ -33,6 +33,11 @@ class AdamW(torch.optim.Optimizer):
         self.norm = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
+    def __getstate__(self):
+        """The base class carries weights, states and groups into a copy; what this class adds goes with them, but not the last norm."""
+        own = {k: getattr(self, k) for k in ("state_bits", "max_norm", "seed", "capturable")}
+        return {**super().__getstate__(), **own, "norm": None}
+
     def _begin(self, p, steps):
         """The state of a tensor that has its first gradient."""
         zeros = lambda n, dtype: torch.zeros(n, dtype=dtype, device=p.device)                   # noqa: E731

@@ -84,3 +84,38 @@ def test_states_from_elsewhere_are_paired_when_they_are_loaded():
     p.grad = torch.zeros_like(p)
     again.step()
     assert float((p.detach() - before).abs().max()) <= 1e-3 and bool((p.detach() == before)[10:20].all())
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("capturable", [False, True])
+def test_copies_of_an_optimizer_go_on(bits, capturable):
+    """Copied, or written and read back, between two steps: its own numbers, states and counters, as the one it was copied from."""
+    import copy
+    import io
+    import pickle
+    import snntc_amd as snn
+    gen = torch.Generator().manual_seed(1)
+    ps = [torch.nn.Parameter(torch.randn(n, generator=gen).to(DEV)) for n in (300, 7)]
+    gs = [[torch.randn(p.shape, generator=gen).to(DEV) for p in ps] for _ in range(4)]
+    opt = snn.optim.AdamW(ps, 1e-2, state_bits=bits, max_norm=0.5, seed=9, capturable=capturable)
+
+    def go(opt, steps):
+        for k in steps:
+            for p, g in zip(opt.param_groups[0]["params"], gs[k]):
+                p.grad = g.clone()
+            opt.step()
+        return [p.detach().clone() for p in opt.param_groups[0]["params"]]
+
+    go(opt, (0, 1))
+    saved = copy.deepcopy(opt.state_dict())                     # (by itself it goes on with the optimizer)
+    copies = [copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))]
+    torch.save(opt, buf := io.BytesIO())
+    copies.append(torch.load(io.BytesIO(buf.getvalue()), weights_only=False))
+    want = go(opt, (2, 3))
+    for other in copies:
+        assert other.norm is None and other.param_groups[0]["params"][0] is not ps[0]
+        got = go(other, (2, 3))
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(other.norm, opt.norm)
+        assert [int(s["step"]) for s in other.state.values()] == [4, 4]
+    copies[0].load_state_dict(saved)
+    assert [int(s["step"]) for s in copies[0].state.values()] == [2, 2]

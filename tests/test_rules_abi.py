@@ -143,3 +143,14 @@ def test_the_optimizer_refuses_numbers_that_mean_nothing():
     for wrong in ({"max_norm": 0}, {"max_norm": -1.0}, {"max_norm": float("nan")}, {"seed": -1}, {"seed": 1 << 32}, {"state_bits": 16}):
         with pytest.raises(ValueError):
             snn.optim.AdamW(w, **wrong)
+
+
+def test_a_copied_optimizer_keeps_its_numbers():
+    import copy
+    import pickle
+    import snntc_amd as snn
+    opt = snn.optim.AdamW([torch.nn.Parameter(torch.ones(3))], state_bits=8, max_norm=0.5, seed=9, capturable=True)
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert (other.state_bits, other.max_norm, other.seed, other.capturable, other.norm) == (8, 0.5, 9, True, None)
+        assert other.step(lambda: 3) == 3
+        other.load_state_dict(opt.state_dict())
