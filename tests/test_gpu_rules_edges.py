@@ -47,3 +47,25 @@ def test_draws_next_to_a_border_are_allowed(J, n, rows, width, dtype):
             at, upto = part.double() * total, cum[r, tokens]
             slack = 66 * 2.0 ** -24 * total
             assert bool(((upto - p[r, tokens] - slack <= at) & (at <= upto + slack)).all())
+
+
+@pytest.mark.parametrize("J", [3, 700, 5000, 20000, 40000])
+@pytest.mark.parametrize("rows", [6, 600])
+def test_times_whose_quotient_by_the_temperature_is_no_float(J, rows):
+    """Differences count, whatever their quotient: a far earlier time is drawn for sure, equal ones alike; times of infinity never are."""
+    import snntc_amd as snn
+    gen = torch.Generator().manual_seed(J)
+    u = torch.rand(rows, generator=gen).to(DEV)
+    at = torch.randint(0, J, (rows,), generator=gen).to(DEV)
+    for early, late, temperature in ((1e10, 2e10, 1e-29), (1e30, 2e30, 1e-10), (-1e38, 3e38, 1.0), (-3e38, 3e38, 0.5), (2.0, float("inf"), 1e-20)):
+        times = torch.full((rows, J), late, device=DEV)
+        times[torch.arange(rows, device=DEV), at] = early
+        tokens, logp = snn.choose_tokens(times, u, temperature)
+        assert torch.equal(tokens, at) and bool((logp == 0).all())
+    for time, temperature in ((1e38, 0.01), (3e38, 1e-29), (-1e38, 1e-3)):
+        times = torch.full((rows, J), time, device=DEV)
+        times[:, 1::2] = float("inf")
+        tokens, logp = snn.choose_tokens(times, u, temperature)
+        n = (J + 1) // 2
+        # equal terms of 1: sums of whole numbers are exact
+        assert torch.equal(tokens, 2 * (u.double() * n).floor().long()) and bool((logp.double() + torch.log(torch.tensor(n, dtype=torch.float64))).abs().max() <= 2.0 ** -20)
