@@ -405,6 +405,7 @@ SNNTC_API int snntc_loss_total(const float* loss, const float* weight, float* to
  *   snntc_rule_times           out[rows,J], of times' type; must not overlap times.
  *   snntc_rule_times_backward  dtimes_j = grad_j times repetition, over it, or as it is, as times_j was; 0 where not allowed.  times may be
  *                              NULL where history is, or no sequence's repetition differs from 1.  presence, frequency, prompts and delay are not read.
+ *                              dtimes must not overlap grad or times.
  *   snntc_choose               tokens[r] (int64): with p = softmax(-out[r] / T), the first j whose running sum of p exceeds uniform[r] of the
  *                              whole (uniform below 0 or NaN counts as 0; from 1 on: the last possible j), logp[r] = log p_j.  T = temperature[r], or
  *                              NULL and temperature_all.  T below 1e-30: the earliest output, the lowest index of equal ones, with its
@@ -413,7 +414,7 @@ SNNTC_API int snntc_loss_total(const float* loss, const float* weight, float* to
  *                              of +infinity, has no chance.  Where nothing is possible (all masked or infinite), a time that is allowed is NaN or
  *                              -infinity, or T is negative or no finite number: token -1 and logp NaN.  rules may be NULL.
  * Errors: a negative size, an unknown type, a NULL required pointer, J = 0 with rows, history_rows that do not divide rows, delay_rows or
- * allowed_rows neither 1 nor rows, a repetition_all that is not positive, penalties or a temperature_all that are not finite or (this) below 0 -> BAD_ARGUMENT;
+ * allowed_rows neither 1 nor rows, a result of the first two that overlaps times or grad, a repetition_all that is not positive, penalties or a temperature_all that are not finite or (this) below 0 -> BAD_ARGUMENT;
  * more than 2^24 - 1 rows, J or history_len above 2^30 -> TOO_LARGE; a workspace below snntc_choose_workspace_bytes -> WORKSPACE.
  * ------------------------------------------------------------------------------------------- */
 typedef struct snntc_rules {

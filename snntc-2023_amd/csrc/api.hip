@@ -765,12 +765,21 @@ static int rule_args(const snntc_rules* rules, int64_t rows, int64_t J, const ch
     return SNNTC_OK;
 }
 
+// Ends of rows are read and written by more than one lane, and by more than one workgroup: a result in place of an input would be ruled twice.
+static int apart(const void* out, const void* in, int64_t rows, int64_t J, int type, const char* who) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(out), b = reinterpret_cast<uintptr_t>(in), bytes = (uintptr_t)(rows * J) * type_bytes(type);
+    if (in && a < b + bytes && b < a + bytes) return fail(SNNTC_ERR_BAD_ARGUMENT, "%s: the result overlaps an input", who);
+    return SNNTC_OK;
+}
+
 int snntc_rule_times(const void* times, int times_type, const snntc_rules* rules, void* out, int64_t rows, int64_t J, void* stream) {
     RuleArgs a;
     int rc = choice_check(rows, J, times_type, "snntc_rule_times");
     if (!rc) rc = rule_args(rules, rows, J, "snntc_rule_times", &a);
     if (rc || rows == 0) return rc;
     if (!times || !out) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_rule_times: null pointer");
+    rc = apart(out, times, rows, J, times_type, "snntc_rule_times");
+    if (rc) return rc;
     return launch_rule_times(times, times_type, a, out, rows, J, static_cast<hipStream_t>(stream));
 }
 
@@ -782,6 +791,9 @@ int snntc_rule_times_backward(const void* grad, const void* times, int times_typ
     if (rc || rows == 0) return rc;
     if (!a.repetition && a.rep == 1.0f) a.history = nullptr;
     if (!grad || !dtimes || (a.history && !times)) return fail(SNNTC_ERR_BAD_ARGUMENT, "snntc_rule_times_backward: null pointer");
+    rc = apart(dtimes, grad, rows, J, times_type, "snntc_rule_times_backward");
+    if (!rc && a.history) rc = apart(dtimes, times, rows, J, times_type, "snntc_rule_times_backward");
+    if (rc) return rc;
     return launch_rule_times_backward(grad, times, times_type, a, dtimes, rows, J, static_cast<hipStream_t>(stream));
 }
 

@@ -154,3 +154,16 @@ def test_a_copied_optimizer_keeps_its_numbers():
         assert (other.state_bits, other.max_norm, other.seed, other.capturable, other.norm) == (8, 0.5, 9, True, None)
         assert other.step(lambda: 3) == 3
         other.load_state_dict(opt.state_dict())
+
+
+@pytest.mark.parametrize("ty,size", [(0, 4), (1, 2), (2, 2)])
+def test_results_in_place_of_an_input_are_refused(lib, ty, size):
+    """Several lanes or workgroups share the ends of rows, so a call in place would rule them twice."""
+    at = lambda n: ctypes.c_void_p((1 << 30) + n)                                       # noqa: E731
+    far, whole = at(1 << 33), 4 * 70000 * size
+    for shift in (0, 2, -2, whole - 2, 2 - whole):
+        assert lib.snntc_rule_times(at(0), ty, _rules(), at(shift), 4, 70000, None) == BAD
+        assert b"overlaps" in lib.snntc_last_error()
+        for grad, times in ((at(0), far), (far, at(0))):
+            assert lib.snntc_rule_times_backward(grad, times, ty, _rules(), at(shift), 4, 70000, None) == BAD
+            assert b"overlaps" in lib.snntc_last_error()
