@@ -457,7 +457,7 @@ SNNTC_API int snntc_choose(const void* times, int times_type, const float* unifo
  *                         every call).
  *   snntc_adamw_moments   first_out[t], second_out[t] (float32[n]) = what the codes stand for.
  * All arrays but `steps` and `norm` are HOST arrays of `count` entries, read before the call returns; tensors of n[t] = 0 are skipped.  No two of
- * the written tensors may overlap, nor a gradient one of them.  The workspace of snntc_adamw_update (SNNTC_ADAMW_WORKSPACE_BYTES) is needed with `steps` only.
+ * the written tensors (steps is one) may overlap, nor a gradient or norm one of them.  The workspace of snntc_adamw_update (SNNTC_ADAMW_WORKSPACE_BYTES) is needed with `steps` only.
  * Errors: a negative count or size, an unknown type, a NULL required pointer, one scale array without the other, lr or weight_decay not
  * finite or negative, a beta outside [0, 1), an eps below the smallest normal float32, a step below 1, a max_norm that is not positive -> BAD_ARGUMENT; n[t] above
  * 2^34 -> TOO_LARGE; a workspace that is missing or too small -> WORKSPACE.

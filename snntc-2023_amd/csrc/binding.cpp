@@ -735,9 +735,11 @@ void no_overlap(std::vector<Span>& spans) {
         any = std::max(any, s.to);
     }
 }
+void add_span(std::vector<Span>& spans, const Tensor& t, bool written) {
+    if (t.defined() && t.numel()) spans.push_back({static_cast<const char*>(t.data_ptr()), static_cast<const char*>(t.data_ptr()) + t.nbytes(), written});
+}
 void add_spans(std::vector<Span>& spans, const TensorList& list, bool written) {
-    for (const Tensor& t : list.keep)
-        if (t.numel()) spans.push_back({static_cast<const char*>(t.data_ptr()), static_cast<const char*>(t.data_ptr()) + t.nbytes(), written});
+    for (const Tensor& t : list.keep) add_span(spans, t, written);
 }
 
 struct Moments { std::vector<Tensor> first, second, first_scale, second_scale; bool coded; };
@@ -773,11 +775,6 @@ void adamw_update(const std::vector<Tensor>& ws, const std::vector<Tensor>& gs, 
         add_written(w, ws[i], ws[0], ws[i].scalar_type(), ws[i].numel(), "weight", i);
     }
     moment_lists(moments, ws, state);
-    std::vector<Span> spans;
-    spans.reserve(6 * ws.size() + 2);
-    add_spans(spans, w, true); add_spans(spans, g, false);
-    for (const TensorList& s : state) add_spans(spans, s, true);
-    no_overlap(spans);
     Tensor scratch_ws;
     if (steps.defined()) {
         on_device(steps, ws[0], "adamw", "step", 0);
@@ -790,6 +787,12 @@ void adamw_update(const std::vector<Tensor>& ws, const std::vector<Tensor>& gs, 
         TORCH_CHECK_TYPE(norm.scalar_type() == at::kFloat && norm.numel() == 1, "adamw: norm is one float32");
         how.norm = f32(norm);
     }
+    std::vector<Span> spans;
+    spans.reserve(6 * ws.size() + 2);
+    add_spans(spans, w, true); add_spans(spans, g, false);
+    for (const TensorList& s : state) add_spans(spans, s, true);
+    add_span(spans, steps, true); add_span(spans, norm, false);
+    no_overlap(spans);
     const auto floats = [](TensorList& l) { return reinterpret_cast<float* const*>(l.at.data()); };
     check(lib.snntc_adamw_update(w.at.data(), g.at.data(), state[0].at.data(), state[1].at.data(), moments.coded ? floats(state[2]) : nullptr,
                                  moments.coded ? floats(state[3]) : nullptr, g.types.data(), w.n.data(), (int64_t)w.n.size(), &how, raw(scratch_ws),

@@ -119,3 +119,21 @@ def test_copies_of_an_optimizer_go_on(bits, capturable):
         assert [int(s["step"]) for s in other.state.values()] == [4, 4]
     copies[0].load_state_dict(saved)
     assert [int(s["step"]) for s in copies[0].state.values()] == [2, 2]
+
+
+def test_numbers_on_the_device_lie_apart_from_what_is_updated():
+    """A norm or a step's number in the memory of a weight, a state or each other: every workgroup would read what others write."""
+    import snntc_amd as snn
+    buf = torch.ones(8, 6, device=DEV)
+    w, g, m, v, a, b = (buf[i] for i in range(6))
+    step = torch.zeros(1, dtype=torch.int64, device=DEV)
+    number = lambda t: t[2:4].view(torch.int64)                                         # noqa: E731
+    call = lambda step=1, norm=None: snn.adamw_update([w], [g], [m], [v], step, norm=norm)               # noqa: E731
+    for how in (dict(norm=w[3]), dict(norm=m[0]), dict(norm=v[5]), dict(step=number(w)), dict(step=number(g)), dict(step=number(v)),
+                dict(step=number(a), norm=a[3])):
+        with pytest.raises(ValueError, match="overlap"):
+            call(**how)
+    assert bool((buf == 1).all())
+    call(step, a[0])
+    call(number(b.zero_()), g[0])                                # beside them, or read on both sides: as ever
+    assert int(step) == int(number(b)) == 1
