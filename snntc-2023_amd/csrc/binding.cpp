@@ -1247,12 +1247,11 @@ Tensor preference_layer(const ChoiceArgs& a, const Tensor& ref, float beta, floa
 struct RuleNode : public Node {
     SavedVariable times, history, lengths, repetition, allowed;
     bool has_history, has_lengths, has_repetition, has_allowed;
-    Tensor shape;                                            // without penalties: in the times' place, whose values the gradient does not need
     float repetition_all;
     std::string name() const override { return "TimeRulesBackward"; }
     void release_variables() override {
         std::lock_guard<std::mutex> lock(mutex_);
-        times.reset_data(); history.reset_data(); lengths.reset_data(); repetition.reset_data(); allowed.reset_data(); shape.reset();
+        times.reset_data(); history.reset_data(); lengths.reset_data(); repetition.reset_data(); allowed.reset_data();
     }
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
@@ -1266,11 +1265,12 @@ struct RuleNode : public Node {
             if (has_repetition) in.repetition.each = repetition.unpack();
         }
         if (has_allowed) in.allowed = allowed.unpack();
-        const Tensor t = has_history ? times.unpack() : shape;
         variable_list out(1);
         {
             at::AutoGradMode no_grad(false);
-            out[0] = rule_times_grad(grads[0], rule_set(t, in));
+            // without penalties the gradient reads no times: a tensor of their shape and type stands for them, and none of them is held
+            const Tensor g = grads[0].contiguous();
+            out[0] = rule_times_grad(g, rule_set(has_history ? times.unpack() : g, in));
         }
         return once(std::move(out), *this, grads, "rule_times");
     }
@@ -1294,8 +1294,6 @@ Tensor rule_layer(const RuleSet& r, const RuleIn& in) {
     if (node->has_history) {
         node->times = SavedVariable(r.times, false);
         node->history = SavedVariable(r.history, false);
-    } else {
-        node->shape = r.times.detach();
     }
     if (node->has_lengths) node->lengths = SavedVariable(r.lengths, false);
     if (node->has_repetition) node->repetition = SavedVariable(r.repetition, false);

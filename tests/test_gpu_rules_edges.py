@@ -69,3 +69,23 @@ def test_times_whose_quotient_by_the_temperature_is_no_float(J, rows):
         n = (J + 1) // 2
         # equal terms of 1: sums of whole numbers are exact
         assert torch.equal(tokens, 2 * (u.double() * n).floor().long()) and bool((logp.double() + torch.log(torch.tensor(n, dtype=torch.float64))).abs().max() <= 2.0 ** -20)
+
+def test_the_gradient_without_penalties_does_not_hold_the_times():
+    """Delays and masks alone: the gradient reads neither the times nor their memory."""
+    import snntc_amd as snn
+    words = snn.pack_allowed(torch.arange(4096, device=DEV) % 3 > 0)
+    leaf = torch.rand(1024, 4096, device=DEV, requires_grad=True)
+    size = leaf.numel() * leaf.element_size()
+
+    def ruled():
+        return snn.rule_times(leaf * 1.0, allowed=words, delay=torch.ones(4096, device=DEV))
+
+    ruled()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    out = ruled()
+    assert torch.cuda.memory_allocated() - before < 1.5 * size               # the result, not the times beside it
+    g = torch.rand_like(out)
+    for grad in (g, g.t().contiguous().t(), g[:1].expand_as(g)):
+        (got,) = torch.autograd.grad(out, [leaf], [grad], retain_graph=True)
+        assert torch.equal(got, torch.where(torch.arange(4096, device=DEV) % 3 > 0, grad, 0.0))
