@@ -180,3 +180,24 @@ def test_every_device_source_of_a_workload_is_counted():
     assert set(bench.COUNTED_SOURCES) == with_kernels
     with open(os.path.join(folder, "api.hip")) as f:
         assert "__global__" not in f.read()
+
+
+def test_no_kernel_with_readings_lives_in_a_source_that_is_not_counted():
+    """In subfolders too: what launches a kernel under a name that has readings is in the digest."""
+    sys.path.insert(0, ROOT)
+    import json
+    import re
+    import bench
+    with open(bench.COUNTERS_FILE) as f:
+        read = {kernel for kernels in json.load(f)["workloads"].values() for kernel in kernels}
+    folder = os.path.join(ROOT, "snntc-2023_amd", "csrc")
+    names = {}
+    for at, _, files in os.walk(folder):
+        for n in files:
+            if n.endswith((".hip", ".h")):
+                with open(os.path.join(at, n)) as f:
+                    launched = [line for line in f.read().split("\n") if "KernelTimerScope timer_(" in line]
+                names[os.path.relpath(os.path.join(at, n), folder)] = {q for line in launched for q in re.findall(r'"(\w+)"', line)}
+    assert os.path.join("policy", "rules.hip") in names and "choose" in names[os.path.join("policy", "rules.hip")]
+    for source, launched in names.items():
+        assert source in bench.COUNTED_SOURCES or not launched & read, (source, launched & read)
