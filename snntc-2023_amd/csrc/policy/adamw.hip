@@ -14,7 +14,7 @@
 // The two moments of an element are rounded apart.  One far below its block's largest can so keep a first moment (down to 2^-18 of the largest)
 // and lose its second (below 2^-34): its next step without a gradient is then lr m / eps.  `paired` drops the first moment
 // with the second.  Largest step in 200, gradients 1e-1 .. 1e-6 of their block's largest and half of them or 97 % 0: 320 .. 1830 lr without, 1.3 .. 2.0 lr
-// with, 1.3 .. 1.8 lr of states in 32 bits.
+// with, 1.3 .. 1.8 lr of states in 32 bits.  It takes 2 % (68 M bf16 weights 155 -> 159 us).
 // A double's upper word with 16 random bits and a half added below its third binary digit is that rounding.  Moments are therefore 64
 // bits wide between the codes: next to a border a sum in 32 bits would leave another code than the definition.
 // 16-bit weights are rounded in the same way and for the same reason: a step of a thousandth of a weight is less than half of what
@@ -193,7 +193,7 @@ __device__ __forceinline__ float stepped(float w, float m, float v, float keep, 
     return fmaf(-rate * m, __builtin_amdgcn_rcpf(root(v * second) + eps), w * keep);
 }
 
-// States in float32.  Bound by memory: 279 us for 68 M float32 weights, 1909 MB at 6.9 TB/s.
+// States in float32.  Bound by memory: 281 us for 68 M float32 weights, 1909 MB at 6.8 TB/s; 231 for bf16 or f16 weights, 1500 MB at 6.5 TB/s.
 template <bool WHOLE, typename E, bool PAST>
 __device__ __forceinline__ void adamw_run(const AdamTable& tab, const AdamScalars& s, int t, long long begin) {
     const long long n = tab.n[t], e0 = begin + threadIdx.x % kWave * 4;
@@ -243,8 +243,9 @@ __device__ __forceinline__ unsigned wave_max(unsigned v) { return wave_join(v, 0
 // A magnitude's bits: ordered as magnitudes are, NaN above all.
 __device__ __forceinline__ unsigned magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
-// States in 8 bits: a wavefront owns kTimes blocks of 256 elements.  Memory and vector instructions bind alike: 161 us for 68 M float32 weights, 1102 MB at
-// 6.9 TB/s, with instructions in 85 % of the issue slots (75 for an element of each lane).  Both blocks' maxima in one tree save a tenth of these, but
+// States in 8 bits: a wavefront owns kTimes blocks of 256 elements.  Memory and vector instructions bind alike: 159 us for 68 M float32 weights, 1102 MB at
+// 6.9 TB/s, with instructions in 84 % of the issue slots (75 for an element of each lane); instructions alone where weights are of 16 bits, 155 us (bf16) and 166
+// (f16) for 682 MB.  Both blocks' maxima in one tree save a tenth of these, but
 // hold 134 registers instead of 84, and the call is slower (322 -> 330 us with norm and moments).
 // Copies of a tensor's last element leave a block's maxima as they are.
 template <bool WHOLE, typename E, bool PAST>
@@ -320,7 +321,7 @@ __global__ void adamw_advance_kernel(long long* __restrict__ steps, AdamStep* __
     *at = AdamStep{lr / (1.0 - pow(b1, (double)t)), 1.0 / (1.0 - pow(b2, (double)t)), (unsigned)t};
 }
 
-// Both moments from their codes, float32.  Bound by memory: 110 us for 68 M, 691 MB at 6.3 TB/s.
+// Both moments from their codes, float32.  Bound by memory: 111 us for 68 M, 691 MB at 6.2 TB/s.
 struct MomentTable {
     const unsigned char* m[kMostTensors];
     const unsigned char* v[kMostTensors];

@@ -312,8 +312,8 @@ __device__ __forceinline__ void rule_piece(Piece<E, VEC>& p, const typename M::M
 }
 
 // Ruled times, or (GRAD) the gradient by the times: in = times or the upstream gradient.  The gradient reads times where a token
-// repeats only: their sign is all it needs.  Bound by memory: 4096 rows of 32000 bf16 times forward 110 us (545 MB, 4.9 TB/s; a copy of the times takes 98),
-// gradient 109 us (636 MB, 5.8 TB/s: lines of scattered times for their signs are 91 MB of it).
+// repeats only: their sign is all it needs.  Bound by memory: 4096 rows of 32000 bf16 times forward 111 us (545 MB, 4.9 TB/s; a copy of the times takes 98),
+// gradient 110 us (636 MB, 5.8 TB/s: lines of scattered times for their signs are 91 MB of it).
 template <typename E, int VEC, int WIDTH, int R, typename COUNT, bool STREAM>
 __global__ void __launch_bounds__(WIDTH)
 rule_kernel(const E* __restrict__ in, const E* __restrict__ times, E* __restrict__ out, RuleArgs a, int64_t rows, int J, int slices) {
@@ -645,7 +645,8 @@ int launch_rule_slices(const void* in, const void* times, void* out, const RuleA
     return SNNTC_OK;
 }
 
-// Slices of 4096 elements, four wavefronts each, and of 2048 by one in rows of up to 8192 elements.  Rows with their gradient:
+// Slices of 4096 elements, four wavefronts each, and of 2048 by one in rows of up to 8192 elements (a border between the two lengths that were measured).
+// Rows with their gradient:
 //     slices                        2048, 1 wavefront   4096, 4   8192, 4   8192, 8
 //     2328 rows of 5003 f16 times         29.1 us         35.3
 //     4096 rows of 32000 bf16 times      230             219       224       218
@@ -685,7 +686,8 @@ int launch_choose_slices(const void* times, const RuleArgs& a, const ChooseArgs&
     }
     {
         KernelTimerScope timer_("choose_join", stream);
-        // (a call on 4096 rows of 32000: 89 us with a wavefront for each, 93 with four; on 64 of 131072 with 2048 tokens: 23.2 and 20.4)
+        // (a call on 4096 rows of 32000: 89 us with a wavefront for each, 93 with four; on 64 of 131072 with 2048 tokens: 23.2 and 20.4; the border,
+        // a row for each CU, lies between them)
         if (rows >= 256)
             hipLaunchKernelGGL((choose_join_kernel<E, VEC, R, COUNT, 64>), wide_grid(rows, 64), dim3(64), 0, stream,
                                static_cast<const E*>(times), a, c, parts, rows, (int)J, slices * kWaves);

@@ -678,7 +678,7 @@ def adamw_update(params, grads, first, second, step, lr=1e-3, betas=(0.9, 0.999)
     device tensor with the number of steps done, which the call advances (for graphs).  norm: grad_norm(grads); gradients are scaled down
     to max_norm where it is larger, and nothing is changed where it is no finite number.  Codes and 16-bit weights are rounded up or
     down by chance, from random bits that follow from seed, the step and the element's place.  paired: a first moment whose second moment's code
-    is 0 is held as 0 too.  Without it the two codes' quotient has no bound: where a block's gradients lie more than a hundredfold apart and
+    is 0 is held as 0 too.  Without it the two codes' quotient has no bound: where a block's gradients lie more than tenfold apart and
     some are 0, an element can keep its first moment alone and move by lr m / eps, hundreds of lr (optim.AdamW pairs them)."""
     params, grads = list(params), list(grads)
     if params or grads:
