@@ -762,9 +762,10 @@ void moment_lists(const Moments& m, const std::vector<Tensor>& sizes, TensorList
 void adamw_update(const std::vector<Tensor>& ws, const std::vector<Tensor>& gs, const Moments& moments, const Tensor& steps, const Tensor& norm,
                   snntc_adamw how) {
     TORCH_CHECK_VALUE(ws.size() == gs.size(), "adamw: ", ws.size(), " weight tensors but ", gs.size(), " gradients");
-    if (ws.empty()) return;
-    on_device(ws[0], ws[0], "adamw", "weight", 0);
-    const c10::DeviceGuard guard(ws[0].device());
+    const Tensor& with = ws.empty() ? steps : ws[0];            // (no tensors: a step's number on the device still counts)
+    if (!with.defined()) return;
+    on_device(with, with, "adamw", ws.empty() ? "step" : "weight", 0);
+    const c10::DeviceGuard guard(with.device());
     TensorList w, state[4];
     const TensorList g = gradients(gs, "adamw");
     w.reserve(ws.size());
@@ -777,13 +778,13 @@ void adamw_update(const std::vector<Tensor>& ws, const std::vector<Tensor>& gs, 
     moment_lists(moments, ws, state);
     Tensor scratch_ws;
     if (steps.defined()) {
-        on_device(steps, ws[0], "adamw", "step", 0);
+        on_device(steps, with, "adamw", "step", 0);
         TORCH_CHECK_TYPE(steps.scalar_type() == at::kLong && steps.numel() == 1, "adamw: a step on the device is one int64");
         how.steps = i64(steps);
-        scratch_ws = scratch(ws[0], SNNTC_ADAMW_WORKSPACE_BYTES);
+        scratch_ws = scratch(with, SNNTC_ADAMW_WORKSPACE_BYTES);
     }
     if (norm.defined()) {
-        on_device(norm, ws[0], "adamw", "norm", 0);
+        on_device(norm, with, "adamw", "norm", 0);
         TORCH_CHECK_TYPE(norm.scalar_type() == at::kFloat && norm.numel() == 1, "adamw: norm is one float32");
         how.norm = f32(norm);
     }
@@ -796,7 +797,7 @@ void adamw_update(const std::vector<Tensor>& ws, const std::vector<Tensor>& gs, 
     const auto floats = [](TensorList& l) { return reinterpret_cast<float* const*>(l.at.data()); };
     check(lib.snntc_adamw_update(w.at.data(), g.at.data(), state[0].at.data(), state[1].at.data(), moments.coded ? floats(state[2]) : nullptr,
                                  moments.coded ? floats(state[3]) : nullptr, g.types.data(), w.n.data(), (int64_t)w.n.size(), &how, raw(scratch_ws),
-                                 bytes_of(scratch_ws), stream_of(ws[0])));
+                                 bytes_of(scratch_ws), stream_of(with)));
     const auto changed = [](const Tensor& t) { if (!t.is_inference()) written_behind_autograd(t); };
     for (const Tensor& t : ws) changed(t);
     for (const TensorList& s : state)

@@ -681,7 +681,7 @@ def adamw_update(params, grads, first, second, step, lr=1e-3, betas=(0.9, 0.999)
     is 0 is held as 0 too.  Without it the two codes' quotient has no bound: where a block's gradients lie more than tenfold apart and
     some are 0, an element can keep its first moment alone and move by lr m / eps, hundreds of lr (optim.AdamW pairs them)."""
     params, grads = list(params), list(grads)
-    if params or grads:
+    if params or grads or isinstance(step, torch.Tensor):
         _lib.native().adamw_update(params, grads, list(first), list(second), None if first_scale is None else list(first_scale),
                                    None if second_scale is None else list(second_scale), step, lr, betas[0], betas[1], eps, weight_decay,
                                    norm, max_norm, seed, paired)

@@ -137,3 +137,16 @@ def test_numbers_on_the_device_lie_apart_from_what_is_updated():
     call(step, a[0])
     call(number(b.zero_()), g[0])                                # beside them, or read on both sides: as ever
     assert int(step) == int(number(b)) == 1
+
+
+def test_a_call_without_elements_still_counts():
+    import snntc_amd as snn
+    step, none = torch.tensor(4, dtype=torch.int64, device=DEV), [torch.zeros(0, device=DEV)]
+    snn.adamw_update([], [], [], [], step)
+    assert int(step) == 5
+    snn.adamw_update(none, none, none, none, step)
+    assert int(step) == 6
+    with pytest.raises(snn.SnntcLibraryError, match="no CPU fallback"):
+        snn.adamw_update([], [], [], [], step.cpu())
+    with pytest.raises(ValueError, match="as many states"):
+        snn.adamw_update([], [], none, none, step)
